@@ -9,11 +9,12 @@ import re
 
 from . import build as _build
 
-U8, S8, S32, S16, F32 = 0, 1, 2, 3, 4  # S16: QSYMM16 (stand-alone stage only); F32: dequantized GEMM output
+U8, S8, S32, S16, F32, F16, BF16 = 0, 1, 2, 3, 4, 5, 6  # F16, BF16: mx_* only. S16: QSYMM16 (stand-alone stage only); F32: dequantized GEMM output
 STAGE_NONE, STAGE_QUANTIZE_DOWN, STAGE_FIXEDPOINT = 0, 1, 2
 # cugl_status values the tests name
 SUCCESS, RUNTIME_ERROR, INVALID_ARGUMENT = 0, 1, 6
 INT32_MIN, INT32_MAX = -(2 ** 31), 2 ** 31 - 1
+MXFP4, NVFP4 = 0, 1  # cugl_mx_format
 
 _vp = C.c_void_p
 _i32 = C.c_int32
@@ -73,6 +74,14 @@ class PoolDesc(C.Structure):
         ("exclude_padding", _i32), ("is_global", _i32),
         ("src_scale", C.c_float), ("src_zero_point", _i32),
         ("dst_scale", C.c_float), ("dst_zero_point", _i32),
+    ]
+
+
+class MxDesc(C.Structure):
+    """cugl_mx_desc"""
+    _fields_ = [
+        ("rows", _i32), ("cols", _i32), ("format", _i32), ("dtype", _i32),
+        ("ld", _i64), ("ld_packed", _i64), ("tensor_exponent", _i32),
     ]
 
 
@@ -175,6 +184,11 @@ _SIGNATURES = {
     "cugl_activation_qasymm8": (C.c_int, [_vp, _vp, _vp, _i64, _i32, C.c_float, C.c_float, C.c_float, _i32,
                                           C.c_float, _i32]),
     "cugl_softmax_qasymm8": (C.c_int, [_vp, _vp, _vp, _i32, _i32, C.c_float, C.c_float, _i32]),
+    "cugl_mx_scale_bytes": (C.c_size_t, [_i32, _i32, _i32]),
+    "cugl_mx_validate": (C.c_int, [C.POINTER(MxDesc), C.POINTER(C.c_char_p)]),
+    "cugl_mx_quantize": (C.c_int, [_vp, C.POINTER(MxDesc), _vp, _vp, _vp]),
+    "cugl_mx_dequantize": (C.c_int, [_vp, C.POINTER(MxDesc), _vp, _vp, _vp]),
+    "cugl_mx_tile_scales": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }
 
 _lib = None
@@ -380,6 +394,18 @@ class Context:
     def transpose_batched(self, src, dst, rows, cols, batch):
         self.check(self.lib.cugl_transpose_batched(self.handle, _dptr(src), _dptr(dst), rows, cols, batch))
 
+    # microscaled 4-bit matrices ------------------------------------------------------------------------
+    def mx_quantize(self, desc: "MxDesc", src, dst, scales):
+        """Plain matrix -> packed codes and scale tiles (mx_scale_bytes)."""
+        self.check(self.lib.cugl_mx_quantize(self.handle, C.byref(desc), _dptr(src), _dptr(dst), _dptr(scales)))
+
+    def mx_dequantize(self, desc: "MxDesc", src, scales, dst):
+        self.check(self.lib.cugl_mx_dequantize(self.handle, C.byref(desc), _dptr(src), _dptr(scales), _dptr(dst)))
+
+    def mx_tile_scales(self, src, ld, rows, cols, format, dst):
+        """Row-major scale bytes -> scale tiles."""
+        self.check(self.lib.cugl_mx_tile_scales(self.handle, _dptr(src), ld, rows, cols, format, _dptr(dst)))
+
     def weights_reshape_nhwc(self, w, dst, K, OFM):
         self.check(self.lib.cugl_weights_reshape_nhwc(self.handle, _dptr(w), _dptr(dst), K, OFM))
 
@@ -440,6 +466,32 @@ def gemm_validate(desc: GemmDesc):
     """Returns (status, reason)."""
     why = C.c_char_p()
     st = load_library().cugl_gemmlowp_validate(C.byref(desc), C.byref(why))
+    return st, (why.value or b"").decode()
+
+
+def mx_pitch(cols: int) -> int:
+    """Bytes between packed rows that every mx_* call takes: the next multiple of 16."""
+    return (cols + 31) // 32 * 16
+
+
+def mx_scale_bytes(rows: int, cols: int, format: int) -> int:
+    return int(load_library().cugl_mx_scale_bytes(rows, cols, format))
+
+
+def make_mx_desc(rows, cols, format, dtype, ld=None, ld_packed=None, tensor_exponent=0) -> MxDesc:
+    """cugl_mx_desc of a dense plain matrix and packed rows mx_pitch(cols) apart unless strides (bytes) are given."""
+    d = MxDesc()
+    d.rows, d.cols, d.format, d.dtype = rows, cols, format, dtype
+    d.ld = cols * (4 if dtype == F32 else 2) if ld is None else ld
+    d.ld_packed = mx_pitch(cols) if ld_packed is None else ld_packed
+    d.tensor_exponent = tensor_exponent
+    return d
+
+
+def mx_validate(desc: MxDesc):
+    """Returns (status, reason)."""
+    why = C.c_char_p()
+    st = load_library().cugl_mx_validate(C.byref(desc), C.byref(why))
     return st, (why.value or b"").decode()
 
 

@@ -1,0 +1,209 @@
+// Microscaled 4-bit floating point (MXFP4 and NVFP4): what the quantiser, the product and the expert layer share.
+//
+// A matrix is cut into blocks along its rows.  A block is kBlock codes E2M1 (sign, two exponent bits, one mantissa bit:
+// 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte:
+//   MXFP4  blocks of 32, scale E8M0: 2^(byte - 127); 255 is NaN
+//   NVFP4  blocks of 16, scale E4M3 (unsigned: bit 7 is 0); 0x7f is NaN
+// Packed rows hold element 2 i in the low half of byte i.  Scale bytes lie in tiles of 128 rows x 4 blocks, 512 bytes,
+// the order in which tcgen05.cp spreads them over tensor memory: row r, block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b.
+// The tiles of one group of 128 rows follow each other.
+#pragma once
+
+#include "kernels.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+namespace cugl
+{
+constexpr int kMxTileBytes = 512;
+
+inline int mx_block(int format)
+{
+    return format == CUGL_NVFP4 ? 16 : 32;
+}
+inline int64_t mx_blocks(int64_t cols, int format)
+{
+    return (cols + mx_block(format) - 1) / mx_block(format);
+}
+inline int64_t mx_scale_tiles(int64_t cols, int format) // tiles along one group of 128 rows
+{
+    return (mx_blocks(cols, format) + 3) / 4;
+}
+inline int64_t mx_scale_size(int64_t rows, int64_t cols, int format)
+{
+    return (rows + 127) / 128 * mx_scale_tiles(cols, format) * kMxTileBytes;
+}
+inline int dtype_size(int dtype)
+{
+    return dtype == CUGL_F32 ? 4 : 2;
+}
+inline bool is_float_dtype(int dtype)
+{
+    return dtype == CUGL_F32 || dtype == CUGL_F16 || dtype == CUGL_BF16;
+}
+
+// The context's device for the duration of one call: the caller's current device may be another one.
+class DeviceScope
+{
+public:
+    explicit DeviceScope(const cugl_context *ctx)
+    {
+        if (cudaGetDevice(&before_) == cudaSuccess && before_ != ctx->device)
+        {
+            changed_ = true;
+            (void)cudaSetDevice(ctx->device);
+        }
+    }
+    ~DeviceScope()
+    {
+        if (changed_)
+        {
+            (void)cudaSetDevice(before_);
+        }
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+
+private:
+    int  before_  = 0;
+    bool changed_ = false;
+};
+
+__device__ __forceinline__ size_t mx_scale_offset(int64_t row, int64_t block, int64_t tiles)
+{
+    return static_cast<size_t>((row >> 7) * tiles + (block >> 2)) * kMxTileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+// Eight values (already divided by their scale) to E2M1, v[0] in the lowest four bits: to nearest, ties to even, saturated.
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float *v)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        w |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_E2M1, cudaRoundNearest)) << (8 * i);
+    }
+    return w;
+}
+
+// Eight codes to f16 pairs (exact), the element of the lowest four bits first.
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t w, __half2 (&h)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        h[i] = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w >> (8 * i)), __NV_E2M1));
+    }
+}
+
+// A block's scale from the largest |value| in it (the bits of a non-negative float; NaN and infinity order above all
+// finite values).  byte: what is stored.  mul: what a value is multiplied by on its way to a code.
+//   MXFP4  2^max(-127, floor(log2 amax) - 2): the largest value lands in [4, 8), above 6 it saturates.  mul is a power of
+//          two, so the codes are those of the exact quotient.
+//   NVFP4  amax * 2^-exponent / 6 to the nearest E4M3 within [2^-9, 448].  Rounding the quotient to 24 bits first changes
+//          nothing: a quotient that is not a midpoint of E4M3 (five bits) stays at least half a step of 24 bits away from it.
+// A block of zeros gets the byte 0; one with a NaN or an infinity gets the NaN scale, all of it reads back as NaN.
+struct MxScale
+{
+    uint32_t byte;
+    float    mul;  // MXFP4: 1 / scale.  NVFP4: 2^-exponent / scale, rounded up (scale_to_code)
+    float    div;  // NVFP4: the scale itself (f32 sources divide)
+};
+template <int kFormat>
+__device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponent_mul)
+{
+    MxScale s;
+    if (kFormat == CUGL_MXFP4)
+    {
+        const uint32_t e = amax_bits >> 23;
+        s.byte           = e > 2 ? e - 2 : 0;
+        s.mul            = __uint_as_float((254 - s.byte) << 23);
+        s.div            = 0.f;
+        if (amax_bits >= 0x7f800000u)
+        {
+            s.byte = 255;
+            s.mul  = 0.f;
+        }
+        return s;
+    }
+    const float                amax = __uint_as_float(amax_bits) * exponent_mul;
+    const float                v    = fminf(fmaxf(__fdiv_rn(amax, 6.f), 0x1p-9f), 448.f);
+    const __nv_fp8_storage_t   b    = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+    const float                f    = __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+    s.byte                          = b;
+    s.div                           = f;
+    s.mul                           = __frcp_ru(f) * exponent_mul;
+    if (amax_bits == 0 || amax_bits >= 0x7f800000u)
+    {
+        s.byte = amax_bits == 0 ? 0 : 0x7f;
+        s.mul  = 0.f;
+        s.div  = 0.f;
+    }
+    return s;
+}
+
+// value / scale, near enough to the exact quotient that rounding it to E2M1 gives the quotient's code.
+//   MXFP4            a product with a power of two
+//   NVFP4, 16 bits   the reciprocal rounded up times the value, rounded towards zero: for every scale (four bits) and every
+//                    value of up to eleven bits it compares with each midpoint of E2M1 as the exact quotient does (checked
+//                    for all of them); one instruction
+//   NVFP4, 32 bits   a division: as for the scale, a quotient that is no midpoint does not round onto one
+template <int kFormat, bool kWide>
+__device__ __forceinline__ float scale_to_code(float v, const MxScale &s, float exponent_mul)
+{
+    if (kFormat == CUGL_MXFP4)
+    {
+        return v * s.mul;
+    }
+    if (kWide)
+    {
+        return s.div != 0.f ? __fdiv_rn(v * exponent_mul, s.div) : 0.f;
+    }
+    return __fmul_rz(v, s.mul);
+}
+
+// The value of a scale byte.
+template <int kFormat>
+__device__ __forceinline__ float mx_scale_value(uint32_t byte)
+{
+    if (kFormat == CUGL_MXFP4)
+    {
+        const uint32_t bits = byte == 0 ? 0x00400000u : byte << 23; // 2^-127 is subnormal
+        return __uint_as_float(byte == 255 ? 0x7fc00000u : bits);
+    }
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte & 0x7f), __NV_E4M3)));
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v)
+{
+    return v;
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v)
+{
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v)
+{
+    return __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ float to_float(float v)
+{
+    return v;
+}
+__device__ __forceinline__ float to_float(__half v)
+{
+    return __half2float(v);
+}
+__device__ __forceinline__ float to_float(__nv_bfloat16 v)
+{
+    return __bfloat162float(v);
+}
+} // namespace cugl

@@ -54,7 +54,9 @@ typedef enum cugl_dtype
     CUGL_S8  = 1,
     CUGL_S32 = 2,
     CUGL_S16 = 3, /* QSYMM16: destination of the stand-alone fixed-point output stage only */
-    CUGL_F32 = 4  /* destination of the GEMM with stage NONE: the int32 result times dequantize_scale */
+    CUGL_F32 = 4, /* destination of the GEMM with stage NONE: the int32 result times dequantize_scale; cugl_mx_* */
+    CUGL_F16 = 5, /* cugl_mx_* only */
+    CUGL_BF16 = 6 /* cugl_mx_* only */
 } cugl_dtype;
 
 /* GEMMLowpOutputStageType (arm_compute/function_info/GEMMInfo.h:40-46).  Only NONE and
@@ -527,6 +529,53 @@ CUGL_API cugl_status cugl_activation_qasymm8(cugl_context *ctx, const void *d_sr
 /* rows x cols, contiguous rows; softmax along a row; output quantization is fixed at (1/256, 0). */
 CUGL_API cugl_status cugl_softmax_qasymm8(cugl_context *ctx, const void *d_src, void *d_dst, int32_t rows, int32_t cols,
                                           float beta, float src_scale, int32_t src_zero_point);
+
+/* ------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point: quantisation, read-back, product and expert layer for language models.  No counterpart
+ * in the reference, whose quantised types are 8-bit integers with one scale per tensor or channel.
+ *
+ * A matrix is cut into blocks along its rows.  A block is E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) and one
+ * scale byte; a value is code * scale * 2^tensor_exponent.
+ *   CUGL_MXFP4  blocks of 32, scale E8M0 = 2^(byte - 127): 2^max(-127, floor(log2 amax) - 2)
+ *   CUGL_NVFP4  blocks of 16, scale E4M3: amax * 2^-tensor_exponent / 6 to the nearest (ties to even) within [2^-9, 448]
+ * where amax is the block's largest |value|.  Codes are value / scale to the nearest, ties to even, saturated at 6.  A block of
+ * zeros has the scale byte 0; a block with a NaN or an infinity has the NaN scale (0xff, 0x7f), and all of it reads back as NaN.
+ * Packed rows hold element 2 i in the low half of byte i; the high half behind an odd row is 0.
+ * Scale bytes lie in tiles of 128 rows x 4 blocks, 512 bytes: row r, block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b;
+ * the ceil(blocks / 4) tiles of 128 rows follow each other, then come those of the next 128 rows (cugl_mx_scale_bytes in all,
+ * 16-byte aligned).  The bytes of blocks behind a row are 0 (a product reads them); the bytes of rows behind the last one are
+ * neither written nor used.
+ * ---------------------------------------------------------------------------------------------- */
+typedef enum cugl_mx_format
+{
+    CUGL_MXFP4 = 0,
+    CUGL_NVFP4 = 1
+} cugl_mx_format;
+
+typedef struct cugl_mx_desc
+{
+    int32_t rows, cols;
+    int32_t format;          /* cugl_mx_format */
+    int32_t dtype;           /* of the plain matrix: CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int64_t ld;              /* bytes between rows of the plain matrix */
+    int64_t ld_packed;       /* bytes between packed rows, at least ceil(cols / 2); a product wants a multiple of 16 */
+    int32_t tensor_exponent; /* CUGL_NVFP4: -64 .. 64, values are stored times 2^-tensor_exponent; CUGL_MXFP4: 0 */
+} cugl_mx_desc;
+
+/* Bytes of the scale tiles of a rows x cols matrix (0: bad argument). */
+CUGL_API size_t      cugl_mx_scale_bytes(int32_t rows, int32_t cols, int32_t format);
+/* Pure host check of a descriptor; reason (optional) receives a static string. */
+CUGL_API cugl_status cugl_mx_validate(const cugl_mx_desc *desc, const char **reason);
+/* Plain matrix d_src -> packed codes d_dst and scale tiles d_scales.  Bytes between the end of a packed row and the next row
+ * are left as they are.  rows == 0: nothing to do. */
+CUGL_API cugl_status cugl_mx_quantize(cugl_context *ctx, const cugl_mx_desc *desc, const void *d_src, void *d_dst,
+                                      void *d_scales);
+/* The way back: code * scale * 2^tensor_exponent, rounded once to the plain matrix' type. */
+CUGL_API cugl_status cugl_mx_dequantize(cugl_context *ctx, const cugl_mx_desc *desc, const void *d_src,
+                                        const void *d_scales, void *d_dst);
+/* Scale bytes from elsewhere, row-major (rows of ceil(cols / block) bytes, ld bytes apart), into tiles. */
+CUGL_API cugl_status cugl_mx_tile_scales(cugl_context *ctx, const void *d_src, int64_t ld, int32_t rows, int32_t cols,
+                                         int32_t format, void *d_dst);
 
 #ifdef __cplusplus
 }
