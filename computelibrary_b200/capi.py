@@ -85,6 +85,14 @@ class MxDesc(C.Structure):
     ]
 
 
+class MxGemmDesc(C.Structure):
+    """cugl_mx_gemm_desc"""
+    _fields_ = [
+        ("M", _i32), ("N", _i32), ("K", _i32), ("format", _i32), ("dst_dtype", _i32), ("has_bias", _i32),
+        ("lda", _i64), ("ldb", _i64), ("ldd", _i64), ("alpha", C.c_float),
+    ]
+
+
 POOL_MAX, POOL_AVG = 0, 1
 ACT_NONE, ACT_RELU, ACT_BOUNDED_RELU, ACT_LU_BOUNDED_RELU = -1, 0, 1, 2
 
@@ -188,6 +196,8 @@ _SIGNATURES = {
     "cugl_mx_validate": (C.c_int, [C.POINTER(MxDesc), C.POINTER(C.c_char_p)]),
     "cugl_mx_quantize": (C.c_int, [_vp, C.POINTER(MxDesc), _vp, _vp, _vp]),
     "cugl_mx_dequantize": (C.c_int, [_vp, C.POINTER(MxDesc), _vp, _vp, _vp]),
+    "cugl_mx_gemm_validate": (C.c_int, [C.POINTER(MxGemmDesc), C.POINTER(C.c_char_p)]),
+    "cugl_mx_gemm": (C.c_int, [_vp, C.POINTER(MxGemmDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
     "cugl_mx_tile_scales": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }
 
@@ -406,6 +416,11 @@ class Context:
         """Row-major scale bytes -> scale tiles."""
         self.check(self.lib.cugl_mx_tile_scales(self.handle, _dptr(src), ld, rows, cols, format, _dptr(dst)))
 
+    def mx_gemm(self, desc: "MxGemmDesc", a, a_scales, b, b_scales, bias, dst):
+        """dst = alpha * a . b^T + bias of packed matrices."""
+        self.check(self.lib.cugl_mx_gemm(self.handle, C.byref(desc), _dptr(a), _dptr(a_scales), _dptr(b), _dptr(b_scales),
+                                         _dptr(bias), _dptr(dst)))
+
     def weights_reshape_nhwc(self, w, dst, K, OFM):
         self.check(self.lib.cugl_weights_reshape_nhwc(self.handle, _dptr(w), _dptr(dst), K, OFM))
 
@@ -492,6 +507,24 @@ def mx_validate(desc: MxDesc):
     """Returns (status, reason)."""
     why = C.c_char_p()
     st = load_library().cugl_mx_validate(C.byref(desc), C.byref(why))
+    return st, (why.value or b"").decode()
+
+
+def make_mx_gemm_desc(M, N, K, format, dst_dtype, lda=None, ldb=None, ldd=None, alpha=1.0, has_bias=False) -> MxGemmDesc:
+    """cugl_mx_gemm_desc; packed rows mx_pitch(K) apart and a dense dst unless strides (bytes) are given."""
+    d = MxGemmDesc()
+    d.M, d.N, d.K, d.format, d.dst_dtype, d.has_bias = M, N, K, format, dst_dtype, int(has_bias)
+    d.lda = mx_pitch(K) if lda is None else lda
+    d.ldb = mx_pitch(K) if ldb is None else ldb
+    d.ldd = N * (4 if dst_dtype == F32 else 2) if ldd is None else ldd
+    d.alpha = alpha
+    return d
+
+
+def mx_gemm_validate(desc: MxGemmDesc):
+    """Returns (status, reason)."""
+    why = C.c_char_p()
+    st = load_library().cugl_mx_gemm_validate(C.byref(desc), C.byref(why))
     return st, (why.value or b"").decode()
 
 

@@ -1,0 +1,167 @@
+// Block-scaled tensor-core products (tcgen05.mma with E2M1 operands): what the product and the expert layer share.
+//
+// Operand roles: the weights are the 128 rows of an MMA (accumulator lanes = output channels), the tokens its columns, as few
+// as sixteen -- so a product with one token uses the same instructions as one with thousands, and a warp that drains the
+// accumulator stores 32 consecutive channels of a token.
+//
+// K is walked in chunks of 256 elements: rows of 128 bytes in the 128-byte swizzle, as TMA writes them.  One MMA takes 64
+// elements (32 bytes of each row) and the scales of its four (NVFP4) or two (MXFP4) blocks per row, which tcgen05.cp has
+// brought from shared to tensor memory: a scale tile of 512 bytes becomes four columns, repeated in the four lane quarters.
+#pragma once
+
+#include "mx.cuh"
+#include "sm100.cuh"
+
+namespace cugl
+{
+namespace
+{
+constexpr int kMxChunk      = 256;            // elements of K per pipeline stage
+constexpr int kMxChunkBytes = kMxChunk / 2;   // one swizzle row
+constexpr int kMxStepK      = 64;             // elements of K per MMA
+constexpr int kMxRows       = 128;            // weight rows per MMA
+constexpr int kMxWBytes     = kMxRows * kMxChunkBytes;
+
+template <int kFormat>
+struct MxTraits
+{
+    static constexpr int kChunkTiles = kFormat == CUGL_NVFP4 ? 4 : 2; // scale tiles per chunk and 128 rows
+    static constexpr int kChunkScale = kChunkTiles * kMxTileBytes;
+    static constexpr int kChunkCols  = kChunkTiles * 4;               // their tensor-memory columns
+};
+
+// Instruction descriptor of kind::mxf4 / mxf4nvf4: E2M1 operands (1) in bits 7 and 10, columns / 8 in 17..22, scale type in 23
+// (0 E4M3, 1 E8M0), rows / 16 in 24..28.  The byte of the scale word an MMA starts at goes to bits 4..5 (columns' operand)
+// and 29..30 (rows' operand), see mx_scale_id.
+inline uint32_t mx_idesc(int format, int rows, int cols)
+{
+    return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(cols >> 3) << 17) | ((format == CUGL_MXFP4 ? 1u : 0u) << 23) |
+           (static_cast<uint32_t>(rows >> 4) << 24);
+}
+template <int kFormat>
+__device__ __forceinline__ constexpr uint32_t mx_scale_id(int step) // two MXFP4 steps share a tile
+{
+    return kFormat == CUGL_MXFP4 ? (static_cast<uint32_t>((step & 1) * 2) << 4) | (static_cast<uint32_t>((step & 1) * 2) << 29) : 0u;
+}
+template <int kFormat>
+__device__ __forceinline__ constexpr int mx_step_tile(int step)
+{
+    return kFormat == CUGL_MXFP4 ? step >> 1 : step;
+}
+
+// D[tmem] (+)= sum over 64 elements of (A code * A scale) * (B code * B scale), float accumulation
+template <int kFormat>
+__device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scale, uint32_t b_scale,
+                                        uint32_t accumulate)
+{
+    if constexpr (kFormat == CUGL_MXFP4)
+    {
+        asm volatile("{\n\t"
+                     ".reg .pred p;\n\t"
+                     "setp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+                     "}"
+                     :
+                     : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+                     : "memory");
+    }
+    else
+    {
+        asm volatile("{\n\t"
+                     ".reg .pred p;\n\t"
+                     "setp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+                     "}"
+                     :
+                     : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+                     : "memory");
+    }
+}
+
+// One scale tile (32 rows of 16 bytes in shared memory) to four tensor-memory columns, in all four lane quarters.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t d_tmem, uint64_t s_desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
+}
+// Descriptor of a scale tile: no swizzle, groups of eight 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr)
+{
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3ffff) >> 4);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :
+                 : "r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Waits for a barrier's phase whatever the abort flag says: a producer that gives up lets its copies in flight land first.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, long long limit)
+{
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 <= limit)
+    {
+    }
+}
+
+// The MMAs of one chunk whose operands and scales have landed in shared memory.  steps: MMAs inside K (1 .. 4).  a_stage,
+// b_stage: shared addresses of the operands; a_sf, b_sf: of their scale tiles; t_a, t_b: tensor-memory columns for those.
+template <int kFormat>
+__device__ __forceinline__ void mx_chunk(uint32_t d_tmem, uint32_t a_stage, uint32_t b_stage, uint32_t t_a, uint32_t t_b, uint32_t idesc, int steps,
+                                         bool first)
+{
+    const uint64_t a_desc = make_kmajor_sw128_desc(a_stage), b_desc = make_kmajor_sw128_desc(b_stage);
+#pragma unroll
+    for (int k = 0; k < kMxChunk / kMxStepK; ++k)
+    {
+        if (k < steps)
+        {
+            const uint32_t col = static_cast<uint32_t>(mx_step_tile<kFormat>(k) * 4);
+            umma_mx<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc | mx_scale_id<kFormat>(k), t_a + col, t_b + col,
+                             first && k == 0 ? 0u : 1u);
+        }
+    }
+}
+template <int kFormat>
+__device__ __forceinline__ void mx_chunk_scales(uint32_t t_dst, uint32_t sf, int tiles)
+{
+    const uint64_t desc = make_scale_desc(sf);
+#pragma unroll
+    for (int t = 0; t < MxTraits<kFormat>::kChunkTiles; ++t)
+    {
+        if (t < tiles)
+        {
+            tmem_copy_scales(t_dst + 4 * t, desc + static_cast<uint64_t>(t * (kMxTileBytes >> 4)));
+        }
+    }
+}
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// packed rows x (inner bytes), ld bytes apart; box = box_rows x 128 bytes in the 128-byte swizzle; what lies outside reads as 0
+inline bool encode_packed_map(CUtensorMap *map, const void *base, int64_t rows, int64_t inner, int64_t ld, int box_rows)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (fn == nullptr)
+    {
+        return false;
+    }
+    const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2]     = {kMxChunkBytes, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2]    = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+} // namespace
+} // namespace cugl

@@ -577,6 +577,25 @@ CUGL_API cugl_status cugl_mx_dequantize(cugl_context *ctx, const cugl_mx_desc *d
 CUGL_API cugl_status cugl_mx_tile_scales(cugl_context *ctx, const void *d_src, int64_t ld, int32_t rows, int32_t cols,
                                          int32_t format, void *d_dst);
 
+/* dst[m][n] = alpha * sum_k a[m][k] * b[n][k] + bias[n]: tokens (A, M rows) times weights (B, N rows of K elements), both
+ * packed with scale tiles of the same format (cugl_mx_quantize), float accumulation, rounded once to dst_dtype.  alpha carries
+ * the tensor exponents (2^(exponent_a + exponent_b)) or any other factor. */
+typedef struct cugl_mx_gemm_desc
+{
+    int32_t M, N, K;
+    int32_t format;        /* cugl_mx_format, of both operands */
+    int32_t dst_dtype;     /* CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int32_t has_bias;      /* float bias [N] */
+    int64_t lda, ldb, ldd; /* bytes between rows; lda and ldb multiples of 16 */
+    float   alpha;
+} cugl_mx_gemm_desc;
+
+CUGL_API cugl_status cugl_mx_gemm_validate(const cugl_mx_gemm_desc *desc, const char **reason);
+/* One launch, no workspace, nothing kept between calls.  Operands and scale tiles are 16-byte aligned.  The sum over k runs in
+ * an order that depends on the sizes only: equal calls give equal bits.  M == 0: nothing to do. */
+CUGL_API cugl_status cugl_mx_gemm(cugl_context *ctx, const cugl_mx_gemm_desc *desc, const void *d_a, const void *d_a_scales,
+                                  const void *d_b, const void *d_b_scales, const float *d_bias, void *d_dst);
+
 #ifdef __cplusplus
 }
 #endif
