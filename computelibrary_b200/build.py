@@ -19,7 +19,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libcugl.so")
 SOURCES = ["context.cu", "bandwidth_kernels.cu", "gemmlowp_simt.cu", "gemmlowp_tcgen05.cu", "plans.cu", "noalloc.cu",
            "layer_kernels.cu", "gemmlowp_tcgen05_epi8.cu", "gemmlowp_tcgen05_epi16.cu",
-           "gemmlowp_dispatch.cu", "mx_quant.cu", "mx_gemm.cu"]
+           "gemmlowp_dispatch.cu", "mx_quant.cu", "mx_gemm.cu", "mx_moe.cu"]
 HEADERS = ["common.cuh", "kernels.cuh", "sm100.cuh", "mx.cuh", "mx_mma.cuh"]
 
 OBJ_DIR = os.path.join(LIB_DIR, "obj")

@@ -93,6 +93,16 @@ class MxGemmDesc(C.Structure):
     ]
 
 
+class MxMoeDesc(C.Structure):
+    """cugl_mx_moe_desc"""
+    _fields_ = [
+        ("tokens", _i32), ("hidden", _i32), ("intermediate", _i32), ("experts", _i32), ("top_k", _i32),
+        ("format", _i32), ("dtype", _i32), ("renormalize", _i32), ("x_exponent", _i32), ("h_exponent", _i32),
+        ("gate_alpha", C.c_float), ("up_alpha", C.c_float), ("down_alpha", C.c_float),
+        ("ld_x", _i64), ("ld_logits", _i64), ("ld_dst", _i64), ("ld_gate_up", _i64), ("ld_down", _i64),
+    ]
+
+
 POOL_MAX, POOL_AVG = 0, 1
 ACT_NONE, ACT_RELU, ACT_BOUNDED_RELU, ACT_LU_BOUNDED_RELU = -1, 0, 1, 2
 
@@ -198,6 +208,9 @@ _SIGNATURES = {
     "cugl_mx_dequantize": (C.c_int, [_vp, C.POINTER(MxDesc), _vp, _vp, _vp]),
     "cugl_mx_gemm_validate": (C.c_int, [C.POINTER(MxGemmDesc), C.POINTER(C.c_char_p)]),
     "cugl_mx_gemm": (C.c_int, [_vp, C.POINTER(MxGemmDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cugl_mx_moe_validate": (C.c_int, [C.POINTER(MxMoeDesc), C.POINTER(C.c_char_p)]),
+    "cugl_mx_moe_workspace_bytes": (C.c_size_t, [C.POINTER(MxMoeDesc)]),
+    "cugl_mx_moe": (C.c_int, [_vp, C.POINTER(MxMoeDesc)] + [_vp] * 10 + [C.c_size_t]),
     "cugl_mx_tile_scales": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }
 
@@ -421,6 +434,15 @@ class Context:
         self.check(self.lib.cugl_mx_gemm(self.handle, C.byref(desc), _dptr(a), _dptr(a_scales), _dptr(b), _dptr(b_scales),
                                          _dptr(bias), _dptr(dst)))
 
+    def mx_moe(self, desc: "MxMoeDesc", x, logits, gate, up, down, dst, workspace, workspace_bytes=None):
+        """One expert layer.  gate, up, down: (packed codes, scale tiles) each; workspace: mx_moe_workspace_bytes(desc) bytes
+        (workspace_bytes: its size where it is a raw pointer)."""
+        if workspace_bytes is None:
+            workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        self.check(self.lib.cugl_mx_moe(self.handle, C.byref(desc), _dptr(x), _dptr(logits), _dptr(gate[0]), _dptr(gate[1]),
+                                        _dptr(up[0]), _dptr(up[1]), _dptr(down[0]), _dptr(down[1]), _dptr(dst),
+                                        _dptr(workspace), workspace_bytes))
+
     def weights_reshape_nhwc(self, w, dst, K, OFM):
         self.check(self.lib.cugl_weights_reshape_nhwc(self.handle, _dptr(w), _dptr(dst), K, OFM))
 
@@ -526,6 +548,33 @@ def mx_gemm_validate(desc: MxGemmDesc):
     why = C.c_char_p()
     st = load_library().cugl_mx_gemm_validate(C.byref(desc), C.byref(why))
     return st, (why.value or b"").decode()
+
+
+def make_mx_moe_desc(tokens, hidden, intermediate, experts, top_k, format, dtype, renormalize=True, x_exponent=0, h_exponent=0,
+                     gate_alpha=1.0, up_alpha=1.0, down_alpha=1.0, ld_x=None, ld_logits=None, ld_dst=None, ld_gate_up=None,
+                     ld_down=None) -> MxMoeDesc:
+    """cugl_mx_moe_desc; dense x, logits and dst and packed rows mx_pitch apart unless strides (bytes) are given."""
+    d = MxMoeDesc()
+    d.tokens, d.hidden, d.intermediate, d.experts, d.top_k = tokens, hidden, intermediate, experts, top_k
+    d.format, d.dtype, d.renormalize, d.x_exponent, d.h_exponent = format, dtype, int(renormalize), x_exponent, h_exponent
+    d.gate_alpha, d.up_alpha, d.down_alpha = gate_alpha, up_alpha, down_alpha
+    d.ld_x = 2 * hidden if ld_x is None else ld_x
+    d.ld_logits = 4 * experts if ld_logits is None else ld_logits
+    d.ld_dst = 2 * hidden if ld_dst is None else ld_dst
+    d.ld_gate_up = mx_pitch(hidden) if ld_gate_up is None else ld_gate_up
+    d.ld_down = mx_pitch(intermediate) if ld_down is None else ld_down
+    return d
+
+
+def mx_moe_validate(desc: MxMoeDesc):
+    """Returns (status, reason)."""
+    why = C.c_char_p()
+    st = load_library().cugl_mx_moe_validate(C.byref(desc), C.byref(why))
+    return st, (why.value or b"").decode()
+
+
+def mx_moe_workspace_bytes(desc: MxMoeDesc) -> int:
+    return int(load_library().cugl_mx_moe_workspace_bytes(C.byref(desc)))
 
 
 def make_pool_desc(B, H, W, C_, pool_type, size=(1, 1), stride=(1, 1), pad=(0, 0, 0, 0), in_q=(1.0, 0),

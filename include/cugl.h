@@ -596,6 +596,40 @@ CUGL_API cugl_status cugl_mx_gemm_validate(const cugl_mx_gemm_desc *desc, const 
 CUGL_API cugl_status cugl_mx_gemm(cugl_context *ctx, const cugl_mx_gemm_desc *desc, const void *d_a, const void *d_a_scales,
                                   const void *d_b, const void *d_b_scales, const float *d_bias, void *d_dst);
 
+/* A mixture-of-experts layer for up to 128 tokens with 4-bit weights, gate included:
+ *   chosen   the top_k largest logits of a token, equal ones by index; NaN and -infinity are never chosen
+ *   p        exp(logit) over its sum, over the chosen ones (renormalize) or over all
+ *   x'       x quantised to the weights' format (x_exponent)
+ *   h[e]     quantise(p[e] * silu(g) * u), g = gate_alpha * x' . gate[e]^T, u = up_alpha * x' . up[e]^T   (h_exponent)
+ *   dst      down_alpha * sum over the chosen e of h[e] . down[e]^T, rounded once
+ * A token with nothing to choose gets zeros.  gate and up are [experts * intermediate] packed rows of hidden elements, down
+ * [experts * hidden] packed rows of intermediate elements, experts one after the other; the scale tiles of every expert are
+ * those of a matrix of its own (cugl_mx_scale_bytes(intermediate, hidden) and (hidden, intermediate) bytes per expert). */
+typedef struct cugl_mx_moe_desc
+{
+    int32_t tokens;                 /* 0 .. 128 */
+    int32_t hidden, intermediate;   /* multiples of 16 */
+    int32_t experts, top_k;         /* 1 .. 512, 1 .. 16 */
+    int32_t format;                 /* cugl_mx_format */
+    int32_t dtype;                  /* of x and dst: CUGL_F16 or CUGL_BF16 */
+    int32_t renormalize;
+    int32_t x_exponent, h_exponent; /* CUGL_NVFP4: tensor exponents x and h are quantised with; CUGL_MXFP4: 0 */
+    float   gate_alpha, up_alpha, down_alpha; /* what the weights' values are to be multiplied by (their tensor exponents) */
+    int64_t ld_x, ld_logits, ld_dst;          /* bytes between rows */
+    int64_t ld_gate_up, ld_down;              /* bytes between packed rows, multiples of 16 */
+} cugl_mx_moe_desc;
+
+CUGL_API cugl_status cugl_mx_moe_validate(const cugl_mx_moe_desc *desc, const char **reason);
+/* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU, and
+ * captured graphs that are replayed at the same time, need one each. */
+CUGL_API size_t      cugl_mx_moe_workspace_bytes(const cugl_mx_moe_desc *desc);
+/* d_logits: float [tokens][experts].  d_workspace: 256-byte aligned, at least cugl_mx_moe_workspace_bytes.  Three launches,
+ * results do not depend on timing.  tokens == 0: nothing to do. */
+CUGL_API cugl_status cugl_mx_moe(cugl_context *ctx, const cugl_mx_moe_desc *desc, const void *d_x, const float *d_logits,
+                                 const void *d_gate, const void *d_gate_scales, const void *d_up, const void *d_up_scales,
+                                 const void *d_down, const void *d_down_scales, void *d_dst, void *d_workspace,
+                                 size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

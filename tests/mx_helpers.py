@@ -103,3 +103,68 @@ def matrix(rng, rows, cols, fmt, std=1.0):
     """A random quantised matrix: (codes, scale bytes, values)."""
     code, byte = quantize(rng.standard_normal((rows, cols)) * std, fmt)
     return code, byte, values(code, byte, fmt)
+
+
+# ---- expert layer -----------------------------------------------------------------------------------------
+def choose(logits, top_k, renormalize):
+    """Chosen experts and their weights per token: lists of (expert, weight)."""
+    out = []
+    for row in np.asarray(logits, np.float64):
+        order = [e for e in np.lexsort((np.arange(row.size), -np.where(np.isnan(row), -np.inf, row)))
+                 if not np.isnan(row[e]) and row[e] > -np.inf]
+        chosen = order[:top_k]
+        among = row[chosen] if renormalize else row[order]
+        top = row[order[0]] if order else 0.0
+        total = np.exp(among - top).sum()
+        out.append([(int(e), np.exp(row[e] - top) / total) for e in chosen])
+    return out
+
+
+def requantized(h, err, fmt, exponent=0):
+    """(values h is stored as, how far a value may be from that where h is only known within err).  A code may fall the other way
+    where its midpoint lies within err; a block whose scale may change is off by at most a step of either scale."""
+    rows, cols = h.shape
+    code, byte = quantize(h, fmt, exponent)
+    v = values(code, byte, fmt, exponent)
+    block, nb = block_of(fmt), blocks_of(cols, fmt)
+    pad = ((0, 0), (0, nb * block - cols))
+    hb, eb = np.pad(np.abs(h), pad).reshape(rows, nb, block), np.pad(err, pad).reshape(rows, nb, block)
+    low = quantize(np.maximum(hb - eb, 0).max(axis=2, keepdims=True).reshape(-1, 1), fmt, exponent)[1].reshape(rows, nb)
+    high = quantize((hb + eb).max(axis=2, keepdims=True).reshape(-1, 1), fmt, exponent)[1].reshape(rows, nb)
+    one = np.full((rows * nb, 1), 2, np.uint8)  # the code of 1
+    s_high = values(one, high.reshape(-1, 1), fmt, exponent).reshape(rows, nb, 1)
+    s = values(one, byte.reshape(-1, 1), fmt, exponent).reshape(rows, nb, 1)
+    q, qe = hb / np.where(s > 0, s, 1), eb / np.where(s > 0, s, 1)
+    near = (np.abs(q[..., None] - MIDPOINTS) <= qe[..., None] * (1 + 1e-9)).any(axis=3) & (s > 0)
+    off = np.where(near, 2 * s, 0)          # the widest step of E2M1 is 2
+    off = np.where((low != high)[:, :, None], 4 * s_high, off)
+    return v, off.reshape(rows, -1)[:, :cols]
+
+
+def moe(vx, logits, gate, up, down, top_k, renormalize, fmt, h_exponent=0, alphas=(1, 1, 1)):
+    """(y, bound of what float sums may change): values of x and of the experts' matrices [E, rows, cols] in float64.  A product
+    of K elements is off by (K / 64 + 18) steps of 2^-23 of its magnitudes (its MMAs, the parts of a split K, the factor), the
+    gate's weight by 2^-20 (expf, division), silu by 2^-20 and by what its argument is off (its slope is below 1.1)."""
+    T, H = vx.shape
+    F = gate.shape[1]
+    y, tol, size = np.zeros((T, H)), np.zeros((T, H)), np.zeros((T, H))
+    steps = 2.0 ** -23 * (-(-H // 64) + 18)
+    picks = choose(logits, top_k, renormalize)
+    for e in range(gate.shape[0]):
+        tokens = [t for t in range(T) if any(i == e for i, _ in picks[t])]
+        if not tokens:
+            continue
+        p = np.array([[w for i, w in picks[t] if i == e] for t in tokens])
+        x = vx[tokens]
+        g, u = alphas[0] * (x @ gate[e].T), alphas[1] * (x @ up[e].T)
+        eg, eu = steps * abs(alphas[0]) * (np.abs(x) @ np.abs(gate[e]).T), steps * abs(alphas[1]) * (np.abs(x) @ np.abs(up[e]).T)
+        with np.errstate(over="ignore"):
+            silu = g / (1 + np.exp(-g))
+        h = p * silu * u
+        err = p * ((1.1 * eg + 2.0 ** -20 * np.abs(silu)) * (np.abs(u) + eu) + np.abs(silu) * eu) + 2.0 ** -19 * np.abs(h)
+        v, off = requantized(h, err, fmt, h_exponent)
+        y[tokens] += alphas[2] * (v @ down[e].T)
+        tol[tokens] += abs(alphas[2]) * (off @ np.abs(down[e]).T)
+        size[tokens] += abs(alphas[2]) * ((np.abs(v) + off) @ np.abs(down[e]).T)
+    active = len({e for pick in picks for e, _ in pick})
+    return y, tol + 2.0 ** -23 * (active * -(-F // 64) + 18) * size
