@@ -16,7 +16,8 @@ namespace
 {
 constexpr int kMmaWarp  = 1;
 constexpr int kFirstEpi = 2;
-constexpr int kThreads  = 192;
+constexpr int kEpiThreads = 128;
+constexpr int kThreads  = 32 * kFirstEpi + kEpiThreads;
 
 struct MxGemmParams
 {
@@ -27,6 +28,7 @@ struct MxGemmParams
     int64_t        k_tiles; // scale tiles along K
     int            tokens, channels, K;
     int            dtype;
+    int            pack_out; // two-byte results: rows of dst are words (4-byte aligned, an even number of channels)
     float          alpha;
     uint32_t       idesc;
     int32_t       *status;
@@ -53,25 +55,46 @@ struct MxPlan
     static_assert(!kSplit || STAGES * STAGE >= NT * kMxRows * 4, "the partial sums of a cluster fit where the stages were");
 };
 
-// Sixteen tokens of one channel.
-template <typename T>
-__device__ __forceinline__ void store_tokens(uint8_t *dst, int64_t ldd, const float (&v)[16], int tokens)
+// N accumulator columns (tokens m, m + 1, ..) of a lane's channel n to dst.  Two-byte results of neighbouring channels leave as
+// one word: lanes exchange a column each, after which the even lane of a pair holds both channels of the first token and the
+// odd lane those of the second.
+template <typename T, int N>
+__device__ __forceinline__ void store_block(const MxGemmParams &p, int m, int n, const uint32_t (&r)[N], int cols, float bias)
 {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
+    uint8_t *dst = p.dst + static_cast<int64_t>(m) * p.ldd + static_cast<int64_t>(n) * static_cast<int>(sizeof(T));
+    if (sizeof(T) == 2 && p.pack_out != 0)
     {
-        if (j < tokens)
+        const int odd = n & 1;
+        dst += odd != 0 ? p.ldd - 2 : 0;
+#pragma unroll
+        for (int j = 0; j < N; j += 2)
         {
-            *reinterpret_cast<T *>(dst + j * ldd) = from_float<T>(v[j]);
+            const float a = __fmaf_rn(__uint_as_float(r[j]), p.alpha, bias), b = __fmaf_rn(__uint_as_float(r[j + 1]), p.alpha, bias);
+            const float got = __shfl_xor_sync(0xffffffffu, odd != 0 ? a : b, 1);
+            T           two[2] = {from_float<T>(odd != 0 ? got : a), from_float<T>(odd != 0 ? b : got)};
+            if (j + odd < cols && n < p.channels)
+            {
+                *reinterpret_cast<uint32_t *>(dst + j * p.ldd) = *reinterpret_cast<const uint32_t *>(two);
+            }
+        }
+        return;
+    }
+    if (n < p.channels)
+    {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+        {
+            if (j < cols) *reinterpret_cast<T *>(dst + j * p.ldd) = from_float<T>(__fmaf_rn(__uint_as_float(r[j]), p.alpha, bias));
         }
     }
+    __syncwarp();
 }
-__device__ __forceinline__ void store_tokens(const MxGemmParams &p, int m, int n, const float (&v)[16])
+template <int N>
+__device__ __forceinline__ void store_block(const MxGemmParams &p, int m, int n, const uint32_t (&r)[N], int cols, float bias)
 {
-    uint8_t *dst = p.dst + static_cast<int64_t>(m) * p.ldd;
-    if (p.dtype == CUGL_F32) store_tokens<float>(dst + 4ll * n, p.ldd, v, p.tokens - m);
-    else if (p.dtype == CUGL_F16) store_tokens<__half>(dst + 2ll * n, p.ldd, v, p.tokens - m);
-    else store_tokens<__nv_bfloat16>(dst + 2ll * n, p.ldd, v, p.tokens - m);
+    if (p.dtype == CUGL_F32) store_block<float>(p, m, n, r, cols, bias);
+    else if (p.dtype == CUGL_F16) store_block<__half>(p, m, n, r, cols, bias);
+    else store_block<__nv_bfloat16>(p, m, n, r, cols, bias);
 }
 
 template <int kFormat, int NT, int STAGES, bool kSplit>
@@ -231,25 +254,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t r[16];
                 tmem_ld_x16(tmem_base + as * NT + j + (static_cast<uint32_t>(q * 32) << 16), r);
                 tmem_ld_wait();
-                float v[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(__uint_as_float(r[i]), p.alpha, b);
-                if (n < p.channels) store_tokens(p, tb * NT + j, n, v);
-                __syncwarp();
+                store_block(p, tb * NT + j, n, r, cols - j, b);
             }
             tc_fence_before();
+            __syncwarp();
             if (lane == 0) mbar_arrive(tempty_bar(as));
         }
     }
 
     if constexpr (kSplit)
     {
-        // Partial sums of the cluster: token j belongs to rank j % ranks; every CTA writes its part of the column (128
-        // channels) into the owner's shared memory, where the stages were, and the owner adds them up in the order of the
-        // ranks -- the same order every time.
         const int  tile = first_tile, wb = tile % w_blocks, tb = tile / w_blocks;
-        const int  cols = min(NT, p.tokens - tb * NT);
-        const int  q = warp & 3, ch = q * 32 + lane;
+        const int  cols = min(NT, p.tokens - tb * NT), shift = 31 - __clz(ranks);
+        const int  q = warp & 3;
         bool       ok = true;
         if (warp >= kFirstEpi)
         {
@@ -257,40 +274,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
         }
         __syncthreads();
-        cluster_sync(); // every CTA's MMAs have read their last stage
-        const int per_owner = (NT + ranks - 1) / ranks;
+        cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
         if (warp >= kFirstEpi && ok)
         {
+            const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, NT);
             for (int j = 0; j < cols; j += 16)
             {
                 uint32_t r[16];
                 tmem_ld_x16(tmem_base + j + (static_cast<uint32_t>(q * 32) << 16), r);
                 tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                {
-                    if (j + i < cols)
-                    {
-                        const float v = c_begin < c_end ? __uint_as_float(r[i]) : 0.f; // a rank without chunks has no accumulator
-                        st_cluster_f32(map_to_cta(s_stage, (j + i) % ranks) + 4u * ((rank * per_owner + (j + i) / ranks) * kMxRows + ch), v);
-                    }
-                }
+                send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, r, cols - j, c_begin < c_end);
             }
         }
         cluster_sync();
         if (warp >= kFirstEpi && ok)
         {
-            const int    n    = wb * kMxRows + ch;
-            const float  b    = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
+            const int    own = kMxRows >> shift, et = threadIdx.x - 32 * kFirstEpi;
+            const int    n = wb * kMxRows + rank * own + (et & (own - 1));
+            const float  b = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
             const float *part = reinterpret_cast<const float *>(smem);
-            for (int i = 0; i * ranks + rank < cols; ++i)
+            if (n < p.channels)
             {
-                float sum = 0.f;
-                for (int src = 0; src < ranks; ++src) sum += part[(src * per_owner + i) * kMxRows + ch];
-                if (n < p.channels)
+                for (int at = et; at < cols * own; at += kEpiThreads)
                 {
-                    const float v   = __fmaf_rn(sum, p.alpha, b);
-                    uint8_t    *dst = p.dst + static_cast<int64_t>(tb * NT + i * ranks + rank) * p.ldd;
+                    const float v   = __fmaf_rn(sum_partial(part, at, shift, NT), p.alpha, b);
+                    uint8_t    *dst = p.dst + static_cast<int64_t>(tb * NT + (at >> (7 - shift))) * p.ldd;
                     if (p.dtype == CUGL_F32) reinterpret_cast<float *>(dst)[n] = v;
                     else if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(v);
                     else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(v);
@@ -312,11 +320,250 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// ---- SM pair -------------------------------------------------------------------------------------------------
+// 256 channels x 256 tokens per cluster of two CTAs: each stages its own 128 weight rows and half of the tokens, and the MMAs
+// (M = 256, N = 256) of the leader read both halves -- 64 instead of 96 bytes from L2 per clock of tensor work and SM.  The
+// scales of all 256 tokens go to both CTAs; they come as boxes of a tensor map because the bytes of both CTAs are credited to
+// the leader's barrier.
+// Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales.
+// The epilogue drains the shared columns first; the next tile's MMAs start when it has, and the rest of the drain runs beside
+// them.
+constexpr int kPairCols   = 256;
+constexpr int kPairShared = 64;
+constexpr int kPairEpi    = 8; // epilogue warps
+constexpr int kPairThreads = 32 * (kFirstEpi + kPairEpi);
+
+template <int kFormat>
+struct MxPairPlan
+{
+    using F                       = MxTraits<kFormat>;
+    static constexpr int STAGES   = kFormat == CUGL_NVFP4 ? 5 : 6;
+    static constexpr int STAGE    = 2 * kMxWBytes;
+    static constexpr int SF_STAGE = 3 * F::kChunkScale;
+    static constexpr int OFF_SF   = STAGES * STAGE;
+    static constexpr int OFF_BAR  = OFF_SF + STAGES * SF_STAGE;
+    static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 3) * 8;
+    static constexpr int DYN_BYTES = OFF_MISC + 16 + 1024;
+    static constexpr int SF_COL   = 2 * kPairCols - kPairShared;
+    static_assert(SF_COL + 3 * F::kChunkCols <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
+};
+
+template <int kFormat>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,
+                        const __grid_constant__ CUtensorMap tmap_wsf, const __grid_constant__ CUtensorMap tmap_tsf,
+                        const __grid_constant__ MxGemmParams p)
+{
+    using P = MxPairPlan<kFormat>;
+    using F = MxTraits<kFormat>;
+    constexpr int STAGES = P::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t       *smem      = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t s_stage   = smem_u32(smem);
+    const uint32_t s_sf      = smem_u32(smem + P::OFF_SF);
+    const uint32_t bar_base  = smem_u32(smem + P::OFF_BAR);
+    auto           full_bar  = [&](int s) { return bar_base + 8u * s; };            // used in the leader only
+    auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    auto           tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+    const uint32_t tempty    = bar_base + 8u * (2 * STAGES + 2);                    // shared columns drained; leader only
+    uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
+    volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int      rank = static_cast<int>(cluster_ctarank());
+
+    const int w_blocks    = (p.channels + 2 * kMxRows - 1) / (2 * kMxRows);
+    const int t_blocks    = (p.tokens + kPairCols - 1) / kPairCols;
+    const int tiles       = w_blocks * t_blocks;
+    const int chunks      = (p.K + kMxChunk - 1) / kMxChunk;
+    const int first_tile  = static_cast<int>(cluster_id_x());
+    const int tile_stride = static_cast<int>(num_clusters_x());
+
+    if (threadIdx.x == 0)
+    {
+        for (int s = 0; s < STAGES; ++s)
+        {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(tfull_bar(0), 1);
+        mbar_init(tfull_bar(1), 1);
+        mbar_init(tempty, 2 * kPairEpi);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp)
+    {
+        tmem_alloc_pair(smem_u32(s_tmem), 512);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // the peer's barriers are initialised before anything is sent to them
+    tc_fence_after();
+    const uint32_t tmem_base = *s_tmem;
+    griddep_launch_dependents();
+    griddep_wait(); // the prologue above touched no global memory
+
+    if (warp == 0)
+    {
+        if (lane == 0)
+        {
+            int g = 0;
+            for (int tile = first_tile; tile < tiles; tile += tile_stride)
+            {
+                const int wb = tile % w_blocks, tb = tile / w_blocks;
+                for (int c = 0; c < chunks; ++c, ++g)
+                {
+                    const int s = g % STAGES;
+                    if (!mbar_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
+                    {
+                        goto produced;
+                    }
+                    if (g == p.withhold && blockIdx.x == 0)
+                    {
+                        continue;
+                    }
+                    // boxes of scale tiles are whole: behind the last tile of a row they read the next row's, which no MMA uses
+                    const uint32_t bar = map_to_cta(full_bar(s), 0);
+                    const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
+                    const int      kt  = static_cast<int>(p.k_tiles), first = c * F::kChunkTiles;
+                    if (rank == 0)
+                    {
+                        mbar_expect_tx(full_bar(s), 2 * (P::STAGE + P::SF_STAGE));
+                    }
+                    tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
+                    tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
+                    tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + first, bar);
+                    tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + first, bar);
+                    tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + first, bar);
+                }
+            }
+        produced:
+            if (*s_abort != 0 && rank == 0) // the leader's barriers count the copies of both CTAs
+            {
+                for (int i = max(0, g - STAGES); i < g; ++i)
+                {
+                    if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    else if (warp == kMmaWarp)
+    {
+        if (rank == 0 && lane == 0)
+        {
+            int  g = 0, it = 0;
+            bool ok = true;
+            const uint32_t t_w = tmem_base + P::SF_COL, t_t = t_w + F::kChunkCols;
+            for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
+            {
+                ok = mbar_wait(tempty, (static_cast<uint32_t>(it) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (it & 1) * (kPairCols - kPairShared);
+                for (int c = 0; c < chunks && ok; ++c, ++g)
+                {
+                    const int s = g % STAGES;
+                    ok = mbar_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int      steps  = min(kMxChunk / kMxStepK, (p.K - c * kMxChunk + kMxStepK - 1) / kMxStepK);
+                    const uint64_t sf     = make_scale_desc(s_sf + s * P::SF_STAGE);
+                    const uint64_t a_desc = make_kmajor_sw128_desc(s_stage + s * P::STAGE), b_desc = a_desc + (kMxWBytes >> 4);
+#pragma unroll
+                    for (int t = 0; t < F::kChunkTiles; ++t) // a step's tokens: rows 0..127 in four columns, 128..255 in the next four
+                    {
+                        const uint64_t at = static_cast<uint64_t>(t * (kMxTileBytes >> 4));
+                        tmem_copy_scales_pair(t_w + 4 * t, sf + at);
+                        tmem_copy_scales_pair(t_t + 8 * t, sf + at + (F::kChunkScale >> 4));
+                        tmem_copy_scales_pair(t_t + 8 * t + 4, sf + at + 2 * (F::kChunkScale >> 4));
+                    }
+#pragma unroll
+                    for (int k = 0; k < kMxChunk / kMxStepK; ++k)
+                    {
+                        if (k < steps)
+                        {
+                            umma_mx_pair<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, p.idesc | mx_scale_id<kFormat>(k),
+                                                  t_w + 4 * mx_step_tile<kFormat>(k), t_t + 8 * mx_step_tile<kFormat>(k), (c | k) != 0 ? 1u : 0u);
+                        }
+                    }
+                    umma_commit_pair(empty_bar(s)); // frees this stage in both CTAs
+                }
+                if (ok)
+                {
+                    umma_commit_pair(tfull_bar(it & 1));
+                }
+            }
+        }
+        __syncwarp();
+    }
+    else
+    {
+        // Two warps per lane quarter, which take turns with groups of 32 columns; the shared ones are the first two groups.
+        const int      q = warp & 3, half = (warp - kFirstEpi) >> 2;
+        const uint32_t release = map_to_cta(tempty, 0);
+        int            it = 0;
+        for (int tile = first_tile; tile < tiles; tile += tile_stride, ++it)
+        {
+            const int   wb = tile % w_blocks, tb = tile / w_blocks, as = it & 1;
+            const int   n  = (wb * 2 + rank) * kMxRows + q * 32 + lane;
+            const float b  = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit)))
+            {
+                break;
+            }
+            tc_fence_after();
+            const int      cols = p.tokens - tb * kPairCols;
+            const uint32_t acc  = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+            for (int i = 0; i < kPairCols / 64; ++i)
+            {
+                const int group = 2 * i + half;
+                const int j     = as == 0 ? (group * 32 + kPairCols - kPairShared) % kPairCols : group * 32;
+                uint32_t  r[32];
+                tmem_ld_x32(acc + j, r);
+                tmem_ld_wait();
+                if (i == 0)
+                {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(release);
+                }
+                store_block(p, tb * kPairCols + j, n, r, cols - j, b);
+            }
+            tc_fence_before();
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync(); // neither CTA leaves (or frees tensor memory) while its peer may still touch it
+    if (warp == kMmaWarp)
+    {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *s_abort != 0)
+    {
+        atomicCAS(p.status, 0, *s_abort);
+    }
+}
+
 struct MxOperands
 {
     const cugl_mx_gemm_desc *d;
     const void              *a, *b;
 };
+
+template <typename K>
+cugl_status allow_smem(cugl_context *ctx, K kernel, int bytes, bool (&set)[64])
+{
+    if (!set[ctx->device & 63])
+    {
+        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        set[ctx->device & 63] = true;
+    }
+    return CUGL_SUCCESS;
+}
 
 template <int kFormat, int NT, int STAGES, bool kSplit>
 cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, int ranks)
@@ -328,22 +575,38 @@ cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, 
     {
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for a packed operand");
     }
-    auto        kernel       = mx_gemm_kernel<kFormat, NT, STAGES, kSplit>;
-    static bool attr_set[64] = {}; // per instantiation and device
-    if (!attr_set[ctx->device & 63])
-    {
-        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::DYN_BYTES));
-        attr_set[ctx->device & 63] = true;
-    }
+    auto        kernel  = mx_gemm_kernel<kFormat, NT, STAGES, kSplit>;
+    static bool set[64] = {}; // per instantiation and device
+    CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc             = mx_idesc(kFormat, kMxRows, NT);
     const int64_t tiles = static_cast<int64_t>((p.channels + kMxRows - 1) / kMxRows) * ((p.tokens + NT - 1) / NT);
-    if (tiles > INT32_MAX / 8)
-    {
-        return fail(ctx, CUGL_INVALID_ARGUMENT, "cugl_mx_gemm: more than 2^28 output tiles");
-    }
     const int grid = kSplit ? static_cast<int>(tiles) * ranks : static_cast<int>(tiles < ctx->sm_count ? tiles : ctx->sm_count);
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, kSplit ? ranks : 1,
                                                 tiles, map_w, map_t, p));
+    return CUGL_SUCCESS;
+}
+
+template <int kFormat>
+cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
+{
+    using P = MxPairPlan<kFormat>;
+    using F = MxTraits<kFormat>;
+    CUtensorMap   map_w, map_t, map_wsf, map_tsf;
+    const int64_t inner = (static_cast<int64_t>(p.K) + 1) / 2;
+    const int64_t w_tiles = (static_cast<int64_t>(p.channels) + 127) / 128 * p.k_tiles, t_tiles = (static_cast<int64_t>(p.tokens) + 127) / 128 * p.k_tiles;
+    if (!encode_packed_map(&map_w, op.b, p.channels, inner, op.d->ldb, kMxRows) || !encode_packed_map(&map_t, op.a, p.tokens, inner, op.d->lda, kMxRows) ||
+        !encode_scale_map(&map_wsf, p.w_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_tsf, p.t_scales, t_tiles, F::kChunkTiles))
+    {
+        return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for an operand");
+    }
+    auto        kernel  = mx_gemm_pair_kernel<kFormat>;
+    static bool set[64] = {};
+    CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
+    p.idesc = mx_idesc(kFormat, 2 * kMxRows, kPairCols);
+    const int64_t   tiles = static_cast<int64_t>((p.channels + 255) / 256) * ((p.tokens + 255) / 256);
+    const long long pairs = tiles < ctx->sm_count / 2 ? tiles : ctx->sm_count / 2;
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(2 * pairs)), kPairThreads, P::DYN_BYTES, 2, 2 * tiles, map_w, map_t,
+                                                map_wsf, map_tsf, p));
     return CUGL_SUCCESS;
 }
 
@@ -353,6 +616,14 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     const int nt     = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
     const int chunks = (p.K + kMxChunk - 1) / kMxChunk;
     const long long tiles = static_cast<long long>((p.channels + kMxRows - 1) / kMxRows) * ((p.tokens + nt - 1) / nt);
+    if (tiles > INT32_MAX / 8)
+    {
+        return fail(ctx, CUGL_INVALID_ARGUMENT, "cugl_mx_gemm: more than 2^28 output tiles");
+    }
+    if (p.tokens > 128 && tiles > ctx->sm_count)
+    {
+        return launch_pair<kFormat>(ctx, op, p);
+    }
     int ranks = 1; // CTAs that share a tile's K: as many as leave no SM idle and every CTA a chunk
     while (ranks < 8 && tiles * ranks * 2 <= ctx->sm_count && ranks * 2 <= chunks) ranks *= 2;
     if (ranks > 1)
@@ -442,6 +713,7 @@ extern "C"
         p.K          = desc->K;
         p.dtype      = desc->dst_dtype;
         p.alpha      = desc->alpha;
+        p.pack_out   = ((reinterpret_cast<uintptr_t>(d_dst) | static_cast<uintptr_t>(desc->ldd)) & 3) == 0 && desc->N % 2 == 0;
         p.status     = ctx->d_status;
         p.spin_limit = ctx->spin_limit;
         p.withhold   = ctx->withhold_kb;

@@ -78,10 +78,45 @@ __device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64
     }
 }
 
+// The same across an SM pair: 256 rows (128 per CTA, each with the scales of its own rows) x up to 256 columns (half of them
+// staged by each CTA, the scales of all of them by both).
+template <int kFormat>
+__device__ __forceinline__ void umma_mx_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scale, uint32_t b_scale,
+                                             uint32_t accumulate)
+{
+    if constexpr (kFormat == CUGL_MXFP4)
+    {
+        asm volatile("{\n\t"
+                     ".reg .pred p;\n\t"
+                     "setp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+                     "}"
+                     :
+                     : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+                     : "memory");
+    }
+    else
+    {
+        asm volatile("{\n\t"
+                     ".reg .pred p;\n\t"
+                     "setp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+                     "}"
+                     :
+                     : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+                     : "memory");
+    }
+}
+
 // One scale tile (32 rows of 16 bytes in shared memory) to four tensor-memory columns, in all four lane quarters.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t d_tmem, uint64_t s_desc)
 {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
+}
+// in both CTAs of a pair, each from its own shared memory
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t d_tmem, uint64_t s_desc)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
 }
 // Descriptor of a scale tile: no swizzle, groups of eight 16-byte rows 128 bytes apart.
 __device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr)
@@ -146,6 +181,59 @@ __device__ __forceinline__ void mx_chunk_scales(uint32_t t_dst, uint32_t sf, int
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v)
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// Partial sums of a cluster whose 2^shift CTAs shared an accumulator's K.  Rank r owns channels r * (128 >> shift) and up.  A
+// warp sends sixteen columns of its 32 accumulator lanes to the owners' shared memory, [rank][column][channel of the owner]:
+// a lane's address only grows by a constant from column to column.  stride: columns of a part.
+__device__ __forceinline__ uint32_t partial_address(uint32_t s_base, int ch, int rank, int shift, int stride)
+{
+    const int own = kMxRows >> shift;
+    return map_to_cta(s_base, static_cast<uint32_t>(ch / own)) + 4u * static_cast<uint32_t>(rank * stride * own + (ch & (own - 1)));
+}
+__device__ __forceinline__ void send_partial(uint32_t to, int shift, const uint32_t (&r)[16], int cols, bool has)
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+    {
+        if (i < cols) // a rank without a share of K has no accumulator: zeros
+        {
+            st_cluster_f32(to + static_cast<uint32_t>(i) * (4u * kMxRows >> shift), has ? __uint_as_float(r[i]) : 0.f);
+        }
+    }
+}
+// Sum over the ranks, always in their order, of element `at` (column * own + channel) of the parts.
+__device__ __forceinline__ float sum_partial(const float *part, int at, int shift, int stride)
+{
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        if (i < (1 << shift)) v[i] = part[i * stride * (kMxRows >> shift) + at];
+    }
+    float sum = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+    {
+        if (i < (1 << shift)) sum += v[i];
+    }
+    return sum;
+}
+
+// scale tiles as rows of 512 bytes; box = box_rows tiles
+inline bool encode_scale_map(CUtensorMap *map, const void *base, int64_t tiles, int box_rows)
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (fn == nullptr)
+    {
+        return false;
+    }
+    const cuuint64_t dims[2]    = {kMxTileBytes / 4, static_cast<cuuint64_t>(tiles)};
+    const cuuint64_t strides[1] = {kMxTileBytes};
+    const cuuint32_t box[2]     = {kMxTileBytes / 4, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2]    = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // packed rows x (inner bytes), ld bytes apart; box = box_rows x 128 bytes in the 128-byte swizzle; what lies outside reads as 0

@@ -21,7 +21,8 @@ namespace
 {
 constexpr int kMmaWarp  = 1;
 constexpr int kFirstEpi = 2;
-constexpr int kThreads  = 192;
+constexpr int kEpiThreads = 128;
+constexpr int kThreads  = 32 * kFirstEpi + kEpiThreads;
 constexpr int kMaxTokens = 128, kMaxExperts = 512, kMaxTopK = 16;
 
 struct MoeParams
@@ -209,26 +210,20 @@ __device__ __forceinline__ int active_experts(const MoeParams &p, uint16_t *list
     return total;
 }
 
-// The gate's weight of expert e for token t; 0 where it was not chosen.
+// The gate's weight of expert e for token t; kNotChosen where the token did not choose it.
+constexpr float kNotChosen = -1.f;
 __device__ __forceinline__ float gate_weight(const MoeParams &p, int t, int e)
 {
-    float w = 0.f;
+    float w = kNotChosen;
     for (int j = 0; j < p.top_k; ++j)
     {
         if (p.ids[t * p.top_k + j] == e) w = p.p[t * p.top_k + j];
     }
     return w;
 }
-__device__ __forceinline__ bool chose(const MoeParams &p, int t, int e)
-{
-    bool c = false;
-    for (int j = 0; j < p.top_k; ++j) c |= p.ids[t * p.top_k + j] == e;
-    return c;
-}
-
 // One token's 32 values of h (a warp's lanes: consecutive f) to codes and scales.  f: the lane's place on the intermediate axis.
 template <int kFormat>
-__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, int f, int lane, float h)
+__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, int f, int lane, float h, bool in = true)
 {
     uint32_t amax = __float_as_uint(h) & 0x7fffffffu;
     if (kFormat == CUGL_MXFP4)
@@ -245,15 +240,33 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, i
     w <<= 4 * (lane & 7);
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-    if ((lane & 7) == 0 && f < p.inner)
+    if (in && (lane & 7) == 0 && f < p.inner)
     {
         *reinterpret_cast<uint32_t *>(p.hq + (static_cast<int64_t>(a) * p.tokens + t) * p.ld_hq + f / 2) = w;
     }
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
-    if ((lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
+    if (in && (lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
     {
         p.hs[static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes + mx_scale_offset(t, f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s.byte);
     }
+}
+// The epilogue warps fill a table of the unit's weights while its MMAs run, a token per thread, and agree on carrying on: a
+// warp that gave up says so here instead of leaving the others at the barrier.
+__device__ __forceinline__ bool fill_weights(const MoeParams &p, float *table, int e, bool ok)
+{
+    const int t = threadIdx.x - 32 * kFirstEpi;
+    if (t < p.tokens) table[t] = gate_weight(p, t, e);
+    uint32_t r;
+    asm volatile("{\n\t"
+                 ".reg .pred p, q;\n\t"
+                 "setp.ne.u32 q, %1, 0;\n\t"
+                 "bar.red.and.pred p, 1, %2, q;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t"
+                 "}"
+                 : "=r"(r)
+                 : "r"(static_cast<uint32_t>(ok)), "n"(kEpiThreads)
+                 : "memory");
+    return r != 0;
 }
 // The same for a token that did not choose the expert: zeros.
 template <int kFormat>
@@ -289,7 +302,7 @@ struct MoePlan
     static constexpr int OFF_BITS   = OFF_MISC + 16;
     static constexpr int OFF_LIST   = OFF_BITS + kMaxExperts / 8;
     static constexpr int OFF_WEIGHT = OFF_LIST + kMaxExperts * 2;
-    static constexpr int DYN_BYTES  = OFF_WEIGHT + kMaxTokens * 4 + 1024;
+    static constexpr int DYN_BYTES  = OFF_WEIGHT + 2 * kMaxTokens * 4 + 1024; // two tables
     static constexpr int ACC_COLS   = kOperands * NT;
     static constexpr int SF_COLS    = (kOperands + 1) * F::kChunkCols;
     static constexpr int COLS       = kAcc * ACC_COLS + STAGES * SF_COLS;
@@ -321,6 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int  *s_abort    = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_bits     = reinterpret_cast<uint32_t *>(smem + P::OFF_BITS);
     uint16_t      *s_list     = reinterpret_cast<uint16_t *>(smem + P::OFF_LIST);
+    float         *s_weight   = reinterpret_cast<float *>(smem + P::OFF_WEIGHT);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0)
@@ -441,22 +455,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         const int q  = warp & 3;
         int       it = 0;
+        bool      ok = true;
         for (int unit = first_unit; unit < units; unit += unit_stride, ++it)
         {
-            const int a = unit / blocks, e = s_list[a], f = (unit % blocks) * kMxRows + q * 32 + lane;
+            const int a = unit / blocks, f = (unit % blocks) * kMxRows + q * 32 + lane;
             const int as = it % kAcc;
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit)))
-            {
-                break;
-            }
+            float    *weight = s_weight + (it & 1) * kMaxTokens; // the other table may still be read by a slower warp
+            if (!fill_weights(p, weight, s_list[a], ok)) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
+            if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
             for (int j = 0; j < p.tokens; j += 16)
             {
-                const int  mine = j + (lane & 15);
-                const bool want = mine < p.tokens && chose(p, mine, e);
-                const float wt  = want ? gate_weight(p, mine, e) : 0.f;
-                const uint32_t any = __ballot_sync(0xffffffffu, want);
-                uint32_t   g[16], u[16];
+                uint32_t g[16], u[16];
                 tmem_ld_x16(tmem_base + as * P::ACC_COLS + j + (static_cast<uint32_t>(q * 32) << 16), g);
                 tmem_ld_x16(tmem_base + as * P::ACC_COLS + NT + j + (static_cast<uint32_t>(q * 32) << 16), u);
                 tmem_ld_wait();
@@ -465,9 +476,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 {
                     if (j + i < p.tokens)
                     {
-                        if ((any >> i) & 1u)
+                        const float w = weight[j + i];
+                        if (w != kNotChosen)
                         {
-                            const float w = __shfl_sync(0xffffffffu, wt, i);
                             const float h = f < p.inner ? swiglu(__uint_as_float(g[i]) * p.gate_alpha, __uint_as_float(u[i]) * p.up_alpha, w) : 0.f;
                             store_hidden<kFormat>(p, a, j + i, f, lane, h);
                         }
@@ -486,60 +497,48 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if constexpr (kSplit)
     {
-        // as in mx_gemm_kernel: token j belongs to rank j % ranks, which adds the cluster's parts up in the order of the ranks
         const bool work = first_unit < units; // the same in the whole cluster
-        const int  q = warp & 3, ch = q * 32 + lane;
+        const int  q = warp & 3, shift = 31 - __clz(ranks);
+        const int  a = work ? first_unit / blocks : 0;
         bool       ok = work;
         if (warp >= kFirstEpi && work)
         {
+            fill_weights(p, s_weight, s_list[a], true);
             ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
             tc_fence_after();
         }
         __syncthreads();
-        cluster_sync();
-        const int per_owner = (NT + ranks - 1) / ranks;
+        cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
         if (warp >= kFirstEpi && ok)
         {
+            const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, 2 * NT);
             for (int j = 0; j < p.tokens; j += 16)
             {
                 uint32_t g[16], u[16];
                 tmem_ld_x16(tmem_base + j + (static_cast<uint32_t>(q * 32) << 16), g);
                 tmem_ld_x16(tmem_base + NT + j + (static_cast<uint32_t>(q * 32) << 16), u);
                 tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                {
-                    if (j + i < p.tokens)
-                    {
-                        const bool     has = c_begin < c_end;
-                        const uint32_t to  = map_to_cta(s_stage, (j + i) % ranks) + 4u * ((rank * per_owner + (j + i) / ranks) * 2 * kMxRows + ch);
-                        st_cluster_f32(to, has ? __uint_as_float(g[i]) : 0.f);
-                        st_cluster_f32(to + 4u * kMxRows, has ? __uint_as_float(u[i]) : 0.f);
-                    }
-                }
+                send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, g, p.tokens - j, c_begin < c_end);
+                send_partial(to + static_cast<uint32_t>(NT + j) * (4u * kMxRows >> shift), shift, u, p.tokens - j, c_begin < c_end);
             }
         }
         cluster_sync();
         if (warp >= kFirstEpi && ok)
         {
-            const int    a = first_unit / blocks, e = s_list[a], f = (first_unit % blocks) * kMxRows + ch;
+            // a warp takes 32 consecutive channels of one token at a time: a rank owns at least 32 (launch_layers)
+            const int    own = kMxRows >> shift;
             const float *part = reinterpret_cast<const float *>(smem);
-            for (int i = 0; i * ranks + rank < p.tokens; ++i)
+            for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < p.tokens * own; at += kEpiThreads)
             {
-                const int t = i * ranks + rank;
-                if (!chose(p, t, e))
+                const bool  in = at < p.tokens * own;
+                const int   t  = in ? at >> (7 - shift) : 0, f = (first_unit % blocks) * kMxRows + rank * own + (at & (own - 1));
+                const float w  = in && f < p.inner ? s_weight[t] : kNotChosen;
+                float       h  = 0.f;
+                if (w != kNotChosen)
                 {
-                    store_hidden_zero<kFormat>(p, a, t, f, lane);
-                    continue;
+                    h = swiglu(sum_partial(part, at, shift, 2 * NT) * p.gate_alpha, sum_partial(part + NT * own, at, shift, 2 * NT) * p.up_alpha, w);
                 }
-                float g = 0.f, u = 0.f;
-                for (int src = 0; src < ranks; ++src)
-                {
-                    g += part[(src * per_owner + i) * 2 * kMxRows + ch];
-                    u += part[(src * per_owner + i) * 2 * kMxRows + kMxRows + ch];
-                }
-                const float h = f < p.inner ? swiglu(g * p.gate_alpha, u * p.up_alpha, gate_weight(p, t, e)) : 0.f;
-                store_hidden<kFormat>(p, a, t, f, lane, h);
+                store_hidden<kFormat>(p, a, t, f, lane, h, in);
             }
         }
     }
@@ -672,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     }
 
-    const int q = warp & 3, ch = q * 32 + lane;
+    const int q = warp & 3, shift = 31 - __clz(ranks);
     bool      ok = true;
     if (warp >= kFirstEpi)
     {
@@ -680,40 +679,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
     }
     __syncthreads();
-    cluster_sync();
-    const int per_owner = (NT + ranks - 1) / ranks;
+    cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
     if (warp >= kFirstEpi && ok)
     {
+        const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, NT);
         for (int j = 0; j < p.tokens; j += 16)
         {
             uint32_t r[16];
             tmem_ld_x16(tmem_base + j + (static_cast<uint32_t>(q * 32) << 16), r);
             tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                if (j + i < p.tokens)
-                {
-                    st_cluster_f32(map_to_cta(s_stage, (j + i) % ranks) + 4u * ((rank * per_owner + (j + i) / ranks) * kMxRows + ch),
-                                   c_begin < c_end ? __uint_as_float(r[i]) : 0.f);
-                }
-            }
+            send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, r, p.tokens - j, c_begin < c_end);
         }
     }
     cluster_sync();
     if (warp >= kFirstEpi && ok)
     {
-        const int    n    = block * kMxRows + ch;
+        const int    own = kMxRows >> shift, et = threadIdx.x - 32 * kFirstEpi;
+        const int    n = block * kMxRows + rank * own + (et & (own - 1));
         const float *part = reinterpret_cast<const float *>(smem);
-        for (int i = 0; i * ranks + rank < p.tokens; ++i)
+        if (n < p.hidden)
         {
-            float sum = 0.f;
-            for (int src = 0; src < ranks; ++src) sum += part[(src * per_owner + i) * kMxRows + ch];
-            if (n < p.hidden)
+            for (int at = et; at < p.tokens * own; at += kEpiThreads)
             {
-                uint8_t *dst = p.dst + static_cast<int64_t>(i * ranks + rank) * p.ld_dst;
-                if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(sum * p.down_alpha);
-                else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(sum * p.down_alpha);
+                const float v   = sum_partial(part, at, shift, NT) * p.down_alpha;
+                uint8_t    *dst = p.dst + static_cast<int64_t>(at >> (7 - shift)) * p.ld_dst;
+                if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(v);
+                else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(v);
             }
         }
     }
@@ -818,7 +809,8 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     const int most_units = most_active * ((p.inner + kMxRows - 1) / kMxRows);
     const int chunks     = (p.hidden + kMxChunk - 1) / kMxChunk;
     int       ranks      = 1; // CTAs that share a unit's K: as many as leave no SM idle and every CTA a chunk
-    while (ranks < 8 && most_units * ranks * 2 <= ctx->sm_count && ranks * 2 <= chunks) ranks *= 2;
+    // (at most four: a rank then owns 32 channels of a unit, one MXFP4 block)
+    while (ranks < 4 && most_units * ranks * 2 <= ctx->sm_count && ranks * 2 <= chunks) ranks *= 2;
     if (ranks > 1)
     {
         CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, true, 1>(ctx, m, p, most_units, ranks)));
