@@ -2,7 +2,7 @@
 //
 //   warp 0      TMA: 128 rows of weights (b) and NT rows of tokens (a), 128 bytes (256 elements) of each per stage, and the
 //               scale tiles that belong to them as plain bulk copies
-//   warp 1      one lane copies the stage's scales to tensor memory and issues its MMAs (M = 128, N = NT, K = 64)
+//   warp 1      copies the stage's scales to tensor memory and issues its MMAs (M = 128, N = NT, K = 64)
 //   warps 2..5  a tensor-memory lane quarter each: accumulator * alpha + bias, rounded once, stored as 32 consecutive
 //               channels per token
 //
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int g = 0;
             for (int tile = first_tile; tile < tiles; tile += tile_stride)
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = c_begin; c < c_end; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    if (!mbar_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
+                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                     {
                         goto produced;
                     }
@@ -180,15 +180,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - first);
                     const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
                     const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
-                    tma_load_2d(dst, &tmap_w, c * kMxChunkBytes, wb * kMxRows, full_bar(s));
-                    tma_load_2d(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * NT, full_bar(s));
-                    bulk_load(sf, w_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
-                    bulk_load(sf + F::kChunkScale, t_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
+                    if (el)
+                    {
+                        mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
+                        tma_load_2d(dst, &tmap_w, c * kMxChunkBytes, wb * kMxRows, full_bar(s));
+                        tma_load_2d(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * NT, full_bar(s));
+                        bulk_load(sf, w_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
+                        bulk_load(sf + F::kChunkScale, t_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
+                    }
+                    __syncwarp();
                 }
             }
         produced:
-            if (*s_abort != 0)
+            if (el && *s_abort != 0)
             {
                 for (int i = max(0, g - STAGES); i < g; ++i)
                 {
@@ -200,32 +204,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     else if (warp == kMmaWarp)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int  g = 0, it = 0;
             bool ok = true;
             for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
             {
                 const int as = it % P::ACC;
-                ok = mbar_wait(tempty_bar(as), (static_cast<uint32_t>(it / P::ACC) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / P::ACC) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + as * NT;
                 for (int c = c_begin; c < c_end && ok; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    ok = mbar_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                    ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - c * F::kChunkTiles);
                     const int      steps = min(kMxChunk / kMxStepK, (p.K - c * kMxChunk + kMxStepK - 1) / kMxStepK);
                     const uint32_t t_w   = tmem_base + P::ACC * NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
                     const uint32_t sf    = s_sf + s * P::SF_STAGE;
-                    mx_chunk_scales<kFormat>(t_w, sf, n);
-                    mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
-                    mx_chunk<kFormat>(d_tmem, s_stage + s * P::STAGE, s_stage + s * P::STAGE + kMxWBytes, t_w, t_t, p.idesc, steps, c == c_begin);
-                    umma_commit(empty_bar(s));
+                    if (el)
+                    {
+                        mx_chunk_scales<kFormat>(t_w, sf, n);
+                        mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
+                        mx_chunk<kFormat>(d_tmem, s_stage + s * P::STAGE, s_stage + s * P::STAGE + kMxWBytes, t_w, t_t, p.idesc, steps, c == c_begin);
+                        umma_commit(empty_bar(s));
+                    }
+                    __syncwarp();
                 }
-                if (ok)
+                if (ok && el)
                 {
                     umma_commit(tfull_bar(as));
                 }
@@ -243,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int   as = it % P::ACC;
             const int   n  = wb * kMxRows + q * 32 + lane;
             const float b  = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it / P::ACC) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit)))
+            if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it / P::ACC) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
                 break;
             }
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool       ok = true;
         if (warp >= kFirstEpi)
         {
-            ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
+            ok = warp_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             tc_fence_after();
         }
         __syncthreads();
@@ -332,6 +340,18 @@ constexpr int kPairCols   = 256;
 constexpr int kPairShared = 64;
 constexpr int kPairEpi    = 8; // epilogue warps
 constexpr int kPairThreads = 32 * (kFirstEpi + kPairEpi);
+
+// Order of the tiles: strips of four blocks of channels, walked token block by token block, so that the tiles in flight share
+// both operands in L2 and on the way to the SMs (channel blocks all the way: 4096 x 14336 x 16384 NVFP4 405 us, strips 346;
+// K = 4096 101 and 102).
+constexpr int kPairStrip = 4;
+__device__ __forceinline__ void pair_tile(int tile, int w_blocks, int t_blocks, int &wb, int &tb)
+{
+    const int strip = tile / (kPairStrip * t_blocks), in = tile - strip * kPairStrip * t_blocks;
+    const int width = min(kPairStrip, w_blocks - strip * kPairStrip);
+    tb              = in / width;
+    wb              = strip * kPairStrip + in - tb * width;
+}
 
 template <int kFormat>
 struct MxPairPlan
@@ -405,16 +425,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
     if (warp == 0)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int g = 0;
             for (int tile = first_tile; tile < tiles; tile += tile_stride)
             {
-                const int wb = tile % w_blocks, tb = tile / w_blocks;
+                int wb, tb;
+                pair_tile(tile, w_blocks, t_blocks, wb, tb);
                 for (int c = 0; c < chunks; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    if (!mbar_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
+                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                     {
                         goto produced;
                     }
@@ -426,15 +447,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     const uint32_t bar = map_to_cta(full_bar(s), 0);
                     const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
                     const int      kt  = static_cast<int>(p.k_tiles), first = c * F::kChunkTiles;
-                    if (rank == 0)
+                    if (el)
                     {
-                        mbar_expect_tx(full_bar(s), 2 * (P::STAGE + P::SF_STAGE));
+                        if (rank == 0)
+                        {
+                            mbar_expect_tx(full_bar(s), 2 * (P::STAGE + P::SF_STAGE));
+                        }
+                        tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
+                        tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
+                        tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + first, bar);
+                        tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + first, bar);
+                        tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + first, bar);
                     }
-                    tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
-                    tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
-                    tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + first, bar);
-                    tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + first, bar);
-                    tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + first, bar);
+                    __syncwarp();
                 }
             }
         produced:
@@ -450,45 +475,50 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     else if (warp == kMmaWarp)
     {
-        if (rank == 0 && lane == 0)
+        const bool el = elect_one();
+        if (rank == 0)
         {
             int  g = 0, it = 0;
             bool ok = true;
             const uint32_t t_w = tmem_base + P::SF_COL, t_t = t_w + F::kChunkCols;
             for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
             {
-                ok = mbar_wait(tempty, (static_cast<uint32_t>(it) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                ok = warp_wait(tempty, (static_cast<uint32_t>(it) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (it & 1) * (kPairCols - kPairShared);
                 for (int c = 0; c < chunks && ok; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    ok = mbar_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                    ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const int      steps  = min(kMxChunk / kMxStepK, (p.K - c * kMxChunk + kMxStepK - 1) / kMxStepK);
                     const uint64_t sf     = make_scale_desc(s_sf + s * P::SF_STAGE);
                     const uint64_t a_desc = make_kmajor_sw128_desc(s_stage + s * P::STAGE), b_desc = a_desc + (kMxWBytes >> 4);
-#pragma unroll
-                    for (int t = 0; t < F::kChunkTiles; ++t) // a step's tokens: rows 0..127 in four columns, 128..255 in the next four
+                    if (el)
                     {
-                        const uint64_t at = static_cast<uint64_t>(t * (kMxTileBytes >> 4));
-                        tmem_copy_scales_pair(t_w + 4 * t, sf + at);
-                        tmem_copy_scales_pair(t_t + 8 * t, sf + at + (F::kChunkScale >> 4));
-                        tmem_copy_scales_pair(t_t + 8 * t + 4, sf + at + 2 * (F::kChunkScale >> 4));
-                    }
 #pragma unroll
-                    for (int k = 0; k < kMxChunk / kMxStepK; ++k)
-                    {
-                        if (k < steps)
+                        for (int t = 0; t < F::kChunkTiles; ++t) // a step's tokens: rows 0..127 in four columns, 128..255 in the next four
                         {
-                            umma_mx_pair<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, p.idesc | mx_scale_id<kFormat>(k),
-                                                  t_w + 4 * mx_step_tile<kFormat>(k), t_t + 8 * mx_step_tile<kFormat>(k), (c | k) != 0 ? 1u : 0u);
+                            const uint64_t at = static_cast<uint64_t>(t * (kMxTileBytes >> 4));
+                            tmem_copy_scales_pair(t_w + 4 * t, sf + at);
+                            tmem_copy_scales_pair(t_t + 8 * t, sf + at + (F::kChunkScale >> 4));
+                            tmem_copy_scales_pair(t_t + 8 * t + 4, sf + at + 2 * (F::kChunkScale >> 4));
                         }
+#pragma unroll
+                        for (int k = 0; k < kMxChunk / kMxStepK; ++k)
+                        {
+                            if (k < steps)
+                            {
+                                umma_mx_pair<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, p.idesc | mx_scale_id<kFormat>(k),
+                                                      t_w + 4 * mx_step_tile<kFormat>(k), t_t + 8 * mx_step_tile<kFormat>(k), (c | k) != 0 ? 1u : 0u);
+                            }
+                        }
+                        umma_commit_pair(empty_bar(s)); // frees this stage in both CTAs
                     }
-                    umma_commit_pair(empty_bar(s)); // frees this stage in both CTAs
+                    __syncwarp();
                 }
-                if (ok)
+                if (ok && el)
                 {
                     umma_commit_pair(tfull_bar(it & 1));
                 }
@@ -504,10 +534,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         int            it = 0;
         for (int tile = first_tile; tile < tiles; tile += tile_stride, ++it)
         {
-            const int   wb = tile % w_blocks, tb = tile / w_blocks, as = it & 1;
+            int wb, tb;
+            pair_tile(tile, w_blocks, t_blocks, wb, tb);
+            const int   as = it & 1;
             const int   n  = (wb * 2 + rank) * kMxRows + q * 32 + lane;
             const float b  = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit)))
+            if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
                 break;
             }

@@ -137,6 +137,27 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  : "memory");
 }
 
+// The lane that issues a warp's tcgen05 and TMA instructions.  The issuing loops are run by the whole warp and only the
+// instructions themselves are guarded by this predicate: control flow stays uniform, so that descriptors and addresses are
+// computed in uniform registers, which these instructions take their operands from.  Under a branch on the lane index each of
+// them has to be moved there first: a copy of scales then takes 46 clocks instead of 16, an MMA of 16 columns 50 instead of 39.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t"
+                 ".reg .pred p;\n\t"
+                 "elect.sync _|p, 0xffffffff;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t"
+                 "}"
+                 : "=r"(p));
+    return p != 0;
+}
+// mbar_wait by a whole warp, which takes the decision to give up together
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code, long long limit)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, limit));
+}
+
 // Waits for a barrier's phase whatever the abort flag says: a producer that gives up lets its copies in flight land first.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, long long limit)
 {

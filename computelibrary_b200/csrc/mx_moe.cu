@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int g = 0;
             for (int unit = first_unit; unit < units; unit += unit_stride)
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = c_begin; c < c_end; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    if (!mbar_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
+                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                     {
                         goto produced;
                     }
@@ -397,17 +397,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
                     const int64_t  at    = static_cast<int64_t>(first) * kMxTileBytes;
                     const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    mbar_expect_tx(full_bar(s), P::STAGE + 3 * bytes);
-                    tma_load_2d(dst, &tmap_g, c * kMxChunkBytes, row, full_bar(s));
-                    tma_load_2d(dst + kMxWBytes, &tmap_u, c * kMxChunkBytes, row, full_bar(s));
-                    tma_load_2d(dst + 2 * kMxWBytes, &tmap_x, c * kMxChunkBytes, 0, full_bar(s));
-                    bulk_load(sf, p.gate_scales + sf_at + at, bytes, full_bar(s));
-                    bulk_load(sf + F::kChunkScale, p.up_scales + sf_at + at, bytes, full_bar(s));
-                    bulk_load(sf + 2 * F::kChunkScale, p.xs + at, bytes, full_bar(s));
+                    if (el)
+                    {
+                        mbar_expect_tx(full_bar(s), P::STAGE + 3 * bytes);
+                        tma_load_2d(dst, &tmap_g, c * kMxChunkBytes, row, full_bar(s));
+                        tma_load_2d(dst + kMxWBytes, &tmap_u, c * kMxChunkBytes, row, full_bar(s));
+                        tma_load_2d(dst + 2 * kMxWBytes, &tmap_x, c * kMxChunkBytes, 0, full_bar(s));
+                        bulk_load(sf, p.gate_scales + sf_at + at, bytes, full_bar(s));
+                        bulk_load(sf + F::kChunkScale, p.up_scales + sf_at + at, bytes, full_bar(s));
+                        bulk_load(sf + 2 * F::kChunkScale, p.xs + at, bytes, full_bar(s));
+                    }
+                    __syncwarp();
                 }
             }
         produced:
-            if (*s_abort != 0)
+            if (el && *s_abort != 0)
             {
                 for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
             }
@@ -416,34 +420,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     else if (warp == kMmaWarp)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int  g = 0, it = 0;
             bool ok = true;
             for (int unit = first_unit; unit < units && ok; unit += unit_stride, ++it)
             {
                 const int as = it % kAcc;
-                ok = mbar_wait(tempty_bar(as), (static_cast<uint32_t>(it / kAcc) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / kAcc) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + as * P::ACC_COLS;
                 for (int c = c_begin; c < c_end && ok; ++c, ++g)
                 {
                     const int s = g % STAGES;
-                    ok = mbar_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                    ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const int      n     = min(F::kChunkTiles, static_cast<int>(p.h_tiles) - c * F::kChunkTiles);
                     const int      steps = min(kMxChunk / kMxStepK, (p.hidden - c * kMxChunk + kMxStepK - 1) / kMxStepK);
                     const uint32_t t_g   = tmem_base + kAcc * P::ACC_COLS + s * P::SF_COLS, t_u = t_g + F::kChunkCols, t_x = t_u + F::kChunkCols;
                     const uint32_t sf = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
-                    mx_chunk_scales<kFormat>(t_x, sf + 2 * F::kChunkScale, n);
-                    mx_chunk_scales<kFormat>(t_g, sf, n);
-                    mx_chunk_scales<kFormat>(t_u, sf + F::kChunkScale, n);
-                    mx_chunk<kFormat>(d_tmem, st, st + 2 * kMxWBytes, t_g, t_x, p.idesc, steps, c == c_begin);
-                    mx_chunk<kFormat>(d_tmem + NT, st + kMxWBytes, st + 2 * kMxWBytes, t_u, t_x, p.idesc, steps, c == c_begin);
-                    umma_commit(empty_bar(s));
+                    if (el)
+                    {
+                        mx_chunk_scales<kFormat>(t_x, sf + 2 * F::kChunkScale, n);
+                        mx_chunk_scales<kFormat>(t_g, sf, n);
+                        mx_chunk_scales<kFormat>(t_u, sf + F::kChunkScale, n);
+                        mx_chunk<kFormat>(d_tmem, st, st + 2 * kMxWBytes, t_g, t_x, p.idesc, steps, c == c_begin);
+                        mx_chunk<kFormat>(d_tmem + NT, st + kMxWBytes, st + 2 * kMxWBytes, t_u, t_x, p.idesc, steps, c == c_begin);
+                        umma_commit(empty_bar(s));
+                    }
+                    __syncwarp();
                 }
-                if (ok)
+                if (ok && el)
                 {
                     umma_commit(tfull_bar(as));
                 }
@@ -462,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int as = it % kAcc;
             float    *weight = s_weight + (it & 1) * kMaxTokens; // the other table may still be read by a slower warp
             if (!fill_weights(p, weight, s_list[a], ok)) break;
-            ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
+            ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
             for (int j = 0; j < p.tokens; j += 16)
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp >= kFirstEpi && work)
         {
             fill_weights(p, s_weight, s_list[a], true);
-            ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
+            ok = warp_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             tc_fence_after();
         }
         __syncthreads();
@@ -613,13 +621,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int g = 0;
             for (int i = c_begin; i < c_end; ++i, ++g)
             {
                 const int s = g % STAGES;
-                if (!mbar_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
+                if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                 {
                     break;
                 }
@@ -628,13 +636,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int      n     = min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first);
                 const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
                 const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
-                tma_load_2d(dst, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
-                tma_load_2d(dst + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
-                bulk_load(sf, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
-                bulk_load(sf + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
+                if (el)
+                {
+                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
+                    tma_load_2d(dst, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
+                    tma_load_2d(dst + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
+                    bulk_load(sf, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
+                    bulk_load(sf + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
+                }
+                __syncwarp();
             }
-            if (*s_abort != 0)
+            if (el && *s_abort != 0)
             {
                 for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
             }
@@ -643,14 +655,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     else if (warp == kMmaWarp)
     {
-        if (lane == 0)
+        const bool el = elect_one();
         {
             int  g  = 0;
             bool ok = true;
             for (int i = c_begin; i < c_end && ok; ++i, ++g)
             {
                 const int s = g % STAGES;
-                ok = mbar_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                 if (!ok) break;
                 tc_fence_after();
                 const int      c     = i % per_expert;
@@ -658,12 +670,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int      steps = min(kMxChunk / kMxStepK, (p.inner - c * kMxChunk + kMxStepK - 1) / kMxStepK);
                 const uint32_t t_w   = tmem_base + NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
                 const uint32_t sf    = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
-                mx_chunk_scales<kFormat>(t_w, sf, n);
-                mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
-                mx_chunk<kFormat>(tmem_base, st, st + kMxWBytes, t_w, t_t, p.idesc, steps, i == c_begin);
-                umma_commit(empty_bar(s));
+                if (el)
+                {
+                    mx_chunk_scales<kFormat>(t_w, sf, n);
+                    mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
+                    mx_chunk<kFormat>(tmem_base, st, st + kMxWBytes, t_w, t_t, p.idesc, steps, i == c_begin);
+                    umma_commit(empty_bar(s));
+                }
+                __syncwarp();
             }
-            if (ok)
+            if (ok && el)
             {
                 umma_commit(tfull);
             }
@@ -675,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool      ok = true;
     if (warp >= kFirstEpi)
     {
-        ok = __all_sync(0xffffffffu, mbar_wait(tfull, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
+        ok = warp_wait(tfull, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
         tc_fence_after();
     }
     __syncthreads();
