@@ -44,15 +44,18 @@ struct MxPlan
     static constexpr int STAGE       = kMxWBytes + T_BYTES;
     static constexpr int SF_STAGE    = 2 * F::kChunkScale;
     static constexpr int OFF_SF      = STAGES * STAGE;
-    static constexpr int OFF_BAR     = OFF_SF + STAGES * SF_STAGE;
-    static constexpr int OFF_MISC    = OFF_BAR + (2 * STAGES + 4) * 8;
+    // the partial sums of a cluster: an area of their own where there is room, else where the stages were
+    static constexpr bool OWN_PART   = NT <= 32;
+    [[maybe_unused]] static constexpr int OFF_PART    = OWN_PART ? OFF_SF + STAGES * SF_STAGE : 0;
+    static constexpr int OFF_BAR     = OFF_SF + STAGES * SF_STAGE + (kSplit && OWN_PART ? NT * kMxRows * 4 : 0);
+    static constexpr int OFF_MISC    = OFF_BAR + (2 * STAGES + 5) * 8;
     static constexpr int DYN_BYTES   = OFF_MISC + 16 + 1024;
-    static constexpr int ACC         = kSplit ? 1 : 2;
+    static constexpr int ACC         = kSplit || NT == 128 ? 1 : 2; // accumulators
     static constexpr int SF_COLS     = 2 * F::kChunkCols; // per stage
     static constexpr int COLS        = ACC * NT + STAGES * SF_COLS;
     static constexpr int TMEM_COLS   = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static_assert(COLS <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
-    static_assert(!kSplit || STAGES * STAGE >= NT * kMxRows * 4, "the partial sums of a cluster fit where the stages were");
+    static_assert(TMEM_COLS <= 256 && DYN_BYTES <= 115200, "half the tensor and shared memory of an SM: two CTAs share it");
+    static_assert(STAGES * STAGE >= NT * kMxRows * 4, "the partial sums of a cluster fit where the stages were");
 };
 
 // N accumulator columns (tokens m, m + 1, ..) of a lane's channel n to dst.  Two-byte results of neighbouring channels leave as
@@ -97,8 +100,27 @@ __device__ __forceinline__ void store_block(const MxGemmParams &p, int m, int n,
     else store_block<__nv_bfloat16>(p, m, n, r, cols, bias);
 }
 
+// four tokens of one channel
+template <typename T>
+__device__ __forceinline__ void store_four(const MxGemmParams &p, int m, int n, const float4 &v, int cols, float bias)
+{
+    uint8_t    *dst  = p.dst + static_cast<int64_t>(m) * p.ldd + static_cast<int64_t>(n) * static_cast<int>(sizeof(T));
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+    {
+        if (j < cols) *reinterpret_cast<T *>(dst + j * p.ldd) = from_float<T>(__fmaf_rn(f[j], p.alpha, bias));
+    }
+}
+__device__ __forceinline__ void store_four(const MxGemmParams &p, int m, int n, const float4 &v, int cols, float bias)
+{
+    if (p.dtype == CUGL_F32) store_four<float>(p, m, n, v, cols, bias);
+    else if (p.dtype == CUGL_F16) store_four<__half>(p, m, n, v, cols, bias);
+    else store_four<__nv_bfloat16>(p, m, n, v, cols, bias);
+}
+
 template <int kFormat, int NT, int STAGES, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ MxGemmParams p)
 {
     using P = MxPlan<kFormat, NT, STAGES, kSplit>;
@@ -112,6 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto           tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     auto           tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+    const uint32_t part_bar  = bar_base + 8u * (2 * STAGES + 4);
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -141,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), 4);
         }
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,6 +174,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (kSplit)
+    {
+        cluster_sync(); // every CTA runs and has its barriers before anything is sent to it
+    }
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
     griddep_launch_dependents();
@@ -281,11 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = warp_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             tc_fence_after();
         }
-        __syncthreads();
-        cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
+        if (!P::OWN_PART)
+        {
+            __syncthreads();
+            cluster_sync(); // every CTA's MMAs have read their last stage
+        }
+        const uint32_t s_part = smem_u32(smem + P::OFF_PART);
         if (warp >= kFirstEpi && ok)
         {
-            const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, NT);
+            const int      ch = q * 32 + lane;
+            const uint32_t to = partial_address(s_part, ch, rank, shift, NT);
             for (int j = 0; j < cols; j += 16)
             {
                 uint32_t r[16];
@@ -293,23 +326,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld_wait();
                 send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, r, cols - j, c_begin < c_end);
             }
+            arrive_partial(part_bar, ch, shift);
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(part_bar, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
         }
-        cluster_sync();
         if (warp >= kFirstEpi && ok)
         {
             const int    own = kMxRows >> shift, et = threadIdx.x - 32 * kFirstEpi;
             const int    n = wb * kMxRows + rank * own + (et & (own - 1));
             const float  b = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
-            const float *part = reinterpret_cast<const float *>(smem);
+            const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
             if (n < p.channels)
             {
-                for (int at = et; at < cols * own; at += kEpiThreads)
+                for (int at = et; at < (cols + 3) / 4 * own; at += kEpiThreads)
                 {
-                    const float v   = __fmaf_rn(sum_partial(part, at, shift, NT), p.alpha, b);
-                    uint8_t    *dst = p.dst + static_cast<int64_t>(tb * NT + (at >> (7 - shift))) * p.ldd;
-                    if (p.dtype == CUGL_F32) reinterpret_cast<float *>(dst)[n] = v;
-                    else if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(v);
-                    else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(v);
+                    const int    j = (at >> (7 - shift)) * 4;
+                    const float4 v = sum_partial(part, at, shift, NT);
+                    store_four(p, tb * NT + j, n, v, cols - j, b);
                 }
             }
         }
@@ -321,6 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
+    }
+    if (kSplit && *s_abort != 0)
+    {
+        cluster_sync(); // this CTA may not have received all parts: it stays until the others have left or given up too
     }
     if (threadIdx.x == 0 && *s_abort != 0)
     {
@@ -612,10 +648,16 @@ cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, 
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc             = mx_idesc(kFormat, kMxRows, NT);
     const int64_t tiles = static_cast<int64_t>((p.channels + kMxRows - 1) / kMxRows) * ((p.tokens + NT - 1) / NT);
-    const int grid = kSplit ? static_cast<int>(tiles) * ranks : static_cast<int>(tiles < ctx->sm_count ? tiles : ctx->sm_count);
+    const int grid = kSplit ? static_cast<int>(tiles) * ranks : static_cast<int>(tiles < 2 * ctx->sm_count ? tiles : 2 * ctx->sm_count);
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, kSplit ? ranks : 1,
                                                 tiles, map_w, map_t, p));
     return CUGL_SUCCESS;
+}
+
+template <int kFormat, int NT, int STAGES>
+cugl_status launch_tokens(cugl_context *ctx, const MxOperands &op, const MxGemmParams &p, int ranks)
+{
+    return ranks > 1 ? launch_one<kFormat, NT, STAGES, true>(ctx, op, p, ranks) : launch_one<kFormat, NT, STAGES, false>(ctx, op, p, 1);
 }
 
 template <int kFormat>
@@ -656,24 +698,13 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     {
         return launch_pair<kFormat>(ctx, op, p);
     }
-    int ranks = 1; // CTAs that share a tile's K: as many as leave no SM idle and every CTA a chunk
-    while (ranks < 8 && tiles * ranks * 2 <= ctx->sm_count && ranks * 2 <= chunks) ranks *= 2;
-    if (ranks > 1)
-    {
-        switch (nt)
-        {
-            case 16: return launch_one<kFormat, 16, 8, true>(ctx, op, p, ranks);
-            case 32: return launch_one<kFormat, 32, 8, true>(ctx, op, p, ranks);
-            case 64: return launch_one<kFormat, 64, 7, true>(ctx, op, p, ranks);
-            default: return launch_one<kFormat, 128, 6, true>(ctx, op, p, ranks);
-        }
-    }
+    const int ranks = mx_split(tiles, chunks, 8);
     switch (nt)
     {
-        case 16: return launch_one<kFormat, 16, 8, false>(ctx, op, p, 1);
-        case 32: return launch_one<kFormat, 32, 8, false>(ctx, op, p, 1);
-        case 64: return launch_one<kFormat, 64, 7, false>(ctx, op, p, 1);
-        default: return launch_one<kFormat, 128, 6, false>(ctx, op, p, 1);
+        case 16: return launch_tokens<kFormat, 16, 4>(ctx, op, p, ranks);
+        case 32: return launch_tokens<kFormat, 32, 3>(ctx, op, p, ranks);
+        case 64: return launch_tokens<kFormat, 64, 3>(ctx, op, p, ranks);
+        default: return launch_tokens<kFormat, 128, 3>(ctx, op, p, ranks);
     }
 }
 

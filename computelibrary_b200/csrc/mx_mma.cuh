@@ -199,44 +199,55 @@ __device__ __forceinline__ void mx_chunk_scales(uint32_t t_dst, uint32_t sf, int
     }
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v)
+// Partial sums of a cluster whose 2^shift CTAs shared an accumulator's K.  Rank r owns channels r * (128 >> shift) and up.  The
+// warp that drains 32 lanes of an accumulator writes them to the owners' shared memory, [rank][columns / 4][channel][4 columns],
+// sixteen bytes per lane, and arrives on the owners' barrier; an owner that has all arrivals adds the parts up in the order of
+// the ranks, the same every time.  stride: columns of a part.
+__device__ __forceinline__ int partial_arrivals(int shift) // on an owner's barrier: its channels lie in one warp of each CTA or several
 {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+    return (1 << shift) * max(1, (kMxRows >> shift) / 32);
 }
-
-// Partial sums of a cluster whose 2^shift CTAs shared an accumulator's K.  Rank r owns channels r * (128 >> shift) and up.  A
-// warp sends sixteen columns of its 32 accumulator lanes to the owners' shared memory, [rank][column][channel of the owner]:
-// a lane's address only grows by a constant from column to column.  stride: columns of a part.
 __device__ __forceinline__ uint32_t partial_address(uint32_t s_base, int ch, int rank, int shift, int stride)
 {
     const int own = kMxRows >> shift;
-    return map_to_cta(s_base, static_cast<uint32_t>(ch / own)) + 4u * static_cast<uint32_t>(rank * stride * own + (ch & (own - 1)));
+    return map_to_cta(s_base, static_cast<uint32_t>(ch / own)) + 4u * static_cast<uint32_t>(rank * stride * own) + 16u * static_cast<uint32_t>(ch & (own - 1));
 }
 __device__ __forceinline__ void send_partial(uint32_t to, int shift, const uint32_t (&r)[16], int cols, bool has)
 {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 16; i += 4)
     {
         if (i < cols) // a rank without a share of K has no accumulator: zeros
         {
-            st_cluster_f32(to + static_cast<uint32_t>(i) * (4u * kMxRows >> shift), has ? __uint_as_float(r[i]) : 0.f);
+            st_cluster_v4(to + static_cast<uint32_t>(i) * (4u * kMxRows >> shift), has ? r[i] : 0u, has ? r[i + 1] : 0u, has ? r[i + 2] : 0u,
+                          has ? r[i + 3] : 0u);
         }
     }
 }
-// Sum over the ranks, always in their order, of element `at` (column * own + channel) of the parts.
-__device__ __forceinline__ float sum_partial(const float *part, int at, int shift, int stride)
+__device__ __forceinline__ void arrive_partial(uint32_t bar, int ch, int shift)
 {
-    float v[8];
+    __syncwarp();
+    if ((ch & (min(kMxRows >> shift, 32) - 1)) == 0)
+    {
+        mbar_arrive_cluster(map_to_cta(bar, static_cast<uint32_t>(ch / (kMxRows >> shift))));
+    }
+}
+// Four columns of one channel; at: (columns / 4) * (128 >> shift) + channel of the owner.
+__device__ __forceinline__ float4 sum_partial(const float *part, int at, int shift, int stride)
+{
+    const float4 *p   = reinterpret_cast<const float4 *>(part) + at;
+    const int     gap = stride * (kMxRows >> shift) / 4;
+    float4        v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
     {
-        if (i < (1 << shift)) v[i] = part[i * stride * (kMxRows >> shift) + at];
+        if (i < (1 << shift)) v[i] = p[i * gap];
     }
-    float sum = v[0];
+    float4 sum = v[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i)
     {
-        if (i < (1 << shift)) sum += v[i];
+        if (i < (1 << shift)) sum.x += v[i].x, sum.y += v[i].y, sum.z += v[i].z, sum.w += v[i].w;
     }
     return sum;
 }
@@ -255,6 +266,17 @@ inline bool encode_scale_map(CUtensorMap *map, const void *base, int64_t tiles, 
     const cuuint32_t estr[2]    = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// CTAs (a power of two up to `most`) that share the K of each of `tiles` tiles as a cluster.  With two CTAs to an SM the device
+// holds 148 clusters of two, 71 of four or 33 of eight at once (cudaOccupancyMaxActiveClusters; clusters do not cross the
+// boundaries between groups of SMs); one cluster more would run alone after all others.
+inline int mx_split(long long tiles, int chunks, int most)
+{
+    if (most >= 8 && tiles <= 33 && chunks >= 8) return 8;
+    if (most >= 4 && tiles <= 71 && chunks >= 4) return 4;
+    if (tiles <= 148 && chunks >= 2) return 2;
+    return 1;
 }
 
 // packed rows x (inner bytes), ld bytes apart; box = box_rows x 128 bytes in the 128-byte swizzle; what lies outside reads as 0

@@ -10,7 +10,8 @@
 // atomics, the same order every time.
 //
 // Three launches, overlapped by programmatic dependent launch: gate + quantisation of x, gate/up products + SwiGLU +
-// quantisation, down product.
+// quantisation, down product.  The second lets the third start only after its own wait, i.e. when the first has completed: so
+// the third knows the experts and loads its first weights while the second is still running.
 #include "mx_mma.cuh"
 
 #include <cmath>
@@ -223,7 +224,7 @@ __device__ __forceinline__ float gate_weight(const MoeParams &p, int t, int e)
 }
 // One token's 32 values of h (a warp's lanes: consecutive f) to codes and scales.  f: the lane's place on the intermediate axis.
 template <int kFormat>
-__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, int f, int lane, float h, bool in = true)
+__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, int f, int lane, float h)
 {
     uint32_t amax = __float_as_uint(h) & 0x7fffffffu;
     if (kFormat == CUGL_MXFP4)
@@ -240,12 +241,12 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, i
     w <<= 4 * (lane & 7);
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-    if (in && (lane & 7) == 0 && f < p.inner)
+    if ((lane & 7) == 0 && f < p.inner)
     {
         *reinterpret_cast<uint32_t *>(p.hq + (static_cast<int64_t>(a) * p.tokens + t) * p.ld_hq + f / 2) = w;
     }
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
-    if (in && (lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
+    if ((lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
     {
         p.hs[static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes + mx_scale_offset(t, f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s.byte);
     }
@@ -283,13 +284,23 @@ __device__ __forceinline__ void store_hidden_zero(const MoeParams &p, int a, int
     }
 }
 
-__device__ __forceinline__ float swiglu(float g, float u, float w)
+// A token's sums g and u at 32 consecutive f to h.
+template <int kFormat>
+__device__ __forceinline__ void store_token(const MoeParams &p, int a, int t, int f, int lane, float g, float u, float w)
 {
-    return w * (g / (1.f + expf(-g))) * u;
+    if (w == kNotChosen)
+    {
+        store_hidden_zero<kFormat>(p, a, t, f, lane);
+        return;
+    }
+    g *= p.gate_alpha;
+    u *= p.up_alpha;
+    const float h = w * (g / (1.f + expf(-g))) * u; // SwiGLU, the gate's weight folded in
+    store_hidden<kFormat>(p, a, t, f, lane, f < p.inner ? h : 0.f);
 }
 
-// kOperands: weight matrices that share a stage's tokens (2: gate and up, 1: down)
-template <int kFormat, int NT, int STAGES, int kOperands, int kAcc>
+// kOperands: weight matrices that share a stage's tokens (2: gate and up, 1: down).  Up to 64 tokens two CTAs share an SM.
+template <int kFormat, int NT, int STAGES, int kOperands, bool kSplit, int kAcc>
 struct MoePlan
 {
     using F                         = MxTraits<kFormat>;
@@ -297,29 +308,34 @@ struct MoePlan
     static constexpr int STAGE      = kOperands * kMxWBytes + T_BYTES;
     static constexpr int SF_STAGE   = (kOperands + 1) * F::kChunkScale;
     static constexpr int OFF_SF     = STAGES * STAGE;
-    static constexpr int OFF_BAR    = OFF_SF + STAGES * SF_STAGE;
-    static constexpr int OFF_MISC   = OFF_BAR + (2 * STAGES + 4) * 8;
+    // the partial sums of a cluster: an area of their own where there is room, else where the stages were
+    static constexpr int  PART      = kOperands * NT * kMxRows * 4;
+    static constexpr bool OWN_PART  = PART <= 16384;
+    [[maybe_unused]] static constexpr int OFF_PART   = OWN_PART ? OFF_SF + STAGES * SF_STAGE : 0;
+    static constexpr int OFF_BAR    = OFF_SF + STAGES * SF_STAGE + (kSplit && OWN_PART ? PART : 0);
+    static constexpr int OFF_MISC   = OFF_BAR + (2 * STAGES + 5) * 8;
     static constexpr int OFF_BITS   = OFF_MISC + 16;
     static constexpr int OFF_LIST   = OFF_BITS + kMaxExperts / 8;
     static constexpr int OFF_WEIGHT = OFF_LIST + kMaxExperts * 2;
-    static constexpr int DYN_BYTES  = OFF_WEIGHT + 2 * kMaxTokens * 4 + 1024; // two tables
+    static constexpr int DYN_BYTES  = OFF_WEIGHT + (kOperands == 2 ? 2 * kMaxTokens * 4 : 0) + 1024; // two tables
     static constexpr int ACC_COLS   = kOperands * NT;
     static constexpr int SF_COLS    = (kOperands + 1) * F::kChunkCols;
     static constexpr int COLS       = kAcc * ACC_COLS + STAGES * SF_COLS;
     static constexpr int TMEM_COLS  = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static constexpr int PER_SM     = TMEM_COLS <= 256 && DYN_BYTES <= 115200 ? 2 : 1;
     static_assert(COLS <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
-    static_assert(STAGES * STAGE >= kOperands * NT * kMxRows * 4, "the partial sums of a cluster fit where the stages were");
+    static_assert(STAGES * STAGE >= PART, "the partial sums of a cluster fit where the stages were");
 };
 
 // ---- second launch -------------------------------------------------------------------------------------------
 // Unit of work: 128 rows of one active expert's gate and up matrices, over all tokens.  kSplit: the CTAs of a cluster share a
 // unit's K (few units); else a CTA works through its units, the stages of the next one arriving during the epilogue.
 template <int kFormat, int NT, int STAGES, bool kSplit, int kAcc>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>::PER_SM)
     moe_gate_up_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_constant__ CUtensorMap tmap_u, const __grid_constant__ CUtensorMap tmap_x,
                        const __grid_constant__ MoeParams p)
 {
-    using P = MoePlan<kFormat, NT, STAGES, 2, kAcc>;
+    using P = MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>;
     using F = MxTraits<kFormat>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t       *smem       = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -330,12 +346,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto           empty_bar  = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto           tfull_bar  = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     auto           tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+    const uint32_t part_bar   = bar_base + 8u * (2 * STAGES + 4);
     uint32_t      *s_tmem     = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort    = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_bits     = reinterpret_cast<uint32_t *>(smem + P::OFF_BITS);
     uint16_t      *s_list     = reinterpret_cast<uint16_t *>(smem + P::OFF_LIST);
     float         *s_weight   = reinterpret_cast<float *>(smem + P::OFF_WEIGHT);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int      rank  = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+    const int      ranks = kSplit ? static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x()) : 1;
 
     if (threadIdx.x == 0)
     {
@@ -349,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), 4);
         }
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -358,17 +378,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (kSplit)
+    {
+        cluster_sync(); // every CTA runs and has its barriers before anything is sent to it
+    }
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
-    griddep_launch_dependents();
     griddep_wait(); // the prologue above touched no global memory
+    griddep_launch_dependents();
 
     const int active      = active_experts(p, s_list, s_bits);
     const int blocks      = (p.inner + kMxRows - 1) / kMxRows;
     const int units       = active * blocks;
     const int chunks      = (p.hidden + kMxChunk - 1) / kMxChunk;
-    const int rank        = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
-    const int ranks       = kSplit ? static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x()) : 1;
     const int first_unit  = kSplit ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
     const int unit_stride = kSplit ? max(units, 1) : static_cast<int>(gridDim.x);
     const int per_rank    = (chunks + ranks - 1) / ranks;
@@ -484,16 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 {
                     if (j + i < p.tokens)
                     {
-                        const float w = weight[j + i];
-                        if (w != kNotChosen)
-                        {
-                            const float h = f < p.inner ? swiglu(__uint_as_float(g[i]) * p.gate_alpha, __uint_as_float(u[i]) * p.up_alpha, w) : 0.f;
-                            store_hidden<kFormat>(p, a, j + i, f, lane, h);
-                        }
-                        else
-                        {
-                            store_hidden_zero<kFormat>(p, a, j + i, f, lane);
-                        }
+                        store_token<kFormat>(p, a, j + i, f, lane, __uint_as_float(g[i]), __uint_as_float(u[i]), weight[j + i]);
                     }
                 }
             }
@@ -515,11 +528,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = warp_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             tc_fence_after();
         }
-        __syncthreads();
-        cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
+        if (!P::OWN_PART)
+        {
+            __syncthreads();
+            cluster_sync(); // every CTA's MMAs have read their last stage
+        }
         if (warp >= kFirstEpi && ok)
         {
-            const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, 2 * NT);
+            const int      ch = q * 32 + lane;
+            const uint32_t to = partial_address(smem_u32(smem + P::OFF_PART), ch, rank, shift, 2 * NT);
             for (int j = 0; j < p.tokens; j += 16)
             {
                 uint32_t g[16], u[16];
@@ -529,24 +546,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, g, p.tokens - j, c_begin < c_end);
                 send_partial(to + static_cast<uint32_t>(NT + j) * (4u * kMxRows >> shift), shift, u, p.tokens - j, c_begin < c_end);
             }
+            arrive_partial(part_bar, ch, shift);
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(part_bar, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
         }
-        cluster_sync();
         if (warp >= kFirstEpi && ok)
         {
-            // a warp takes 32 consecutive channels of one token at a time: a rank owns at least 32 (launch_layers)
+            // a warp takes 32 consecutive channels of four tokens at a time: a rank owns at least 32 (launch_layers)
             const int    own = kMxRows >> shift;
-            const float *part = reinterpret_cast<const float *>(smem);
-            for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < p.tokens * own; at += kEpiThreads)
+            const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
+            for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < (p.tokens + 3) / 4 * own; at += kEpiThreads)
             {
-                const bool  in = at < p.tokens * own;
-                const int   t  = in ? at >> (7 - shift) : 0, f = (first_unit % blocks) * kMxRows + rank * own + (at & (own - 1));
-                const float w  = in && f < p.inner ? s_weight[t] : kNotChosen;
-                float       h  = 0.f;
-                if (w != kNotChosen)
+                const int    t0 = (at >> (7 - shift)) * 4, f = (first_unit % blocks) * kMxRows + rank * own + (at & (own - 1));
+                const float4 g4 = sum_partial(part, at, shift, 2 * NT), u4 = sum_partial(part + NT * own, at, shift, 2 * NT);
+                const float  g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
                 {
-                    h = swiglu(sum_partial(part, at, shift, 2 * NT) * p.gate_alpha, sum_partial(part + NT * own, at, shift, 2 * NT) * p.up_alpha, w);
+                    if (t0 + i < p.tokens)
+                    {
+                        store_token<kFormat>(p, a, t0 + i, f, lane, g[i], u[i], s_weight[t0 + i]);
+                    }
                 }
-                store_hidden<kFormat>(p, a, t, f, lane, h, in);
             }
         }
     }
@@ -558,6 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
     }
+    if (kSplit && *s_abort != 0)
+    {
+        cluster_sync(); // this CTA may not have received all parts: it stays until the others have left or given up too
+    }
     if (threadIdx.x == 0 && *s_abort != 0)
     {
         atomicCAS(p.status, 0, *s_abort);
@@ -567,10 +591,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---- third launch --------------------------------------------------------------------------------------------
 // Unit of work: 128 output channels; K is (active expert, intermediate), shared by the CTAs of a cluster.
 template <int kFormat, int NT, int STAGES>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     moe_down_kernel(const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ MoeParams p)
 {
-    using P = MoePlan<kFormat, NT, STAGES, 1, 1>;
+    using P = MoePlan<kFormat, NT, STAGES, 1, true, 1>;
+    static_assert(P::PER_SM == 2, "two CTAs share an SM");
     using F = MxTraits<kFormat>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t       *smem      = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -579,12 +604,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t bar_base  = smem_u32(smem + P::OFF_BAR);
     auto           full_bar  = [&](int s) { return bar_base + 8u * s; };
     auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
-    const uint32_t tfull     = bar_base + 8u * (2 * STAGES);
+    const uint32_t tfull     = bar_base + 8u * (2 * STAGES), part_bar = bar_base + 8u * (2 * STAGES + 4);
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_bits    = reinterpret_cast<uint32_t *>(smem + P::OFF_BITS);
     uint16_t      *s_list    = reinterpret_cast<uint16_t *>(smem + P::OFF_LIST);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int      rank  = static_cast<int>(cluster_ctarank());
+    const int      ranks = static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x());
 
     if (threadIdx.x == 0)
     {
@@ -594,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(tfull, 1);
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -603,17 +631,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync(); // every CTA runs and has its barriers before anything is sent to it
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
     griddep_launch_dependents();
-    griddep_wait(); // the prologue above touched no global memory
 
+    // before the wait for the second launch: what the first one wrote, and the weights
     const int active     = active_experts(p, s_list, s_bits);
     const int per_expert = (p.inner + kMxChunk - 1) / kMxChunk;
     const int chunks     = active * per_expert;
     const int blocks     = (p.hidden + kMxRows - 1) / kMxRows;
-    const int rank       = static_cast<int>(cluster_ctarank());
-    const int ranks      = static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x());
     const int block      = static_cast<int>(cluster_id_x());
     const int per_rank   = (chunks + ranks - 1) / ranks;
     const int c_begin    = min(chunks, rank * per_rank);
@@ -623,28 +650,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         const bool el = elect_one();
         {
-            int g = 0;
-            for (int i = c_begin; i < c_end; ++i, ++g)
+            auto load_weights = [&](int g) {
+                const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, e = s_list[a], first = c * F::kChunkTiles;
+                const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
+                if (el)
+                {
+                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
+                    tma_load_2d(s_stage + s * P::STAGE, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
+                    bulk_load(s_sf + s * P::SF_STAGE, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes,
+                              full_bar(s));
+                }
+                __syncwarp();
+            };
+            auto load_tokens = [&](int g) {
+                const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, first = c * F::kChunkTiles;
+                const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
+                if (el)
+                {
+                    tma_load_2d(s_stage + s * P::STAGE + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
+                    bulk_load(s_sf + s * P::SF_STAGE + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
+                }
+                __syncwarp();
+            };
+            const int mine = c_end - c_begin, early = min(mine, STAGES);
+            int       g = 0;
+            for (; g < early; ++g) load_weights(g);
+            griddep_wait();
+            for (int i = 0; i < early; ++i) load_tokens(i);
+            for (; g < mine; ++g)
             {
                 const int s = g % STAGES;
                 if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                 {
                     break;
                 }
-                const int      a = i / per_expert, c = i - a * per_expert, e = s_list[a];
-                const int      first = c * F::kChunkTiles;
-                const int      n     = min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first);
-                const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
-                const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                if (el)
-                {
-                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
-                    tma_load_2d(dst, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
-                    tma_load_2d(dst + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
-                    bulk_load(sf, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
-                    bulk_load(sf + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
-                }
-                __syncwarp();
+                load_weights(g);
+                load_tokens(g);
             }
             if (el && *s_abort != 0)
             {
@@ -691,14 +732,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool      ok = true;
     if (warp >= kFirstEpi)
     {
+        griddep_wait(); // nothing is written before the launches ahead have completed
         ok = warp_wait(tfull, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
         tc_fence_after();
     }
-    __syncthreads();
-    cluster_sync(); // every CTA's MMAs have read their last stage: partial sums go where the stages were
+    if (!P::OWN_PART)
+    {
+        __syncthreads();
+        cluster_sync(); // every CTA's MMAs have read their last stage
+    }
     if (warp >= kFirstEpi && ok)
     {
-        const uint32_t to = partial_address(s_stage, q * 32 + lane, rank, shift, NT);
+        const int      ch = q * 32 + lane;
+        const uint32_t to = partial_address(smem_u32(smem + P::OFF_PART), ch, rank, shift, NT);
         for (int j = 0; j < p.tokens; j += 16)
         {
             uint32_t r[16];
@@ -706,21 +752,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_wait();
             send_partial(to + static_cast<uint32_t>(j) * (4u * kMxRows >> shift), shift, r, p.tokens - j, c_begin < c_end);
         }
+        arrive_partial(part_bar, ch, shift);
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(part_bar, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit));
     }
-    cluster_sync();
     if (warp >= kFirstEpi && ok)
     {
         const int    own = kMxRows >> shift, et = threadIdx.x - 32 * kFirstEpi;
         const int    n = block * kMxRows + rank * own + (et & (own - 1));
-        const float *part = reinterpret_cast<const float *>(smem);
+        const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
         if (n < p.hidden)
         {
-            for (int at = et; at < p.tokens * own; at += kEpiThreads)
+            for (int at = et; at < (p.tokens + 3) / 4 * own; at += kEpiThreads)
             {
-                const float v   = sum_partial(part, at, shift, NT) * p.down_alpha;
-                uint8_t    *dst = p.dst + static_cast<int64_t>(at >> (7 - shift)) * p.ld_dst;
-                if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(v);
-                else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(v);
+                const int    j  = (at >> (7 - shift)) * 4;
+                const float4 v4 = sum_partial(part, at, shift, NT);
+                const float  v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    if (j + i < p.tokens)
+                    {
+                        uint8_t *dst = p.dst + static_cast<int64_t>(j + i) * p.ld_dst;
+                        if (p.dtype == CUGL_F16) reinterpret_cast<__half *>(dst)[n] = from_float<__half>(v[i] * p.down_alpha);
+                        else reinterpret_cast<__nv_bfloat16 *>(dst)[n] = from_float<__nv_bfloat16>(v[i] * p.down_alpha);
+                    }
+                }
             }
         }
     }
@@ -731,6 +787,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
+    }
+    if (*s_abort != 0)
+    {
+        cluster_sync(); // this CTA may not have received all parts: it stays until the others have left or given up too
     }
     if (threadIdx.x == 0 && *s_abort != 0)
     {
@@ -809,11 +869,12 @@ struct MoeMaps
 template <int kFormat, int NT, int STAGES, bool kSplit, int kAcc>
 cugl_status launch_gate_up(cugl_context *ctx, const MoeMaps &m, const MoeParams &p, int most_units, int ranks)
 {
-    using P     = MoePlan<kFormat, NT, STAGES, 2, kAcc>;
+    using P     = MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>;
     auto kernel = moe_gate_up_kernel<kFormat, NT, STAGES, kSplit, kAcc>;
     static bool set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
-    const int grid = kSplit ? most_units * ranks : (most_units < ctx->sm_count ? most_units : ctx->sm_count);
+    const int slots = P::PER_SM * ctx->sm_count;
+    const int grid  = kSplit ? most_units * ranks : (most_units < slots ? most_units : slots);
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, kSplit ? ranks : 1, most_units,
                                                 m.gate, m.up, m.x, p));
     return CUGL_SUCCESS;
@@ -824,9 +885,8 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
 {
     const int most_units = most_active * ((p.inner + kMxRows - 1) / kMxRows);
     const int chunks     = (p.hidden + kMxChunk - 1) / kMxChunk;
-    int       ranks      = 1; // CTAs that share a unit's K: as many as leave no SM idle and every CTA a chunk
-    // (at most four: a rank then owns 32 channels of a unit, one MXFP4 block)
-    while (ranks < 4 && most_units * ranks * 2 <= ctx->sm_count && ranks * 2 <= chunks) ranks *= 2;
+    // at most four: a rank then owns 32 channels of a unit, one MXFP4 block; and only where two CTAs share an SM (mx_split)
+    int ranks = NT <= 64 ? mx_split(most_units, chunks, 4) : 1;
     if (ranks > 1)
     {
         CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, true, 1>(ctx, m, p, most_units, ranks)));
@@ -835,13 +895,12 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     {
         CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, false, kUpAcc>(ctx, m, p, most_units, 1)));
     }
-    using P     = MoePlan<kFormat, NT, kDownStages, 1, 1>;
+    using P     = MoePlan<kFormat, NT, kDownStages, 1, true, 1>;
     auto kernel = moe_down_kernel<kFormat, NT, kDownStages>;
     static bool set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int blocks = (p.hidden + kMxRows - 1) / kMxRows, most_chunks = most_active * ((p.inner + kMxChunk - 1) / kMxChunk);
-    ranks            = 1;
-    while (ranks < 8 && blocks * ranks * 2 <= ctx->sm_count && ranks * 2 <= most_chunks) ranks *= 2;
+    ranks = mx_split(blocks, most_chunks, 8);
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kThreads, P::DYN_BYTES, ranks, blocks * ranks,
                                                 m.down, m.h, p));
     return CUGL_SUCCESS;
@@ -862,10 +921,10 @@ cugl_status launch_moe(cugl_context *ctx, const MoeMaps &m, MoeParams p, int nt,
     p.idesc = mx_idesc(kFormat, kMxRows, nt);
     switch (nt)
     {
-        case 16: return launch_layers<kFormat, 16, 5, 2, 8>(ctx, m, p, most_active);
-        case 32: return launch_layers<kFormat, 32, 5, 2, 8>(ctx, m, p, most_active);
-        case 64: return launch_layers<kFormat, 64, 4, 2, 7>(ctx, m, p, most_active);
-        default: return launch_layers<kFormat, 128, 4, 1, 6>(ctx, m, p, most_active);
+        case 16: return launch_layers<kFormat, 16, 2, 2, 4>(ctx, m, p, most_active);
+        case 32: return launch_layers<kFormat, 32, 2, 2, 3>(ctx, m, p, most_active);
+        case 64: return launch_layers<kFormat, 64, 2, 1, 3>(ctx, m, p, most_active);
+        default: return launch_layers<kFormat, 128, 4, 1, 3>(ctx, m, p, most_active);
     }
 }
 } // namespace
