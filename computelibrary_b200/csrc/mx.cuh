@@ -112,7 +112,8 @@ struct MxScale
     float    mul;  // MXFP4: 1 / scale.  NVFP4: 2^-exponent / scale, rounded up (scale_to_code)
     float    div;  // NVFP4: the scale itself (f32 sources divide)
 };
-template <int kFormat>
+// kExact false: values that were computed in float just now and carry its error; a product with 1 / 6 instead of the division.
+template <int kFormat, bool kExact = true>
 __device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponent_mul)
 {
     MxScale s;
@@ -130,7 +131,7 @@ __device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponen
         return s;
     }
     const float                amax = __uint_as_float(amax_bits) * exponent_mul;
-    const float                v    = fminf(fmaxf(__fdiv_rn(amax, 6.f), 0x1p-9f), 448.f);
+    const float                v    = fminf(fmaxf(kExact ? __fdiv_rn(amax, 6.f) : amax * (1.f / 6.f), 0x1p-9f), 448.f);
     const __nv_fp8_storage_t   b    = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
     const float                f    = __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
     s.byte                          = b;

@@ -50,13 +50,14 @@ struct MoeParams
 // ---- first launch ----------------------------------------------------------------------------------------
 // The gate: a warp per token.  Logits become unsigned keys in their order (0: not to be chosen: NaN and -infinity, or chosen
 // already); a choice is the largest key, the lowest index among equal ones.
+template <int kPer> // experts per lane
 __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
 {
     const float *row = reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(p.logits) + t * p.ld_logits);
-    uint32_t     key[kMaxExperts / 32];
+    uint32_t     key[kPer];
     float        top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kMaxExperts / 32; ++i)
+    for (int i = 0; i < kPer; ++i)
     {
         const int   e = i * 32 + lane;
         const float v = e < p.experts ? __ldg(row + e) : -INFINITY;
@@ -70,7 +71,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
     if (p.renormalize == 0)
     {
 #pragma unroll
-        for (int i = 0; i < kMaxExperts / 32; ++i)
+        for (int i = 0; i < kPer; ++i)
         {
             const int e = i * 32 + lane;
             if (e < p.experts && key[i] != 0) all += expf(__ldg(row + e) - top);
@@ -84,18 +85,18 @@ __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
     {
         uint32_t best = 0;
 #pragma unroll
-        for (int i = 0; i < kMaxExperts / 32; ++i) best = max(best, key[i]);
+        for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
         best = __reduce_max_sync(0xffffffffu, best);
         int at = kMaxExperts;
 #pragma unroll
-        for (int i = kMaxExperts / 32 - 1; i >= 0; --i)
+        for (int i = kPer - 1; i >= 0; --i)
         {
             if (best != 0 && key[i] == best) at = i * 32 + lane;
         }
         at = __reduce_min_sync(0xffffffffu, at);
         if (best == 0) break;
 #pragma unroll
-        for (int i = 0; i < kMaxExperts / 32; ++i)
+        for (int i = 0; i < kPer; ++i)
         {
             if (at == i * 32 + lane) key[i] = 0;
         }
@@ -177,7 +178,9 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const __grid_constant__ 
         const int t = block * 8 + warp;
         if (t < p.tokens)
         {
-            route_token(p, t, lane);
+            if (p.experts <= 64) route_token<2>(p, t, lane);
+            else if (p.experts <= 128) route_token<4>(p, t, lane);
+            else route_token<kMaxExperts / 32>(p, t, lane);
         }
         return;
     }
@@ -222,41 +225,29 @@ __device__ __forceinline__ float gate_weight(const MoeParams &p, int t, int e)
     }
     return w;
 }
-// One token's 32 values of h (a warp's lanes: consecutive f) to codes and scales.  f: the lane's place on the intermediate axis.
+// While a unit's MMAs run, the epilogue warps fill a table of its gate weights, a token per thread, and write the zeros of the
+// tokens that did not choose the expert.  They agree on carrying on: a warp that gave up says so here instead of leaving the
+// others at the barrier.
 template <int kFormat>
-__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t, int f, int lane, float h)
-{
-    uint32_t amax = __float_as_uint(h) & 0x7fffffffu;
-    if (kFormat == CUGL_MXFP4)
-    {
-        amax = __reduce_max_sync(0xffffffffu, amax);
-    }
-    else
-    {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    }
-    const MxScale s = mx_scale_of<kFormat>(amax, p.h_mul);
-    uint32_t      w = static_cast<uint32_t>(__nv_cvt_float_to_fp4(scale_to_code<kFormat, true>(h, s, p.h_mul), __NV_E2M1, cudaRoundNearest)) & 15u;
-    w <<= 4 * (lane & 7);
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-    if ((lane & 7) == 0 && f < p.inner)
-    {
-        *reinterpret_cast<uint32_t *>(p.hq + (static_cast<int64_t>(a) * p.tokens + t) * p.ld_hq + f / 2) = w;
-    }
-    constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
-    if ((lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
-    {
-        p.hs[static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes + mx_scale_offset(t, f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s.byte);
-    }
-}
-// The epilogue warps fill a table of the unit's weights while its MMAs run, a token per thread, and agree on carrying on: a
-// warp that gave up says so here instead of leaving the others at the barrier.
-__device__ __forceinline__ bool fill_weights(const MoeParams &p, float *table, int e, bool ok)
+__device__ __forceinline__ bool begin_unit(const MoeParams &p, float *table, int a, int e, int f0, bool ok)
 {
     const int t = threadIdx.x - 32 * kFirstEpi;
-    if (t < p.tokens) table[t] = gate_weight(p, t, e);
+    if (t < p.tokens)
+    {
+        const float w = gate_weight(p, t, e);
+        table[t]      = w;
+        if (w == kNotChosen)
+        {
+            uint2 *codes = reinterpret_cast<uint2 *>(p.hq + (static_cast<int64_t>(a) * p.tokens + t) * p.ld_hq + f0 / 2);
+            for (int i = 0; i < min(kMxRows, p.inner - f0) / 16; ++i) codes[i] = make_uint2(0, 0);
+            constexpr int kTiles = kMxRows / (4 * (kFormat == CUGL_NVFP4 ? 16 : 32)); // scale tiles along a unit
+            uint8_t      *scales = p.hs + static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes;
+            for (int i = f0 / kMxRows * kTiles; i < min(f0 / kMxRows * kTiles + kTiles, static_cast<int>(p.f_tiles)); ++i)
+            {
+                *reinterpret_cast<uint32_t *>(scales + mx_scale_offset(t, 4 * i, p.f_tiles)) = 0;
+            }
+        }
+    }
     uint32_t r;
     asm volatile("{\n\t"
                  ".reg .pred p, q;\n\t"
@@ -269,34 +260,63 @@ __device__ __forceinline__ bool fill_weights(const MoeParams &p, float *table, i
                  : "memory");
     return r != 0;
 }
-// The same for a token that did not choose the expert: zeros.
+
+// Four tokens' sums g and u at a warp's 32 consecutive f to h, its codes and scales; chosen: bit i, token t0 + i chose the
+// expert (the others' zeros are written already).  Four at a time because each is one long chain of dependent instructions.
 template <int kFormat>
-__device__ __forceinline__ void store_hidden_zero(const MoeParams &p, int a, int t, int f, int lane)
+__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t0, int f, int lane, const float (&g)[4], const float (&u)[4], const float *weight,
+                                             uint32_t chosen)
 {
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
-    if ((lane & 7) == 0 && f < p.inner)
+    float         h[4];
+    uint32_t      amax[4], w[4];
+    MxScale       s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
     {
-        *reinterpret_cast<uint32_t *>(p.hq + (static_cast<int64_t>(a) * p.tokens + t) * p.ld_hq + f / 2) = 0;
+        const float x = g[i] * p.gate_alpha;
+        const float v = weight[t0 + i] * __fdividef(x, 1.f + expf(-x)) * (u[i] * p.up_alpha); // SwiGLU, the gate's weight folded in
+        h[i]          = f < p.inner ? v : 0.f;
+        amax[i]       = __float_as_uint(h[i]) & 0x7fffffffu;
     }
-    if ((lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4)
+    if (kFormat == CUGL_MXFP4)
     {
-        p.hs[static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes + mx_scale_offset(t, f / kBlock, p.f_tiles)] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax[i] = __reduce_max_sync(0xffffffffu, amax[i]);
     }
-}
-
-// A token's sums g and u at 32 consecutive f to h.
-template <int kFormat>
-__device__ __forceinline__ void store_token(const MoeParams &p, int a, int t, int f, int lane, float g, float u, float w)
-{
-    if (w == kNotChosen)
+    else
     {
-        store_hidden_zero<kFormat>(p, a, t, f, lane);
-        return;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+        {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax[i] = max(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+        }
     }
-    g *= p.gate_alpha;
-    u *= p.up_alpha;
-    const float h = w * (g / (1.f + expf(-g))) * u; // SwiGLU, the gate's weight folded in
-    store_hidden<kFormat>(p, a, t, f, lane, f < p.inner ? h : 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        s[i] = mx_scale_of<kFormat, false>(amax[i], p.h_mul); // h carries the error of float sums: no exact quotients
+        w[i] = (static_cast<uint32_t>(__nv_cvt_float_to_fp4(h[i] * s[i].mul, __NV_E2M1, cudaRoundNearest)) & 15u) << (4 * (lane & 7));
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], o);
+    }
+    uint8_t *codes  = p.hq + (static_cast<int64_t>(a) * p.tokens + t0) * p.ld_hq + f / 2;
+    uint8_t *scales = p.hs + static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes;
+    const bool code_lane = (lane & 7) == 0 && f < p.inner, scale_lane = (lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        if ((chosen >> i) & 1u)
+        {
+            if (code_lane) *reinterpret_cast<uint32_t *>(codes + i * p.ld_hq) = w[i];
+            if (scale_lane) scales[mx_scale_offset(t0 + i, f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s[i].byte);
+        }
+    }
 }
 
 // kOperands: weight matrices that share a stage's tokens (2: gate and up, 1: down).  Up to 64 tokens two CTAs share an SM.
@@ -488,25 +508,29 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
         bool      ok = true;
         for (int unit = first_unit; unit < units; unit += unit_stride, ++it)
         {
-            const int a = unit / blocks, f = (unit % blocks) * kMxRows + q * 32 + lane;
+            const int a = unit / blocks, f0 = (unit % blocks) * kMxRows, f = f0 + q * 32 + lane;
             const int as = it % kAcc;
             float    *weight = s_weight + (it & 1) * kMaxTokens; // the other table may still be read by a slower warp
-            if (!fill_weights(p, weight, s_list[a], ok)) break;
+            if (!begin_unit<kFormat>(p, weight, a, s_list[a], f0, ok)) break;
             ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
             for (int j = 0; j < p.tokens; j += 16)
             {
+                const uint32_t chosen = __ballot_sync(0xffffffffu, lane < 16 && j + lane < p.tokens && weight[j + lane] != kNotChosen);
+                if (chosen == 0) continue;
                 uint32_t g[16], u[16];
                 tmem_ld_x16(tmem_base + as * P::ACC_COLS + j + (static_cast<uint32_t>(q * 32) << 16), g);
                 tmem_ld_x16(tmem_base + as * P::ACC_COLS + NT + j + (static_cast<uint32_t>(q * 32) << 16), u);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+                for (int i = 0; i < 16; i += 4)
                 {
-                    if (j + i < p.tokens)
+                    if (((chosen >> i) & 15u) != 0)
                     {
-                        store_token<kFormat>(p, a, j + i, f, lane, __uint_as_float(g[i]), __uint_as_float(u[i]), weight[j + i]);
+                        const float g4[4] = {__uint_as_float(g[i]), __uint_as_float(g[i + 1]), __uint_as_float(g[i + 2]), __uint_as_float(g[i + 3])};
+                        const float u4[4] = {__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])};
+                        store_hidden<kFormat>(p, a, j + i, f, lane, g4, u4, weight, (chosen >> i) & 15u);
                     }
                 }
             }
@@ -524,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
         bool       ok = work;
         if (warp >= kFirstEpi && work)
         {
-            fill_weights(p, s_weight, s_list[a], true);
+            (void)begin_unit<kFormat>(p, s_weight, a, s_list[a], first_unit % blocks * kMxRows, true);
             ok = warp_wait(tfull_bar(0), 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             tc_fence_after();
         }
@@ -557,15 +581,12 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
             for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < (p.tokens + 3) / 4 * own; at += kEpiThreads)
             {
                 const int    t0 = (at >> (7 - shift)) * 4, f = (first_unit % blocks) * kMxRows + rank * own + (at & (own - 1));
-                const float4 g4 = sum_partial(part, at, shift, 2 * NT), u4 = sum_partial(part + NT * own, at, shift, 2 * NT);
-                const float  g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                const uint32_t chosen = __ballot_sync(0xffffffffu, lane < 4 && t0 + lane < p.tokens && s_weight[t0 + lane] != kNotChosen);
+                if (chosen != 0)
                 {
-                    if (t0 + i < p.tokens)
-                    {
-                        store_token<kFormat>(p, a, t0 + i, f, lane, g[i], u[i], s_weight[t0 + i]);
-                    }
+                    const float4 g4 = sum_partial(part, at, shift, 2 * NT), u4 = sum_partial(part + NT * own, at, shift, 2 * NT);
+                    const float  g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+                    store_hidden<kFormat>(p, a, t0, f, lane, g, u, s_weight, chosen);
                 }
             }
         }
@@ -672,9 +693,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 __syncwarp();
             };
+            // further weights are asked for kAhead chunks before their stage is free: they come from L2 then
+            constexpr int kAhead   = 8;
+            auto          prefetch = [&](int g) {
+                const int i = c_begin + g, a = i / per_expert, c = i - a * per_expert;
+                if (el) tma_prefetch_2d(&tmap_d, c * kMxChunkBytes, s_list[a] * p.hidden + block * kMxRows);
+                __syncwarp();
+            };
             const int mine = c_end - c_begin, early = min(mine, STAGES);
             int       g = 0;
             for (; g < early; ++g) load_weights(g);
+            for (int i = early; i < min(mine, STAGES + kAhead); ++i) prefetch(i);
             griddep_wait();
             for (int i = 0; i < early; ++i) load_tokens(i);
             for (; g < mine; ++g)
@@ -686,6 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 load_weights(g);
                 load_tokens(g);
+                if (g + kAhead < mine) prefetch(g + kAhead);
             }
             if (el && *s_abort != 0)
             {
