@@ -3,8 +3,8 @@
 //   warp 0      TMA: 128 rows of weights (b) and NT rows of tokens (a), 128 bytes (256 elements) of each per stage, and the
 //               scale tiles that belong to them as plain bulk copies
 //   warp 1      copies the stage's scales to tensor memory and issues its MMAs (M = 128, N = NT, K = 64)
-//   warps 2..5  a tensor-memory lane quarter each: accumulator * alpha + bias, rounded once, stored as 32 consecutive
-//               channels per token
+//   warps 2..   a tensor-memory lane quarter each (or half of its columns): accumulator * alpha + bias, rounded once, stored
+//               as 32 consecutive channels per token
 //
 // Every stage has scale columns of its own in tensor memory: they are written again only after the stage's MMAs have been
 // committed, like its shared memory.
@@ -16,9 +16,6 @@ namespace
 {
 constexpr int kMmaWarp  = 1;
 constexpr int kFirstEpi = 2;
-constexpr int kEpiThreads = 128;
-constexpr int kThreads  = 32 * kFirstEpi + kEpiThreads;
-
 struct MxGemmParams
 {
     const uint8_t *w_scales, *t_scales;
@@ -40,6 +37,10 @@ template <int kFormat, int NT, int STAGES, bool kSplit>
 struct MxPlan
 {
     using F                          = MxTraits<kFormat>;
+    // Epilogue warps: one per tensor-memory lane quarter, two where a tile has 64 columns or more (a warp has a scheduler
+    // to itself and waits for its own instructions most of the time).
+    static constexpr int EPI         = NT >= 64 ? 8 : 4;
+    static constexpr int THREADS     = 32 * (kFirstEpi + EPI);
     static constexpr int T_BYTES     = NT * kMxChunkBytes;
     static constexpr int STAGE       = kMxWBytes + T_BYTES;
     static constexpr int SF_STAGE    = 2 * F::kChunkScale;
@@ -120,11 +121,12 @@ __device__ __forceinline__ void store_four(const MxGemmParams &p, int m, int n, 
 }
 
 template <int kFormat, int NT, int STAGES, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS), 2)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ MxGemmParams p)
 {
     using P = MxPlan<kFormat, NT, STAGES, kSplit>;
     using F = MxTraits<kFormat>;
+    constexpr int kEpi = P::EPI;
     extern __shared__ uint8_t smem_raw[];
     uint8_t       *smem      = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t s_stage   = smem_u32(smem);
@@ -162,9 +164,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int a = 0; a < 2; ++a)
         {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 4);
+            mbar_init(tempty_bar(a), kEpi);
         }
-        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kEpi));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     else if (!kSplit)
     {
-        const int q  = warp & 3;
+        const int q = warp & 3, half = (warp - kFirstEpi) >> 2;
         int       it = 0;
         for (int tile = first_tile; tile < tiles; tile += tile_stride, ++it)
         {
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             tc_fence_after();
             const int cols = min(NT, p.tokens - tb * NT);
-            for (int j = 0; j < cols; j += 16)
+            for (int j = 16 * half; j < cols; j += 4 * kEpi)
             {
                 uint32_t r[16];
                 tmem_ld_x16(tmem_base + as * NT + j + (static_cast<uint32_t>(q * 32) << 16), r);
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     {
         const int  tile = first_tile, wb = tile % w_blocks, tb = tile / w_blocks;
         const int  cols = min(NT, p.tokens - tb * NT), shift = 31 - __clz(ranks);
-        const int  q = warp & 3;
+        const int  q = warp & 3, half = (warp - kFirstEpi) >> 2;
         bool       ok = true;
         if (warp >= kFirstEpi)
         {
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         {
             const int      ch = q * 32 + lane;
             const uint32_t to = partial_address(s_part, ch, rank, shift, NT);
-            for (int j = 0; j < cols; j += 16)
+            for (int j = 16 * half; j < cols; j += 4 * kEpi)
             {
                 uint32_t r[16];
                 tmem_ld_x16(tmem_base + j + (static_cast<uint32_t>(q * 32) << 16), r);
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
             if (n < p.channels)
             {
-                for (int at = et; at < (cols + 3) / 4 * own; at += kEpiThreads)
+                for (int at = et; at < (cols + 3) / 4 * own; at += 32 * kEpi)
                 {
                     const int    j = (at >> (7 - shift)) * 4;
                     const float4 v = sum_partial(part, at, shift, NT);
@@ -649,7 +651,7 @@ cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, 
     p.idesc             = mx_idesc(kFormat, kMxRows, NT);
     const int64_t tiles = static_cast<int64_t>((p.channels + kMxRows - 1) / kMxRows) * ((p.tokens + NT - 1) / NT);
     const int grid = kSplit ? static_cast<int>(tiles) * ranks : static_cast<int>(tiles < 2 * ctx->sm_count ? tiles : 2 * ctx->sm_count);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, kSplit ? ranks : 1,
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), P::THREADS, P::DYN_BYTES, kSplit ? ranks : 1,
                                                 tiles, map_w, map_t, p));
     return CUGL_SUCCESS;
 }
@@ -698,7 +700,10 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     {
         return launch_pair<kFormat>(ctx, op, p);
     }
-    const int ranks = mx_split(tiles, chunks, 8);
+    // Sharing K pays until the SMs are busy; the parts of 128 columns cost more to add up (64 KB per CTA).  us with 1 / 2 / 4 / 8
+    // CTAs per tile: 1 x 4096 x 4096 (32 tiles) 7.8 / 5.8 / 4.9 / 5.7, 16 x 4096 x 14336 20.6 / 13.0 / 9.9 / 10.3, 64 x 4096 x 4096
+    // 9.0 / 8.2 / 7.3 / 8.2, 100 x 4096 x 4096 10.1 / 9.5 / 8.9 / 9.9, 256 x 4096 x 4096 (64 tiles) 11.3 / 11.9 / 11.5 / 22.
+    const int ranks = nt < 128 || tiles * 4 <= ctx->sm_count ? mx_split(tiles, chunks, 4) : 1;
     switch (nt)
     {
         case 16: return launch_tokens<kFormat, 16, 4>(ctx, op, p, ranks);

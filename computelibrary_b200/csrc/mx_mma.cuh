@@ -137,12 +137,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  : "memory");
 }
 
-// Asks for a box of a tensor map to be brought into L2.
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int c0, int c1)
-{
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
-}
-
 // The lane that issues a warp's tcgen05 and TMA instructions.  The issuing loops are run by the whole warp and only the
 // instructions themselves are guarded by this predicate: control flow stays uniform, so that descriptors and addresses are
 // computed in uniform registers, which these instructions take their operands from.  Under a branch on the lane index each of
@@ -209,9 +203,10 @@ __device__ __forceinline__ void mx_chunk_scales(uint32_t t_dst, uint32_t sf, int
 // warp that drains 32 lanes of an accumulator writes them to the owners' shared memory, [rank][columns / 4][channel][4 columns],
 // sixteen bytes per lane, and arrives on the owners' barrier; an owner that has all arrivals adds the parts up in the order of
 // the ranks, the same every time.  stride: columns of a part.
-__device__ __forceinline__ int partial_arrivals(int shift) // on an owner's barrier: its channels lie in one warp of each CTA or several
+// warps: of a CTA that drain the accumulator, one or two per lane quarter.  An owner's channels lie in one quarter or several.
+__device__ __forceinline__ int partial_arrivals(int shift, int warps)
 {
-    return (1 << shift) * max(1, (kMxRows >> shift) / 32);
+    return (1 << shift) * max(1, (kMxRows >> shift) / 32) * (warps / 4);
 }
 __device__ __forceinline__ uint32_t partial_address(uint32_t s_base, int ch, int rank, int shift, int stride)
 {
@@ -281,7 +276,7 @@ inline int mx_split(long long tiles, int chunks, int most)
 {
     if (most >= 8 && tiles <= 33 && chunks >= 8) return 8;
     if (most >= 4 && tiles <= 71 && chunks >= 4) return 4;
-    if (tiles <= 148 && chunks >= 2) return 2;
+    if (most >= 2 && tiles <= 148 && chunks >= 2) return 2;
     return 1;
 }
 

@@ -22,8 +22,10 @@ namespace
 {
 constexpr int kMmaWarp  = 1;
 constexpr int kFirstEpi = 2;
-constexpr int kEpiThreads = 128;
-constexpr int kThreads  = 32 * kFirstEpi + kEpiThreads;
+// epilogue warps: two per tensor-memory lane quarter for gate and up (SwiGLU and the re-quantisation are long chains of
+// dependent instructions), one for down
+constexpr int kUpEpi = 8, kDownEpi = 4;
+constexpr int kUpThreads = 32 * (kFirstEpi + kUpEpi), kDownThreads = 32 * (kFirstEpi + kDownEpi);
 constexpr int kMaxTokens = 128, kMaxExperts = 512, kMaxTopK = 16;
 
 struct MoeParams
@@ -193,7 +195,7 @@ __device__ __forceinline__ int active_experts(const MoeParams &p, uint16_t *list
 {
     if (threadIdx.x < kMaxExperts / 32) bits[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.tokens * p.top_k; i += kThreads)
+    for (int i = threadIdx.x; i < p.tokens * p.top_k; i += static_cast<int>(blockDim.x))
     {
         const int e = p.ids[i];
         if (e >= 0) atomicOr(&bits[e >> 5], 1u << (e & 31));
@@ -201,7 +203,7 @@ __device__ __forceinline__ int active_experts(const MoeParams &p, uint16_t *list
     __syncthreads();
     int total = 0;
     for (int w = 0; w < kMaxExperts / 32; ++w) total += __popc(bits[w]);
-    for (int e = threadIdx.x; e < p.experts; e += kThreads)
+    for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
     {
         if ((bits[e >> 5] >> (e & 31)) & 1u)
         {
@@ -256,7 +258,7 @@ __device__ __forceinline__ bool begin_unit(const MoeParams &p, float *table, int
                  "selp.u32 %0, 1, 0, p;\n\t"
                  "}"
                  : "=r"(r)
-                 : "r"(static_cast<uint32_t>(ok)), "n"(kEpiThreads)
+                 : "r"(static_cast<uint32_t>(ok)), "n"(32 * kUpEpi)
                  : "memory");
     return r != 0;
 }
@@ -351,7 +353,7 @@ struct MoePlan
 // Unit of work: 128 rows of one active expert's gate and up matrices, over all tokens.  kSplit: the CTAs of a cluster share a
 // unit's K (few units); else a CTA works through its units, the stages of the next one arriving during the epilogue.
 template <int kFormat, int NT, int STAGES, bool kSplit, int kAcc>
-__global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>::PER_SM)
+__global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>::PER_SM)
     moe_gate_up_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_constant__ CUtensorMap tmap_u, const __grid_constant__ CUtensorMap tmap_x,
                        const __grid_constant__ MoeParams p)
 {
@@ -386,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
         for (int a = 0; a < 2; ++a)
         {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 4);
+            mbar_init(tempty_bar(a), kUpEpi);
         }
-        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kUpEpi));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -503,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
     }
     else if (!kSplit)
     {
-        const int q  = warp & 3;
+        const int q = warp & 3, half = (warp - kFirstEpi) >> 2;
         int       it = 0;
         bool      ok = true;
         for (int unit = first_unit; unit < units; unit += unit_stride, ++it)
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
             ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
-            for (int j = 0; j < p.tokens; j += 16)
+            for (int j = 16 * half; j < p.tokens; j += 4 * kUpEpi)
             {
                 const uint32_t chosen = __ballot_sync(0xffffffffu, lane < 16 && j + lane < p.tokens && weight[j + lane] != kNotChosen);
                 if (chosen == 0) continue;
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
     if constexpr (kSplit)
     {
         const bool work = first_unit < units; // the same in the whole cluster
-        const int  q = warp & 3, shift = 31 - __clz(ranks);
+        const int  q = warp & 3, half = (warp - kFirstEpi) >> 2, shift = 31 - __clz(ranks);
         const int  a = work ? first_unit / blocks : 0;
         bool       ok = work;
         if (warp >= kFirstEpi && work)
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
         {
             const int      ch = q * 32 + lane;
             const uint32_t to = partial_address(smem_u32(smem + P::OFF_PART), ch, rank, shift, 2 * NT);
-            for (int j = 0; j < p.tokens; j += 16)
+            for (int j = 16 * half; j < p.tokens; j += 4 * kUpEpi)
             {
                 uint32_t g[16], u[16];
                 tmem_ld_x16(tmem_base + j + (static_cast<uint32_t>(q * 32) << 16), g);
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
             // a warp takes 32 consecutive channels of four tokens at a time: a rank owns at least 32 (launch_layers)
             const int    own = kMxRows >> shift;
             const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
-            for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < (p.tokens + 3) / 4 * own; at += kEpiThreads)
+            for (int at = (warp - kFirstEpi) * 32 + lane; at - lane < (p.tokens + 3) / 4 * own; at += 32 * kUpEpi)
             {
                 const int    t0 = (at >> (7 - shift)) * 4, f = (first_unit % blocks) * kMxRows + rank * own + (at & (own - 1));
                 const uint32_t chosen = __ballot_sync(0xffffffffu, lane < 4 && t0 + lane < p.tokens && s_weight[t0 + lane] != kNotChosen);
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, MoePlan<kFormat, NT, STAGES, 2, kSpl
 // ---- third launch --------------------------------------------------------------------------------------------
 // Unit of work: 128 output channels; K is (active expert, intermediate), shared by the CTAs of a cluster.
 template <int kFormat, int NT, int STAGES>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kDownThreads, 2)
     moe_down_kernel(const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ MoeParams p)
 {
     using P = MoePlan<kFormat, NT, STAGES, 1, true, 1>;
@@ -642,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(tfull, 1);
-        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks)));
+        mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kDownEpi));
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -693,17 +695,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 __syncwarp();
             };
-            // further weights are asked for kAhead chunks before their stage is free: they come from L2 then
-            constexpr int kAhead   = 8;
-            auto          prefetch = [&](int g) {
-                const int i = c_begin + g, a = i / per_expert, c = i - a * per_expert;
-                if (el) tma_prefetch_2d(&tmap_d, c * kMxChunkBytes, s_list[a] * p.hidden + block * kMxRows);
-                __syncwarp();
-            };
             const int mine = c_end - c_begin, early = min(mine, STAGES);
             int       g = 0;
             for (; g < early; ++g) load_weights(g);
-            for (int i = early; i < min(mine, STAGES + kAhead); ++i) prefetch(i);
             griddep_wait();
             for (int i = 0; i < early; ++i) load_tokens(i);
             for (; g < mine; ++g)
@@ -715,7 +709,6 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 load_weights(g);
                 load_tokens(g);
-                if (g + kAhead < mine) prefetch(g + kAhead);
             }
             if (el && *s_abort != 0)
             {
@@ -792,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
         if (n < p.hidden)
         {
-            for (int at = et; at < (p.tokens + 3) / 4 * own; at += kEpiThreads)
+            for (int at = et; at < (p.tokens + 3) / 4 * own; at += 32 * kDownEpi)
             {
                 const int    j  = (at >> (7 - shift)) * 4;
                 const float4 v4 = sum_partial(part, at, shift, NT);
@@ -905,7 +898,7 @@ cugl_status launch_gate_up(cugl_context *ctx, const MoeMaps &m, const MoeParams 
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int slots = P::PER_SM * ctx->sm_count;
     const int grid  = kSplit ? most_units * ranks : (most_units < slots ? most_units : slots);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, kSplit ? ranks : 1, most_units,
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kUpThreads, P::DYN_BYTES, kSplit ? ranks : 1, most_units,
                                                 m.gate, m.up, m.x, p));
     return CUGL_SUCCESS;
 }
@@ -931,7 +924,7 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int blocks = (p.hidden + kMxRows - 1) / kMxRows, most_chunks = most_active * ((p.inner + kMxChunk - 1) / kMxChunk);
     ranks = mx_split(blocks, most_chunks, 8);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kThreads, P::DYN_BYTES, ranks, blocks * ranks,
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kDownThreads, P::DYN_BYTES, ranks, blocks * ranks,
                                                 m.down, m.h, p));
     return CUGL_SUCCESS;
 }
