@@ -10,6 +10,8 @@
 // committed, like its shared memory.
 #include "mx_mma.cuh"
 
+#include <cstring>
+
 namespace cugl
 {
 namespace
@@ -374,6 +376,9 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
 // Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales.
 // The epilogue drains the shared columns first; the next tile's MMAs start when it has, and the rest of the drain runs beside
 // them.
+// kBulk: two-byte results of 32 channels x 32 tokens are transposed by stmatrix into a warp's staging area and leave as one
+// bulk tensor store (16-byte aligned rows of dst, channels a multiple of 8); a quarter of the instructions of stores from
+// registers.
 constexpr int kPairCols   = 256;
 constexpr int kPairShared = 64;
 constexpr int kPairEpi    = 8; // epilogue warps
@@ -395,10 +400,11 @@ template <int kFormat>
 struct MxPairPlan
 {
     using F                       = MxTraits<kFormat>;
-    static constexpr int STAGES   = kFormat == CUGL_NVFP4 ? 5 : 6;
+    static constexpr int STAGES   = 5;
     static constexpr int STAGE    = 2 * kMxWBytes;
     static constexpr int SF_STAGE = 3 * F::kChunkScale;
-    static constexpr int OFF_SF   = STAGES * STAGE;
+    static constexpr int OFF_OUT  = STAGES * STAGE; // staging: two areas of 32 tokens x 64 bytes per epilogue warp
+    static constexpr int OFF_SF   = OFF_OUT + kPairEpi * 2 * 2048;
     static constexpr int OFF_BAR  = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 3) * 8;
     static constexpr int DYN_BYTES = OFF_MISC + 16 + 1024;
@@ -406,11 +412,32 @@ struct MxPairPlan
     static_assert(SF_COL + 3 * F::kChunkCols <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
 };
 
-template <int kFormat>
+// 32 channels x 32 tokens of an accumulator (two halves of 16 lanes as fragments) to a staging area of 32 rows of 64 bytes in
+// the 64-byte swizzle.  bias: of channels lane / 4 + 8 i.
+template <typename T>
+__device__ __forceinline__ void stage_block(uint32_t s_out, int lane, const uint32_t (&lo)[16], const uint32_t (&hi)[16], float alpha, const float (&bias)[4])
+{
+    auto pack = [&](uint32_t a, uint32_t b, float c) {
+        const T  two[2] = {from_float<T>(__fmaf_rn(__uint_as_float(a), alpha, c)), from_float<T>(__fmaf_rn(__uint_as_float(b), alpha, c))};
+        uint32_t w;
+        memcpy(&w, two, 4);
+        return w;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) // eight tokens: matrix m holds channels 8 m .. 8 m + 7
+    {
+        const int      row  = 8 * i + (lane & 7), chunk = lane >> 3;
+        const uint32_t addr = s_out + static_cast<uint32_t>(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+        stmatrix_x4_trans(addr, pack(lo[4 * i], lo[4 * i + 1], bias[0]), pack(lo[4 * i + 2], lo[4 * i + 3], bias[1]),
+                          pack(hi[4 * i], hi[4 * i + 1], bias[2]), pack(hi[4 * i + 2], hi[4 * i + 3], bias[3]));
+    }
+}
+
+template <int kFormat, bool kBulk>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,
                         const __grid_constant__ CUtensorMap tmap_wsf, const __grid_constant__ CUtensorMap tmap_tsf,
-                        const __grid_constant__ MxGemmParams p)
+                        const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmParams p)
 {
     using P = MxPairPlan<kFormat>;
     using F = MxTraits<kFormat>;
@@ -574,9 +601,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         {
             int wb, tb;
             pair_tile(tile, w_blocks, t_blocks, wb, tb);
-            const int   as = it & 1;
-            const int   n  = (wb * 2 + rank) * kMxRows + q * 32 + lane;
-            const float b  = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
+            const int   as = it & 1, n0 = (wb * 2 + rank) * kMxRows + q * 32;
             if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
                 break;
@@ -584,13 +609,32 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const int      cols = p.tokens - tb * kPairCols;
             const uint32_t acc  = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
+            float          bias[4] = {}; // kBulk: of the fragments' rows, else of this lane's channel
+            if (p.bias != nullptr)
+            {
+#pragma unroll
+                for (int i = 0; i < (kBulk ? 4 : 1); ++i)
+                {
+                    const int n = n0 + (kBulk ? lane / 4 + 8 * i : lane);
+                    bias[i]     = n < p.channels ? __ldg(p.bias + n) : 0.f;
+                }
+            }
 #pragma unroll 1
             for (int i = 0; i < kPairCols / 64; ++i)
             {
                 const int group = 2 * i + half;
                 const int j     = as == 0 ? (group * 32 + kPairCols - kPairShared) % kPairCols : group * 32;
-                uint32_t  r[32];
-                tmem_ld_x32(acc + j, r);
+                uint32_t  r[2][16];
+                if constexpr (kBulk)
+                {
+                    tmem_ld_frag32(acc + j, r[0]);
+                    tmem_ld_frag32(acc + j + (16u << 16), r[1]);
+                }
+                else
+                {
+                    tmem_ld_x16(acc + j, r[0]);
+                    tmem_ld_x16(acc + j + 16, r[1]);
+                }
                 tmem_ld_wait();
                 if (i == 0)
                 {
@@ -598,9 +642,32 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(release);
                 }
-                store_block(p, tb * kPairCols + j, n, r, cols - j, b);
+                if constexpr (kBulk)
+                {
+                    const uint32_t s_out = s_stage + P::OFF_OUT + ((warp - kFirstEpi) * 2 + (i & 1)) * 2048;
+                    if (lane == 0) tma_store_wait_read_but_one(); // the store that read this area two groups ago
+                    __syncwarp();
+                    if (p.dtype == CUGL_F16) stage_block<__half>(s_out, lane, r[0], r[1], p.alpha, bias);
+                    else stage_block<__nv_bfloat16>(s_out, lane, r[0], r[1], p.alpha, bias);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0)
+                    {
+                        if (j < cols && n0 < p.channels) tma_store_2d(&tmap_out, s_out, n0, tb * kPairCols + j);
+                        tma_store_commit();
+                    }
+                }
+                else
+                {
+                    store_block(p, tb * kPairCols + j, n0 + lane, r[0], cols - j, bias[0]);
+                    store_block(p, tb * kPairCols + j + 16, n0 + lane, r[1], cols - j - 16, bias[0]);
+                }
             }
             tc_fence_before();
+        }
+        if (kBulk && lane == 0)
+        {
+            tma_store_wait_all(); // shared memory stays valid until the stores have read it
         }
     }
 
@@ -623,6 +690,18 @@ struct MxOperands
     const cugl_mx_gemm_desc *d;
     const void              *a, *b;
 };
+
+// dst in boxes of 32 tokens x 32 two-byte channels (rows of 64 bytes in the 64-byte swizzle)
+bool encode_dst_map(CUtensorMap *map, const MxGemmParams &p)
+{
+    EncodeTiledFn    fn         = get_encode_fn();
+    const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(p.channels), static_cast<cuuint64_t>(p.tokens)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ldd)};
+    const cuuint32_t box[2]     = {32, 32};
+    const cuuint32_t estr[2]    = {1, 1};
+    return fn != nullptr && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 template <typename K>
 cugl_status allow_smem(cugl_context *ctx, K kernel, int bytes, bool (&set)[64])
@@ -662,27 +741,28 @@ cugl_status launch_tokens(cugl_context *ctx, const MxOperands &op, const MxGemmP
     return ranks > 1 ? launch_one<kFormat, NT, STAGES, true>(ctx, op, p, ranks) : launch_one<kFormat, NT, STAGES, false>(ctx, op, p, 1);
 }
 
-template <int kFormat>
+template <int kFormat, bool kBulk>
 cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
 {
     using P = MxPairPlan<kFormat>;
     using F = MxTraits<kFormat>;
-    CUtensorMap   map_w, map_t, map_wsf, map_tsf;
+    CUtensorMap   map_w, map_t, map_wsf, map_tsf, map_out{};
     const int64_t inner = (static_cast<int64_t>(p.K) + 1) / 2;
     const int64_t w_tiles = (static_cast<int64_t>(p.channels) + 127) / 128 * p.k_tiles, t_tiles = (static_cast<int64_t>(p.tokens) + 127) / 128 * p.k_tiles;
     if (!encode_packed_map(&map_w, op.b, p.channels, inner, op.d->ldb, kMxRows) || !encode_packed_map(&map_t, op.a, p.tokens, inner, op.d->lda, kMxRows) ||
-        !encode_scale_map(&map_wsf, p.w_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_tsf, p.t_scales, t_tiles, F::kChunkTiles))
+        !encode_scale_map(&map_wsf, p.w_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_tsf, p.t_scales, t_tiles, F::kChunkTiles) ||
+        (kBulk && !encode_dst_map(&map_out, p)))
     {
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for an operand");
     }
-    auto        kernel  = mx_gemm_pair_kernel<kFormat>;
+    auto        kernel  = mx_gemm_pair_kernel<kFormat, kBulk>;
     static bool set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc = mx_idesc(kFormat, 2 * kMxRows, kPairCols);
     const int64_t   tiles = static_cast<int64_t>((p.channels + 255) / 256) * ((p.tokens + 255) / 256);
     const long long pairs = tiles < ctx->sm_count / 2 ? tiles : ctx->sm_count / 2;
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(2 * pairs)), kPairThreads, P::DYN_BYTES, 2, 2 * tiles, map_w, map_t,
-                                                map_wsf, map_tsf, p));
+                                                map_wsf, map_tsf, map_out, p));
     return CUGL_SUCCESS;
 }
 
@@ -698,7 +778,10 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     }
     if (p.tokens > 128 && tiles > ctx->sm_count)
     {
-        return launch_pair<kFormat>(ctx, op, p);
+        // a bulk store wants 16-byte aligned rows and clips at the end of a row in whole 16-byte units
+        const bool bulk = p.dtype != CUGL_F32 && ((reinterpret_cast<uintptr_t>(p.dst) | static_cast<uintptr_t>(p.ldd)) & 15) == 0 && p.channels % 8 == 0 &&
+                          p.ldd < (1ll << 40);
+        return bulk ? launch_pair<kFormat, true>(ctx, op, p) : launch_pair<kFormat, false>(ctx, op, p);
     }
     // Sharing K pays until the SMs are busy; the parts of 128 columns cost more to add up (64 KB per CTA).  us with 1 / 2 / 4 / 8
     // CTAs per tile: 1 x 4096 x 4096 (32 tiles) 7.8 / 5.8 / 4.9 / 5.7, 16 x 4096 x 14336 20.6 / 13.0 / 9.9 / 10.3, 64 x 4096 x 4096

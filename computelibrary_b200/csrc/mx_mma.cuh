@@ -158,6 +158,24 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, limit));
 }
 
+// 16 accumulator lanes x 32 columns in the fragment layout of the matrix instructions: v[4 i + 0, 1] are columns 8 i + 2 (lane % 4)
+// and the next of row lane / 4, v[4 i + 2, 3] the same columns of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values, transposed on the way to shared memory: lane l gives the address of row l % 8 of the
+// transposed matrix l / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // Waits for a barrier's phase whatever the abort flag says: a producer that gives up lets its copies in flight land first.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, long long limit)
 {
