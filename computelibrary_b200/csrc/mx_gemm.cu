@@ -376,9 +376,9 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
 // Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales.
 // The epilogue drains the shared columns first; the next tile's MMAs start when it has, and the rest of the drain runs beside
 // them.
-// kBulk: two-byte results of 32 channels x 32 tokens are transposed by stmatrix into a warp's staging area and leave as one
-// bulk tensor store (16-byte aligned rows of dst, channels a multiple of 8); a quarter of the instructions of stores from
-// registers.
+// kBulk: blocks of 32 channels x 32 tokens leave through a warp's staging area as one bulk tensor store (rows of dst 16-byte
+// aligned and whole 16-byte units long); two-byte results (kBulk = 2) are transposed by stmatrix on the way, floats (4) are
+// stored as they lie.  A quarter of the instructions of stores from registers: 4096 x 14336 x 1024 to BF16 73 -> 44 us.
 constexpr int kPairCols   = 256;
 constexpr int kPairShared = 64;
 constexpr int kPairEpi    = 8; // epilogue warps
@@ -403,8 +403,8 @@ struct MxPairPlan
     static constexpr int STAGES   = 5;
     static constexpr int STAGE    = 2 * kMxWBytes;
     static constexpr int SF_STAGE = 3 * F::kChunkScale;
-    static constexpr int OFF_OUT  = STAGES * STAGE; // staging: two areas of 32 tokens x 64 bytes per epilogue warp
-    static constexpr int OFF_SF   = OFF_OUT + kPairEpi * 2 * 2048;
+    static constexpr int OFF_OUT  = STAGES * STAGE; // staging: 4 KB per epilogue warp
+    static constexpr int OFF_SF   = OFF_OUT + kPairEpi * 4096;
     static constexpr int OFF_BAR  = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 3) * 8;
     static constexpr int DYN_BYTES = OFF_MISC + 16 + 1024;
@@ -433,7 +433,7 @@ __device__ __forceinline__ void stage_block(uint32_t s_out, int lane, const uint
     }
 }
 
-template <int kFormat, bool kBulk>
+template <int kFormat, int kBulk>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,
                         const __grid_constant__ CUtensorMap tmap_wsf, const __grid_constant__ CUtensorMap tmap_tsf,
@@ -609,13 +609,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const int      cols = p.tokens - tb * kPairCols;
             const uint32_t acc  = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
-            float          bias[4] = {}; // kBulk: of the fragments' rows, else of this lane's channel
+            float          bias[4] = {}; // kBulk = 2: of the fragments' rows, else of this lane's channel
             if (p.bias != nullptr)
             {
 #pragma unroll
-                for (int i = 0; i < (kBulk ? 4 : 1); ++i)
+                for (int i = 0; i < (kBulk == 2 ? 4 : 1); ++i)
                 {
-                    const int n = n0 + (kBulk ? lane / 4 + 8 * i : lane);
+                    const int n = n0 + (kBulk == 2 ? lane / 4 + 8 * i : lane);
                     bias[i]     = n < p.channels ? __ldg(p.bias + n) : 0.f;
                 }
             }
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const int group = 2 * i + half;
                 const int j     = as == 0 ? (group * 32 + kPairCols - kPairShared) % kPairCols : group * 32;
                 uint32_t  r[2][16];
-                if constexpr (kBulk)
+                if constexpr (kBulk == 2)
                 {
                     tmem_ld_frag32(acc + j, r[0]);
                     tmem_ld_frag32(acc + j + (16u << 16), r[1]);
@@ -642,12 +642,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(release);
                 }
-                if constexpr (kBulk)
+                if constexpr (kBulk != 0)
                 {
-                    const uint32_t s_out = s_stage + P::OFF_OUT + ((warp - kFirstEpi) * 2 + (i & 1)) * 2048;
-                    if (lane == 0) tma_store_wait_read_but_one(); // the store that read this area two groups ago
+                    // two-byte results: two areas in turn; floats: one
+                    const int      area  = (warp - kFirstEpi) * 4096 + (kBulk == 2 ? (i & 1) * 2048 : 0);
+                    const uint32_t s_out = s_stage + P::OFF_OUT + area;
+                    if (lane == 0) // the store that reads this area has done so
+                    {
+                        if (kBulk == 2) tma_store_wait_read_but_one();
+                        else tma_store_wait_read();
+                    }
                     __syncwarp();
-                    if (p.dtype == CUGL_F16) stage_block<__half>(s_out, lane, r[0], r[1], p.alpha, bias);
+                    if constexpr (kBulk == 4)
+                    {
+                        float *out = reinterpret_cast<float *>(smem + P::OFF_OUT + area) + lane;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) out[32 * k] = __fmaf_rn(__uint_as_float(r[k / 16][k % 16]), p.alpha, bias[0]);
+                    }
+                    else if (p.dtype == CUGL_F16) stage_block<__half>(s_out, lane, r[0], r[1], p.alpha, bias);
                     else stage_block<__nv_bfloat16>(s_out, lane, r[0], r[1], p.alpha, bias);
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -665,7 +677,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
             tc_fence_before();
         }
-        if (kBulk && lane == 0)
+        if (kBulk != 0 && lane == 0)
         {
             tma_store_wait_all(); // shared memory stays valid until the stores have read it
         }
@@ -691,7 +703,7 @@ struct MxOperands
     const void              *a, *b;
 };
 
-// dst in boxes of 32 tokens x 32 two-byte channels (rows of 64 bytes in the 64-byte swizzle)
+// dst in boxes of 32 tokens x 32 channels: rows of 64 bytes in the 64-byte swizzle, or of 128 bytes
 bool encode_dst_map(CUtensorMap *map, const MxGemmParams &p)
 {
     EncodeTiledFn    fn         = get_encode_fn();
@@ -699,8 +711,8 @@ bool encode_dst_map(CUtensorMap *map, const MxGemmParams &p)
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ldd)};
     const cuuint32_t box[2]     = {32, 32};
     const cuuint32_t estr[2]    = {1, 1};
-    return fn != nullptr && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return fn != nullptr && fn(map, p.dtype == CUGL_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, p.dtype == CUGL_F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename K>
@@ -741,7 +753,7 @@ cugl_status launch_tokens(cugl_context *ctx, const MxOperands &op, const MxGemmP
     return ranks > 1 ? launch_one<kFormat, NT, STAGES, true>(ctx, op, p, ranks) : launch_one<kFormat, NT, STAGES, false>(ctx, op, p, 1);
 }
 
-template <int kFormat, bool kBulk>
+template <int kFormat, int kBulk>
 cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
 {
     using P = MxPairPlan<kFormat>;
@@ -751,7 +763,7 @@ cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
     const int64_t w_tiles = (static_cast<int64_t>(p.channels) + 127) / 128 * p.k_tiles, t_tiles = (static_cast<int64_t>(p.tokens) + 127) / 128 * p.k_tiles;
     if (!encode_packed_map(&map_w, op.b, p.channels, inner, op.d->ldb, kMxRows) || !encode_packed_map(&map_t, op.a, p.tokens, inner, op.d->lda, kMxRows) ||
         !encode_scale_map(&map_wsf, p.w_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_tsf, p.t_scales, t_tiles, F::kChunkTiles) ||
-        (kBulk && !encode_dst_map(&map_out, p)))
+        (kBulk != 0 && !encode_dst_map(&map_out, p)))
     {
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for an operand");
     }
@@ -776,12 +788,23 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     {
         return fail(ctx, CUGL_INVALID_ARGUMENT, "cugl_mx_gemm: more than 2^28 output tiles");
     }
-    if (p.tokens > 128 && tiles > ctx->sm_count)
+    if (p.tokens > 128 && (tiles >= 128 || (tiles >= 64 && chunks >= 8)))
     {
-        // a bulk store wants 16-byte aligned rows and clips at the end of a row in whole 16-byte units
-        const bool bulk = p.dtype != CUGL_F32 && ((reinterpret_cast<uintptr_t>(p.dst) | static_cast<uintptr_t>(p.ldd)) & 15) == 0 && p.channels % 8 == 0 &&
+        // us on one CTA per tile / an SM pair: 256 x 4096 x 4096 (64 tiles) 11.3 / 10.1, 256 x 7168 x 4096 12.5 / 11.0, 512 x 14336 x 4096
+        // 23.2 / 18.7, 2048 x 4096 x 512 9.6 / 8.5; 1024 x 1024 x 1024 (64 tiles) 5.6 / 6.0, 150 x 2048 x 14336 (32 tiles, shared K)
+        // 13.8 / 21.3.  Without bulk stores the pair's epilogue is the slower one unless K is long: F32 2048 x 4096 x 1024 12.6 / 16.4.
+        // A bulk store wants 16-byte aligned rows and clips at the end of a row in whole 16-byte units.
+        const int  size = dtype_size(p.dtype);
+        const bool bulk = ((reinterpret_cast<uintptr_t>(p.dst) | static_cast<uintptr_t>(p.ldd)) & 15) == 0 && p.channels * static_cast<int64_t>(size) % 16 == 0 &&
                           p.ldd < (1ll << 40);
-        return bulk ? launch_pair<kFormat, true>(ctx, op, p) : launch_pair<kFormat, false>(ctx, op, p);
+        if (bulk)
+        {
+            return size == 4 ? launch_pair<kFormat, 4>(ctx, op, p) : launch_pair<kFormat, 2>(ctx, op, p);
+        }
+        if (tiles >= 2 * ctx->sm_count && chunks >= 16)
+        {
+            return launch_pair<kFormat, 0>(ctx, op, p);
+        }
     }
     // Sharing K pays until the SMs are busy; the parts of 128 columns cost more to add up (64 KB per CTA).  us with 1 / 2 / 4 / 8
     // CTAs per tile: 1 x 4096 x 4096 (32 tiles) 7.8 / 5.8 / 4.9 / 5.7, 16 x 4096 x 14336 20.6 / 13.0 / 9.9 / 10.3, 64 x 4096 x 4096
