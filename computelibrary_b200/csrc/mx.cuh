@@ -109,20 +109,20 @@ __device__ __forceinline__ void unpack_e2m1x8(uint32_t w, __half2 (&h)[4])
 struct MxScale
 {
     uint32_t byte;
-    float    mul;  // MXFP4: 1 / scale.  NVFP4: 2^-exponent / scale, rounded up (scale_to_code)
-    float    div;  // NVFP4: the scale itself (f32 sources divide)
+    float    mul;  // MXFP4: 1 / scale.  NVFP4: 2^-exponent / scale, rounded up, or to nearest where the source has 32 bits
+    float    unit; // NVFP4, 32 bits: scale * 2^exponent, what a code of 1 stands for
 };
 // kExact false: values that were computed in float just now and carry its error; a product with 1 / 6 instead of the division.
-template <int kFormat, bool kExact = true>
+template <int kFormat, bool kWide = false, bool kExact = true>
 __device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponent_mul)
 {
     MxScale s;
+    s.unit = 0.f;
     if (kFormat == CUGL_MXFP4)
     {
         const uint32_t e = amax_bits >> 23;
         s.byte           = e > 2 ? e - 2 : 0;
         s.mul            = __uint_as_float((254 - s.byte) << 23);
-        s.div            = 0.f;
         if (amax_bits >= 0x7f800000u)
         {
             s.byte = 255;
@@ -130,18 +130,19 @@ __device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponen
         }
         return s;
     }
-    const float                amax = __uint_as_float(amax_bits) * exponent_mul;
-    const float                v    = fminf(fmaxf(kExact ? __fdiv_rn(amax, 6.f) : amax * (1.f / 6.f), 0x1p-9f), 448.f);
+    const float                amax = fminf(__uint_as_float(amax_bits) * exponent_mul, 4096.f); // all above 6 * 448 saturate alike
+    float                      v    = amax * (1.f / 6.f);
+    if (kExact) v                   = __fmaf_rn(__fmaf_rn(-6.f, v, amax), 1.f / 6.f, v); // correctly rounded, see scale_to_codes
+    v                               = fminf(fmaxf(v, 0x1p-9f), 448.f);
     const __nv_fp8_storage_t   b    = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
     const float                f    = __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
     s.byte                          = b;
-    s.div                           = f;
-    s.mul                           = __frcp_ru(f) * exponent_mul;
+    s.mul                           = (kWide ? __frcp_rn(f) : __frcp_ru(f)) * exponent_mul;
+    if (kWide) s.unit               = f * __uint_as_float((254u << 23) - __float_as_uint(exponent_mul)); // exponent_mul: a power of two
     if (amax_bits == 0 || amax_bits >= 0x7f800000u)
     {
         s.byte = amax_bits == 0 ? 0 : 0x7f;
         s.mul  = 0.f;
-        s.div  = 0.f;
     }
     return s;
 }
@@ -151,19 +152,30 @@ __device__ __forceinline__ MxScale mx_scale_of(uint32_t amax_bits, float exponen
 //   NVFP4, 16 bits   the reciprocal rounded up times the value, rounded towards zero: for every scale (four bits) and every
 //                    value of up to eleven bits it compares with each midpoint of E2M1 as the exact quotient does (checked
 //                    for all of them); one instruction
-//   NVFP4, 32 bits   a division: as for the scale, a quotient that is no midpoint does not round onto one
-template <int kFormat, bool kWide>
-__device__ __forceinline__ float scale_to_code(float v, const MxScale &s, float exponent_mul)
+//   NVFP4, 32 bits   the correctly rounded quotient: as for the scale, a quotient that is no midpoint does not round onto one.
+//                    Product with the reciprocal and one correction by the exact remainder (Markstein, Computation of
+//                    elementary functions on the IBM RISC System/6000 processor, 1990).  A saturated block is bounded first:
+//                    its products may overflow.
+template <int kFormat, bool kWide, int kCount>
+__device__ __forceinline__ void scale_to_codes(float (&v)[kCount], const MxScale &s)
 {
-    if (kFormat == CUGL_MXFP4)
+    if (kFormat == CUGL_NVFP4 && kWide)
     {
-        return v * s.mul;
+        if (s.byte == 0x7e)
+        {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) v[i] = fminf(fmaxf(v[i], -8.f * s.unit), 8.f * s.unit);
+        }
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+        {
+            const float q = __fmul_rn(v[i], s.mul);
+            v[i]          = __fmaf_rn(__fmaf_rn(-q, s.unit, v[i]), s.mul, q);
+        }
+        return;
     }
-    if (kWide)
-    {
-        return s.div != 0.f ? __fdiv_rn(v * exponent_mul, s.div) : 0.f;
-    }
-    return __fmul_rz(v, s.mul);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] = kFormat == CUGL_MXFP4 ? v[i] * s.mul : __fmul_rz(v[i], s.mul);
 }
 
 // The value of a scale byte.

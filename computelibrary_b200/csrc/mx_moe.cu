@@ -164,8 +164,7 @@ __device__ __forceinline__ void quantize_tokens(const MoeParams &p, int block, i
     }
     if (c0 < p.hidden)
     {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = scale_to_code<kFormat, false>(v[i], s, p.x_mul);
+        scale_to_codes<kFormat, false>(v, s);
         *reinterpret_cast<uint2 *>(p.xq + row * p.ld_xq + c0 / 2) = make_uint2(pack_e2m1x8(v), pack_e2m1x8(v + 8));
     }
 }
@@ -298,7 +297,7 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t0, 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        s[i] = mx_scale_of<kFormat, false>(amax[i], p.h_mul); // h carries the error of float sums: no exact quotients
+        s[i] = mx_scale_of<kFormat, false, false>(amax[i], p.h_mul); // h carries the error of float sums: no exact quotients
         w[i] = (static_cast<uint32_t>(__nv_cvt_float_to_fp4(h[i] * s[i].mul, __NV_E2M1, cudaRoundNearest)) & 15u) << (4 * (lane & 7));
     }
 #pragma unroll

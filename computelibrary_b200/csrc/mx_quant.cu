@@ -4,45 +4,96 @@
 
 #include <cmath>
 #include <cstring>
-#include <utility>
 
 namespace cugl
 {
 namespace
 {
 constexpr int kWarps = 8;
+constexpr int kLaneCols = 8;               // consecutive columns of a lane
+constexpr int kItemCols = 32 * kLaneCols;  // columns of a warp
 
-// Sixteen consecutive values of a row as floats, and the bits of the largest |value|.
+struct QuantParams
+{
+    const uint8_t *src;
+    uint8_t       *dst, *scales;
+    int64_t        ld, ld_packed, tiles; // bytes, bytes, scale tiles along a row
+    int            rows, cols, groups;   // groups of rows: what a block takes at a time
+    int            lane_shift;           // 2^lane_shift lanes of a warp share a row
+    float          exponent_mul;
+    int            vec_plain, vec_packed; // the plain matrix is 16-byte aligned, the packed one 4-byte
+};
+
+// What a warp takes: kRows rows (or groups of narrow rows) of kSegs segments of 256 columns.  Segments lie 256 columns apart at
+// addresses that differ by constants, so that a row's address is computed once.
+struct Place
+{
+    int row, step; // first row, rows between items
+    int c0;        // first column of the first segment
+};
+template <int kSegs, int kRows>
+__device__ __forceinline__ Place place_of(const QuantParams &p, int group, int lane)
+{
+    Place q;
+    q.step = 32 >> p.lane_shift;
+    q.row  = (group * kWarps + static_cast<int>(threadIdx.x >> 5)) * kRows * q.step + (lane >> p.lane_shift);
+    q.c0   = static_cast<int>(blockIdx.x) * kSegs * kItemCols + (lane & ((1 << p.lane_shift) - 1)) * kLaneCols;
+    return q;
+}
+
+// Rows that start anywhere: a warp moves its 256 values as consecutive elements and turns them over in shared memory, where a
+// lane's eight lie in a row.  row: of lane 0's columns; c0: the segment's first column.
 template <typename T>
-__device__ __forceinline__ uint32_t load16(const T *p, float (&v)[16])
+__device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c0, int lane, T *area)
+{
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kLaneCols; ++i)
+    {
+        const int at = i * 32 + lane, l = at / kLaneCols, r = row + (l >> p.lane_shift);
+        const int c  = c0 + (l & ((1 << p.lane_shift) - 1)) * kLaneCols + at % kLaneCols;
+        T         v  = from_float<T>(0.f);
+        if (r < p.rows && c < p.cols) v = reinterpret_cast<const T *>(p.src + r * p.ld)[c];
+        area[at] = v;
+    }
+    __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void store_ragged(const QuantParams &p, int row, int c0, int lane, const T *area)
+{
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kLaneCols; ++i)
+    {
+        const int at = i * 32 + lane, l = at / kLaneCols, r = row + (l >> p.lane_shift);
+        const int c  = c0 + (l & ((1 << p.lane_shift) - 1)) * kLaneCols + at % kLaneCols;
+        if (r < p.rows && c < p.cols) reinterpret_cast<T *>(p.dst + r * p.ld)[c] = area[at];
+    }
+    __syncwarp();
+}
+
+// The bits of the largest |value| of eight (NaN above infinity above all others), and the values as floats.
+template <typename T>
+__device__ __forceinline__ uint32_t widen(const uint4 (&raw)[sizeof(T) / 2], float (&v)[kLaneCols])
 {
     uint32_t m = 0;
     if constexpr (sizeof(T) == 4)
     {
+        memcpy(v, raw, sizeof(v));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-            const float4 q = __ldg(reinterpret_cast<const float4 *>(p) + i);
-            v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int i = 0; i < kLaneCols; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
     }
     else
     {
-        uint32_t    w[8];
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 4; ++i)
         {
             m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-            T lo, hi;
-            const uint16_t l = static_cast<uint16_t>(w[i]), h = static_cast<uint16_t>(w[i] >> 16);
-            memcpy(&lo, &l, 2);
-            memcpy(&hi, &h, 2);
-            v[2 * i]     = to_float(lo);
-            v[2 * i + 1] = to_float(hi);
+            T two[2];
+            memcpy(two, &w[i], 4);
+            v[2 * i]     = to_float(two[0]);
+            v[2 * i + 1] = to_float(two[1]);
         }
         const uint16_t top = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
         T              t;
@@ -51,151 +102,179 @@ __device__ __forceinline__ uint32_t load16(const T *p, float (&v)[16])
     }
     return m;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t load16_part(const T *p, int n, float (&v)[16])
+
+// A lane owns eight columns of a segment: half an NVFP4 block or a quarter of an MXFP4 one; the largest value and the scale bytes
+// of four blocks are gathered by shuffles, and the bytes leave as one word of their tile.  A warp has the loads of all its
+// segments in flight.
+template <typename T, int kFormat, bool kVec, int kSegs, int kRows>
+__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const __grid_constant__ QuantParams p)
 {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
+    constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
+    constexpr int kLanes = kBlock / kLaneCols; // of a block
+    constexpr int kLoads = sizeof(T) / 2;
+    constexpr int kTiles = kItemCols / (4 * kBlock); // scale tiles of a segment
+    __shared__ __align__(16) T areas[kVec ? 1 : kWarps][kVec ? 8 : kItemCols];
+    dependent_prologue();
+    const int lane = threadIdx.x & 31;
+    for (int group = blockIdx.y; group < p.groups; group += gridDim.y)
     {
-        v[i] = i < n ? to_float(p[i]) : 0.f;
-        m    = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        const Place at = place_of<kSegs, kRows>(p, group, lane);
+        uint4       raw[kRows][kSegs][kLoads];
+        if constexpr (kVec)
+        {
+#pragma unroll
+            for (int u = 0; u < kRows; ++u)
+            {
+                const int row = at.row + u * at.step;
+                const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + at.c0;
+#pragma unroll
+                for (int g = 0; g < kSegs; ++g)
+                {
+                    const int n = row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
+#pragma unroll
+                    for (int l = 0; l < kLoads; ++l)
+                    {
+                        raw[u][g][l] = make_uint4(0, 0, 0, 0);
+                        if (n >= kLaneCols) raw[u][g][l] = __ldg(reinterpret_cast<const uint4 *>(src + g * kItemCols) + l);
+                    }
+                    if (n > 0 && n < kLaneCols)
+                    {
+                        T part[kLaneCols];
+#pragma unroll
+                        for (int i = 0; i < kLaneCols; ++i) part[i] = i < n ? src[g * kItemCols + i] : from_float<T>(0.f);
+                        memcpy(raw[u][g], part, sizeof(part));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+        {
+            const int      row    = at.row + u * at.step;
+            const int      block  = at.c0 / kBlock;
+            uint8_t *const scales = p.scales + mx_scale_offset(row, block, p.tiles);
+            uint8_t *const dst    = p.dst + row * p.ld_packed + at.c0 / 2;
+#pragma unroll
+            for (int g = 0; g < kSegs; ++g)
+            {
+                if constexpr (!kVec)
+                {
+                    T *area = areas[threadIdx.x >> 5];
+                    load_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
+#pragma unroll
+                    for (int l = 0; l < kLoads; ++l) raw[u][g][l] = reinterpret_cast<const uint4 *>(area + lane * kLaneCols)[l];
+                }
+                float    v[kLaneCols];
+                uint32_t amax = widen<T>(raw[u][g], v);
+#pragma unroll
+                for (int o = 1; o < kLanes; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const MxScale s    = mx_scale_of<kFormat, sizeof(T) == 4>(amax, p.exponent_mul);
+                uint32_t      word = s.byte << (8 * ((lane / kLanes) & 3));
+                word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
+                word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
+                scale_to_codes<kFormat, sizeof(T) == 4>(v, s);
+                const uint32_t w = pack_e2m1x8(v);
+                const int      n = p.cols - at.c0 - g * kItemCols;
+                if (row < p.rows)
+                {
+                    if ((lane & (4 * kLanes - 1)) == 0 && block + g * 4 * kTiles < 4 * p.tiles)
+                    {
+                        *reinterpret_cast<uint32_t *>(scales + g * kTiles * kMxTileBytes) = word; // blocks behind the row: 0
+                    }
+                    uint8_t *d = dst + g * kItemCols / 2;
+                    if (n >= kLaneCols && p.vec_packed != 0)
+                    {
+                        *reinterpret_cast<uint32_t *>(d) = w;
+                    }
+                    else
+                    {
+                        for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) d[i] = static_cast<uint8_t>(w >> (8 * i)); // the half byte behind an odd row is 0
+                    }
+                }
+            }
+        }
     }
-    return m;
 }
 
-struct QuantParams
+template <typename T, int kFormat, bool kVec, int kSegs, int kRows>
+__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const __grid_constant__ QuantParams p)
 {
-    const void *src;
-    uint8_t    *dst, *scales;
-    int64_t     ld, ld_packed, tiles; // bytes, bytes, scale tiles along a row
-    int         rows, cols;
-    int         chunks;     // pieces of sixteen columns a row is walked in: whole scale tiles
-    int         lane_shift; // 2^lane_shift lanes of a warp share a row
-    float       exponent_mul;
-    int         vec_src, vec_dst; // 16-byte loads / 8-byte stores are aligned
-};
-
-// A lane owns sixteen columns: one NVFP4 block, or half an MXFP4 block whose other half is the neighbouring lane's.  The scale
-// bytes of four blocks are gathered by shuffles and leave as one word of their tile.
-template <typename T, int kFormat>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantParams p)
-{
+    constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
+    constexpr int kTiles = kItemCols / (4 * kBlock); // scale tiles of a segment
+    __shared__ __align__(16) T areas[kVec ? 1 : kWarps][kVec ? 8 : kItemCols];
     dependent_prologue();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per_row  = 1 << p.lane_shift;
-    const int rows_per = 32 >> p.lane_shift;
-    const int sub      = lane >> p.lane_shift;
-    const int chunk    = blockIdx.x * per_row + (lane & (per_row - 1));
-    const int c0       = chunk * 16;
-    const int n        = min(16, p.cols - c0); // <= 0: behind the row, only the tile's zero scales
-    for (int64_t row = (static_cast<int64_t>(blockIdx.y) * kWarps + warp) * rows_per + sub; __any_sync(0xffffffffu, row < p.rows);
-         row += static_cast<int64_t>(gridDim.y) * kWarps * rows_per)
+    const int lane = threadIdx.x & 31;
+    for (int group = blockIdx.y; group < p.groups; group += gridDim.y)
     {
-        const bool in = row < p.rows && chunk < p.chunks;
-        float      v[16];
-        uint32_t   amax = 0;
-        if (in && n > 0)
-        {
-            const T *src = reinterpret_cast<const T *>(static_cast<const uint8_t *>(p.src) + row * p.ld) + c0;
-            amax         = (n == 16 && p.vec_src != 0) ? load16(src, v) : load16_part(src, n, v);
-        }
-        constexpr int kLanesPerBlock = kFormat == CUGL_NVFP4 ? 1 : 2;
-        if (kLanesPerBlock == 2)
-        {
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        }
-        const MxScale s = mx_scale_of<kFormat>(amax, p.exponent_mul);
-        uint32_t      word = s.byte << (8 * ((lane / kLanesPerBlock) & 3));
-        word |= __shfl_xor_sync(0xffffffffu, word, kLanesPerBlock);
-        word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanesPerBlock);
-        if (!in)
-        {
-            continue;
-        }
-        if ((chunk & (4 * kLanesPerBlock - 1)) == 0)
-        {
-            *reinterpret_cast<uint32_t *>(p.scales + mx_scale_offset(row, chunk / kLanesPerBlock, p.tiles)) = word;
-        }
-        if (n > 0)
-        {
+        const Place at = place_of<kSegs, kRows>(p, group, lane);
+        uint32_t    w[kRows][kSegs], byte[kRows][kSegs];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = scale_to_code<kFormat, sizeof(T) == 4>(v[i], s, p.exponent_mul);
-            const uint32_t lo = pack_e2m1x8(v), hi = pack_e2m1x8(v + 8);
-            uint8_t       *d  = p.dst + row * p.ld_packed + c0 / 2;
-            if (n == 16 && p.vec_dst != 0)
+        for (int u = 0; u < kRows; ++u)
+        {
+            const int      row    = at.row + u * at.step;
+            const uint8_t *src    = p.src + row * p.ld_packed + at.c0 / 2;
+            const uint8_t *scales = p.scales + mx_scale_offset(row, at.c0 / kBlock, p.tiles);
+#pragma unroll
+            for (int g = 0; g < kSegs; ++g)
             {
-                *reinterpret_cast<uint2 *>(d) = make_uint2(lo, hi);
-            }
-            else
-            {
-                const uint64_t w = (static_cast<uint64_t>(hi) << 32) | lo;
-                for (int i = 0; i < (n + 1) / 2; ++i) d[i] = static_cast<uint8_t>(w >> (8 * i)); // values behind the row count as 0
+                const int n = row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
+                w[u][g] = byte[u][g] = 0;
+                if (n > 0) byte[u][g] = __ldg(scales + g * kTiles * kMxTileBytes);
+                if (n >= kLaneCols && p.vec_packed != 0)
+                {
+                    w[u][g] = __ldg(reinterpret_cast<const uint32_t *>(src + g * kItemCols / 2));
+                }
+                else
+                {
+                    for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) w[u][g] |= static_cast<uint32_t>(__ldg(src + g * kItemCols / 2 + i)) << (8 * i);
+                }
             }
         }
-    }
-}
-
-template <typename T, int kFormat>
-__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const QuantParams p, void *out)
-{
-    dependent_prologue();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per_row  = 1 << p.lane_shift;
-    const int rows_per = 32 >> p.lane_shift;
-    const int chunk    = blockIdx.x * per_row + (lane & (per_row - 1));
-    const int c0       = chunk * 16;
-    const int n        = min(16, p.cols - c0);
-    if (n <= 0)
-    {
-        return;
-    }
-    for (int64_t row = (static_cast<int64_t>(blockIdx.y) * kWarps + warp) * rows_per + (lane >> p.lane_shift); row < p.rows;
-         row += static_cast<int64_t>(gridDim.y) * kWarps * rows_per)
-    {
-        const uint8_t *src = static_cast<const uint8_t *>(p.src) + row * p.ld_packed + c0 / 2;
-        uint32_t       w[2];
-        if (n == 16 && p.vec_src != 0)
-        {
-            const uint2 q = __ldg(reinterpret_cast<const uint2 *>(src));
-            w[0] = q.x, w[1] = q.y;
-        }
-        else
-        {
-            uint64_t q = 0;
-            for (int i = 0; i < (n + 1) / 2; ++i) q |= static_cast<uint64_t>(__ldg(src + i)) << (8 * i);
-            w[0] = static_cast<uint32_t>(q), w[1] = static_cast<uint32_t>(q >> 32);
-        }
-        const int   block = kFormat == CUGL_NVFP4 ? chunk : chunk >> 1;
-        const float s     = mx_scale_value<kFormat>(__ldg(p.scales + mx_scale_offset(row, block, p.tiles))) * p.exponent_mul;
-        T           v[16];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int u = 0; u < kRows; ++u)
         {
-            __half2 h[4];
-            unpack_e2m1x8(w[j], h);
+            const int row = at.row + u * at.step;
+            T        *dst = reinterpret_cast<T *>(p.dst + row * p.ld) + at.c0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int g = 0; g < kSegs; ++g)
             {
-                const float2 f         = __half22float2(h[i]);
-                v[8 * j + 2 * i]     = from_float<T>(f.x * s);
-                v[8 * j + 2 * i + 1] = from_float<T>(f.y * s);
-            }
-        }
-        T *dst = reinterpret_cast<T *>(static_cast<uint8_t *>(out) + row * p.ld) + c0;
-        if (n == 16 && p.vec_dst != 0)
-        {
-            uint4 q[sizeof(T)];
-            memcpy(q, v, sizeof(v));
+                const float s = mx_scale_value<kFormat>(byte[u][g]) * p.exponent_mul;
+                __half2     h[4];
+                unpack_e2m1x8(w[u][g], h);
+                T v[kLaneCols];
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) reinterpret_cast<uint4 *>(dst)[i] = q[i];
-        }
-        else
-        {
+                for (int i = 0; i < 4; ++i)
+                {
+                    const float2 f = __half22float2(h[i]);
+                    v[2 * i]       = from_float<T>(f.x * s);
+                    v[2 * i + 1]   = from_float<T>(f.y * s);
+                }
+                uint4 q[sizeof(T) / 2];
+                memcpy(q, v, sizeof(v));
+                if constexpr (!kVec)
+                {
+                    T *area = areas[threadIdx.x >> 5];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                if (i < n) dst[i] = v[i];
+                    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(area + lane * kLaneCols)[i] = q[i];
+                    store_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
+                }
+                else if (row < p.rows)
+                {
+                    const int n = p.cols - at.c0 - g * kItemCols;
+                    if (n >= kLaneCols)
+                    {
+#pragma unroll
+                        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(dst + g * kItemCols)[i] = q[i];
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int i = 0; i < kLaneCols; ++i)
+                        {
+                            if (i < n) dst[g * kItemCols + i] = v[i];
+                        }
+                    }
+                }
             }
         }
     }
@@ -232,38 +311,50 @@ QuantParams make_params(const cugl_mx_desc &d, const void *plain, const void *pa
     p.tiles     = mx_scale_tiles(d.cols, d.format);
     p.rows      = d.rows;
     p.cols      = d.cols;
-    p.chunks    = static_cast<int>(p.tiles * 4 * mx_block(d.format) / 16);
+    const int64_t lanes = p.tiles * 4 * mx_block(d.format) / kLaneCols; // of a row, whole scale tiles
     p.lane_shift = 5;
-    // narrow rows: a power of two of lanes that holds one, at least those that share a word of scales
-    while (p.lane_shift > (d.format == CUGL_NVFP4 ? 2 : 3) && (1 << (p.lane_shift - 1)) >= p.chunks) --p.lane_shift;
-    const bool plain_vec = aligned(plain, 16) && d.ld % 16 == 0, packed_vec = aligned(packed, 8) && d.ld_packed % 8 == 0;
-    p.vec_src = plain_vec;
-    p.vec_dst = packed_vec;
+    // narrow rows: a power of two of lanes that holds one; those that share a word of scales stay together
+    while (p.lane_shift > 3 && (1 << (p.lane_shift - 1)) >= lanes) --p.lane_shift;
+    p.vec_plain  = aligned(plain, 16) && d.ld % 16 == 0;
+    p.vec_packed = aligned(packed, 4) && d.ld_packed % 4 == 0;
     return p;
 }
 
-dim3 grid_of(const QuantParams &p)
+template <typename K>
+cudaError_t launch_rows(cugl_context *ctx, K kernel, QuantParams p, int segs, int rows_per_warp)
 {
-    const int     per_row = 1 << p.lane_shift;
-    const int64_t y       = (static_cast<int64_t>(p.rows) + kWarps * (32 / per_row) - 1) / (kWarps * (32 / per_row));
-    return dim3(static_cast<unsigned>((p.chunks + per_row - 1) / per_row), static_cast<unsigned>(y < 65535 ? y : 65535));
+    const int64_t per_block = static_cast<int64_t>(kWarps) * rows_per_warp * (32 >> p.lane_shift);
+    const int64_t cols      = p.lane_shift < 5 ? p.cols : segs * kItemCols; // of a block: narrow rows lie in one
+    p.groups                = static_cast<int>((p.rows + per_block - 1) / per_block);
+    const dim3 grid(static_cast<unsigned>((p.cols + cols - 1) / cols), static_cast<unsigned>(p.groups < 65535 ? p.groups : 65535));
+    return launch_dependent(ctx, kernel, grid, kWarps * 32, 0, static_cast<long long>(grid.x) * grid.y, p);
 }
-
+// Four segments of a row where there are enough rows and columns to keep the device busy that way, else one
+bool wide(const cugl_context *ctx, const QuantParams &p)
+{
+    return p.cols >= 4 * kItemCols && static_cast<int64_t>(p.rows) * (p.cols / (4 * kItemCols)) >= 16ll * ctx->sm_count;
+}
+template <typename T, int kFormat>
+cudaError_t launch_quantize(cugl_context *ctx, const QuantParams &p)
+{
+    if (p.vec_plain == 0) return launch_rows(ctx, quantize_kernel<T, kFormat, false, 1, 1>, p, 1, 1);
+    return wide(ctx, p) ? launch_rows(ctx, quantize_kernel<T, kFormat, true, 4, 1>, p, 4, 1) : launch_rows(ctx, quantize_kernel<T, kFormat, true, 1, 1>, p, 1, 1);
+}
+template <typename T, int kFormat>
+cudaError_t launch_dequantize(cugl_context *ctx, const QuantParams &p)
+{
+    if (p.vec_plain == 0) return launch_rows(ctx, dequantize_kernel<T, kFormat, false, 1, 1>, p, 1, 1);
+    return wide(ctx, p) ? launch_rows(ctx, dequantize_kernel<T, kFormat, true, 4, 1>, p, 4, 1) : launch_rows(ctx, dequantize_kernel<T, kFormat, true, 1, 1>, p, 1, 1);
+}
 template <typename T>
 cudaError_t launch_quantize(cugl_context *ctx, int format, const QuantParams &p)
 {
-    const dim3      g     = grid_of(p);
-    const long long units = static_cast<long long>(g.x) * g.y;
-    return format == CUGL_NVFP4 ? launch_dependent(ctx, quantize_kernel<T, CUGL_NVFP4>, g, kWarps * 32, 0, units, p)
-                                : launch_dependent(ctx, quantize_kernel<T, CUGL_MXFP4>, g, kWarps * 32, 0, units, p);
+    return format == CUGL_NVFP4 ? launch_quantize<T, CUGL_NVFP4>(ctx, p) : launch_quantize<T, CUGL_MXFP4>(ctx, p);
 }
 template <typename T>
-cudaError_t launch_dequantize(cugl_context *ctx, int format, const QuantParams &p, void *out)
+cudaError_t launch_dequantize(cugl_context *ctx, int format, const QuantParams &p)
 {
-    const dim3      g     = grid_of(p);
-    const long long units = static_cast<long long>(g.x) * g.y;
-    return format == CUGL_NVFP4 ? launch_dependent(ctx, dequantize_kernel<T, CUGL_NVFP4>, g, kWarps * 32, 0, units, p, out)
-                                : launch_dependent(ctx, dequantize_kernel<T, CUGL_MXFP4>, g, kWarps * 32, 0, units, p, out);
+    return format == CUGL_NVFP4 ? launch_dequantize<T, CUGL_NVFP4>(ctx, p) : launch_dequantize<T, CUGL_MXFP4>(ctx, p);
 }
 
 const char *validate_mx(const cugl_mx_desc *d, cugl_status *code)
@@ -272,6 +363,7 @@ const char *validate_mx(const cugl_mx_desc *d, cugl_status *code)
     if (d == nullptr) return "descriptor is NULL";
     if (d->rows < 0 || d->cols < 1) return "rows must not be negative and cols must be positive";
     if (d->cols > INT32_MAX - 1024) return "cols is too large";
+    if (d->rows > INT32_MAX - (1 << 20)) return "rows is too large"; // row numbers behind the last one stay within 32 bits
     if (d->format != CUGL_MXFP4 && d->format != CUGL_NVFP4) return "format must be CUGL_MXFP4 or CUGL_NVFP4";
     if (!is_float_dtype(d->dtype)) return "dtype must be CUGL_F32, CUGL_F16 or CUGL_BF16";
     if (d->ld < static_cast<int64_t>(d->cols) * dtype_size(d->dtype) || d->ld % dtype_size(d->dtype) != 0)
@@ -333,7 +425,7 @@ extern "C"
         if (desc->rows == 0) return CUGL_SUCCESS;
         const DeviceScope device(ctx);
         QuantParams       p = make_params(*desc, d_src, d_dst);
-        p.src          = d_src;
+        p.src          = static_cast<const uint8_t *>(d_src);
         p.dst          = static_cast<uint8_t *>(d_dst);
         p.scales       = static_cast<uint8_t *>(d_scales);
         p.exponent_mul = std::ldexp(1.f, -desc->tensor_exponent);
@@ -349,13 +441,13 @@ extern "C"
         if (desc->rows == 0) return CUGL_SUCCESS;
         const DeviceScope device(ctx);
         QuantParams       p = make_params(*desc, d_dst, d_src);
-        std::swap(p.vec_src, p.vec_dst);
-        p.src          = d_src;
+        p.src          = static_cast<const uint8_t *>(d_src);
+        p.dst          = static_cast<uint8_t *>(d_dst);
         p.scales       = const_cast<uint8_t *>(static_cast<const uint8_t *>(d_scales));
         p.exponent_mul = std::ldexp(1.f, desc->tensor_exponent);
-        CUGL_CUDA_TRY(ctx, desc->dtype == CUGL_F32   ? launch_dequantize<float>(ctx, desc->format, p, d_dst)
-                           : desc->dtype == CUGL_F16 ? launch_dequantize<__half>(ctx, desc->format, p, d_dst)
-                                                     : launch_dequantize<__nv_bfloat16>(ctx, desc->format, p, d_dst));
+        CUGL_CUDA_TRY(ctx, desc->dtype == CUGL_F32   ? launch_dequantize<float>(ctx, desc->format, p)
+                           : desc->dtype == CUGL_F16 ? launch_dequantize<__half>(ctx, desc->format, p)
+                                                     : launch_dequantize<__nv_bfloat16>(ctx, desc->format, p));
         return CUGL_SUCCESS;
     }
 
