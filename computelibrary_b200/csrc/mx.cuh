@@ -80,13 +80,10 @@ __device__ __forceinline__ size_t mx_scale_offset(int64_t row, int64_t block, in
 // Eight values (already divided by their scale) to E2M1, v[0] in the lowest four bits: to nearest, ties to even, saturated.
 __device__ __forceinline__ uint32_t pack_e2m1x8(const float *v)
 {
-    uint32_t w = 0;
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        w |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_E2M1, cudaRoundNearest)) << (8 * i);
-    }
-    return w;
+    for (int i = 0; i < 4; ++i) b[i] = __nv_cvt_float2_to_fp4x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_E2M1, cudaRoundNearest);
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
 // Eight codes to f16 pairs (exact), the element of the lowest four bits first.

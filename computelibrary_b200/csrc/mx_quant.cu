@@ -106,89 +106,192 @@ __device__ __forceinline__ uint32_t widen(const uint4 (&raw)[sizeof(T) / 2], flo
 // A lane owns eight columns of a segment: half an NVFP4 block or a quarter of an MXFP4 one; the largest value and the scale bytes
 // of four blocks are gathered by shuffles, and the bytes leave as one word of their tile.  A warp has the loads of all its
 // segments in flight.
-template <typename T, int kFormat, bool kVec, int kSegs, int kRows>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const __grid_constant__ QuantParams p)
+//
+// Floats: a lane's eight are two 16-byte units.  Lanes of a pair swap one each, so that an access of the warp covers whole
+// 32-byte sectors (read-back of 4096 x 4096: 23.7 -> 16 us).
+__device__ __forceinline__ void swap_units(uint4 &a, uint4 &b, int lane) // the even lane's b and the odd lane's a change places
+{
+    const bool odd  = (lane & 1) != 0;
+    uint4      send = odd ? a : b;
+    send.x = __shfl_xor_sync(0xffffffffu, send.x, 1);
+    send.y = __shfl_xor_sync(0xffffffffu, send.y, 1);
+    send.z = __shfl_xor_sync(0xffffffffu, send.z, 1);
+    send.w = __shfl_xor_sync(0xffffffffu, send.w, 1);
+    if (odd) a = send;
+    else b = send;
+}
+
+// kWhole: every segment lies inside the matrix and all rows are aligned; nothing to test.
+template <typename T, int kFormat, bool kVec, bool kWhole, int kSegs, int kRows>
+__device__ __forceinline__ void quantize_group(const QuantParams &p, int group, T *area)
 {
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
     constexpr int kLanes = kBlock / kLaneCols; // of a block
     constexpr int kLoads = sizeof(T) / 2;
     constexpr int kTiles = kItemCols / (4 * kBlock); // scale tiles of a segment
-    __shared__ __align__(16) T areas[kVec ? 1 : kWarps][kVec ? 8 : kItemCols];
-    dependent_prologue();
-    const int lane = threadIdx.x & 31;
-    for (int group = blockIdx.y; group < p.groups; group += gridDim.y)
+    const int     lane   = threadIdx.x & 31;
+    const Place   at     = place_of<kSegs, kRows>(p, group, lane);
+    uint4         raw[kRows][kSegs][kLoads];
+    if constexpr (kVec)
     {
-        const Place at = place_of<kSegs, kRows>(p, group, lane);
-        uint4       raw[kRows][kSegs][kLoads];
-        if constexpr (kVec)
-        {
-#pragma unroll
-            for (int u = 0; u < kRows; ++u)
-            {
-                const int row = at.row + u * at.step;
-                const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + at.c0;
-#pragma unroll
-                for (int g = 0; g < kSegs; ++g)
-                {
-                    const int n = row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
-#pragma unroll
-                    for (int l = 0; l < kLoads; ++l)
-                    {
-                        raw[u][g][l] = make_uint4(0, 0, 0, 0);
-                        if (n >= kLaneCols) raw[u][g][l] = __ldg(reinterpret_cast<const uint4 *>(src + g * kItemCols) + l);
-                    }
-                    if (n > 0 && n < kLaneCols)
-                    {
-                        T part[kLaneCols];
-#pragma unroll
-                        for (int i = 0; i < kLaneCols; ++i) part[i] = i < n ? src[g * kItemCols + i] : from_float<T>(0.f);
-                        memcpy(raw[u][g], part, sizeof(part));
-                    }
-                }
-            }
-        }
 #pragma unroll
         for (int u = 0; u < kRows; ++u)
         {
-            const int      row    = at.row + u * at.step;
-            const int      block  = at.c0 / kBlock;
-            uint8_t *const scales = p.scales + mx_scale_offset(row, block, p.tiles);
-            uint8_t *const dst    = p.dst + row * p.ld_packed + at.c0 / 2;
+            const int row = at.row + u * at.step;
+            const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + at.c0;
 #pragma unroll
             for (int g = 0; g < kSegs; ++g)
             {
-                if constexpr (!kVec)
+                if constexpr (kWhole && kLoads == 2)
                 {
-                    T *area = areas[threadIdx.x >> 5];
-                    load_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
-#pragma unroll
-                    for (int l = 0; l < kLoads; ++l) raw[u][g][l] = reinterpret_cast<const uint4 *>(area + lane * kLaneCols)[l];
+                    const uint4 *unit = reinterpret_cast<const uint4 *>(src + g * kItemCols) - (lane & 1); // of the pair's first lane: + 2 per lane before it
+                    raw[u][g][0]      = __ldg(unit);
+                    raw[u][g][1]      = __ldg(unit + 2);
+                    continue;
                 }
-                float    v[kLaneCols];
-                uint32_t amax = widen<T>(raw[u][g], v);
+                const int n = kWhole || row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
 #pragma unroll
-                for (int o = 1; o < kLanes; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                const MxScale s    = mx_scale_of<kFormat, sizeof(T) == 4>(amax, p.exponent_mul);
-                uint32_t      word = s.byte << (8 * ((lane / kLanes) & 3));
-                word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
-                word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
-                scale_to_codes<kFormat, sizeof(T) == 4>(v, s);
-                const uint32_t w = pack_e2m1x8(v);
-                const int      n = p.cols - at.c0 - g * kItemCols;
-                if (row < p.rows)
+                for (int l = 0; l < kLoads; ++l)
                 {
-                    if ((lane & (4 * kLanes - 1)) == 0 && block + g * 4 * kTiles < 4 * p.tiles)
+                    raw[u][g][l] = make_uint4(0, 0, 0, 0);
+                    if (kWhole || n >= kLaneCols) raw[u][g][l] = __ldg(reinterpret_cast<const uint4 *>(src + g * kItemCols) + l);
+                }
+                if (!kWhole && n > 0 && n < kLaneCols)
+                {
+                    T part[kLaneCols];
+#pragma unroll
+                    for (int i = 0; i < kLaneCols; ++i) part[i] = i < n ? src[g * kItemCols + i] : from_float<T>(0.f);
+                    memcpy(raw[u][g], part, sizeof(part));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+    {
+        const int      row    = at.row + u * at.step;
+        const int      block  = at.c0 / kBlock;
+        uint8_t *const scales = p.scales + mx_scale_offset(row, block, p.tiles);
+        uint8_t *const dst    = p.dst + row * p.ld_packed + at.c0 / 2;
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g)
+        {
+            if constexpr (!kVec)
+            {
+                load_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
+#pragma unroll
+                for (int l = 0; l < kLoads; ++l) raw[u][g][l] = reinterpret_cast<const uint4 *>(area + lane * kLaneCols)[l];
+            }
+            if constexpr (kWhole && kLoads == 2) swap_units(raw[u][g][0], raw[u][g][1], lane);
+            float    v[kLaneCols];
+            uint32_t amax = widen<T>(raw[u][g], v);
+#pragma unroll
+            for (int o = 1; o < kLanes; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const MxScale s    = mx_scale_of<kFormat, sizeof(T) == 4>(amax, p.exponent_mul);
+            uint32_t      word = s.byte << (8 * ((lane / kLanes) & 3));
+            word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
+            word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
+            scale_to_codes<kFormat, sizeof(T) == 4>(v, s);
+            const uint32_t w = pack_e2m1x8(v);
+            if (kWhole || row < p.rows)
+            {
+                if ((lane & (4 * kLanes - 1)) == 0 && (kWhole || block + g * 4 * kTiles < 4 * p.tiles))
+                {
+                    *reinterpret_cast<uint32_t *>(scales + g * kTiles * kMxTileBytes) = word; // blocks behind the row: 0
+                }
+                const int n = p.cols - at.c0 - g * kItemCols;
+                uint8_t  *d = dst + g * kItemCols / 2;
+                if (kWhole || (n >= kLaneCols && p.vec_packed != 0))
+                {
+                    *reinterpret_cast<uint32_t *>(d) = w;
+                }
+                else
+                {
+                    for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) d[i] = static_cast<uint8_t>(w >> (8 * i)); // the half byte behind an odd row is 0
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int kFormat, bool kVec, bool kWhole, int kSegs, int kRows>
+__device__ __forceinline__ void dequantize_group(const QuantParams &p, int group, T *area)
+{
+    constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
+    constexpr int kTiles = kItemCols / (4 * kBlock); // scale tiles of a segment
+    const int     lane   = threadIdx.x & 31;
+    const Place   at     = place_of<kSegs, kRows>(p, group, lane);
+    uint32_t      w[kRows][kSegs], byte[kRows][kSegs];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+    {
+        const int      row    = at.row + u * at.step;
+        const uint8_t *src    = p.src + row * p.ld_packed + at.c0 / 2;
+        const uint8_t *scales = p.scales + mx_scale_offset(row, at.c0 / kBlock, p.tiles);
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g)
+        {
+            const int n = kWhole ? kLaneCols : row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
+            w[u][g] = byte[u][g] = 0;
+            if (n > 0) byte[u][g] = __ldg(scales + g * kTiles * kMxTileBytes);
+            if (kWhole || (n >= kLaneCols && p.vec_packed != 0))
+            {
+                w[u][g] = __ldg(reinterpret_cast<const uint32_t *>(src + g * kItemCols / 2));
+            }
+            else
+            {
+                for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) w[u][g] |= static_cast<uint32_t>(__ldg(src + g * kItemCols / 2 + i)) << (8 * i);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+    {
+        const int row = at.row + u * at.step;
+        T        *dst = reinterpret_cast<T *>(p.dst + row * p.ld) + at.c0;
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g)
+        {
+            const float s = mx_scale_value<kFormat>(byte[u][g]) * p.exponent_mul;
+            __half2     h[4];
+            unpack_e2m1x8(w[u][g], h);
+            T v[kLaneCols];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                const float2 f = __half22float2(h[i]);
+                v[2 * i]       = from_float<T>(f.x * s);
+                v[2 * i + 1]   = from_float<T>(f.y * s);
+            }
+            uint4 q[sizeof(T) / 2];
+            memcpy(q, v, sizeof(v));
+            if constexpr (!kVec)
+            {
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(area + lane * kLaneCols)[i] = q[i];
+                store_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
+            }
+            else if constexpr (kWhole && sizeof(T) == 4)
+            {
+                swap_units(q[0], q[1], lane);
+                uint4 *unit = reinterpret_cast<uint4 *>(dst + g * kItemCols) - (lane & 1);
+                unit[0]     = q[0];
+                unit[2]     = q[1];
+            }
+            else if (kWhole || row < p.rows)
+            {
+                const int n = p.cols - at.c0 - g * kItemCols;
+                if (kWhole || n >= kLaneCols)
+                {
+#pragma unroll
+                    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(dst + g * kItemCols)[i] = q[i];
+                }
+                else
+                {
+#pragma unroll
+                    for (int i = 0; i < kLaneCols; ++i)
                     {
-                        *reinterpret_cast<uint32_t *>(scales + g * kTiles * kMxTileBytes) = word; // blocks behind the row: 0
-                    }
-                    uint8_t *d = dst + g * kItemCols / 2;
-                    if (n >= kLaneCols && p.vec_packed != 0)
-                    {
-                        *reinterpret_cast<uint32_t *>(d) = w;
-                    }
-                    else
-                    {
-                        for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) d[i] = static_cast<uint8_t>(w >> (8 * i)); // the half byte behind an odd row is 0
+                        if (i < n) dst[g * kItemCols + i] = v[i];
                     }
                 }
             }
@@ -196,86 +299,25 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const __grid_cons
     }
 }
 
-template <typename T, int kFormat, bool kVec, int kSegs, int kRows>
-__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const __grid_constant__ QuantParams p)
+template <typename T, int kFormat, bool kVec, int kSegs, int kRows, bool kBack>
+__global__ void __launch_bounds__(kWarps * 32) mx_rows_kernel(const __grid_constant__ QuantParams p)
 {
-    constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
-    constexpr int kTiles = kItemCols / (4 * kBlock); // scale tiles of a segment
     __shared__ __align__(16) T areas[kVec ? 1 : kWarps][kVec ? 8 : kItemCols];
     dependent_prologue();
-    const int lane = threadIdx.x & 31;
+    T *area = areas[kVec ? 0 : threadIdx.x >> 5];
     for (int group = blockIdx.y; group < p.groups; group += gridDim.y)
     {
-        const Place at = place_of<kSegs, kRows>(p, group, lane);
-        uint32_t    w[kRows][kSegs], byte[kRows][kSegs];
-#pragma unroll
-        for (int u = 0; u < kRows; ++u)
+        const bool whole = kVec && p.lane_shift == 5 && p.vec_packed != 0 && static_cast<int>(blockIdx.x + 1) * kSegs * kItemCols <= p.cols &&
+                           (group + 1) * kWarps * kRows <= p.rows; // the same for the block
+        if constexpr (kBack)
         {
-            const int      row    = at.row + u * at.step;
-            const uint8_t *src    = p.src + row * p.ld_packed + at.c0 / 2;
-            const uint8_t *scales = p.scales + mx_scale_offset(row, at.c0 / kBlock, p.tiles);
-#pragma unroll
-            for (int g = 0; g < kSegs; ++g)
-            {
-                const int n = row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
-                w[u][g] = byte[u][g] = 0;
-                if (n > 0) byte[u][g] = __ldg(scales + g * kTiles * kMxTileBytes);
-                if (n >= kLaneCols && p.vec_packed != 0)
-                {
-                    w[u][g] = __ldg(reinterpret_cast<const uint32_t *>(src + g * kItemCols / 2));
-                }
-                else
-                {
-                    for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) w[u][g] |= static_cast<uint32_t>(__ldg(src + g * kItemCols / 2 + i)) << (8 * i);
-                }
-            }
+            if (whole) dequantize_group<T, kFormat, kVec, kVec, kSegs, kRows>(p, group, area);
+            else dequantize_group<T, kFormat, kVec, false, kSegs, kRows>(p, group, area);
         }
-#pragma unroll
-        for (int u = 0; u < kRows; ++u)
+        else
         {
-            const int row = at.row + u * at.step;
-            T        *dst = reinterpret_cast<T *>(p.dst + row * p.ld) + at.c0;
-#pragma unroll
-            for (int g = 0; g < kSegs; ++g)
-            {
-                const float s = mx_scale_value<kFormat>(byte[u][g]) * p.exponent_mul;
-                __half2     h[4];
-                unpack_e2m1x8(w[u][g], h);
-                T v[kLaneCols];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    const float2 f = __half22float2(h[i]);
-                    v[2 * i]       = from_float<T>(f.x * s);
-                    v[2 * i + 1]   = from_float<T>(f.y * s);
-                }
-                uint4 q[sizeof(T) / 2];
-                memcpy(q, v, sizeof(v));
-                if constexpr (!kVec)
-                {
-                    T *area = areas[threadIdx.x >> 5];
-#pragma unroll
-                    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(area + lane * kLaneCols)[i] = q[i];
-                    store_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
-                }
-                else if (row < p.rows)
-                {
-                    const int n = p.cols - at.c0 - g * kItemCols;
-                    if (n >= kLaneCols)
-                    {
-#pragma unroll
-                        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(dst + g * kItemCols)[i] = q[i];
-                    }
-                    else
-                    {
-#pragma unroll
-                        for (int i = 0; i < kLaneCols; ++i)
-                        {
-                            if (i < n) dst[g * kItemCols + i] = v[i];
-                        }
-                    }
-                }
-            }
+            if (whole) quantize_group<T, kFormat, kVec, kVec, kSegs, kRows>(p, group, area);
+            else quantize_group<T, kFormat, kVec, false, kSegs, kRows>(p, group, area);
         }
     }
 }
@@ -334,27 +376,24 @@ bool wide(const cugl_context *ctx, const QuantParams &p)
 {
     return p.cols >= 4 * kItemCols && static_cast<int64_t>(p.rows) * (p.cols / (4 * kItemCols)) >= 16ll * ctx->sm_count;
 }
-template <typename T, int kFormat>
-cudaError_t launch_quantize(cugl_context *ctx, const QuantParams &p)
+template <typename T, int kFormat, bool kBack>
+cudaError_t launch_matrix(cugl_context *ctx, const QuantParams &p)
 {
-    if (p.vec_plain == 0) return launch_rows(ctx, quantize_kernel<T, kFormat, false, 1, 1>, p, 1, 1);
-    return wide(ctx, p) ? launch_rows(ctx, quantize_kernel<T, kFormat, true, 4, 1>, p, 4, 1) : launch_rows(ctx, quantize_kernel<T, kFormat, true, 1, 1>, p, 1, 1);
+    if (p.vec_plain == 0) return launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 1, 1, kBack>, p, 1, 1);
+    return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 4, 1, kBack>, p, 4, 1)
+                        : launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 1, 1, kBack>, p, 1, 1);
 }
-template <typename T, int kFormat>
-cudaError_t launch_dequantize(cugl_context *ctx, const QuantParams &p)
+template <typename T, bool kBack>
+cudaError_t launch_matrix(cugl_context *ctx, int format, const QuantParams &p)
 {
-    if (p.vec_plain == 0) return launch_rows(ctx, dequantize_kernel<T, kFormat, false, 1, 1>, p, 1, 1);
-    return wide(ctx, p) ? launch_rows(ctx, dequantize_kernel<T, kFormat, true, 4, 1>, p, 4, 1) : launch_rows(ctx, dequantize_kernel<T, kFormat, true, 1, 1>, p, 1, 1);
+    return format == CUGL_NVFP4 ? launch_matrix<T, CUGL_NVFP4, kBack>(ctx, p) : launch_matrix<T, CUGL_MXFP4, kBack>(ctx, p);
 }
-template <typename T>
-cudaError_t launch_quantize(cugl_context *ctx, int format, const QuantParams &p)
+template <bool kBack>
+cudaError_t launch_matrix(cugl_context *ctx, const cugl_mx_desc &d, const QuantParams &p)
 {
-    return format == CUGL_NVFP4 ? launch_quantize<T, CUGL_NVFP4>(ctx, p) : launch_quantize<T, CUGL_MXFP4>(ctx, p);
-}
-template <typename T>
-cudaError_t launch_dequantize(cugl_context *ctx, int format, const QuantParams &p)
-{
-    return format == CUGL_NVFP4 ? launch_dequantize<T, CUGL_NVFP4>(ctx, p) : launch_dequantize<T, CUGL_MXFP4>(ctx, p);
+    return d.dtype == CUGL_F32 ? launch_matrix<float, kBack>(ctx, d.format, p)
+           : d.dtype == CUGL_F16 ? launch_matrix<__half, kBack>(ctx, d.format, p)
+                                 : launch_matrix<__nv_bfloat16, kBack>(ctx, d.format, p);
 }
 
 const char *validate_mx(const cugl_mx_desc *d, cugl_status *code)
@@ -429,9 +468,7 @@ extern "C"
         p.dst          = static_cast<uint8_t *>(d_dst);
         p.scales       = static_cast<uint8_t *>(d_scales);
         p.exponent_mul = std::ldexp(1.f, -desc->tensor_exponent);
-        CUGL_CUDA_TRY(ctx, desc->dtype == CUGL_F32   ? launch_quantize<float>(ctx, desc->format, p)
-                           : desc->dtype == CUGL_F16 ? launch_quantize<__half>(ctx, desc->format, p)
-                                                     : launch_quantize<__nv_bfloat16>(ctx, desc->format, p));
+        CUGL_CUDA_TRY(ctx, launch_matrix<false>(ctx, *desc, p));
         return CUGL_SUCCESS;
     }
 
@@ -445,9 +482,7 @@ extern "C"
         p.dst          = static_cast<uint8_t *>(d_dst);
         p.scales       = const_cast<uint8_t *>(static_cast<const uint8_t *>(d_scales));
         p.exponent_mul = std::ldexp(1.f, desc->tensor_exponent);
-        CUGL_CUDA_TRY(ctx, desc->dtype == CUGL_F32   ? launch_dequantize<float>(ctx, desc->format, p)
-                           : desc->dtype == CUGL_F16 ? launch_dequantize<__half>(ctx, desc->format, p)
-                                                     : launch_dequantize<__nv_bfloat16>(ctx, desc->format, p));
+        CUGL_CUDA_TRY(ctx, launch_matrix<true>(ctx, *desc, p));
         return CUGL_SUCCESS;
     }
 
