@@ -29,7 +29,8 @@ struct MxGemmParams
     int            dtype;
     int            pack_out; // two-byte results: rows of dst are words (4-byte aligned, an even number of channels)
     float          alpha;
-    uint32_t       idesc;
+    uint32_t       idesc, idesc_half; // SM pair: of a whole tile and of half a tile
+    int            whole;             // SM pair: tiles that are not split
     int32_t       *status;
     long long      spin_limit;
     int            withhold; // see cugl_context_withhold_copy_once
@@ -388,6 +389,17 @@ constexpr int kPairThreads = 32 * (kFirstEpi + kPairEpi);
 // both operands in L2 and on the way to the SMs (channel blocks all the way: 4096 x 14336 x 16384 NVFP4 405 us, strips 346;
 // K = 4096 101 and 102).
 constexpr int kPairStrip = 4;
+
+// Tiles of a last wave that fills at most half of the SM pairs are worked on as two halves of 128 tokens.  Items: whole tiles, then
+// the halves.
+struct PairItem
+{
+    int tile, half; // -1: whole
+};
+__device__ __forceinline__ PairItem pair_item(int item, int whole)
+{
+    return item < whole ? PairItem{item, -1} : PairItem{whole + ((item - whole) >> 1), (item - whole) & 1};
+}
 __device__ __forceinline__ void pair_tile(int tile, int w_blocks, int t_blocks, int &wb, int &tb)
 {
     const int strip = tile / (kPairStrip * t_blocks), in = tile - strip * kPairStrip * t_blocks;
@@ -436,6 +448,7 @@ __device__ __forceinline__ void stage_block(uint32_t s_out, int lane, const uint
 template <int kFormat, int kBulk>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,
+                        const __grid_constant__ CUtensorMap tmap_half,
                         const __grid_constant__ CUtensorMap tmap_wsf, const __grid_constant__ CUtensorMap tmap_tsf,
                         const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmParams p)
 {
@@ -456,12 +469,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int      rank = static_cast<int>(cluster_ctarank());
 
-    const int w_blocks    = (p.channels + 2 * kMxRows - 1) / (2 * kMxRows);
-    const int t_blocks    = (p.tokens + kPairCols - 1) / kPairCols;
-    const int tiles       = w_blocks * t_blocks;
-    const int chunks      = (p.K + kMxChunk - 1) / kMxChunk;
-    const int first_tile  = static_cast<int>(cluster_id_x());
-    const int tile_stride = static_cast<int>(num_clusters_x());
+    const int w_blocks = (p.channels + 2 * kMxRows - 1) / (2 * kMxRows);
+    const int t_blocks = (p.tokens + kPairCols - 1) / kPairCols;
+    const int items    = p.whole + 2 * (w_blocks * t_blocks - p.whole);
+    const int chunks   = (p.K + kMxChunk - 1) / kMxChunk;
+    const int first    = static_cast<int>(cluster_id_x());
+    const int stride   = static_cast<int>(num_clusters_x());
 
     if (threadIdx.x == 0)
     {
@@ -493,10 +506,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const bool el = elect_one();
         {
             int g = 0;
-            for (int tile = first_tile; tile < tiles; tile += tile_stride)
+            for (int v = first; v < items; v += stride)
             {
-                int wb, tb;
-                pair_tile(tile, w_blocks, t_blocks, wb, tb);
+                const PairItem item = pair_item(v, p.whole);
+                int            wb, tb;
+                pair_tile(item.tile, w_blocks, t_blocks, wb, tb);
                 for (int c = 0; c < chunks; ++c, ++g)
                 {
                     const int s = g % STAGES;
@@ -511,18 +525,27 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     // boxes of scale tiles are whole: behind the last tile of a row they read the next row's, which no MMA uses
                     const uint32_t bar = map_to_cta(full_bar(s), 0);
                     const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    const int      kt  = static_cast<int>(p.k_tiles), first = c * F::kChunkTiles;
+                    const int      kt  = static_cast<int>(p.k_tiles), sf0 = c * F::kChunkTiles;
                     if (el)
                     {
+                        const bool whole = item.half < 0;
                         if (rank == 0)
                         {
-                            mbar_expect_tx(full_bar(s), 2 * (P::STAGE + P::SF_STAGE));
+                            mbar_expect_tx(full_bar(s), whole ? 2 * (P::STAGE + P::SF_STAGE) : 2 * (kMxWBytes + kMxWBytes / 2 + 2 * F::kChunkScale));
                         }
                         tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
-                        tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
-                        tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + first, bar);
-                        tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + first, bar);
-                        tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + first, bar);
+                        tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + sf0, bar);
+                        if (whole)
+                        {
+                            tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
+                            tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + sf0, bar);
+                            tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + sf0, bar);
+                        }
+                        else
+                        {
+                            tma_load_2d_pair(dst + kMxWBytes, &tmap_half, c * kMxChunkBytes, tb * kPairCols + item.half * kMxRows + rank * (kMxRows / 2), bar);
+                            tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, (tb * 2 + item.half) * kt + sf0, bar);
+                        }
                     }
                     __syncwarp();
                 }
@@ -546,8 +569,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             int  g = 0, it = 0;
             bool ok = true;
             const uint32_t t_w = tmem_base + P::SF_COL, t_t = t_w + F::kChunkCols;
-            for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
+            for (int v = first; v < items && ok; v += stride, ++it)
             {
+                const bool     whole = v < p.whole;
+                const uint32_t idesc = whole ? p.idesc : p.idesc_half;
                 ok = warp_wait(tempty, (static_cast<uint32_t>(it) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (it & 1) * (kPairCols - kPairShared);
@@ -568,14 +593,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                             const uint64_t at = static_cast<uint64_t>(t * (kMxTileBytes >> 4));
                             tmem_copy_scales_pair(t_w + 4 * t, sf + at);
                             tmem_copy_scales_pair(t_t + 8 * t, sf + at + (F::kChunkScale >> 4));
-                            tmem_copy_scales_pair(t_t + 8 * t + 4, sf + at + 2 * (F::kChunkScale >> 4));
+                            if (whole) tmem_copy_scales_pair(t_t + 8 * t + 4, sf + at + 2 * (F::kChunkScale >> 4));
                         }
 #pragma unroll
                         for (int k = 0; k < kMxChunk / kMxStepK; ++k)
                         {
                             if (k < steps)
                             {
-                                umma_mx_pair<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, p.idesc | mx_scale_id<kFormat>(k),
+                                umma_mx_pair<kFormat>(d_tmem, a_desc + 2u * k, b_desc + 2u * k, idesc | mx_scale_id<kFormat>(k),
                                                       t_w + 4 * mx_step_tile<kFormat>(k), t_t + 8 * mx_step_tile<kFormat>(k), (c | k) != 0 ? 1u : 0u);
                             }
                         }
@@ -597,17 +622,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int      q = warp & 3, half = (warp - kFirstEpi) >> 2;
         const uint32_t release = map_to_cta(tempty, 0);
         int            it = 0;
-        for (int tile = first_tile; tile < tiles; tile += tile_stride, ++it)
+        for (int v = first; v < items; v += stride, ++it)
         {
-            int wb, tb;
-            pair_tile(tile, w_blocks, t_blocks, wb, tb);
+            const PairItem item = pair_item(v, p.whole);
+            int            wb, tb;
+            pair_tile(item.tile, w_blocks, t_blocks, wb, tb);
             const int   as = it & 1, n0 = (wb * 2 + rank) * kMxRows + q * 32;
             if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
                 break;
             }
             tc_fence_after();
-            const int      cols = p.tokens - tb * kPairCols;
+            const int      m0   = tb * kPairCols + (item.half > 0 ? kMxRows : 0), cols = p.tokens - m0;
             const uint32_t acc  = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
             float          bias[4] = {}; // kBulk = 2: of the fragments' rows, else of this lane's channel
             if (p.bias != nullptr)
@@ -620,10 +646,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 }
             }
 #pragma unroll 1
-            for (int i = 0; i < kPairCols / 64; ++i)
+            for (int i = 0; i < (item.half < 0 ? kPairCols / 64 : kMxRows / 64); ++i)
             {
                 const int group = 2 * i + half;
-                const int j     = as == 0 ? (group * 32 + kPairCols - kPairShared) % kPairCols : group * 32;
+                const int j     = as == 0 && item.half < 0 ? (group * 32 + kPairCols - kPairShared) % kPairCols : group * 32; // (a half has none of the first accumulator's shared columns)
                 uint32_t  r[2][16];
                 if constexpr (kBulk == 2)
                 {
@@ -665,14 +691,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     __syncwarp();
                     if (lane == 0)
                     {
-                        if (j < cols && n0 < p.channels) tma_store_2d(&tmap_out, s_out, n0, tb * kPairCols + j);
+                        if (j < cols && n0 < p.channels) tma_store_2d(&tmap_out, s_out, n0, m0 + j);
                         tma_store_commit();
                     }
                 }
                 else
                 {
-                    store_block(p, tb * kPairCols + j, n0 + lane, r[0], cols - j, bias[0]);
-                    store_block(p, tb * kPairCols + j + 16, n0 + lane, r[1], cols - j - 16, bias[0]);
+                    store_block(p, m0 + j, n0 + lane, r[0], cols - j, bias[0]);
+                    store_block(p, m0 + j + 16, n0 + lane, r[1], cols - j - 16, bias[0]);
                 }
             }
             tc_fence_before();
@@ -758,10 +784,11 @@ cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
 {
     using P = MxPairPlan<kFormat>;
     using F = MxTraits<kFormat>;
-    CUtensorMap   map_w, map_t, map_wsf, map_tsf, map_out{};
+    CUtensorMap   map_w, map_t, map_half, map_wsf, map_tsf, map_out{};
     const int64_t inner = (static_cast<int64_t>(p.K) + 1) / 2;
     const int64_t w_tiles = (static_cast<int64_t>(p.channels) + 127) / 128 * p.k_tiles, t_tiles = (static_cast<int64_t>(p.tokens) + 127) / 128 * p.k_tiles;
     if (!encode_packed_map(&map_w, op.b, p.channels, inner, op.d->ldb, kMxRows) || !encode_packed_map(&map_t, op.a, p.tokens, inner, op.d->lda, kMxRows) ||
+        !encode_packed_map(&map_half, op.a, p.tokens, inner, op.d->lda, kMxRows / 2) ||
         !encode_scale_map(&map_wsf, p.w_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_tsf, p.t_scales, t_tiles, F::kChunkTiles) ||
         (kBulk != 0 && !encode_dst_map(&map_out, p)))
     {
@@ -770,10 +797,13 @@ cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
     auto        kernel  = mx_gemm_pair_kernel<kFormat, kBulk>;
     static bool set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
-    p.idesc = mx_idesc(kFormat, 2 * kMxRows, kPairCols);
-    const int64_t   tiles = static_cast<int64_t>((p.channels + 255) / 256) * ((p.tokens + 255) / 256);
-    const long long pairs = tiles < ctx->sm_count / 2 ? tiles : ctx->sm_count / 2;
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(2 * pairs)), kPairThreads, P::DYN_BYTES, 2, 2 * tiles, map_w, map_t,
+    p.idesc      = mx_idesc(kFormat, 2 * kMxRows, kPairCols);
+    p.idesc_half = mx_idesc(kFormat, 2 * kMxRows, kPairCols / 2);
+    const int tiles = static_cast<int>(static_cast<int64_t>((p.channels + 255) / 256) * ((p.tokens + 255) / 256)), pairs = ctx->sm_count / 2;
+    const int tail  = tiles % pairs;
+    p.whole         = tail > 0 && 2 * tail <= pairs ? tiles - tail : tiles;
+    const int items = p.whole + 2 * (tiles - p.whole), grid = 2 * (items < pairs ? items : pairs);
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kPairThreads, P::DYN_BYTES, 2, 2ll * items, map_w, map_t, map_half,
                                                 map_wsf, map_tsf, map_out, p));
     return CUGL_SUCCESS;
 }

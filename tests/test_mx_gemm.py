@@ -119,6 +119,43 @@ def test_larger(ctx, fmt, dtype, M, N, K):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(512, 4096, 700), (257, 8200, 2048), (385, 4104, 2304), (140, 9472, 2050), (2100, 2800, 300)])
+def test_halves_of_tiles(ctx, fmt, M, N, K):
+    """Few tiles, or a few beyond whole waves: worked on as two halves of 128 tokens, the second of which may be empty."""
+    check(ctx, M, N, K, fmt, capi.BF16)
+    check(ctx, M, N, K, fmt, capi.F32, bias=True)
+    check(ctx, M, N - 1, K, fmt, capi.F16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,k_block", [(1, 4096, 4096, 1), (8, 512, 1024, 0), (64, 20000, 1024, 3), (100, 4096, 2048, 0), (512, 4096, 2048, 3),
+                                           (2048, 4096, 2048, 9), (300, 1001, 2048, 1)])
+def test_wait_limit(ctx, M, N, K, k_block):
+    """Operand copies that never come: the call ends by its wait limit and says so; the next one is as always."""
+    import torch
+    rng = np.random.default_rng(0)
+    a, sa, _ = operand(rng, M, K, capi.NVFP4)
+    b, sb, _ = operand(rng, N, K, capi.NVFP4)
+    want, out = (torch.zeros((M, N), dtype=torch.float32, device="cuda") for _ in range(2))
+    d = capi.make_mx_gemm_desc(M, N, K, capi.NVFP4, capi.F32)
+    ctx.mx_gemm(d, a, sa, b, sb, None, want)
+    ctx.sync()
+    ctx.set_wait_limit_us(20000)
+    try:
+        ctx.withhold_copy_once(k_block)
+        ctx.mx_gemm(d, a, sa, b, sb, None, out)
+        with pytest.raises(capi.CuglError) as e:
+            ctx.sync()
+        assert e.value.status == capi.RUNTIME_ERROR
+    finally:
+        ctx.set_wait_limit_us(0)
+    ctx.mx_gemm(d, a, sa, b, sb, None, out)
+    ctx.sync()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_long_k(ctx, fmt):
     check(ctx, 3, 130, 70001, fmt, capi.F32)
     check(ctx, 200, 300, 16384, fmt, capi.F32)
