@@ -944,8 +944,8 @@ cugl_status launch_moe(cugl_context *ctx, const MoeMaps &m, MoeParams p, int nt,
     switch (nt)
     {
         case 16: return launch_layers<kFormat, 16, 2, 2, 4>(ctx, m, p, most_active);
-        case 32: return launch_layers<kFormat, 32, 2, 2, 3>(ctx, m, p, most_active);
-        case 64: return launch_layers<kFormat, 64, 2, 1, 3>(ctx, m, p, most_active);
+        case 32: return launch_layers<kFormat, 32, 2, 2, kFormat == CUGL_MXFP4 ? 4 : 3>(ctx, m, p, most_active);
+        case 64: return launch_layers<kFormat, 64, 2, 1, kFormat == CUGL_MXFP4 ? 4 : 3>(ctx, m, p, most_active);
         default: return launch_layers<kFormat, 128, 4, 1, 3>(ctx, m, p, most_active);
     }
 }
