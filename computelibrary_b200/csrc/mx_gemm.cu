@@ -773,10 +773,13 @@ cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, 
     return CUGL_SUCCESS;
 }
 
-template <int kFormat, int NT, int STAGES>
+// as many stages as half an SM's shared memory holds
+template <int kFormat, int NT>
 cugl_status launch_tokens(cugl_context *ctx, const MxOperands &op, const MxGemmParams &p, int ranks)
 {
-    return ranks > 1 ? launch_one<kFormat, NT, STAGES, true>(ctx, op, p, ranks) : launch_one<kFormat, NT, STAGES, false>(ctx, op, p, 1);
+    constexpr bool kSmall  = kFormat == CUGL_MXFP4; // half the scale bytes
+    constexpr int  kStages = NT <= 32 || (NT == 64 && kSmall) ? 4 : 3, kShared = NT == 32 && !kSmall ? 3 : kStages;
+    return ranks > 1 ? launch_one<kFormat, NT, kShared, true>(ctx, op, p, ranks) : launch_one<kFormat, NT, kStages, false>(ctx, op, p, 1);
 }
 
 template <int kFormat, int kBulk>
@@ -842,10 +845,10 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     const int ranks = nt < 128 || tiles * 4 <= ctx->sm_count ? mx_split(tiles, chunks, 4) : 1;
     switch (nt)
     {
-        case 16: return launch_tokens<kFormat, 16, 4>(ctx, op, p, ranks);
-        case 32: return launch_tokens<kFormat, 32, 3>(ctx, op, p, ranks);
-        case 64: return launch_tokens<kFormat, 64, 3>(ctx, op, p, ranks);
-        default: return launch_tokens<kFormat, 128, 3>(ctx, op, p, ranks);
+        case 16: return launch_tokens<kFormat, 16>(ctx, op, p, ranks);
+        case 32: return launch_tokens<kFormat, 32>(ctx, op, p, ranks);
+        case 64: return launch_tokens<kFormat, 64>(ctx, op, p, ranks);
+        default: return launch_tokens<kFormat, 128>(ctx, op, p, ranks);
     }
 }
 
