@@ -18,6 +18,8 @@ namespace
 {
 constexpr int kMmaWarp  = 1;
 constexpr int kFirstEpi = 2;
+constexpr int kPrefetch = 16; // chunks, 256 KB of weights per CTA
+
 struct MxGemmParams
 {
     const uint8_t *w_scales, *t_scales;
@@ -153,9 +155,8 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     const int ranks       = kSplit ? static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x()) : 1;
     const int first_tile  = kSplit ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
     const int tile_stride = kSplit ? tiles : static_cast<int>(gridDim.x);
-    const int per_rank    = (chunks + ranks - 1) / ranks;
-    const int c_begin     = min(chunks, rank * per_rank);
-    const int c_end       = min(chunks, c_begin + per_rank);
+    const int c_begin     = chunk_share(chunks, rank, ranks);
+    const int c_end       = chunk_share(chunks, rank + 1, ranks);
 
     if (threadIdx.x == 0)
     {
@@ -186,51 +187,60 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
     griddep_launch_dependents();
-    griddep_wait(); // the prologue above touched no global memory
+    if (warp == 0 && first_tile < tiles)
+    {
+        // The weights of the first tile start on their way from memory while the kernels ahead finish: bringing them into L2
+        // reads nothing that those kernels could still change.
+        const bool el = elect_one();
+        for (int c = c_begin; c < min(c_end, c_begin + kPrefetch); ++c)
+        {
+            if (el) tma_prefetch_2d(&tmap_w, c * kMxChunkBytes, first_tile % w_blocks * kMxRows);
+            __syncwarp();
+        }
+    }
+    griddep_wait(); // everything else touches global memory after the kernels ahead
 
     if (warp == 0)
     {
         const bool el = elect_one();
+        int g = 0;
+        for (int tile = first_tile; tile < tiles; tile += tile_stride)
         {
-            int g = 0;
-            for (int tile = first_tile; tile < tiles; tile += tile_stride)
+            const int      wb = tile % w_blocks, tb = tile / w_blocks;
+            const uint8_t *w_sf = p.w_scales + static_cast<int64_t>(wb) * p.k_tiles * kMxTileBytes;
+            const uint8_t *t_sf = p.t_scales + static_cast<int64_t>(tb) * p.k_tiles * kMxTileBytes; // NT < 128: one block only
+            for (int c = c_begin; c < c_end; ++c, ++g)
             {
-                const int      wb = tile % w_blocks, tb = tile / w_blocks;
-                const uint8_t *w_sf = p.w_scales + static_cast<int64_t>(wb) * p.k_tiles * kMxTileBytes;
-                const uint8_t *t_sf = p.t_scales + static_cast<int64_t>(tb) * p.k_tiles * kMxTileBytes; // NT < 128: one block only
-                for (int c = c_begin; c < c_end; ++c, ++g)
+                const int s = g % STAGES;
+                if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                 {
-                    const int s = g % STAGES;
-                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
-                    {
-                        goto produced;
-                    }
-                    if (g == p.withhold && blockIdx.x == 0)
-                    {
-                        continue;
-                    }
-                    const int      first = c * F::kChunkTiles;
-                    const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - first);
-                    const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
-                    const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    if (el)
-                    {
-                        mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
-                        tma_load_2d(dst, &tmap_w, c * kMxChunkBytes, wb * kMxRows, full_bar(s));
-                        tma_load_2d(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * NT, full_bar(s));
-                        bulk_load(sf, w_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
-                        bulk_load(sf + F::kChunkScale, t_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
-                    }
-                    __syncwarp();
+                    goto produced;
                 }
+                if (g == p.withhold && blockIdx.x == 0)
+                {
+                    continue;
+                }
+                const int      first = c * F::kChunkTiles;
+                const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - first);
+                const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
+                const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
+                if (el)
+                {
+                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
+                    tma_load_2d(dst, &tmap_w, c * kMxChunkBytes, wb * kMxRows, full_bar(s));
+                    tma_load_2d(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * NT, full_bar(s));
+                    bulk_load(sf, w_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
+                    bulk_load(sf + F::kChunkScale, t_sf + static_cast<int64_t>(first) * kMxTileBytes, bytes, full_bar(s));
+                }
+                __syncwarp();
             }
-        produced:
-            if (el && *s_abort != 0)
+        }
+    produced:
+        if (el && *s_abort != 0)
+        {
+            for (int i = max(0, g - STAGES); i < g; ++i)
             {
-                for (int i = max(0, g - STAGES); i < g; ++i)
-                {
-                    if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-                }
+                if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
             }
         }
         __syncwarp();
@@ -238,38 +248,36 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     else if (warp == kMmaWarp)
     {
         const bool el = elect_one();
+        int  g = 0, it = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
         {
-            int  g = 0, it = 0;
-            bool ok = true;
-            for (int tile = first_tile; tile < tiles && ok; tile += tile_stride, ++it)
+            const int as = it % P::ACC;
+            ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / P::ACC) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + as * NT;
+            for (int c = c_begin; c < c_end && ok; ++c, ++g)
             {
-                const int as = it % P::ACC;
-                ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / P::ACC) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                const int s = g % STAGES;
+                ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + as * NT;
-                for (int c = c_begin; c < c_end && ok; ++c, ++g)
+                const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - c * F::kChunkTiles);
+                const int      steps = min(kMxChunk / kMxStepK, (p.K - c * kMxChunk + kMxStepK - 1) / kMxStepK);
+                const uint32_t t_w   = tmem_base + P::ACC * NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
+                const uint32_t sf    = s_sf + s * P::SF_STAGE;
+                if (el)
                 {
-                    const int s = g % STAGES;
-                    ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int      n     = min(F::kChunkTiles, static_cast<int>(p.k_tiles) - c * F::kChunkTiles);
-                    const int      steps = min(kMxChunk / kMxStepK, (p.K - c * kMxChunk + kMxStepK - 1) / kMxStepK);
-                    const uint32_t t_w   = tmem_base + P::ACC * NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
-                    const uint32_t sf    = s_sf + s * P::SF_STAGE;
-                    if (el)
-                    {
-                        mx_chunk_scales<kFormat>(t_w, sf, n);
-                        mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
-                        mx_chunk<kFormat>(d_tmem, s_stage + s * P::STAGE, s_stage + s * P::STAGE + kMxWBytes, t_w, t_t, p.idesc, steps, c == c_begin);
-                        umma_commit(empty_bar(s));
-                    }
-                    __syncwarp();
+                    mx_chunk_scales<kFormat>(t_w, sf, n);
+                    mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
+                    mx_chunk<kFormat>(d_tmem, s_stage + s * P::STAGE, s_stage + s * P::STAGE + kMxWBytes, t_w, t_t, p.idesc, steps, c == c_begin);
+                    umma_commit(empty_bar(s));
                 }
-                if (ok && el)
-                {
-                    umma_commit(tfull_bar(as));
-                }
+                __syncwarp();
+            }
+            if (ok && el)
+            {
+                umma_commit(tfull_bar(as));
             }
         }
         __syncwarp();
@@ -504,59 +512,57 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (warp == 0)
     {
         const bool el = elect_one();
+        int g = 0;
+        for (int v = first; v < items; v += stride)
         {
-            int g = 0;
-            for (int v = first; v < items; v += stride)
+            const PairItem item = pair_item(v, p.whole);
+            int            wb, tb;
+            pair_tile(item.tile, w_blocks, t_blocks, wb, tb);
+            for (int c = 0; c < chunks; ++c, ++g)
             {
-                const PairItem item = pair_item(v, p.whole);
-                int            wb, tb;
-                pair_tile(item.tile, w_blocks, t_blocks, wb, tb);
-                for (int c = 0; c < chunks; ++c, ++g)
+                const int s = g % STAGES;
+                if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                 {
-                    const int s = g % STAGES;
-                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
-                    {
-                        goto produced;
-                    }
-                    if (g == p.withhold && blockIdx.x == 0)
-                    {
-                        continue;
-                    }
-                    // boxes of scale tiles are whole: behind the last tile of a row they read the next row's, which no MMA uses
-                    const uint32_t bar = map_to_cta(full_bar(s), 0);
-                    const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    const int      kt  = static_cast<int>(p.k_tiles), sf0 = c * F::kChunkTiles;
-                    if (el)
-                    {
-                        const bool whole = item.half < 0;
-                        if (rank == 0)
-                        {
-                            mbar_expect_tx(full_bar(s), whole ? 2 * (P::STAGE + P::SF_STAGE) : 2 * (kMxWBytes + kMxWBytes / 2 + 2 * F::kChunkScale));
-                        }
-                        tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
-                        tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + sf0, bar);
-                        if (whole)
-                        {
-                            tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
-                            tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + sf0, bar);
-                            tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + sf0, bar);
-                        }
-                        else
-                        {
-                            tma_load_2d_pair(dst + kMxWBytes, &tmap_half, c * kMxChunkBytes, tb * kPairCols + item.half * kMxRows + rank * (kMxRows / 2), bar);
-                            tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, (tb * 2 + item.half) * kt + sf0, bar);
-                        }
-                    }
-                    __syncwarp();
+                    goto produced;
                 }
+                if (g == p.withhold && blockIdx.x == 0)
+                {
+                    continue;
+                }
+                // boxes of scale tiles are whole: behind the last tile of a row they read the next row's, which no MMA uses
+                const uint32_t bar = map_to_cta(full_bar(s), 0);
+                const uint32_t dst = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
+                const int      kt  = static_cast<int>(p.k_tiles), sf0 = c * F::kChunkTiles;
+                if (el)
+                {
+                    const bool whole = item.half < 0;
+                    if (rank == 0)
+                    {
+                        mbar_expect_tx(full_bar(s), whole ? 2 * (P::STAGE + P::SF_STAGE) : 2 * (kMxWBytes + kMxWBytes / 2 + 2 * F::kChunkScale));
+                    }
+                    tma_load_2d_pair(dst, &tmap_w, c * kMxChunkBytes, (wb * 2 + rank) * kMxRows, bar);
+                    tma_load_2d_pair(sf, &tmap_wsf, 0, (wb * 2 + rank) * kt + sf0, bar);
+                    if (whole)
+                    {
+                        tma_load_2d_pair(dst + kMxWBytes, &tmap_t, c * kMxChunkBytes, tb * kPairCols + rank * kMxRows, bar);
+                        tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, tb * 2 * kt + sf0, bar);
+                        tma_load_2d_pair(sf + 2 * F::kChunkScale, &tmap_tsf, 0, (tb * 2 + 1) * kt + sf0, bar);
+                    }
+                    else
+                    {
+                        tma_load_2d_pair(dst + kMxWBytes, &tmap_half, c * kMxChunkBytes, tb * kPairCols + item.half * kMxRows + rank * (kMxRows / 2), bar);
+                        tma_load_2d_pair(sf + F::kChunkScale, &tmap_tsf, 0, (tb * 2 + item.half) * kt + sf0, bar);
+                    }
+                }
+                __syncwarp();
             }
-        produced:
-            if (*s_abort != 0 && rank == 0) // the leader's barriers count the copies of both CTAs
+        }
+    produced:
+        if (*s_abort != 0 && rank == 0) // the leader's barriers count the copies of both CTAs
+        {
+            for (int i = max(0, g - STAGES); i < g; ++i)
             {
-                for (int i = max(0, g - STAGES); i < g; ++i)
-                {
-                    if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-                }
+                if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
             }
         }
         __syncwarp();

@@ -137,6 +137,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  : "memory");
 }
 
+// Asks for a box of a tensor map to be brought into L2.  A hint: what another kernel writes there later is seen by whoever reads
+// after it, so it may run ahead of griddepcontrol.wait.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
+}
+
 // The lane that issues a warp's tcgen05 and TMA instructions.  The issuing loops are run by the whole warp and only the
 // instructions themselves are guarded by this predicate: control flow stays uniform, so that descriptors and addresses are
 // computed in uniform registers, which these instructions take their operands from.  Under a branch on the lane index each of
@@ -215,6 +222,12 @@ __device__ __forceinline__ void mx_chunk_scales(uint32_t t_dst, uint32_t sf, int
             tmem_copy_scales(t_dst + 4 * t, desc + static_cast<uint64_t>(t * (kMxTileBytes >> 4)));
         }
     }
+}
+
+// First chunk of a rank's share of K.
+__device__ __forceinline__ int chunk_share(int chunks, int rank, int ranks)
+{
+    return static_cast<int>(static_cast<int64_t>(chunks) * rank / ranks);
 }
 
 // Partial sums of a cluster whose 2^shift CTAs shared an accumulator's K.  Rank r owns channels r * (128 >> shift) and up.  The

@@ -414,90 +414,85 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
     const int chunks      = (p.hidden + kMxChunk - 1) / kMxChunk;
     const int first_unit  = kSplit ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
     const int unit_stride = kSplit ? max(units, 1) : static_cast<int>(gridDim.x);
-    const int per_rank    = (chunks + ranks - 1) / ranks;
-    const int c_begin     = min(chunks, rank * per_rank);
-    const int c_end       = min(chunks, c_begin + per_rank);
+    const int c_begin     = chunk_share(chunks, rank, ranks);
+    const int c_end       = chunk_share(chunks, rank + 1, ranks);
 
     if (warp == 0)
     {
         const bool el = elect_one();
+        int g = 0;
+        for (int unit = first_unit; unit < units; unit += unit_stride)
         {
-            int g = 0;
-            for (int unit = first_unit; unit < units; unit += unit_stride)
+            const int      e = s_list[unit / blocks], fb = unit % blocks;
+            const int64_t  sf_at = (static_cast<int64_t>(e) * blocks + fb) * p.h_tiles * kMxTileBytes;
+            const int      row = e * p.inner + fb * kMxRows;
+            for (int c = c_begin; c < c_end; ++c, ++g)
             {
-                const int      e = s_list[unit / blocks], fb = unit % blocks;
-                const int64_t  sf_at = (static_cast<int64_t>(e) * blocks + fb) * p.h_tiles * kMxTileBytes;
-                const int      row = e * p.inner + fb * kMxRows;
-                for (int c = c_begin; c < c_end; ++c, ++g)
+                const int s = g % STAGES;
+                if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
                 {
-                    const int s = g % STAGES;
-                    if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
-                    {
-                        goto produced;
-                    }
-                    const int      first = c * F::kChunkTiles;
-                    const int      n     = min(F::kChunkTiles, static_cast<int>(p.h_tiles) - first);
-                    const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
-                    const int64_t  at    = static_cast<int64_t>(first) * kMxTileBytes;
-                    const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                    if (el)
-                    {
-                        mbar_expect_tx(full_bar(s), P::STAGE + 3 * bytes);
-                        tma_load_2d(dst, &tmap_g, c * kMxChunkBytes, row, full_bar(s));
-                        tma_load_2d(dst + kMxWBytes, &tmap_u, c * kMxChunkBytes, row, full_bar(s));
-                        tma_load_2d(dst + 2 * kMxWBytes, &tmap_x, c * kMxChunkBytes, 0, full_bar(s));
-                        bulk_load(sf, p.gate_scales + sf_at + at, bytes, full_bar(s));
-                        bulk_load(sf + F::kChunkScale, p.up_scales + sf_at + at, bytes, full_bar(s));
-                        bulk_load(sf + 2 * F::kChunkScale, p.xs + at, bytes, full_bar(s));
-                    }
-                    __syncwarp();
+                    goto produced;
                 }
+                const int      first = c * F::kChunkTiles;
+                const int      n     = min(F::kChunkTiles, static_cast<int>(p.h_tiles) - first);
+                const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
+                const int64_t  at    = static_cast<int64_t>(first) * kMxTileBytes;
+                const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
+                if (el)
+                {
+                    mbar_expect_tx(full_bar(s), P::STAGE + 3 * bytes);
+                    tma_load_2d(dst, &tmap_g, c * kMxChunkBytes, row, full_bar(s));
+                    tma_load_2d(dst + kMxWBytes, &tmap_u, c * kMxChunkBytes, row, full_bar(s));
+                    tma_load_2d(dst + 2 * kMxWBytes, &tmap_x, c * kMxChunkBytes, 0, full_bar(s));
+                    bulk_load(sf, p.gate_scales + sf_at + at, bytes, full_bar(s));
+                    bulk_load(sf + F::kChunkScale, p.up_scales + sf_at + at, bytes, full_bar(s));
+                    bulk_load(sf + 2 * F::kChunkScale, p.xs + at, bytes, full_bar(s));
+                }
+                __syncwarp();
             }
-        produced:
-            if (el && *s_abort != 0)
-            {
-                for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-            }
+        }
+    produced:
+        if (el && *s_abort != 0)
+        {
+            for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
         }
         __syncwarp();
     }
     else if (warp == kMmaWarp)
     {
         const bool el = elect_one();
+        int  g = 0, it = 0;
+        bool ok = true;
+        for (int unit = first_unit; unit < units && ok; unit += unit_stride, ++it)
         {
-            int  g = 0, it = 0;
-            bool ok = true;
-            for (int unit = first_unit; unit < units && ok; unit += unit_stride, ++it)
+            const int as = it % kAcc;
+            ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / kAcc) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + as * P::ACC_COLS;
+            for (int c = c_begin; c < c_end && ok; ++c, ++g)
             {
-                const int as = it % kAcc;
-                ok = warp_wait(tempty_bar(as), (static_cast<uint32_t>(it / kAcc) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                const int s = g % STAGES;
+                ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + as * P::ACC_COLS;
-                for (int c = c_begin; c < c_end && ok; ++c, ++g)
+                const int      n     = min(F::kChunkTiles, static_cast<int>(p.h_tiles) - c * F::kChunkTiles);
+                const int      steps = min(kMxChunk / kMxStepK, (p.hidden - c * kMxChunk + kMxStepK - 1) / kMxStepK);
+                const uint32_t t_g   = tmem_base + kAcc * P::ACC_COLS + s * P::SF_COLS, t_u = t_g + F::kChunkCols, t_x = t_u + F::kChunkCols;
+                const uint32_t sf = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
+                if (el)
                 {
-                    const int s = g % STAGES;
-                    ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int      n     = min(F::kChunkTiles, static_cast<int>(p.h_tiles) - c * F::kChunkTiles);
-                    const int      steps = min(kMxChunk / kMxStepK, (p.hidden - c * kMxChunk + kMxStepK - 1) / kMxStepK);
-                    const uint32_t t_g   = tmem_base + kAcc * P::ACC_COLS + s * P::SF_COLS, t_u = t_g + F::kChunkCols, t_x = t_u + F::kChunkCols;
-                    const uint32_t sf = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
-                    if (el)
-                    {
-                        mx_chunk_scales<kFormat>(t_x, sf + 2 * F::kChunkScale, n);
-                        mx_chunk_scales<kFormat>(t_g, sf, n);
-                        mx_chunk_scales<kFormat>(t_u, sf + F::kChunkScale, n);
-                        mx_chunk<kFormat>(d_tmem, st, st + 2 * kMxWBytes, t_g, t_x, p.idesc, steps, c == c_begin);
-                        mx_chunk<kFormat>(d_tmem + NT, st + kMxWBytes, st + 2 * kMxWBytes, t_u, t_x, p.idesc, steps, c == c_begin);
-                        umma_commit(empty_bar(s));
-                    }
-                    __syncwarp();
+                    mx_chunk_scales<kFormat>(t_x, sf + 2 * F::kChunkScale, n);
+                    mx_chunk_scales<kFormat>(t_g, sf, n);
+                    mx_chunk_scales<kFormat>(t_u, sf + F::kChunkScale, n);
+                    mx_chunk<kFormat>(d_tmem, st, st + 2 * kMxWBytes, t_g, t_x, p.idesc, steps, c == c_begin);
+                    mx_chunk<kFormat>(d_tmem + NT, st + kMxWBytes, st + 2 * kMxWBytes, t_u, t_x, p.idesc, steps, c == c_begin);
+                    umma_commit(empty_bar(s));
                 }
-                if (ok && el)
-                {
-                    umma_commit(tfull_bar(as));
-                }
+                __syncwarp();
+            }
+            if (ok && el)
+            {
+                umma_commit(tfull_bar(as));
             }
         }
         __syncwarp();
@@ -664,88 +659,83 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     const int chunks     = active * per_expert;
     const int blocks     = (p.hidden + kMxRows - 1) / kMxRows;
     const int block      = static_cast<int>(cluster_id_x());
-    const int per_rank   = (chunks + ranks - 1) / ranks;
-    const int c_begin    = min(chunks, rank * per_rank);
-    const int c_end      = min(chunks, c_begin + per_rank);
+    const int c_begin    = chunk_share(chunks, rank, ranks);
+    const int c_end      = chunk_share(chunks, rank + 1, ranks);
 
     if (warp == 0)
     {
         const bool el = elect_one();
+        auto load_weights = [&](int g) {
+            const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, e = s_list[a], first = c * F::kChunkTiles;
+            const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
+            if (el)
+            {
+                mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
+                tma_load_2d(s_stage + s * P::STAGE, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
+                bulk_load(s_sf + s * P::SF_STAGE, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes,
+                          full_bar(s));
+            }
+            __syncwarp();
+        };
+        auto load_tokens = [&](int g) {
+            const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, first = c * F::kChunkTiles;
+            const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
+            if (el)
+            {
+                tma_load_2d(s_stage + s * P::STAGE + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
+                bulk_load(s_sf + s * P::SF_STAGE + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
+            }
+            __syncwarp();
+        };
+        const int mine = c_end - c_begin, early = min(mine, STAGES);
+        int       g = 0;
+        for (; g < early; ++g) load_weights(g);
+        griddep_wait();
+        for (int i = 0; i < early; ++i) load_tokens(i);
+        for (; g < mine; ++g)
         {
-            auto load_weights = [&](int g) {
-                const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, e = s_list[a], first = c * F::kChunkTiles;
-                const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
-                if (el)
-                {
-                    mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
-                    tma_load_2d(s_stage + s * P::STAGE, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
-                    bulk_load(s_sf + s * P::SF_STAGE, p.down_scales + ((static_cast<int64_t>(e) * blocks + block) * p.f_tiles + first) * kMxTileBytes, bytes,
-                              full_bar(s));
-                }
-                __syncwarp();
-            };
-            auto load_tokens = [&](int g) {
-                const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, first = c * F::kChunkTiles;
-                const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
-                if (el)
-                {
-                    tma_load_2d(s_stage + s * P::STAGE + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
-                    bulk_load(s_sf + s * P::SF_STAGE + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
-                }
-                __syncwarp();
-            };
-            const int mine = c_end - c_begin, early = min(mine, STAGES);
-            int       g = 0;
-            for (; g < early; ++g) load_weights(g);
-            griddep_wait();
-            for (int i = 0; i < early; ++i) load_tokens(i);
-            for (; g < mine; ++g)
+            const int s = g % STAGES;
+            if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
             {
-                const int s = g % STAGES;
-                if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit))
-                {
-                    break;
-                }
-                load_weights(g);
-                load_tokens(g);
+                break;
             }
-            if (el && *s_abort != 0)
-            {
-                for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-            }
+            load_weights(g);
+            load_tokens(g);
+        }
+        if (el && *s_abort != 0)
+        {
+            for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
         }
         __syncwarp();
     }
     else if (warp == kMmaWarp)
     {
         const bool el = elect_one();
+        int  g  = 0;
+        bool ok = true;
+        for (int i = c_begin; i < c_end && ok; ++i, ++g)
         {
-            int  g  = 0;
-            bool ok = true;
-            for (int i = c_begin; i < c_end && ok; ++i, ++g)
+            const int s = g % STAGES;
+            ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+            if (!ok) break;
+            tc_fence_after();
+            const int      c     = i % per_expert;
+            const int      n     = min(F::kChunkTiles, static_cast<int>(p.f_tiles) - c * F::kChunkTiles);
+            const int      steps = min(kMxChunk / kMxStepK, (p.inner - c * kMxChunk + kMxStepK - 1) / kMxStepK);
+            const uint32_t t_w   = tmem_base + NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
+            const uint32_t sf    = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
+            if (el)
             {
-                const int s = g % STAGES;
-                ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
-                if (!ok) break;
-                tc_fence_after();
-                const int      c     = i % per_expert;
-                const int      n     = min(F::kChunkTiles, static_cast<int>(p.f_tiles) - c * F::kChunkTiles);
-                const int      steps = min(kMxChunk / kMxStepK, (p.inner - c * kMxChunk + kMxStepK - 1) / kMxStepK);
-                const uint32_t t_w   = tmem_base + NT + s * P::SF_COLS, t_t = t_w + F::kChunkCols;
-                const uint32_t sf    = s_sf + s * P::SF_STAGE, st = s_stage + s * P::STAGE;
-                if (el)
-                {
-                    mx_chunk_scales<kFormat>(t_w, sf, n);
-                    mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
-                    mx_chunk<kFormat>(tmem_base, st, st + kMxWBytes, t_w, t_t, p.idesc, steps, i == c_begin);
-                    umma_commit(empty_bar(s));
-                }
-                __syncwarp();
+                mx_chunk_scales<kFormat>(t_w, sf, n);
+                mx_chunk_scales<kFormat>(t_t, sf + F::kChunkScale, n);
+                mx_chunk<kFormat>(tmem_base, st, st + kMxWBytes, t_w, t_t, p.idesc, steps, i == c_begin);
+                umma_commit(empty_bar(s));
             }
-            if (ok && el)
-            {
-                umma_commit(tfull);
-            }
+            __syncwarp();
+        }
+        if (ok && el)
+        {
+            umma_commit(tfull);
         }
         __syncwarp();
     }
