@@ -272,11 +272,10 @@ def calculate_quantized_multipliers(i_scale: float, w_scales, o_scale: float):
 
 def _dptr(t):
     """Device pointer of a torch tensor / raw int / None."""
-    if t is None:
-        return None
-    if isinstance(t, int):
+    try:
+        return t.data_ptr()
+    except AttributeError:
         return t
-    return t.data_ptr()
 
 
 class Context:

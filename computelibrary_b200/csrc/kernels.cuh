@@ -189,13 +189,17 @@ inline bool use_dependent_launch(const cugl_context *ctx, long long units)
     {
         return false;
     }
+    if (units <= static_cast<long long>(kShortWaves) * ctx->sm_count)
+    {
+        return true; // captured or not
+    }
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess)
     {
         (void)cudaGetLastError();
         return false;
     }
-    return st == cudaStreamCaptureStatusNone || units <= static_cast<long long>(kShortWaves) * ctx->sm_count;
+    return st == cudaStreamCaptureStatusNone;
 }
 
 // First thing in a kernel launched with launch_dependent that has no prologue worth overlapping: the next kernel of the
