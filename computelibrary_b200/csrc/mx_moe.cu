@@ -15,6 +15,7 @@
 #include "mx_mma.cuh"
 
 #include <cmath>
+#include <initializer_list>
 
 namespace cugl
 {
@@ -858,7 +859,10 @@ const char *validate_moe(const cugl_mx_moe_desc *d)
         return "ld_gate_up and ld_down must hold a packed row and be multiples of 16 below 2^40";
     if (d->format == CUGL_MXFP4 && (d->x_exponent != 0 || d->h_exponent != 0)) return "x_exponent and h_exponent are for CUGL_NVFP4";
     if (d->x_exponent < -64 || d->x_exponent > 64 || d->h_exponent < -64 || d->h_exponent > 64) return "x_exponent and h_exponent must lie within -64 .. 64";
-    if (!(d->gate_alpha - d->gate_alpha == 0.f) || !(d->up_alpha - d->up_alpha == 0.f) || !(d->down_alpha - d->down_alpha == 0.f)) return "alphas must be finite";
+    for (const float v : {std::ldexp(d->gate_alpha, d->x_exponent), std::ldexp(d->up_alpha, d->x_exponent), std::ldexp(d->down_alpha, d->h_exponent)})
+    {
+        if (!(v - v == 0.f)) return "an alpha times 2 to its operand's exponent must be finite";
+    }
     return nullptr;
 }
 

@@ -591,8 +591,9 @@ typedef struct cugl_mx_gemm_desc
 } cugl_mx_gemm_desc;
 
 CUGL_API cugl_status cugl_mx_gemm_validate(const cugl_mx_gemm_desc *desc, const char **reason);
-/* One launch, no workspace, nothing kept between calls.  Operands and scale tiles are 16-byte aligned.  The sum over k runs in
- * an order that depends on the sizes only: equal calls give equal bits.  M == 0: nothing to do. */
+/* One launch, no workspace, nothing kept between calls.  Operands and scale tiles are 16-byte aligned, dst overlaps none of
+ * them.  The sum over k runs in an order that depends on the sizes, the type and dst's alignment only: equal calls give equal
+ * bits.  M == 0: nothing to do. */
 CUGL_API cugl_status cugl_mx_gemm(cugl_context *ctx, const cugl_mx_gemm_desc *desc, const void *d_a, const void *d_a_scales,
                                   const void *d_b, const void *d_b_scales, const float *d_bias, void *d_dst);
 
@@ -604,7 +605,9 @@ CUGL_API cugl_status cugl_mx_gemm(cugl_context *ctx, const cugl_mx_gemm_desc *de
  *   dst      down_alpha * sum over the chosen e of h[e] . down[e]^T, rounded once
  * A token with nothing to choose gets zeros.  gate and up are [experts * intermediate] packed rows of hidden elements, down
  * [experts * hidden] packed rows of intermediate elements, experts one after the other; the scale tiles of every expert are
- * those of a matrix of its own (cugl_mx_scale_bytes(intermediate, hidden) and (hidden, intermediate) bytes per expert). */
+ * those of a matrix of its own (cugl_mx_scale_bytes(intermediate, hidden) and (hidden, intermediate) bytes per expert).
+ * The weights of an expert that some token chose are finite: down's products run over all tokens, with zeros for those that did
+ * not choose the expert, and a NaN scale there would reach them too.  (A NaN in x stays with its token.) */
 typedef struct cugl_mx_moe_desc
 {
     int32_t tokens;                 /* 0 .. 128 */
@@ -624,7 +627,7 @@ CUGL_API cugl_status cugl_mx_moe_validate(const cugl_mx_moe_desc *desc, const ch
  * captured graphs that are replayed at the same time, need one each. */
 CUGL_API size_t      cugl_mx_moe_workspace_bytes(const cugl_mx_moe_desc *desc);
 /* d_logits: float [tokens][experts].  d_workspace: 256-byte aligned, at least cugl_mx_moe_workspace_bytes.  Three launches,
- * results do not depend on timing.  tokens == 0: nothing to do. */
+ * results do not depend on timing.  d_dst may be d_x (then ld_dst == ld_x).  tokens == 0: nothing to do. */
 CUGL_API cugl_status cugl_mx_moe(cugl_context *ctx, const cugl_mx_moe_desc *desc, const void *d_x, const float *d_logits,
                                  const void *d_gate, const void *d_gate_scales, const void *d_up, const void *d_up_scales,
                                  const void *d_down, const void *d_down_scales, void *d_dst, void *d_workspace,
