@@ -165,6 +165,12 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, limit));
 }
 
+// one column of a warp's 32 accumulator lanes
+__device__ __forceinline__ void tmem_ld_x1(uint32_t taddr, uint32_t &v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
+}
+
 // 16 accumulator lanes x 32 columns in the fragment layout of the matrix instructions: v[4 i + 0, 1] are columns 8 i + 2 (lane % 4)
 // and the next of row lane / 4, v[4 i + 2, 3] the same columns of row lane / 4 + 8.
 __device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&v)[16])

@@ -263,11 +263,11 @@ __device__ __forceinline__ bool begin_unit(const MoeParams &p, float *table, int
     return r != 0;
 }
 
-// Four tokens' sums g and u at a warp's 32 consecutive f to h, its codes and scales; chosen: bit i, token t0 + i chose the
-// expert (the others' zeros are written already).  Four at a time because each is one long chain of dependent instructions.
+// Sums g and u of four tokens at a warp's 32 consecutive f to h, its codes and scales; valid: bit i, token t[i] is to be stored.
+// Four at a time because each is one long chain of dependent instructions.
 template <int kFormat>
-__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t0, int f, int lane, const float (&g)[4], const float (&u)[4], const float *weight,
-                                             uint32_t chosen)
+__device__ __forceinline__ void store_hidden(const MoeParams &p, int a, const int (&t)[4], int f, int lane, const float (&g)[4], const float (&u)[4],
+                                             const float *weight, uint32_t valid)
 {
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
     float         h[4];
@@ -277,7 +277,7 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t0, 
     for (int i = 0; i < 4; ++i)
     {
         const float x = g[i] * p.gate_alpha;
-        const float v = weight[t0 + i] * __fdividef(x, 1.f + expf(-x)) * (u[i] * p.up_alpha); // SwiGLU, the gate's weight folded in
+        const float v = weight[t[i]] * __fdividef(x, 1.f + expf(-x)) * (u[i] * p.up_alpha); // SwiGLU, the gate's weight folded in
         h[i]          = f < p.inner ? v : 0.f;
         amax[i]       = __float_as_uint(h[i]) & 0x7fffffffu;
     }
@@ -307,16 +307,16 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, int t0, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], o);
     }
-    uint8_t *codes  = p.hq + (static_cast<int64_t>(a) * p.tokens + t0) * p.ld_hq + f / 2;
+    uint8_t *codes  = p.hq + static_cast<int64_t>(a) * p.tokens * p.ld_hq + f / 2;
     uint8_t *scales = p.hs + static_cast<int64_t>(a) * p.f_tiles * kMxTileBytes;
     const bool code_lane = (lane & 7) == 0 && f < p.inner, scale_lane = (lane & (kBlock - 1)) == 0 && f / kBlock < p.f_tiles * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        if ((chosen >> i) & 1u)
+        if ((valid >> i) & 1u)
         {
-            if (code_lane) *reinterpret_cast<uint32_t *>(codes + i * p.ld_hq) = w[i];
-            if (scale_lane) scales[mx_scale_offset(t0 + i, f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s[i].byte);
+            if (code_lane) *reinterpret_cast<uint32_t *>(codes + t[i] * p.ld_hq) = w[i];
+            if (scale_lane) scales[mx_scale_offset(t[i], f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s[i].byte);
         }
     }
 }
@@ -512,23 +512,35 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
             ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
-            for (int j = 16 * half; j < p.tokens; j += 4 * kUpEpi)
+            // the tokens that chose the expert, four at a time; the two warps of a lane quarter take turns
+            const uint32_t acc  = tmem_base + as * P::ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
+            int            turn = 0;
+            for (int w = 0; w < p.tokens; w += 32)
             {
-                const uint32_t chosen = __ballot_sync(0xffffffffu, lane < 16 && j + lane < p.tokens && weight[j + lane] != kNotChosen);
-                if (chosen == 0) continue;
-                uint32_t g[16], u[16];
-                tmem_ld_x16(tmem_base + as * P::ACC_COLS + j + (static_cast<uint32_t>(q * 32) << 16), g);
-                tmem_ld_x16(tmem_base + as * P::ACC_COLS + NT + j + (static_cast<uint32_t>(q * 32) << 16), u);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
+                uint32_t left = __ballot_sync(0xffffffffu, w + lane < p.tokens && weight[min(w + lane, kMaxTokens - 1)] != kNotChosen);
+                for (; left != 0; ++turn)
                 {
-                    if (((chosen >> i) & 15u) != 0)
+                    int      t[4];
+                    uint32_t valid = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
                     {
-                        const float g4[4] = {__uint_as_float(g[i]), __uint_as_float(g[i + 1]), __uint_as_float(g[i + 2]), __uint_as_float(g[i + 3])};
-                        const float u4[4] = {__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])};
-                        store_hidden<kFormat>(p, a, j + i, f, lane, g4, u4, weight, (chosen >> i) & 15u);
+                        t[i] = left != 0 ? w + __ffs(left) - 1 : t[0];
+                        valid |= left != 0 ? 1u << i : 0u;
+                        left &= left - 1;
                     }
+                    if ((turn & 1) != half) continue;
+                    uint32_t g[4], u[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        tmem_ld_x1(acc + t[i], g[i]);
+                        tmem_ld_x1(acc + NT + t[i], u[i]);
+                    }
+                    tmem_ld_wait();
+                    const float g4[4] = {__uint_as_float(g[0]), __uint_as_float(g[1]), __uint_as_float(g[2]), __uint_as_float(g[3])};
+                    const float u4[4] = {__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3])};
+                    store_hidden<kFormat>(p, a, t, f, lane, g4, u4, weight, valid);
                 }
             }
             tc_fence_before();
@@ -583,7 +595,8 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
                 {
                     const float4 g4 = sum_partial(part, at, shift, 2 * NT), u4 = sum_partial(part + NT * own, at, shift, 2 * NT);
                     const float  g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-                    store_hidden<kFormat>(p, a, t0, f, lane, g, u, s_weight, chosen);
+                    const int    t[4] = {t0, t0 + 1, t0 + 2, t0 + 3};
+                    store_hidden<kFormat>(p, a, t, f, lane, g, u, s_weight, chosen);
                 }
             }
         }
