@@ -8,6 +8,11 @@
 //
 // Every stage has scale columns of its own in tensor memory: they are written again only after the stage's MMAs have been
 // committed, like its shared memory.
+//
+// What bounds it: few tokens, the weights' bytes and the latency of one launch (1 x 4096 x 4096 NVFP4, 9.4 MB: 4.7 us in a
+// captured run, 1.5 us at the copy rate; 24 x 14336 x 4096 MXFP4, 31 MB: 8.4 us, 3.7 TB/s).  Hence 64 to 74 KB of operands in
+// flight per CTA, two CTAs per SM, K shared by a cluster where there are few tiles, and weights asked for before the launch
+// ahead has ended.  Many tokens, the tensor cores: see the SM-pair kernel below.
 #include "mx_mma.cuh"
 
 #include <cstring>
@@ -382,7 +387,12 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
 // (M = 256, N = 256) of the leader read both halves -- 64 instead of 96 bytes from L2 per clock of tensor work and SM.  The
 // scales of all 256 tokens go to both CTAs; they come as boxes of a tensor map because the bytes of both CTAs are credited to
 // the leader's barrier.
-// Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales.
+// What bounds it: power.  4096 x 14336 x 4096 NVFP4 takes 96 us by itself (5.0 PFLOP/s) and 112 to 116 back to back, where the
+// clock falls to 1.3 GHz; with operands of zeros K = 16384 runs at 7.1 PFLOP/s, with random ones at 5.65.
+// Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales of
+// one chunk.  A chunk's scales overwrite those of the chunk before: the copies and MMAs that one thread issues are carried out
+// in the order of issue.  (Two sets of columns in turn, each copied to only after the commit of the MMAs that read it, cost a
+// tenth: 4096 x 14336 x 4096 100 -> 110 us, 512 x 4096 x 4096 10.0 -> 11.3.)
 // The epilogue drains the shared columns first; the next tile's MMAs start when it has, and the rest of the drain runs beside
 // them.
 // kBulk: blocks of 32 channels x 32 tokens leave through a warp's staging area as one bulk tensor store (rows of dst 16-byte

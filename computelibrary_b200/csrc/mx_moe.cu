@@ -12,6 +12,10 @@
 // Three launches, overlapped by programmatic dependent launch: gate + quantisation of x, gate/up products + SwiGLU +
 // quantisation, down product.  The second lets the third start only after its own wait, i.e. when the first has completed: so
 // the third knows the experts and loads its first weights while the second is still running.
+//
+// us (floor: the chosen experts' weights at the copy rate), hidden 2048, intermediate 768, 64 experts: 1 token, top 8, NVFP4 14.3
+// (3.3), three launches of little else than latency; 48 tokens, top 4, MXFP4 40 (24); 128 tokens, top 8, NVFP4 56 (26), MXFP4
+// 51 (25), where the exchange of the down product's partial sums (64 KB per CTA) and an epilogue that no MMA overlaps are next.
 #include "mx_mma.cuh"
 
 #include <cmath>
@@ -118,7 +122,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
     }
 }
 
-// x to codes and scales, sixteen columns per lane as in quantize_kernel.
+// x to codes and scales (the rounding of mx.cuh), sixteen columns per lane.
 template <typename T, int kFormat>
 __device__ __forceinline__ void quantize_tokens(const MoeParams &p, int block, int warp, int lane)
 {
@@ -512,7 +516,8 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
             ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
             if (!ok) continue; // the next barrier ends it for all four warps
             tc_fence_after();
-            // the tokens that chose the expert, four at a time; the two warps of a lane quarter take turns
+            // The tokens that chose the expert, four at a time; the two warps of a lane quarter take turns.  (Four neighbours of which
+            // one or more chose it: 128 tokens 65 us instead of 56.)
             const uint32_t acc  = tmem_base + as * P::ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
             int            turn = 0;
             for (int w = 0; w < p.tokens; w += 32)
@@ -930,6 +935,10 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int blocks = (p.hidden + kMxRows - 1) / kMxRows, most_chunks = most_active * ((p.inner + kMxChunk - 1) / kMxChunk);
     ranks = mx_split(blocks, most_chunks, 8);
+    // One CTA per SM where it then still loads its whole share of K ahead of the second launch's end: 1 token, hidden 4096,
+    // intermediate 2048, top 2, NVFP4 (32 blocks, 16 chunks) 15.9 us with eight CTAs per block, 14.5 with four.  Fewer than one per
+    // SM lose: 2 tokens, hidden 2048, intermediate 1024, top 1 (16 blocks, 8 chunks) 11.7 and 12.4.
+    while (ranks > 2 && blocks * ranks > ctx->sm_count && most_chunks * 2 <= kDownStages * ranks) ranks /= 2;
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kDownThreads, P::DYN_BYTES, ranks, blocks * ranks,
                                                 m.down, m.h, p));
     return CUGL_SUCCESS;

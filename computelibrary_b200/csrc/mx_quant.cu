@@ -1,5 +1,9 @@
 // Microscaled 4-bit matrices: quantisation, read-back and the re-ordering of scales.  One pass over the data each; the bytes
 // moved bound all three.
+//
+// us, and of the measured copy rate: 8192 x 4096 BF16 -> MXFP4 and back (170 MB, two launches) 31.0, 85 %; 4096 x 4096 F32 ->
+// NVFP4 and back (153 MB) 28.0, 85 %; 8192 x 4096 NVFP4 -> BF16 (86 MB) 15.8, 84 %.  Rows that are not 16-byte aligned:
+// 1023 x 2049 F16 there and back (10.6 MB) 8.9, two launches of about 4.
 #include "mx.cuh"
 
 #include <cmath>
