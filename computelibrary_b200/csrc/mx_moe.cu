@@ -935,10 +935,12 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int blocks = (p.hidden + kMxRows - 1) / kMxRows, most_chunks = most_active * ((p.inner + kMxChunk - 1) / kMxChunk);
     ranks = mx_split(blocks, most_chunks, 8);
-    // One CTA per SM where it then still loads its whole share of K ahead of the second launch's end: 1 token, hidden 4096,
-    // intermediate 2048, top 2, NVFP4 (32 blocks, 16 chunks) 15.9 us with eight CTAs per block, 14.5 with four.  Fewer than one per
-    // SM lose: 2 tokens, hidden 2048, intermediate 1024, top 1 (16 blocks, 8 chunks) 11.7 and 12.4.
-    while (ranks > 2 && blocks * ranks > ctx->sm_count && most_chunks * 2 <= kDownStages * ranks) ranks /= 2;
+    // One CTA per SM instead of two where that leaves no more than a quarter of them idle: fewer parts to exchange, and room beside
+    // the second launch.  Few chunks per CTA gain by it, 1 token, hidden 4096, intermediate 2048, top 2, NVFP4 (16 chunks) 15.9 -> 14.5
+    // us, intermediate 1536, top 8 (48) 23.7 -> 22.9; many lose, 48 tokens, intermediate 768, 64 experts (192) 71 -> 76; but the parts
+    // of 128 columns are the greater cost: 100 tokens, intermediate 512, 4 experts 34 -> 28, 128 tokens, 1536, 64 experts 158 -> 148.
+    // Half the SMs idle: 128 tokens, hidden 2560 (20 blocks) 41.7 -> 46; two parts instead of four, hidden 8192: 43.7 -> 46.3.
+    if (ranks == 8 && blocks * 8 > ctx->sm_count && blocks * 4 >= ctx->sm_count * 3 / 4 && (NT == 128 || most_chunks <= 12 * 4)) ranks = 4;
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kDownThreads, P::DYN_BYTES, ranks, blocks * ranks,
                                                 m.down, m.h, p));
     return CUGL_SUCCESS;
