@@ -939,8 +939,13 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     // the second launch.  Few chunks per CTA gain by it, 1 token, hidden 4096, intermediate 2048, top 2, NVFP4 (16 chunks) 15.9 -> 14.5
     // us, intermediate 1536, top 8 (48) 23.7 -> 22.9; many lose, 48 tokens, intermediate 768, 64 experts (192) 71 -> 76; but the parts
     // of 128 columns are the greater cost: 100 tokens, intermediate 512, 4 experts 34 -> 28, 128 tokens, 1536, 64 experts 158 -> 148.
-    // Half the SMs idle: 128 tokens, hidden 2560 (20 blocks) 41.7 -> 46; two parts instead of four, hidden 8192: 43.7 -> 46.3.
-    if (ranks == 8 && blocks * 8 > ctx->sm_count && blocks * 4 >= ctx->sm_count * 3 / 4 && (NT == 128 || most_chunks <= 12 * 4)) ranks = 4;
+    // Half the SMs idle: 128 tokens, hidden 2560 (20 blocks) 41.7 -> 46;
+    // two parts of 128 columns instead of four, hidden 8192: 43.7 -> 46.3 (1 token, 8 chunks: 16.0 -> 15.3).
+    while (ranks > 2 && blocks * ranks > ctx->sm_count && blocks * ranks / 2 >= ctx->sm_count * 3 / 4 &&
+           (NT == 128 ? ranks == 8 : most_chunks <= 6 * ranks))
+    {
+        ranks /= 2;
+    }
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(blocks * ranks)), kDownThreads, P::DYN_BYTES, ranks, blocks * ranks,
                                                 m.down, m.h, p));
     return CUGL_SUCCESS;
