@@ -10,7 +10,7 @@
 // committed, like its shared memory.
 //
 // What bounds it: few tokens, the weights' bytes and the latency of one launch (1 x 4096 x 4096 NVFP4, 9.4 MB: 4.7 us in a
-// captured run, 1.5 us at the copy rate; 24 x 14336 x 4096 MXFP4, 31 MB: 8.4 us, 3.7 TB/s).  Hence 64 to 74 KB of operands in
+// captured run, 1.5 us at the copy rate; 24 x 14336 x 4096 MXFP4, 31 MB: 8.4 to 8.8 us, 3.6 TB/s).  Hence 64 to 74 KB of operands in
 // flight per CTA, two CTAs per SM, K shared by a cluster where there are few tiles, and weights asked for before the launch
 // ahead has ended.  Many tokens, the tensor cores: see the SM-pair kernel below.
 #include "mx_mma.cuh"
