@@ -205,6 +205,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     }
     griddep_wait(); // everything else touches global memory after the kernels ahead
 
+    int issued = 0; // stages that the producer has filled
     if (warp == 0)
     {
         const bool el = elect_one();
@@ -241,14 +242,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
             }
         }
     produced:
-        if (el && *s_abort != 0)
-        {
-            for (int i = max(0, g - STAGES); i < g; ++i)
-            {
-                if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-            }
-        }
-        __syncwarp();
+        issued = g;
     }
     else if (warp == kMmaWarp)
     {
@@ -367,6 +361,10 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
 
     tc_fence_before();
     __syncthreads();
+    if (warp == 0 && *s_abort != 0)
+    {
+        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit);
+    }
     if (warp == kMmaWarp)
     {
         tc_fence_after();
@@ -519,6 +517,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     griddep_launch_dependents();
     griddep_wait(); // the prologue above touched no global memory
 
+    int issued = 0; // stages that the producer has filled
     if (warp == 0)
     {
         const bool el = elect_one();
@@ -568,14 +567,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
         }
     produced:
-        if (*s_abort != 0 && rank == 0) // the leader's barriers count the copies of both CTAs
-        {
-            for (int i = max(0, g - STAGES); i < g; ++i)
-            {
-                if (!(i == p.withhold && blockIdx.x == 0)) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-            }
-        }
-        __syncwarp();
+        issued = g;
     }
     else if (warp == kMmaWarp)
     {
@@ -727,6 +719,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    if (warp == 0 && rank == 0 && *s_abort != 0)
+    {
+        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit); // the leader's barriers count the copies of both CTAs
+    }
     cluster_sync(); // neither CTA leaves (or frees tensor memory) while its peer may still touch it
     if (warp == kMmaWarp)
     {

@@ -189,13 +189,20 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Waits for a barrier's phase whatever the abort flag says: a producer that gives up lets its copies in flight land first.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, long long limit)
+// Of a kernel that has given up: waits for the copies still in flight into the last STAGES of `issued` stages (their full barriers
+// start at `bars`; withheld: a stage whose copies were left out) before the CTA leaves its shared memory.  Copies take
+// microseconds; the bound is there for one that never comes, and long enough whatever limit the caller set.
+template <int STAGES>
+__device__ __forceinline__ void drain_stages(uint32_t bars, int issued, int withheld, long long limit)
 {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity) && clock64() - t0 <= limit)
+    for (int i = max(0, issued - STAGES); i < issued; ++i)
     {
+        const long long t0 = clock64(), bound = limit + 2000000;
+        while (i != withheld && !mbar_try_wait(bars + 8u * (i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u) && clock64() - t0 <= bound)
+        {
+        }
     }
+    __syncwarp();
 }
 
 // The MMAs of one chunk whose operands and scales have landed in shared memory.  steps: MMAs inside K (1 .. 4).  a_stage,

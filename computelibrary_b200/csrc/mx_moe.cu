@@ -32,6 +32,7 @@ constexpr int kFirstEpi = 2;
 constexpr int kUpEpi = 8, kDownEpi = 4;
 constexpr int kUpThreads = 32 * (kFirstEpi + kUpEpi), kDownThreads = 32 * (kFirstEpi + kDownEpi);
 constexpr int kMaxTokens = 128, kMaxExperts = 512, kMaxTopK = 16;
+constexpr int kWithholdDown = 1 << 16; // ordinals of cugl_context_withhold_copy_once from here on: the third launch's
 
 struct MoeParams
 {
@@ -52,6 +53,7 @@ struct MoeParams
     uint32_t       idesc;
     int32_t       *status;
     long long      spin_limit;
+    int            withhold_up, withhold_down; // see cugl_context_withhold_copy_once
 };
 
 // ---- first launch ----------------------------------------------------------------------------------------
@@ -421,11 +423,13 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
     const int unit_stride = kSplit ? max(units, 1) : static_cast<int>(gridDim.x);
     const int c_begin     = chunk_share(chunks, rank, ranks);
     const int c_end       = chunk_share(chunks, rank + 1, ranks);
+    int       issued      = 0; // stages that the producer has filled
 
     if (warp == 0)
     {
         const bool el = elect_one();
-        int g = 0;
+        const int  withheld = blockIdx.x == 0 ? p.withhold_up : -1;
+        int        g = 0;
         for (int unit = first_unit; unit < units; unit += unit_stride)
         {
             const int      e = s_list[unit / blocks], fb = unit % blocks;
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
                 const uint32_t bytes = static_cast<uint32_t>(n) * kMxTileBytes;
                 const int64_t  at    = static_cast<int64_t>(first) * kMxTileBytes;
                 const uint32_t dst   = s_stage + s * P::STAGE, sf = s_sf + s * P::SF_STAGE;
-                if (el)
+                if (el && g != withheld)
                 {
                     mbar_expect_tx(full_bar(s), P::STAGE + 3 * bytes);
                     tma_load_2d(dst, &tmap_g, c * kMxChunkBytes, row, full_bar(s));
@@ -457,11 +461,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
             }
         }
     produced:
-        if (el && *s_abort != 0)
-        {
-            for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-        }
-        __syncwarp();
+        issued = g;
     }
     else if (warp == kMmaWarp)
     {
@@ -609,6 +609,10 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
 
     tc_fence_before();
     __syncthreads();
+    if (warp == 0 && *s_abort != 0)
+    {
+        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold_up : -1, p.spin_limit);
+    }
     if (warp == kMmaWarp)
     {
         tc_fence_after();
@@ -680,14 +684,16 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     const int block      = static_cast<int>(cluster_id_x());
     const int c_begin    = chunk_share(chunks, rank, ranks);
     const int c_end      = chunk_share(chunks, rank + 1, ranks);
+    int       issued     = 0; // stages that the producer has filled
 
     if (warp == 0)
     {
         const bool el = elect_one();
+        const int  withheld = blockIdx.x == 0 ? p.withhold_down : -1;
         auto load_weights = [&](int g) {
             const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, e = s_list[a], first = c * F::kChunkTiles;
             const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
-            if (el)
+            if (el && g != withheld)
             {
                 mbar_expect_tx(full_bar(s), P::STAGE + 2 * bytes);
                 tma_load_2d(s_stage + s * P::STAGE, &tmap_d, c * kMxChunkBytes, e * p.hidden + block * kMxRows, full_bar(s));
@@ -699,7 +705,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
         auto load_tokens = [&](int g) {
             const int      i = c_begin + g, s = g % STAGES, a = i / per_expert, c = i - a * per_expert, first = c * F::kChunkTiles;
             const uint32_t bytes = static_cast<uint32_t>(min(F::kChunkTiles, static_cast<int>(p.f_tiles) - first)) * kMxTileBytes;
-            if (el)
+            if (el && g != withheld)
             {
                 tma_load_2d(s_stage + s * P::STAGE + kMxWBytes, &tmap_h, c * kMxChunkBytes, a * p.tokens, full_bar(s));
                 bulk_load(s_sf + s * P::SF_STAGE + F::kChunkScale, p.hs + (static_cast<int64_t>(a) * p.f_tiles + first) * kMxTileBytes, bytes, full_bar(s));
@@ -721,11 +727,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
             load_weights(g);
             load_tokens(g);
         }
-        if (el && *s_abort != 0)
-        {
-            for (int i = max(0, g - STAGES); i < g; ++i) mbar_drain(full_bar(i % STAGES), static_cast<uint32_t>(i / STAGES) & 1u, p.spin_limit);
-        }
-        __syncwarp();
+        issued = g;
     }
     else if (warp == kMmaWarp)
     {
@@ -814,6 +816,10 @@ __global__ void __launch_bounds__(kDownThreads, 2)
 
     tc_fence_before();
     __syncthreads();
+    if (warp == 0 && *s_abort != 0)
+    {
+        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold_down : -1, p.spin_limit);
+    }
     if (warp == kMmaWarp)
     {
         tc_fence_after();
@@ -1066,6 +1072,9 @@ extern "C"
         p.down_alpha   = std::ldexp(desc->down_alpha, desc->h_exponent);
         p.status       = ctx->d_status;
         p.spin_limit   = ctx->spin_limit;
+        p.withhold_up   = ctx->withhold_kb < kWithholdDown ? ctx->withhold_kb : -1;
+        p.withhold_down = ctx->withhold_kb >= kWithholdDown ? ctx->withhold_kb - kWithholdDown : -1;
+        ctx->withhold_kb = -1;
         const int nt   = desc->tokens <= 16 ? 16 : desc->tokens <= 32 ? 32 : desc->tokens <= 64 ? 64 : 128;
         const int64_t rows_f = static_cast<int64_t>(desc->experts) * desc->intermediate, rows_h = static_cast<int64_t>(desc->experts) * desc->hidden;
         MoeMaps       m;

@@ -108,11 +108,13 @@ CUGL_API cugl_status cugl_context_set_trace_buffer(cugl_context *ctx, void *d_bu
 CUGL_API cugl_status cugl_context_set_wait_limit_us(cugl_context *ctx, uint64_t microseconds);
 /* Test instrument of that path, no reference counterpart: in the NEXT tensor-core GEMM launch of this context the
  * producer of CTA 0 leaves out the operand copies of k-block ordinal `k_block` (counted over the CTA's tile
- * sequence), so that the wait for them runs out.  One shot: the launch after it is normal again. */
+ * sequence), so that the wait for them runs out.  One shot: the launch after it is normal again.  cugl_mx_gemm and cugl_mx_moe
+ * take it too (the latter in its gate and up products, from 65536 on, less 65536, in its down product). */
 CUGL_API cugl_status cugl_context_withhold_copy_once(cugl_context *ctx, int k_block);
 /* The tensor-core kernels are launched with programmatic stream serialization (on by default): a kernel lets the next
  * one in the stream start its prologue (barrier set-up, tensor-memory allocation) while its own last tiles finish, and
- * every kernel waits for its predecessor's completion (griddepcontrol.wait) before its first access to global memory.
+ * every kernel waits for its predecessor's completion (griddepcontrol.wait) before its first access to global memory (but
+ * for cugl_mx_moe's third launch, which reads what was complete before its second, and prefetches into L2).
  * The operand preparation and the short kernels between the products (at most one block per SM) are launched the same way.
  * A stream that is being captured into a CUDA graph gets programmatic edges for short launches only (at most four tiles or
  * blocks per SM; measured slower for longer ones).  0 restores plain stream order everywhere.  No

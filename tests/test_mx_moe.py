@@ -267,6 +267,34 @@ def test_calls_in_a_row_share_a_workspace_and_a_graph(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,k_block", [(1, 6, 0), (40, 40, 3), (128, 40, 2), (1, 6, 65536), (40, 40, 65539), (128, 40, 65537)])
+def test_wait_limit(ctx, tokens, experts, k_block):
+    """Operand copies that never come, in the gate and up products or in the down product: the call ends by its wait limit and says
+    so; the next one is as always.  (1 token: four chunks of K over four CTAs, one copy each to withhold.)"""
+    import torch
+    layer = Layer(51, 1024, 1152, experts, capi.NVFP4)
+    g = torch.Generator().manual_seed(tokens)
+    x, logits = torch.randn((tokens, 1024), generator=g).to(torch.bfloat16).cuda(), torch.randn((tokens, experts), generator=g).cuda()
+    d = layer.desc(tokens, 4, capi.BF16)
+    ws, want, out = workspace(d), torch.zeros_like(x), torch.zeros_like(x)
+    args = (d, x, logits, layer.gate, layer.up, layer.down)
+    ctx.mx_moe(*args, want, ws)
+    ctx.sync()
+    ctx.set_wait_limit_us(20000)
+    try:
+        ctx.withhold_copy_once(k_block)
+        ctx.mx_moe(*args, out, ws)
+        with pytest.raises(capi.CuglError) as e:
+            ctx.sync()
+        assert e.value.status == capi.RUNTIME_ERROR
+    finally:
+        ctx.set_wait_limit_us(0)
+    ctx.mx_moe(*args, out, ws)
+    ctx.sync()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_nothing_to_do_and_refusals(ctx):
     import torch
     p = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda").data_ptr()
