@@ -569,7 +569,7 @@ CUGL_API size_t      cugl_mx_scale_bytes(int32_t rows, int32_t cols, int32_t for
 /* Pure host check of a descriptor; reason (optional) receives a static string. */
 CUGL_API cugl_status cugl_mx_validate(const cugl_mx_desc *desc, const char **reason);
 /* Plain matrix d_src -> packed codes d_dst and scale tiles d_scales.  Bytes between the end of a packed row and the next row
- * are left as they are.  rows == 0: nothing to do. */
+ * are left as they are.  No buffer overlaps another.  rows == 0: nothing to do. */
 CUGL_API cugl_status cugl_mx_quantize(cugl_context *ctx, const cugl_mx_desc *desc, const void *d_src, void *d_dst,
                                       void *d_scales);
 /* The way back: code * scale * 2^tensor_exponent, rounded once to the plain matrix' type. */

@@ -155,6 +155,14 @@ def test_wait_limit(ctx, M, N, K, k_block):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,pad", [(4097, 0), (4098, 0), (4098, 1), (4100, 2)])
+def test_large_ragged_rows(ctx, dtype, N, pad):
+    """Many tiles, long K and rows that bulk stores cannot write: odd, two-byte and four-byte aligned ones."""
+    check(ctx, 1210, N, 3900, capi.NVFP4 if N % 2 else capi.MXFP4, dtype, bias=True, pad=pad)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_long_k(ctx, fmt):
     check(ctx, 3, 130, 70001, fmt, capi.F32)
