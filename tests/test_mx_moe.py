@@ -139,6 +139,15 @@ def test_tokens(ctx, fmt, tokens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(1, 768, 640, 10, 8), (3, 1104, 512, 12, 4), (8, 2032, 208, 24, 3), (1, 3600, 1056, 4, 2),
+                                                               (100, 3600, 1056, 4, 2), (2, 7184, 272, 8, 4), (70, 7184, 272, 4, 2)])
+def test_parts_of_k(ctx, fmt, tokens, hidden, inner, experts, top_k):
+    """Sizes whose K is shared by two or four CTAs in either product, in uneven parts."""
+    check(ctx, Layer(hidden + inner, hidden, inner, experts, fmt), tokens, top_k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_many_experts(ctx, fmt):
     """More units of work than SMs: a CTA works through several."""
     layer = Layer(6, 256, 144, 512, fmt)
