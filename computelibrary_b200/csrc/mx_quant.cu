@@ -48,18 +48,23 @@ __device__ __forceinline__ Place place_of(const QuantParams &p, int group, int l
 // Rows that start anywhere: a warp moves its 256 values as consecutive elements and turns them over in shared memory, where a
 // lane's eight lie in a row.  row: of lane 0's columns; c0: the segment's first column.
 template <typename T>
-__device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c0, int lane, T *area)
+__device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c0, int lane, T (&v)[kLaneCols])
 {
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < kLaneCols; ++i)
     {
         const int at = i * 32 + lane, l = at / kLaneCols, r = row + (l >> p.lane_shift);
         const int c  = c0 + (l & ((1 << p.lane_shift) - 1)) * kLaneCols + at % kLaneCols;
-        T         v  = from_float<T>(0.f);
-        if (r < p.rows && c < p.cols) v = reinterpret_cast<const T *>(p.src + r * p.ld)[c];
-        area[at] = v;
+        v[i]         = from_float<T>(0.f);
+        if (r < p.rows && c < p.cols) v[i] = reinterpret_cast<const T *>(p.src + r * p.ld)[c];
     }
+}
+template <typename T>
+__device__ __forceinline__ void turn_over(int lane, const T (&v)[kLaneCols], T *area)
+{
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kLaneCols; ++i) area[i * 32 + lane] = v[i];
     __syncwarp();
 }
 template <typename T>
@@ -136,7 +141,20 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
     const int     lane   = threadIdx.x & 31;
     const Place   at     = place_of<kSegs, kRows>(p, group, lane);
     uint4         raw[kRows][kSegs][kLoads];
-    if constexpr (kVec)
+    T             loose[kRows][kVec ? 1 : kSegs][kLaneCols];
+    if constexpr (!kVec)
+    {
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+        {
+#pragma unroll
+            for (int g = 0; g < kSegs; ++g)
+            {
+                load_ragged(p, at.row + u * at.step - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, loose[u][g]);
+            }
+        }
+    }
+    else
     {
 #pragma unroll
         for (int u = 0; u < kRows; ++u)
@@ -182,7 +200,7 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
         {
             if constexpr (!kVec)
             {
-                load_ragged(p, row - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, area);
+                turn_over(lane, loose[u][g], area);
 #pragma unroll
                 for (int l = 0; l < kLoads; ++l) raw[u][g][l] = reinterpret_cast<const uint4 *>(area + lane * kLaneCols)[l];
             }
@@ -383,7 +401,11 @@ bool wide(const cugl_context *ctx, const QuantParams &p)
 template <typename T, int kFormat, bool kBack>
 cudaError_t launch_matrix(cugl_context *ctx, const QuantParams &p)
 {
-    if (p.vec_plain == 0) return launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 1, 1, kBack>, p, 1, 1);
+    if (p.vec_plain == 0)
+    {
+        return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 4, 1, kBack>, p, 4, 1)
+                            : launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 1, 1, kBack>, p, 1, 1);
+    }
     return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 4, 1, kBack>, p, 4, 1)
                         : launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 1, 1, kBack>, p, 1, 1);
 }

@@ -207,6 +207,16 @@ def test_strides_and_alignment(ctx, fmt, offset, extra, pitch_extra):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [4097, 4350, 5002])
+def test_many_ragged_rows(ctx, fmt, dtype, cols):
+    import torch
+    g = torch.Generator().manual_seed(cols)
+    round_trip(ctx, torch.randn((607, cols), generator=g).to(torch_dtype(dtype)).cuda(), fmt)
+
+
+@pytest.mark.gpu
 def test_many_rows(ctx):
     """More rows than one launch has blocks of; the last ones are right."""
     import torch
