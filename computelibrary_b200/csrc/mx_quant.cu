@@ -50,6 +50,14 @@ __device__ __forceinline__ Place place_of(const QuantParams &p, int group, int l
 template <typename T>
 __device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c0, int lane, T (&v)[kLaneCols])
 {
+    if (p.lane_shift == 5) // the warp's values lie in one row
+    {
+        const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + c0 + lane;
+        const int n   = row < p.rows ? p.cols - c0 - lane : 0;
+#pragma unroll
+        for (int i = 0; i < kLaneCols; ++i) v[i] = i * 32 < n ? src[i * 32] : from_float<T>(0.f);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kLaneCols; ++i)
     {
@@ -71,6 +79,18 @@ template <typename T>
 __device__ __forceinline__ void store_ragged(const QuantParams &p, int row, int c0, int lane, const T *area)
 {
     __syncwarp();
+    if (p.lane_shift == 5)
+    {
+        T        *dst = reinterpret_cast<T *>(p.dst + row * p.ld) + c0 + lane;
+        const int n   = row < p.rows ? p.cols - c0 - lane : 0;
+#pragma unroll
+        for (int i = 0; i < kLaneCols; ++i)
+        {
+            if (i * 32 < n) dst[i * 32] = area[i * 32 + lane];
+        }
+        __syncwarp();
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kLaneCols; ++i)
     {
