@@ -13,7 +13,7 @@
 // quantisation, down product.  The second lets the third start only after its own wait, i.e. when the first has completed: so
 // the third knows the experts and loads its first weights while the second is still running.
 //
-// us (floor: the chosen experts' weights at the copy rate), hidden 2048, intermediate 768, 64 experts: 1 token, top 8, NVFP4 15
+// us (floor: the chosen experts' weights at the copy rate), hidden 2048, intermediate 768, 64 experts: 1 token, top 8, NVFP4 14.5
 // (3.3), three launches of little else than latency; 48 tokens, top 4, MXFP4 40 (24); 128 tokens, top 8, NVFP4 56 (26), MXFP4
 // 51 (25), where the exchange of the down product's partial sums (64 KB per CTA) and an epilogue that no MMA overlaps are next.
 #include "mx_mma.cuh"
