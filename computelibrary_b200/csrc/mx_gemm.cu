@@ -59,7 +59,7 @@ struct MxPlan
     static constexpr bool OWN_PART   = NT <= 32;
     [[maybe_unused]] static constexpr int OFF_PART    = OWN_PART ? OFF_SF + STAGES * SF_STAGE : 0;
     static constexpr int OFF_BAR     = OFF_SF + STAGES * SF_STAGE + (kSplit && OWN_PART ? NT * kMxRows * 4 : 0);
-    static constexpr int OFF_MISC    = OFF_BAR + (2 * STAGES + 5) * 8;
+    static constexpr int OFF_MISC    = OFF_BAR + (2 * STAGES + 6) * 8;
     static constexpr int DYN_BYTES   = OFF_MISC + 16 + 1024;
     static constexpr int ACC         = kSplit || NT == 128 ? 1 : 2; // accumulators
     static constexpr int SF_COLS     = 2 * F::kChunkCols; // per stage
@@ -147,6 +147,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     auto           tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     auto           tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
     const uint32_t part_bar  = bar_base + 8u * (2 * STAGES + 4);
+    const uint32_t gone_bar  = bar_base + 8u * (2 * STAGES + 5); // see drain_mmas
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -176,6 +177,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
             mbar_init(tempty_bar(a), kEpi);
         }
         mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kEpi));
+        mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
     }
     if (warp == kMmaWarp)
     {
+        if (*s_abort != 0) drain_mmas<false>(gone_bar, p.spin_limit);
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
     }
@@ -434,7 +437,7 @@ struct MxPairPlan
     static constexpr int OFF_OUT  = STAGES * STAGE; // staging: 4 KB per epilogue warp
     static constexpr int OFF_SF   = OFF_OUT + kPairEpi * 4096;
     static constexpr int OFF_BAR  = OFF_SF + STAGES * SF_STAGE;
-    static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 3) * 8;
+    static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 4) * 8;
     static constexpr int DYN_BYTES = OFF_MISC + 16 + 1024;
     static constexpr int SF_COL   = 2 * kPairCols - kPairShared;
     static_assert(SF_COL + 3 * F::kChunkCols <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
@@ -480,6 +483,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto           tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     const uint32_t tempty    = bar_base + 8u * (2 * STAGES + 2);                    // shared columns drained; leader only
+    const uint32_t gone_bar  = bar_base + 8u * (2 * STAGES + 3);                    // see drain_mmas
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -502,6 +506,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         mbar_init(tfull_bar(0), 1);
         mbar_init(tfull_bar(1), 1);
         mbar_init(tempty, 2 * kPairEpi);
+        mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -722,6 +727,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (warp == 0 && rank == 0 && *s_abort != 0)
     {
         drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit); // the leader's barriers count the copies of both CTAs
+    }
+    if (warp == kMmaWarp && rank == 0 && *s_abort != 0)
+    {
+        drain_mmas<true>(gone_bar, p.spin_limit); // a leader that has not given up has drained every accumulator
     }
     cluster_sync(); // neither CTA leaves (or frees tensor memory) while its peer may still touch it
     if (warp == kMmaWarp)

@@ -205,6 +205,26 @@ __device__ __forceinline__ void drain_stages(uint32_t bars, int issued, int with
     __syncwarp();
 }
 
+// Of a kernel that has given up, by the warp that issues its tcgen05 instructions: MMAs and copies of scales may still be reading
+// shared and writing tensor memory, and their commits are still to arrive on this CTA's barriers.  Commits all of them once more to
+// a barrier of its own and waits for it, before the tensor memory is freed and the CTA leaves.  (A commit covers what its thread
+// has issued; elect.sync names the same lane every time.)  kPair: by the leader of an SM pair, whose barriers both get the arrival.
+template <bool kPair>
+__device__ __forceinline__ void drain_mmas(uint32_t bar, long long limit)
+{
+    if (elect_one())
+    {
+        if constexpr (kPair) umma_commit_pair(bar);
+        else umma_commit(bar);
+    }
+    __syncwarp();
+    const long long t0 = clock64(), bound = limit + 2000000;
+    while (!mbar_try_wait(bar, 0) && clock64() - t0 <= bound)
+    {
+    }
+    __syncwarp();
+}
+
 // The MMAs of one chunk whose operands and scales have landed in shared memory.  steps: MMAs inside K (1 .. 4).  a_stage,
 // b_stage: shared addresses of the operands; a_sf, b_sf: of their scale tiles; t_a, t_b: tensor-memory columns for those.
 template <int kFormat>

@@ -341,7 +341,7 @@ struct MoePlan
     static constexpr bool OWN_PART  = PART <= 16384;
     [[maybe_unused]] static constexpr int OFF_PART   = OWN_PART ? OFF_SF + STAGES * SF_STAGE : 0;
     static constexpr int OFF_BAR    = OFF_SF + STAGES * SF_STAGE + (kSplit && OWN_PART ? PART : 0);
-    static constexpr int OFF_MISC   = OFF_BAR + (2 * STAGES + 5) * 8;
+    static constexpr int OFF_MISC   = OFF_BAR + (2 * STAGES + 6) * 8;
     static constexpr int OFF_BITS   = OFF_MISC + 16;
     static constexpr int OFF_LIST   = OFF_BITS + kMaxExperts / 8;
     static constexpr int OFF_WEIGHT = OFF_LIST + kMaxExperts * 2;
@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
     auto           tfull_bar  = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     auto           tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
     const uint32_t part_bar   = bar_base + 8u * (2 * STAGES + 4);
+    const uint32_t gone_bar   = bar_base + 8u * (2 * STAGES + 5); // see drain_mmas
     uint32_t      *s_tmem     = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort    = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_bits     = reinterpret_cast<uint32_t *>(smem + P::OFF_BITS);
@@ -397,6 +398,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
             mbar_init(tempty_bar(a), kUpEpi);
         }
         mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kUpEpi));
+        mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -615,6 +617,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
     }
     if (warp == kMmaWarp)
     {
+        if (*s_abort != 0) drain_mmas<false>(gone_bar, p.spin_limit);
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
     }
@@ -645,6 +648,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     auto           full_bar  = [&](int s) { return bar_base + 8u * s; };
     auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
     const uint32_t tfull     = bar_base + 8u * (2 * STAGES), part_bar = bar_base + 8u * (2 * STAGES + 4);
+    const uint32_t gone_bar  = bar_base + 8u * (2 * STAGES + 5); // see drain_mmas
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_bits    = reinterpret_cast<uint32_t *>(smem + P::OFF_BITS);
@@ -662,6 +666,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
         }
         mbar_init(tfull, 1);
         mbar_init(part_bar, partial_arrivals(31 - __clz(ranks), kDownEpi));
+        mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -822,6 +827,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     }
     if (warp == kMmaWarp)
     {
+        if (*s_abort != 0) drain_mmas<false>(gone_bar, p.spin_limit);
         tc_fence_after();
         tmem_dealloc(tmem_base, P::TMEM_COLS);
     }
