@@ -464,6 +464,31 @@ __device__ __forceinline__ void stage_block(uint32_t s_out, int lane, const uint
     }
 }
 
+// drain_stages of an SM pair, by its leader, whose barriers count the copies of both CTAs: the producers may have stopped at different
+// stages, so what the barrier of a stage that only one of them has filled still expects, or does not expect yet, is put right first.
+// bytes: of one CTA's copies of a stage.  (The counts are at most STAGES apart: both wait for the same MMAs.)
+template <int STAGES, typename Bytes>
+__device__ __forceinline__ void drain_pair_stages(uint32_t bars, int issued, int peer, int withheld, long long limit, Bytes bytes)
+{
+    const int end = max(issued, peer);
+    for (int i = max(0, end - STAGES); i < end; ++i)
+    {
+        const uint32_t bar = bars + 8u * (i % STAGES);
+        const bool     own = i < issued && i != withheld, other = i < peer;
+        if (own != other && elect_one())
+        {
+            if (own) mbar_complete_tx(bar, bytes(i)); // expected, but the peer never asked for it
+            else mbar_expect_tx(bar, bytes(i));       // the other way round
+        }
+        __syncwarp();
+        const long long t0 = clock64(), bound = limit + 2000000;
+        while ((own || other) && !mbar_try_wait(bar, static_cast<uint32_t>(i / STAGES) & 1u) && clock64() - t0 <= bound)
+        {
+        }
+    }
+    __syncwarp();
+}
+
 template <int kFormat, int kBulk>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,
@@ -486,6 +511,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t gone_bar  = bar_base + 8u * (2 * STAGES + 3);                    // see drain_mmas
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
+    uint32_t      *s_peer    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC + 8); // stages the peer has filled; bit 31: it has given up
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int      rank = static_cast<int>(cluster_ctarank());
 
@@ -724,15 +750,29 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 0 && rank == 0 && *s_abort != 0)
+    if (threadIdx.x == 0)
     {
-        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit); // the leader's barriers count the copies of both CTAs
+        st_cluster_u32(map_to_cta(smem_u32(s_peer), rank ^ 1), static_cast<uint32_t>(issued) | (*s_abort != 0 ? 0x80000000u : 0u));
     }
-    if (warp == kMmaWarp && rank == 0 && *s_abort != 0)
-    {
-        drain_mmas<true>(gone_bar, p.spin_limit); // a leader that has not given up has drained every accumulator
-    }
+    __syncwarp();
     cluster_sync(); // neither CTA leaves (or frees tensor memory) while its peer may still touch it
+    const uint32_t peer = *s_peer;
+    if (*s_abort != 0 || (peer >> 31) != 0) // given up, here or there: the same in both CTAs
+    {
+        if (rank == 0 && warp == 0)
+        {
+            drain_pair_stages<STAGES>(
+                bar_base, issued, static_cast<int>(peer & 0x7fffffffu), blockIdx.x == 0 ? p.withhold : -1, p.spin_limit, [&](int g) {
+                    return first + static_cast<int64_t>(g / chunks) * stride < p.whole ? P::STAGE + P::SF_STAGE
+                                                                                     : kMxWBytes + kMxWBytes / 2 + 2 * F::kChunkScale;
+                });
+        }
+        if (rank == 0 && warp == kMmaWarp)
+        {
+            drain_mmas<true>(gone_bar, p.spin_limit);
+        }
+        cluster_sync();
+    }
     if (warp == kMmaWarp)
     {
         tc_fence_after();

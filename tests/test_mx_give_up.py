@@ -47,7 +47,8 @@ def check(ctx, call, out, sure=True):
 
 @pytest.mark.parametrize("fmt", [capi.MXFP4, capi.NVFP4])
 @pytest.mark.parametrize("M,N,K", [(16, 128, 2 ** 24), (30, 256, 2 ** 24), (64, 128, 2 ** 24), (100, 128, 2 ** 24),  # K shared by a cluster
-                                   (40, 19200, 2 ** 20), (100, 4864, 2 ** 21)])                                     # a CTA per tile
+                                   (40, 19200, 2 ** 20), (100, 4864, 2 ** 21),                                      # a CTA per tile
+                                   (512, 4096, 2 ** 21), (2048, 8192, 2 ** 20)])                                    # SM pairs, halves of tiles, both
 def test_products(ctx, fmt, M, N, K):
     import torch
     g = torch.Generator(device="cuda").manual_seed(M)
