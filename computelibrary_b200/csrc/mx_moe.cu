@@ -196,14 +196,27 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const __grid_constant__ 
 }
 
 // ---- what the two product launches share ---------------------------------------------------------------------
+// A choice as the first launch left it.  kEarly: read ahead of griddepcontrol.wait, by the third launch.  The first launch had
+// completed before the second let the third start, so its writes are performed on the device; but nothing makes a line that an
+// earlier call left in this SM's L1 stale, and a workspace has the same addresses every time.  Hence a load at device scope, which
+// goes to L2 (and, unlike acquiring ones, does not hold up the next).
+template <bool kEarly>
+__device__ __forceinline__ int chosen_id(const int32_t *at)
+{
+    if constexpr (!kEarly) return *at;
+    int32_t v;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+    return v;
+}
 // Experts that some token chose, in order.  list: [kMaxExperts], bits: [kMaxExperts / 32] in shared memory.
+template <bool kEarly>
 __device__ __forceinline__ int active_experts(const MoeParams &p, uint16_t *list, uint32_t *bits)
 {
     if (threadIdx.x < kMaxExperts / 32) bits[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.tokens * p.top_k; i += static_cast<int>(blockDim.x))
     {
-        const int e = p.ids[i];
+        const int e = chosen_id<kEarly>(p.ids + i);
         if (e >= 0) atomicOr(&bits[e >> 5], 1u << (e & 31));
     }
     __syncthreads();
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
     griddep_wait(); // the prologue above touched no global memory
     griddep_launch_dependents();
 
-    const int active      = active_experts(p, s_list, s_bits);
+    const int active      = active_experts<false>(p, s_list, s_bits);
     const int blocks      = (p.inner + kMxRows - 1) / kMxRows;
     const int units       = active * blocks;
     const int chunks      = (p.hidden + kMxChunk - 1) / kMxChunk;
@@ -682,7 +695,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     griddep_launch_dependents();
 
     // before the wait for the second launch: what the first one wrote, and the weights
-    const int active     = active_experts(p, s_list, s_bits);
+    const int active     = active_experts<true>(p, s_list, s_bits);
     const int per_expert = (p.inner + kMxChunk - 1) / kMxChunk;
     const int chunks     = active * per_expert;
     const int blocks     = (p.hidden + kMxRows - 1) / kMxRows;

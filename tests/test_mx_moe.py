@@ -276,6 +276,31 @@ def test_calls_in_a_row_share_a_workspace_and_a_graph(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 20])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_many_calls_in_a_row_on_one_workspace(ctx, fmt, tokens):
+    """Other experts in every call, nothing awaited in between: a launch that runs ahead reads the choices of its own call."""
+    import torch
+    layer = Layer(61, 512, 256, 48, fmt)
+    g = torch.Generator().manual_seed(tokens)
+    calls = 300
+    x = torch.randn((calls, tokens, 512), generator=g).to(torch.bfloat16).cuda()
+    logits = torch.randn((calls, tokens, 48), generator=g).cuda()
+    d = layer.desc(tokens, 4, capi.BF16)
+    ws = workspace(d)
+    alone, row = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    for i in range(calls):
+        ctx.mx_moe(d, x[i], logits[i], layer.gate, layer.up, layer.down, alone[i], ws)
+        ctx.sync()
+    for i in range(calls):
+        ctx.mx_moe(d, x[i], logits[i], layer.gate, layer.up, layer.down, row[i], ws)
+    ctx.sync()
+    assert torch.equal(row, alone)
+    want, tol = expected(layer, x[calls - 1], logits[calls - 1], 4, capi.BF16)
+    assert (np.abs(row[-1].double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,experts,k_block", [(1, 6, 0), (40, 40, 3), (128, 40, 2), (1, 6, 65536), (40, 40, 65539), (128, 40, 65537)])
 def test_wait_limit(ctx, tokens, experts, k_block):
     """Operand copies that never come, in the gate and up products or in the down product: the call ends by its wait limit and says
