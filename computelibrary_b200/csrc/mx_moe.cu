@@ -749,6 +749,7 @@ __global__ void __launch_bounds__(kDownThreads, 2)
     }
     else if (warp == kMmaWarp)
     {
+        griddep_wait(); // the tokens' half of a stage comes after the second launch, whose time is not to count in this one's waits
         const bool el = elect_one();
         int  g  = 0;
         bool ok = true;

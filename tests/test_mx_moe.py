@@ -329,6 +329,34 @@ def test_wait_limit(ctx, tokens, experts, k_block):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hidden,inner,experts", [(1024, 256, 6), (1024, 128, 20)])
+def test_time_of_the_second_launch_counts_in_no_wait_of_the_third(ctx, fmt, hidden, inner, experts):
+    """A copy withheld in the gate and up products keeps the second launch busy for the whole limit.  The third, all of which is on the
+    device by then, has waited for nothing of its own: it carries on and writes its results, whatever they are, although the call
+    says that a wait ran out.  (Both would run out of the limit within microseconds of each other: which comes first is chance, so
+    this can pass without the wait it is about.)"""
+    import torch
+    layer = Layer(71, hidden, inner, experts, fmt)
+    g = torch.Generator().manual_seed(1)
+    x, logits = torch.randn((1, hidden), generator=g).to(torch.bfloat16).cuda(), torch.randn((1, experts), generator=g).cuda()
+    d = layer.desc(1, 4, capi.BF16)
+    ws = workspace(d)
+    for limit in (3000, 20000):
+        out = torch.full_like(x, 7.0)
+        ctx.set_wait_limit_us(limit)
+        try:
+            ctx.withhold_copy_once(0)
+            ctx.mx_moe(d, x, logits, layer.gate, layer.up, layer.down, out, ws)
+            with pytest.raises(capi.CuglError) as e:
+                ctx.sync()
+            assert e.value.status == capi.RUNTIME_ERROR
+        finally:
+            ctx.set_wait_limit_us(0)
+        assert not (out == 7).any()
+
+
+@pytest.mark.gpu
 def test_nothing_to_do_and_refusals(ctx):
     import torch
     p = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda").data_ptr()
