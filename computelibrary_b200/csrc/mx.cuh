@@ -167,7 +167,7 @@ __device__ __forceinline__ void scale_to_codes(float (&v)[kCount], const MxScale
         for (int i = 0; i < kCount; ++i)
         {
             const float q = __fmul_rn(v[i], s.mul);
-            v[i]          = __fmaf_rn(__fmaf_rn(-q, s.unit, v[i]), s.mul, q);
+            v[i]          = copysignf(__fmaf_rn(__fmaf_rn(-q, s.unit, v[i]), s.mul, q), v[i]); // -0: the remainder 0 would turn it into 0
         }
         return;
     }

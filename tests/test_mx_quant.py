@@ -184,6 +184,32 @@ def test_32_bit_corners(ctx, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols,exponent", [(96, 0), (2048, 0), (77, 0), (96, -5), (1030, 7)])
+def test_signs_of_zeros(ctx, fmt, dtype, cols, exponent):
+    """A zero, or a value that rounds to it, keeps its sign in its code and on the way back, whatever type it comes from: codes bit for
+    bit in every finite block."""
+    import torch
+    exponent = exponent if fmt == capi.NVFP4 else 0
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn((40, cols), generator=g)
+    x[torch.rand((40, cols), generator=g) < 0.3] *= 1e-3
+    x[torch.rand((40, cols), generator=g) < 0.3] *= 0.0
+    x[1], x[2], x[3, ::2] = 0.0, -0.0, -0.0
+    x = (x * 2.0 ** exponent).to(torch_dtype(dtype)).cuda()
+    assert (torch.signbit(x) & (x == 0)).any()
+    q = Stored(40, cols, fmt)
+    d = capi.make_mx_desc(40, cols, fmt, dtype, tensor_exponent=exponent)
+    ctx.mx_quantize(d, x, q.raw, q.scales)
+    code, byte = mx.quantize(x.double().cpu().numpy(), fmt, exponent)
+    assert np.array_equal(q.bytes(), byte) and np.array_equal(q.codes(), code)
+    y = torch.full_like(x, 7.0)
+    ctx.mx_dequantize(d, q.raw, q.scales, y)
+    assert torch.equal(torch.signbit(y), torch.signbit(x))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("exponent", [-64, -6, 3, 64])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tensor_exponent(ctx, dtype, exponent):
