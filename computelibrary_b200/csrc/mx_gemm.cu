@@ -91,6 +91,7 @@ __device__ __forceinline__ void store_block(const MxGemmParams &p, int m, int n,
                 *reinterpret_cast<uint32_t *>(dst + j * p.ldd) = *reinterpret_cast<const uint32_t *>(two);
             }
         }
+        __syncwarp(); // aligned loads of tensor memory may be next
         return;
     }
     if (n < p.channels)
@@ -733,6 +734,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         if (j < cols && n0 < p.channels) tma_store_2d(&tmap_out, s_out, n0, m0 + j);
                         tma_store_commit();
                     }
+                    __syncwarp();
                 }
                 else
                 {

@@ -269,6 +269,7 @@ __device__ __forceinline__ bool begin_unit(const MoeParams &p, float *table, int
             }
         }
     }
+    __syncwarp(); // the barrier is an aligned one
     uint32_t r;
     asm volatile("{\n\t"
                  ".reg .pred p, q;\n\t"
@@ -338,6 +339,7 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, const in
             if (scale_lane) scales[mx_scale_offset(t[i], f / kBlock, p.f_tiles)] = static_cast<uint8_t>(s[i].byte);
         }
     }
+    __syncwarp(); // aligned loads of tensor memory may be next
 }
 
 // kOperands: weight matrices that share a stage's tokens (2: gate and up, 1: down).  Up to 64 tokens two CTAs share an SM.
