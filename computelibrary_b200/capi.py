@@ -275,7 +275,9 @@ def _dptr(t):
     try:
         return t.data_ptr()
     except AttributeError:
-        return t
+        if t is None or isinstance(t, int):
+            return t
+        raise
 
 
 class Context:

@@ -104,3 +104,16 @@ def test_product_does_not_touch_the_oracle():
             if f.endswith((".py", ".cu", ".cuh", ".cpp", ".h", ".hpp")):
                 text = open(os.path.join(root, f), errors="ignore").read()
                 assert "import oracle" not in text and "gemmlowp_oracle" not in text and "libacl_ref" not in text, f
+
+
+@pytest.mark.parametrize("what", [b"0123456789abcdef", "text", bytearray(16), 1.5, [1], np.zeros(4, np.float32), (C.c_char * 16)(), C.c_void_p(16)])
+def test_device_pointers_are_tensors_integers_or_none(what):
+    """What is no device buffer is refused by the binding; a bytes or ctypes object would go down as a host address."""
+    with pytest.raises(AttributeError):
+        capi._dptr(what)
+
+
+def test_device_pointers():
+    import torch
+    t = torch.zeros(4)
+    assert capi._dptr(t) == t.data_ptr() and capi._dptr(4096) == 4096 and capi._dptr(None) is None
