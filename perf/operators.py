@@ -277,13 +277,13 @@ _kept = {}
 
 
 def _context():
-    """The context a program keeps for its stream."""
+    """The context a program keeps for its stream (the default stream's handle is the same on every device)."""
     import computelibrary_b200 as cl
 
-    stream = torch.cuda.current_stream().cuda_stream
-    if stream not in _kept:
-        _kept[stream] = cl.Context(torch.cuda.current_device(), stream)
-    return _kept[stream]
+    at = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    if at not in _kept:
+        _kept[at] = cl.Context(*at)
+    return _kept[at]
 
 
 def _describe(s):
