@@ -3230,6 +3230,7 @@ using EncodeIm2colFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32
                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeIm2colFn get_encode_im2col_fn()
 {
+    need_thread_context();
     static EncodeIm2colFn fn = []() -> EncodeIm2colFn {
         void                           *p = nullptr;
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;

@@ -409,8 +409,33 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// The driver's encoders want a context that is current in the calling thread.  A thread that has made no CUDA call yet, or only asked
+// for its device, has none: its device's primary one is made current, as the runtime's first launch would.
+void need_thread_context()
+{
+    thread_local bool has = false;
+    if (has)
+    {
+        return;
+    }
+    void                           *p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    CUcontext                       current = nullptr;
+    int                             device  = 0;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+    {
+        (void)reinterpret_cast<CUresult (*)(CUcontext *)>(p)(&current);
+    }
+    has = current != nullptr || (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess);
+    if (!has)
+    {
+        (void)cudaGetLastError(); // the encoder will say what is wrong
+    }
+}
+
 EncodeTiledFn get_encode_fn()
 {
+    need_thread_context();
     static EncodeTiledFn fn = []() -> EncodeTiledFn {
         void                           *p = nullptr;
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;

@@ -131,6 +131,65 @@ def test_two_streams_at_a_time(ctx):
 
 
 @pytest.mark.gpu
+def test_threads_at_a_time(ctx):
+    """Threads with contexts of their own make their calls at once (a kernel's first ones among them): the bits are those of one thread."""
+    import threading
+    import torch
+    import computelibrary_b200 as cl
+    rng = np.random.default_rng(6)
+    jobs = []
+    for fmt in FORMATS:
+        for M, N, K in ((1, 500, 300), (20, 300, 600), (50, 300, 600), (100, 260, 900), (300, 2048, 2048)):
+            a, sa, _ = test_mx_gemm.operand(rng, M, K, fmt)
+            b, sb, _ = test_mx_gemm.operand(rng, N, K, fmt)
+            jobs.append((capi.make_mx_gemm_desc(M, N, K, fmt, capi.F32), a, sa, b, sb))
+    layers = []
+    for fmt in FORMATS:
+        layer = test_mx_moe.Layer(81, 256, 160, 12, fmt)
+        for tokens in (2, 30, 60, 100):
+            x, logits = torch.from_numpy(rng.standard_normal((tokens, 256))).to(torch.bfloat16).cuda(), torch.from_numpy(rng.standard_normal((tokens, 12))).float().cuda()
+            layers.append((layer.desc(tokens, 3, capi.BF16), x, logits, layer.gate, layer.up, layer.down))
+
+    def buffers():
+        return ([torch.zeros((j[0].M, j[0].N), device="cuda") for j in jobs], [torch.zeros_like(x) for _, x, *_ in layers],
+                [test_mx_moe.workspace(d) for d, *_ in layers])
+
+    def run(context, out):
+        for j, y in zip(jobs, out[0]):
+            context.mx_gemm(*j, None, y)
+        for j, y, ws in zip(layers, out[1], out[2]):
+            context.mx_moe(*j, y, ws)
+
+    sets = [buffers() for _ in range(5)]
+    contexts = [cl.Context(0, torch.cuda.Stream().cuda_stream) for _ in range(4)]
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(4), []
+
+    def thread(context, out):
+        try:
+            start.wait()
+            for _ in range(3):
+                run(context, out)
+            context.sync()
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=a) for a in zip(contexts, sets)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    run(ctx, sets[4])
+    ctx.sync()
+    for out in sets[:4]:
+        for got, alone in zip(out[0] + out[1], sets[4][0] + sets[4][1]):
+            assert torch.equal(got, alone)
+    for context in contexts:
+        context.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_without_overlapped_launches(ctx, fmt):
     import torch
