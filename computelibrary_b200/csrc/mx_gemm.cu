@@ -804,17 +804,6 @@ bool encode_dst_map(CUtensorMap *map, const MxGemmParams &p)
                                CU_TENSOR_MAP_INTERLEAVE_NONE, p.dtype == CUGL_F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename K>
-cugl_status allow_smem(cugl_context *ctx, K kernel, int bytes, bool (&set)[64])
-{
-    if (!set[ctx->device & 63])
-    {
-        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        set[ctx->device & 63] = true;
-    }
-    return CUGL_SUCCESS;
-}
-
 template <int kFormat, int NT, int STAGES, bool kSplit>
 cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, int ranks)
 {
@@ -826,7 +815,7 @@ cugl_status launch_one(cugl_context *ctx, const MxOperands &op, MxGemmParams p, 
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for a packed operand");
     }
     auto        kernel  = mx_gemm_kernel<kFormat, NT, STAGES, kSplit>;
-    static bool set[64] = {}; // per instantiation and device
+    static std::atomic<bool> set[64] = {}; // per instantiation and device
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc             = mx_idesc(kFormat, kMxRows, NT);
     const int64_t tiles = static_cast<int64_t>((p.channels + kMxRows - 1) / kMxRows) * ((p.tokens + NT - 1) / NT);
@@ -861,7 +850,7 @@ cugl_status launch_pair(cugl_context *ctx, const MxOperands &op, MxGemmParams p)
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for an operand");
     }
     auto        kernel  = mx_gemm_pair_kernel<kFormat, kBulk>;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc      = mx_idesc(kFormat, 2 * kMxRows, kPairCols);
     p.idesc_half = mx_idesc(kFormat, 2 * kMxRows, kPairCols / 2);

@@ -12,6 +12,8 @@
 #include "mx.cuh"
 #include "sm100.cuh"
 
+#include <atomic>
+
 namespace cugl
 {
 namespace
@@ -342,6 +344,19 @@ inline int mx_split(long long tiles, int chunks, int most)
     if (most >= 4 && tiles <= 71 && chunks >= 4) return 4;
     if (most >= 2 && tiles <= 148 && chunks >= 2) return 2;
     return 1;
+}
+
+// Lets a kernel have its dynamic shared memory, once per device: set is the kernel's own.  Threads with contexts of their own may come
+// here at once; each then sets the attribute, to the same value.
+template <typename K>
+cugl_status allow_smem(cugl_context *ctx, K kernel, int bytes, std::atomic<bool> (&set)[64])
+{
+    if (!set[ctx->device & 63].load(std::memory_order_acquire))
+    {
+        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        set[ctx->device & 63].store(true, std::memory_order_release);
+    }
+    return CUGL_SUCCESS;
 }
 
 // packed rows x (inner bytes), ld bytes apart; box = box_rows x 128 bytes in the 128-byte swizzle; what lies outside reads as 0

@@ -912,17 +912,6 @@ const char *validate_moe(const cugl_mx_moe_desc *d)
     return nullptr;
 }
 
-template <typename K>
-cugl_status allow_smem(cugl_context *ctx, K kernel, int bytes, bool (&set)[64])
-{
-    if (!set[ctx->device & 63])
-    {
-        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        set[ctx->device & 63] = true;
-    }
-    return CUGL_SUCCESS;
-}
-
 struct MoeMaps
 {
     CUtensorMap gate, up, x, down, h;
@@ -933,7 +922,7 @@ cugl_status launch_gate_up(cugl_context *ctx, const MoeMaps &m, const MoeParams 
 {
     using P     = MoePlan<kFormat, NT, STAGES, 2, kSplit, kAcc>;
     auto kernel = moe_gate_up_kernel<kFormat, NT, STAGES, kSplit, kAcc>;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int slots = P::PER_SM * ctx->sm_count;
     const int grid  = kSplit ? most_units * ranks : (most_units < slots ? most_units : slots);
@@ -962,7 +951,7 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     }
     using P     = MoePlan<kFormat, NT, kDownStages, 1, true, 1>;
     auto kernel = moe_down_kernel<kFormat, NT, kDownStages>;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64] = {};
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     const int blocks = (p.hidden + kMxRows - 1) / kMxRows, most_chunks = most_active * ((p.inner + kMxChunk - 1) / kMxChunk);
     ranks = mx_split(blocks, most_chunks, 8);
