@@ -941,11 +941,11 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     // Up to eight tokens and eight chunks: one CTA per SM instead of two (intermediate 768, 64 experts, top 8: 48 units).  1 token, hidden
     // 2048, NVFP4 15.2 -> 14.4 us, MXFP4 14.5 -> 13.5; longer rows lose (hidden 8192 23.7 -> 27.1), 16 tokens do (15.9 -> 16.3).
     if (ranks == 4 && most_units * 4 > ctx->sm_count && chunks <= 8 && p.tokens <= 8) ranks = 2;
-    if (ranks > 1)
+    if constexpr (NT <= 64)
     {
-        CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, true, 1>(ctx, m, p, most_units, ranks)));
+        if (ranks > 1) CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, true, 1>(ctx, m, p, most_units, ranks)));
     }
-    else
+    if (ranks == 1)
     {
         CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, false, kUpAcc>(ctx, m, p, most_units, 1)));
     }
