@@ -414,11 +414,14 @@ cudaError_t launch_rows(cugl_context *ctx, K kernel, QuantParams p, int segs, in
     const dim3 grid(static_cast<unsigned>((p.cols + cols - 1) / cols), static_cast<unsigned>(p.groups < 65535 ? p.groups : 65535));
     return launch_dependent(ctx, kernel, grid, kWarps * 32, 0, static_cast<long long>(grid.x) * grid.y, p);
 }
-// Four segments of a row where there are enough rows and columns to keep the device busy that way, else one.  (Read-back
-// of 5780 x 3014 F32: one 27.7 us, four 19.1; of 300 x 9001, 2400 items of four: one 5.3, four 5.7.)
+// Four segments of a row where there are enough rows and columns to keep the device busy that way, else one: from 24 items of four per
+// SM on.  us with one segment / four, items rows * (cols / 1024): BF16 -> MXFP4 of 4096 columns, 2400 items 3.07 / 2.76, 3552 3.80 / 3.06,
+// 11840 9.34 / 6.32, and back 2.59 / 2.98, 3.24 / 3.28, 7.47 / 5.78; F32 -> NVFP4 3.71 / 4.01, 4.84 / 4.10, 12.5 / 10.4, and back
+// 3.09 / 3.82, 3.89 / 3.48, 8.84 / 8.70; read-back of F32 rows of 3014 4.9 / 5.8, 6.4 / 5.9, 18.0 / 14.2.  (Rows that end early in their
+// last block of four are quantised slower by it at any size: 1281 columns, BF16 -> MXFP4, 11840 items 21.5 / 23.0.)
 bool wide(const cugl_context *ctx, const QuantParams &p)
 {
-    return p.cols >= 4 * kItemCols && static_cast<int64_t>(p.rows) * (p.cols / (4 * kItemCols)) >= 16ll * ctx->sm_count;
+    return p.cols >= 4 * kItemCols && static_cast<int64_t>(p.rows) * (p.cols / (4 * kItemCols)) >= 24ll * ctx->sm_count;
 }
 template <typename T, int kFormat, bool kBack>
 cudaError_t launch_matrix(cugl_context *ctx, const QuantParams &p)

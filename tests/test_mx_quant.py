@@ -243,6 +243,17 @@ def test_many_ragged_rows(ctx, fmt, dtype, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(911, 4096), (1801, 2304), (911, 4097), (3600, 1031), (1203, 5002)])
+def test_many_rows_of_several_segments(ctx, fmt, dtype, rows, cols):
+    """As many items as the kernels that take four segments at a time want, aligned rows and others, last segments that are not full."""
+    import torch
+    g = torch.Generator().manual_seed(rows)
+    round_trip(ctx, torch.randn((rows, cols), generator=g).to(torch_dtype(dtype)).cuda(), fmt)
+
+
+@pytest.mark.gpu
 def test_many_rows(ctx):
     """More rows than one launch has blocks of; the last ones are right."""
     import torch
