@@ -938,9 +938,10 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     const int chunks     = (p.hidden + kMxChunk - 1) / kMxChunk;
     // at most four: a rank then owns 32 channels of a unit, one MXFP4 block; and only where two CTAs share an SM (mx_split)
     int ranks = NT <= 64 ? mx_split(most_units, chunks, 4) : 1;
-    // Up to eight tokens and eight chunks: one CTA per SM instead of two (intermediate 768, 64 experts, top 8: 48 units).  1 token, hidden
-    // 2048, NVFP4 15.2 -> 14.4 us, MXFP4 14.5 -> 13.5; longer rows lose (hidden 8192 23.7 -> 27.1), 16 tokens do (15.9 -> 16.3).
-    if (ranks == 4 && most_units * 4 > ctx->sm_count && chunks <= 8 && p.tokens <= 8) ranks = 2;
+    // Up to eight tokens and twelve chunks: one CTA per SM instead of two.  us with 2 / 4 CTAs per unit, 48 units: hidden 1536, 1 token NVFP4
+    // 13.2 / 14.3, 2048 14.1 / 15.1 and MXFP4 13.3 / 14.5, 2560 14.7 / 15.5, 13.7 / 14.9, 2880 15.1 / 16.0, 14.7 / 15.4, 3584 16.1 / 16.5 (8 tokens
+    // 16.9 / 16.5), 4096 17.5 / 16.9, 16.4 / 16.1, 6144 20.5 / 19.1, 8192 26.2 / 22.6; 16 tokens, hidden 2048, 16.3 / 15.9.
+    if (ranks == 4 && most_units * 4 > ctx->sm_count && chunks <= 12 && p.tokens <= 8) ranks = 2;
     if constexpr (NT <= 64)
     {
         if (ranks > 1) CUGL_TRY((launch_gate_up<kFormat, NT, kUpStages, true, 1>(ctx, m, p, most_units, ranks)));
@@ -961,6 +962,8 @@ cugl_status launch_layers(cugl_context *ctx, const MoeMaps &m, const MoeParams &
     // of 128 columns are the greater cost: 100 tokens, intermediate 512, 4 experts 34 -> 28, 128 tokens, 1536, 64 experts 158 -> 148.
     // Half the SMs idle: 128 tokens, hidden 2560 (20 blocks) 41.7 -> 46;
     // two parts of 128 columns instead of four, hidden 8192: 43.7 -> 46.3 (1 token, 8 chunks: 16.0 -> 15.3).
+    // Ten layers (hidden 1024 .. 8192, 4 .. 64 experts) with 1, 8, 48, 100 and 128 tokens in both formats: within 5 % of the best of 2, 4 and 8
+    // parts, but for MXFP4, hidden 4096, intermediate 1536, 64 experts and 48 tokens (eight 130, four 119).
     while (ranks > 2 && blocks * ranks > ctx->sm_count && blocks * ranks / 2 >= ctx->sm_count * 3 / 4 &&
            (NT == 128 ? ranks == 8 : most_chunks <= 6 * ranks))
     {

@@ -148,6 +148,14 @@ def test_parts_of_k(ctx, fmt, tokens, hidden, inner, experts, top_k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(1, 2320, 640, 10, 8), (8, 2864, 640, 10, 8), (1, 3056, 768, 8, 8), (7, 3344, 640, 10, 8)])
+def test_parts_of_longer_rows(ctx, fmt, tokens, hidden, inner, experts, top_k):
+    """Rows of ten to fourteen chunks over two or four CTAs, few tokens and enough units for one CTA per SM."""
+    check(ctx, Layer(hidden + inner, hidden, inner, experts, fmt), tokens, top_k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_many_experts(ctx, fmt):
     """More units of work than SMs: a CTA works through several."""
     layer = Layer(6, 256, 144, 512, fmt)
