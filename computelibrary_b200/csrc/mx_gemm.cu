@@ -877,7 +877,9 @@ cugl_status launch_product(cugl_context *ctx, const MxOperands &op, const MxGemm
     {
         // us on one CTA per tile / an SM pair: 256 x 4096 x 4096 (64 tiles) 11.3 / 10.1, 256 x 7168 x 4096 12.5 / 11.0, 512 x 14336 x 4096
         // 23.2 / 18.7, 2048 x 4096 x 512 9.6 / 8.5; 1024 x 1024 x 1024 (64 tiles) 5.6 / 6.0, 150 x 2048 x 14336 (32 tiles, shared K)
-        // 13.8 / 21.3.  Without bulk stores the pair's epilogue is the slower one unless K is long: F32 2048 x 4096 x 1024 12.6 / 16.4.
+        // 13.8 / 21.3.  Without bulk stores the pair's epilogue is the slower one unless K is long: 2048 x 4097 F32 NVFP4, K = 1024 13.7 / 16.5,
+        // 2048 17.6 / 18.4, 3584 23.1 / 21.6, 4096 24.8 / 22.8, 8192 38.4 / 32.8; BF16 15.2 / 21.0, 19.7 / 23.0, 25.9 / 26.0, 26.0 / 25.1, 40.0 /
+        // 34.5; MXFP4 BF16 13.7 / 19.2, 16.9 / 20.8, 22.2 / 23.5, 24.2 / 24.3, 36.6 / 32.7; 3000 x 6001 turns at K of 2048 to 3584.
         // A bulk store wants 16-byte aligned rows and clips at the end of a row in whole 16-byte units.
         const int  size = dtype_size(p.dtype);
         const bool bulk = ((reinterpret_cast<uintptr_t>(p.dst) | static_cast<uintptr_t>(p.ldd)) & 15) == 0 && p.channels * static_cast<int64_t>(size) % 16 == 0 &&
