@@ -156,6 +156,14 @@ def test_parts_of_longer_rows(ctx, fmt, tokens, hidden, inner, experts, top_k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,hidden,inner", [(2, 18944, 48), (2, 18960, 48), (30, 19088, 32), (60, 19200, 16), (100, 19216, 32), (3, 38032, 16)])
+def test_long_rows(ctx, fmt, tokens, hidden, inner):
+    """From 148 output blocks on the down product runs without clusters, from 296 on in several waves."""
+    check(ctx, Layer(hidden, hidden, inner, 3, fmt), tokens, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_many_experts(ctx, fmt):
     """More units of work than SMs: a CTA works through several."""
     layer = Layer(6, 256, 144, 512, fmt)
