@@ -554,7 +554,8 @@ def mx_gemm_validate(desc: MxGemmDesc):
 def make_mx_moe_desc(tokens, hidden, intermediate, experts, top_k, format, dtype, renormalize=True, x_exponent=0, h_exponent=0,
                      gate_alpha=1.0, up_alpha=1.0, down_alpha=1.0, ld_x=None, ld_logits=None, ld_dst=None, ld_gate_up=None,
                      ld_down=None) -> MxMoeDesc:
-    """cugl_mx_moe_desc; dense x, logits and dst and packed rows mx_pitch apart unless strides (bytes) are given."""
+    """cugl_mx_moe_desc; dense x, logits and dst and packed rows mx_pitch apart unless strides (bytes) are given.  NVFP4: h_exponent has to
+    follow the size of what h stores, the gate's weight included (include/cugl.h)."""
     d = MxMoeDesc()
     d.tokens, d.hidden, d.intermediate, d.experts, d.top_k = tokens, hidden, intermediate, experts, top_k
     d.format, d.dtype, d.renormalize, d.x_exponent, d.h_exponent = format, dtype, int(renormalize), x_exponent, h_exponent

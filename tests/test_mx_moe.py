@@ -57,6 +57,24 @@ def test_choice_of_the_reference():
     assert picks[0][0][1] == 0.5 and picks[1][0][1] == 1.0
 
 
+@pytest.mark.parametrize("size", [1.0, 0.1])
+def test_h_exponent_follows_the_gate_weight(size):
+    """What the header says of it: with small weights E4M3 scales of h run out at exponent 0, and with one that follows their size the
+    error is that of h quantised without them."""
+    rng = np.random.default_rng(3)
+    h, p = rng.standard_normal((256, 256)) * size, 1 / 128
+    w = rng.standard_normal((256, 64))
+
+    def error(stored):
+        return np.linalg.norm((stored - p * h) @ w) / np.linalg.norm(p * h @ w)
+
+    apart = error(p * mx.values(*mx.quantize(h, mx.NVFP4), mx.NVFP4))
+    folded = {e: error(mx.values(*mx.quantize(p * h, mx.NVFP4, e), mx.NVFP4, e)) for e in (0, -6, -9)}
+    assert folded[0] > 1.3 * apart and folded[-9] < 1.05 * apart
+    if size == 1.0:
+        assert folded[-6] < 1.05 * apart
+
+
 # ---- on the GPU -------------------------------------------------------------------------------------------
 class Layer:
     def __init__(self, seed, hidden, inner, experts, fmt, pitch_extra=0):
