@@ -392,8 +392,10 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
 // What bounds it: power.  4096 x 14336 x 4096 NVFP4 takes 96 us by itself (5.0 PFLOP/s) and 112 to 116 back to back, where the
 // clock falls to 1.3 GHz; with operands of zeros K = 16384 runs at 7.1 PFLOP/s, with random ones at 5.65.
 // Tensor memory: two accumulators of 256 columns that share 64 (0 .. 255 and 192 .. 447), so that the rest holds the scales of
-// one chunk.  A chunk's scales overwrite those of the chunk before: the copies and MMAs that one thread issues are carried out
-// in the order of issue.  (Two sets of columns in turn, each copied to only after the commit of the MMAs that read it, cost a
+// one chunk.  A chunk's scales overwrite those of the chunk before, by copies issued behind the MMAs that read them.  PTX lists copy
+// before MMA among the pairs of tcgen05 instructions that keep the order of their issue, but not MMA before copy: this rests on one
+// thread's copies and MMAs going through one queue, as public block-scaled main loops rely on too, and on every test of a tile with
+// several chunks.  (Two sets of columns in turn, each copied to only after the commit of the MMAs that read it, cost a
 // tenth: 4096 x 14336 x 4096 100 -> 110 us, 512 x 4096 x 4096 10.0 -> 11.3.)
 // The epilogue drains the shared columns first; the next tile's MMAs start when it has, and the rest of the drain runs beside
 // them.

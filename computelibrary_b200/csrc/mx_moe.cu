@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kUpThreads, MoePlan<kFormat, NT, STAGES, 2, kS
             float    *weight = s_weight + (it & 1) * kMaxTokens; // the other table may still be read by a slower warp
             if (!begin_unit<kFormat>(p, weight, a, s_list[a], f0, ok)) break;
             ok = warp_wait(tfull_bar(as), static_cast<uint32_t>(it / kAcc) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
-            if (!ok) continue; // the next barrier ends it for all four warps
+            if (!ok) continue; // the next barrier ends it for all eight warps
             tc_fence_after();
             // The tokens that chose the expert, four at a time; the two warps of a lane quarter take turns.  (Four neighbours of which
             // one or more chose it: 128 tokens 65 us instead of 56.)

@@ -89,7 +89,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // Programmatic dependent launch.  launch_dependents: the next kernel of the stream may be scheduled (it starts on SMs
 // this grid has left, or never used) and run its prologue; wait: returns once the preceding kernel has completed and
-// its memory operations are visible -- every access to global memory of a kernel launched that way comes after it.
+// its memory operations are visible -- every access to global memory of a kernel launched that way comes after it, but for
+// prefetches into L2 and the expert layer's third launch, which reads what was complete before its predecessor let it start.
 // Without the launch attribute both are no-ops.
 __device__ __forceinline__ void griddep_launch_dependents()
 {
