@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(kWarps * 32) mx_rows_kernel(const __grid_const
     }
 }
 
-// Row-major scale bytes into tiles: a thread per four blocks of a row.
+// Row-major scale bytes into tiles: a thread per four blocks of a row, read byte by byte, stored as a word.  Done once per weight, not
+// made fast: 14336 x 4096 NVFP4 8.3 us (7.3 MB, 14 % of the copy rate), 65536 x 16384 113 (18 %).
 __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t *src, int64_t ld, int rows, int blocks, int64_t tiles, uint8_t *dst)
 {
     dependent_prologue();

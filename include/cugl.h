@@ -101,8 +101,10 @@ CUGL_API cugl_status cugl_context_set_trace_buffer(cugl_context *ctx, void *d_bu
 
 /* Every wait of a tensor-core kernel on a barrier (operands landed, stage free, accumulator complete / drained) is
  * bounded: when it has lasted longer than the limit the kernel stops issuing work, waits for the copies it has in
- * flight, frees its tensor memory, returns, and the next cugl_sync() reports CUGL_RUNTIME_ERROR; the context stays
- * usable.  The limit is two seconds unless set here, in microseconds (0 restores the default).  It is the
+ * flight (those of cugl_mx_* for their MMAs too), frees its tensor memory, returns, and the next cugl_sync() reports
+ * CUGL_RUNTIME_ERROR; the context stays usable.  A limit is for what never comes: choose it well above the time a call
+ * takes (it is looked at up to a millisecond late).  It is two seconds unless set here, in microseconds (0 restores the
+ * default).  It is the
  * counterpart of the scheduler-side run-time checks of the reference (IScheduler::schedule errors); the reference
  * has no device waits. */
 CUGL_API cugl_status cugl_context_set_wait_limit_us(cugl_context *ctx, uint64_t microseconds);
