@@ -301,14 +301,14 @@ def _source(slots, rows):
 
 
 def _decode(packed, tiles, fmt, cols):
-    """Values of packed rows with their scale tiles, float32 [rows, cols]."""
+    """Values of packed rows with their scale tiles, float32 [..., rows, cols] (leading dimensions alike)."""
     table = torch.tensor(GRID + tuple(-v for v in GRID), dtype=torch.float32, device=packed.device)
-    rows, nb = packed.shape[0], _blocks(cols, fmt)
-    codes = torch.stack((packed & 15, packed >> 4), dim=-1).flatten(-2)[:, :cols]
-    byte = tiles.reshape(-(-rows // 128), -(-nb // 4), 32, 4, 4).permute(0, 3, 2, 1, 4)
-    byte = byte.reshape(-(-rows // 128) * 128, -1)[:rows, :nb]
+    lead, rows, nb = packed.shape[:-2], packed.shape[-2], _blocks(cols, fmt)
+    codes = torch.stack((packed & 15, packed >> 4), dim=-1).flatten(-2)[..., :cols]
+    byte = tiles.reshape(lead + (-(-rows // 128), -(-nb // 4), 32, 4, 4)).movedim(-2, -4).movedim(-2, -3)
+    byte = byte.reshape(lead + (-(-rows // 128) * 128, -(-nb // 4) * 4))[..., :rows, :nb]
     scale = _pow2(byte.to(torch.int64) - 127) if fmt == "mxfp4" else byte.contiguous().view(torch.float8_e4m3fn).to(torch.float32)
-    return table[codes.to(torch.int32)] * scale.repeat_interleave(BLOCK[fmt], dim=1)[:, :cols]
+    return table[codes.to(torch.int32)] * scale.repeat_interleave(BLOCK[fmt], dim=-1)[..., :cols]
 
 
 def _plain(s):
@@ -327,16 +327,18 @@ def _plain(s):
         N, K, fmt = s["N"], s["K"], s["fmt"]
         a = _decode(s["a"], s["a_tiles"], fmt, K)
         out = torch.zeros_like(s["out"])
-        for e, (start, count) in enumerate(s["group_list"]):
-            if count == 0:
-                continue
+        hit = [e for e, (_, count) in enumerate(s["group_list"]) if count > 0]  # only the chosen experts are decoded
 
-            def product(w):
-                return torch.matmul(a[start:start + count], _decode(w[0][e * N:(e + 1) * N], w[1][e], fmt, K).T) * w[2][e]
+        def values(w):
+            return _decode(w[0].view(s["experts"], N, -1)[hit], w[1][hit], fmt, K) * w[2][hit, None, None]
 
-            y = product(s["b"])
+        b, up = values(s["b"]), values(s["up"]) if s["swiglu"] else None
+        for i, e in enumerate(hit):
+            start, count = s["group_list"][e]
+            rows = a[start:start + count]
+            y = torch.matmul(rows, b[i].T)
             if s["swiglu"]:
-                y = y * torch.sigmoid(y) * product(s["up"])
+                y = y * torch.sigmoid(y) * torch.matmul(rows, up[i].T)
             if s["bias"] is not None:
                 y = y + s["bias"][e]
             out[start:start + count] = y.to(dtype)
@@ -346,14 +348,13 @@ def _plain(s):
         for j in range(s["top_k"]):
             y = y + s["p"][:, j:j + 1] * s["src"][s["slots"][:, j].long()].float()
         return y.to(dtype)
-    out, at = s["base"].clone(), 0
-    for n, i in zip(s["lengths"], s["picks"]):
-        if n > 0 and i >= 0:
-            r = s["rank_list"][i]
-            v = torch.matmul(s["x"][at:at + n].float(), s["a"][i, :r].float().T)
-            delta = torch.matmul(v, s["b"][i, :, :r].float().T) * s["scales"][i]
-            out[at:at + n] = (s["base"][at:at + n].float() + delta).to(dtype)
-        at += n
+    adapters = np.repeat(s["picks"], s["lengths"])  # of every token
+    out = s["base"].clone()
+    for i in sorted(set(adapters.tolist()) - {-1}):
+        r, rows = s["rank_list"][i], torch.from_numpy(np.nonzero(adapters == i)[0]).cuda()
+        v = torch.matmul(s["x"][rows].float(), s["a"][i, :r].float().T)
+        delta = torch.matmul(v, s["b"][i, :, :r].float().T) * s["scales"][i]
+        out[rows] = (s["base"][rows].float() + delta).to(dtype)
     return out
 
 
