@@ -103,6 +103,36 @@ class MxMoeDesc(C.Structure):
     ]
 
 
+class MxGroupedGemmDesc(C.Structure):
+    """cugl_mx_grouped_gemm_desc"""
+    _fields_ = [
+        ("groups", _i32), ("rows", _i32), ("expected_rows", _i32), ("N", _i32), ("K", _i32), ("format", _i32),
+        ("dst_dtype", _i32), ("swiglu", _i32), ("has_bias", _i32), ("alpha", C.c_float), ("up_alpha", C.c_float),
+        ("lda", _i64), ("ldb", _i64), ("ldd", _i64),
+    ]
+
+
+class MoeRouteDesc(C.Structure):
+    """cugl_moe_route_desc"""
+    _fields_ = [("tokens", _i32), ("experts", _i32), ("top_k", _i32), ("dtype", _i32), ("renormalize", _i32), ("ld_logits", _i64)]
+
+
+class MxGroupDesc(C.Structure):
+    """cugl_mx_group_desc"""
+    _fields_ = [
+        ("tokens", _i32), ("top_k", _i32), ("rows", _i32), ("cols", _i32), ("format", _i32), ("dtype", _i32),
+        ("src_grouped", _i32), ("tensor_exponent", _i32), ("ld", _i64), ("ld_packed", _i64),
+    ]
+
+
+class MoeCombineDesc(C.Structure):
+    """cugl_moe_combine_desc"""
+    _fields_ = [
+        ("tokens", _i32), ("top_k", _i32), ("rows", _i32), ("cols", _i32), ("src_dtype", _i32), ("dst_dtype", _i32),
+        ("ld_src", _i64), ("ld_dst", _i64),
+    ]
+
+
 POOL_MAX, POOL_AVG = 0, 1
 ACT_NONE, ACT_RELU, ACT_BOUNDED_RELU, ACT_LU_BOUNDED_RELU = -1, 0, 1, 2
 
@@ -211,6 +241,16 @@ _SIGNATURES = {
     "cugl_mx_moe_validate": (C.c_int, [C.POINTER(MxMoeDesc), C.POINTER(C.c_char_p)]),
     "cugl_mx_moe_workspace_bytes": (C.c_size_t, [C.POINTER(MxMoeDesc)]),
     "cugl_mx_moe": (C.c_int, [_vp, C.POINTER(MxMoeDesc)] + [_vp] * 10 + [C.c_size_t]),
+    "cugl_moe_route_validate": (C.c_int, [C.POINTER(MoeRouteDesc), C.POINTER(C.c_char_p)]),
+    "cugl_moe_route_workspace_bytes": (C.c_size_t, [C.POINTER(MoeRouteDesc)]),
+    "cugl_moe_route": (C.c_int, [_vp, C.POINTER(MoeRouteDesc)] + [_vp] * 6 + [C.c_size_t]),
+    "cugl_mx_group_validate": (C.c_int, [C.POINTER(MxGroupDesc), C.POINTER(C.c_char_p)]),
+    "cugl_mx_quantize_grouped": (C.c_int, [_vp, C.POINTER(MxGroupDesc)] + [_vp] * 4),
+    "cugl_moe_combine_validate": (C.c_int, [C.POINTER(MoeCombineDesc), C.POINTER(C.c_char_p)]),
+    "cugl_moe_combine": (C.c_int, [_vp, C.POINTER(MoeCombineDesc)] + [_vp] * 4),
+    "cugl_mx_group_rows": (_i64, [_i32, _i64]),
+    "cugl_mx_grouped_gemm_validate": (C.c_int, [C.POINTER(MxGroupedGemmDesc), C.POINTER(C.c_char_p)]),
+    "cugl_mx_grouped_gemm": (C.c_int, [_vp, C.POINTER(MxGroupedGemmDesc)] + [_vp] * 11),
     "cugl_mx_tile_scales": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }
 
@@ -444,6 +484,29 @@ class Context:
                                         _dptr(up[0]), _dptr(up[1]), _dptr(down[0]), _dptr(down[1]), _dptr(dst),
                                         _dptr(workspace), workspace_bytes))
 
+    def moe_route(self, desc: "MoeRouteDesc", logits, ids, weights, slots, groups, workspace, workspace_bytes=None):
+        """The gate of an expert layer; workspace: moe_route_workspace_bytes(desc) bytes (workspace_bytes: its size where it is a raw
+        pointer)."""
+        if workspace_bytes is None:
+            workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        self.check(self.lib.cugl_moe_route(self.handle, C.byref(desc), _dptr(logits), _dptr(ids), _dptr(weights), _dptr(slots),
+                                           _dptr(groups), _dptr(workspace), workspace_bytes))
+
+    def mx_quantize_grouped(self, desc: "MxGroupDesc", src, slots, dst, scales):
+        """Plain rows -> packed rows of groups."""
+        self.check(self.lib.cugl_mx_quantize_grouped(self.handle, C.byref(desc), _dptr(src), _dptr(slots), _dptr(dst), _dptr(scales)))
+
+    def moe_combine(self, desc: "MoeCombineDesc", src, slots, weights, dst):
+        """Rows of groups, times their weights -> tokens."""
+        self.check(self.lib.cugl_moe_combine(self.handle, C.byref(desc), _dptr(src), _dptr(slots), _dptr(weights), _dptr(dst)))
+
+    def mx_grouped_gemm(self, desc: "MxGroupedGemmDesc", a, a_scales, groups, b, dst, up=None, bias=None):
+        """Products of groups of rows.  b, up: (packed codes, scale tiles) or (packed codes, scale tiles, factors per group)."""
+        def parts(w):
+            return [_dptr(t) for t in (tuple(w) + (None, None, None))[:3]] if w is not None else [None] * 3
+        self.check(self.lib.cugl_mx_grouped_gemm(self.handle, C.byref(desc), _dptr(a), _dptr(a_scales), _dptr(groups), *parts(b),
+                                                 *parts(up), _dptr(bias), _dptr(dst)))
+
     def weights_reshape_nhwc(self, w, dst, K, OFM):
         self.check(self.lib.cugl_weights_reshape_nhwc(self.handle, _dptr(w), _dptr(dst), K, OFM))
 
@@ -577,6 +640,81 @@ def mx_moe_validate(desc: MxMoeDesc):
 
 def mx_moe_workspace_bytes(desc: MxMoeDesc) -> int:
     return int(load_library().cugl_mx_moe_workspace_bytes(C.byref(desc)))
+
+
+def mx_group_rows(groups: int, rows: int) -> int:
+    """Rows of a matrix that holds any `rows` rows in `groups` groups, each of which starts at a multiple of 128."""
+    return int(load_library().cugl_mx_group_rows(groups, rows))
+
+
+def _validated(call, desc):
+    """(status, reason) of one of the library's checks of descriptors."""
+    why = C.c_char_p()
+    st = call(C.byref(desc), C.byref(why))
+    return st, (why.value or b"").decode()
+
+
+def make_moe_route_desc(tokens, experts, top_k, dtype=F32, renormalize=True, ld_logits=None) -> MoeRouteDesc:
+    """cugl_moe_route_desc; dense logits unless a stride (bytes) is given."""
+    d = MoeRouteDesc()
+    d.tokens, d.experts, d.top_k, d.dtype, d.renormalize = tokens, experts, top_k, dtype, int(renormalize)
+    d.ld_logits = experts * (4 if dtype == F32 else 2) if ld_logits is None else ld_logits
+    return d
+
+
+def moe_route_validate(desc: MoeRouteDesc):
+    """Returns (status, reason)."""
+    return _validated(load_library().cugl_moe_route_validate, desc)
+
+
+def moe_route_workspace_bytes(desc: MoeRouteDesc) -> int:
+    return int(load_library().cugl_moe_route_workspace_bytes(C.byref(desc)))
+
+
+def make_mx_group_desc(tokens, top_k, cols, rows, format, dtype, ld=None, ld_packed=None, tensor_exponent=0, src_grouped=False) -> MxGroupDesc:
+    """cugl_mx_group_desc of a dense plain matrix and packed rows mx_pitch(cols) apart unless strides (bytes) are given."""
+    d = MxGroupDesc()
+    d.tokens, d.top_k, d.rows, d.cols, d.format, d.dtype = tokens, top_k, rows, cols, format, dtype
+    d.src_grouped, d.tensor_exponent = int(src_grouped), tensor_exponent
+    d.ld = cols * (4 if dtype == F32 else 2) if ld is None else ld
+    d.ld_packed = mx_pitch(cols) if ld_packed is None else ld_packed
+    return d
+
+
+def mx_group_validate(desc: MxGroupDesc):
+    """Returns (status, reason)."""
+    return _validated(load_library().cugl_mx_group_validate, desc)
+
+
+def make_moe_combine_desc(tokens, top_k, cols, rows, src_dtype, dst_dtype, ld_src=None, ld_dst=None) -> MoeCombineDesc:
+    """cugl_moe_combine_desc; dense matrices unless strides (bytes) are given."""
+    d = MoeCombineDesc()
+    d.tokens, d.top_k, d.rows, d.cols, d.src_dtype, d.dst_dtype = tokens, top_k, rows, cols, src_dtype, dst_dtype
+    d.ld_src = cols * (4 if src_dtype == F32 else 2) if ld_src is None else ld_src
+    d.ld_dst = cols * (4 if dst_dtype == F32 else 2) if ld_dst is None else ld_dst
+    return d
+
+
+def moe_combine_validate(desc: MoeCombineDesc):
+    """Returns (status, reason)."""
+    return _validated(load_library().cugl_moe_combine_validate, desc)
+
+
+def make_mx_grouped_gemm_desc(groups, rows, N, K, format, dst_dtype, expected_rows=0, swiglu=False, has_bias=False, alpha=1.0,
+                              up_alpha=1.0, lda=None, ldb=None, ldd=None) -> MxGroupedGemmDesc:
+    """cugl_mx_grouped_gemm_desc; packed rows mx_pitch(K) apart and a dense dst unless strides (bytes) are given."""
+    d = MxGroupedGemmDesc()
+    d.groups, d.rows, d.expected_rows, d.N, d.K, d.format, d.dst_dtype = groups, rows, expected_rows, N, K, format, dst_dtype
+    d.swiglu, d.has_bias, d.alpha, d.up_alpha = int(swiglu), int(has_bias), alpha, up_alpha
+    d.lda = mx_pitch(K) if lda is None else lda
+    d.ldb = mx_pitch(K) if ldb is None else ldb
+    d.ldd = N * (4 if dst_dtype == F32 else 2) if ldd is None else ldd
+    return d
+
+
+def mx_grouped_gemm_validate(desc: MxGroupedGemmDesc):
+    """Returns (status, reason)."""
+    return _validated(load_library().cugl_mx_grouped_gemm_validate, desc)
 
 
 def make_pool_desc(B, H, W, C_, pool_type, size=(1, 1), stride=(1, 1), pad=(0, 0, 0, 0), in_q=(1.0, 0),

@@ -58,7 +58,8 @@ enum : int32_t
     DEV_TIMEOUT_PRODUCER = 1,
     DEV_TIMEOUT_MMA      = 2,
     DEV_TIMEOUT_EPILOGUE = 3,
-    DEV_TIMEOUT_DRAIN    = 4
+    DEV_TIMEOUT_DRAIN    = 4,
+    DEV_BAD_GROUP        = 5 // cugl_mx_grouped_gemm: a group that does not lie within the rows
 };
 
 // Everything an epilogue needs to turn a raw sum_k A*B accumulator into the function's output.

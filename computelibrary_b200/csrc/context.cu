@@ -379,6 +379,10 @@ extern "C"
             *ctx->h_status     = 0;
             cudaMemsetAsync(ctx->d_status, 0, sizeof(int32_t), ctx->stream);
             cudaStreamSynchronize(ctx->stream);
+            if (code == cugl::DEV_BAD_GROUP)
+            {
+                return fail(ctx, CUGL_RUNTIME_ERROR, "cugl_mx_grouped_gemm: a group did not start at a multiple of 128 or did not lie within the rows; it was left out");
+            }
             return fail(ctx, CUGL_RUNTIME_ERROR,
                         "device-side bounded wait ran out (code " + std::to_string(code) +
                             ": 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 4 = drain); results are invalid");

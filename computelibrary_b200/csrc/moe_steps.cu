@@ -1,0 +1,524 @@
+// The steps of an expert layer around its products: the gate, which also gives every choice a row of a group, and the combination of a
+// token's rows.
+#include "mx.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace cugl
+{
+namespace
+{
+constexpr int kMaxExperts = 512, kMaxTopK = 16;
+constexpr int kSlab = 128; // rows at whose multiples groups start
+
+// ---- the gate ------------------------------------------------------------------------------------------------
+// A warp chooses for a token; a block takes a chunk of consecutive tokens.  The rows of a group are in the order of the tokens, so a
+// choice's row is its group's start, the choices of that expert in the chunks before, and those of the tokens before it in its own
+// chunk (bits of a mask per expert).  One chunk: one launch.  Several: the first launch leaves the number of choices per chunk and expert,
+// the second adds up those of the chunks before (no block waits for another one, nothing depends on the order of atomics).
+//
+// What bounds it: latency.  64 tokens a chunk, two per warp: a choice is a dozen dependent instructions, top_k of them follow each
+// other.
+constexpr int kRouteWarps  = 32;
+constexpr int kRouteChunk  = 64;  // tokens of a block, where there are several
+constexpr int kRouteSingle = 128; // tokens of a single block
+constexpr int kMaskWords   = kRouteSingle / 32;
+
+struct RouteParams
+{
+    const uint8_t *logits;
+    int32_t       *ids, *slots;
+    float         *weights;
+    int2          *groups;
+    int32_t       *counts; // [chunks][experts]
+    int64_t        ld;
+    int            tokens, experts, top_k, renormalize, chunk, chunks;
+};
+
+template <typename T>
+__device__ __forceinline__ float load_logit(const T *p)
+{
+    return to_float(*p);
+}
+
+// Logits become unsigned keys in their order (0: not to be chosen: NaN and -infinity, or chosen already); a choice is the largest key,
+// the lowest index among equal ones.  Lane j returns the j-th choice (-1: none) and its weight.
+template <typename T, int kPer> // experts per lane
+__device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane, float &weight)
+{
+    const T *row = reinterpret_cast<const T *>(p.logits + t * p.ld);
+    uint32_t key[kPer];
+    float    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+    {
+        const int      e = i * 32 + lane;
+        const float    v = e < p.experts ? load_logit(row + e) : -INFINITY;
+        const uint32_t b = __float_as_uint(v + 0.f); // -0 and 0 are equal logits
+        key[i] = v > -INFINITY ? ((b >> 31) != 0 ? ~b : b | 0x80000000u) : 0u;
+        if (v > top) top = v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float all = 0.f;
+    if (p.renormalize == 0)
+    {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+        {
+            if (key[i] != 0) all += expf(__uint_as_float((key[i] >> 31) != 0 ? key[i] & 0x7fffffffu : ~key[i]) - top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    int   mine = -1;
+    float own = 0.f, sum = 0.f;
+    for (int j = 0; j < p.top_k; ++j)
+    {
+        uint32_t best = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
+        best = __reduce_max_sync(0xffffffffu, best);
+        if (best == 0) break;
+        int at = kMaxExperts;
+#pragma unroll
+        for (int i = kPer - 1; i >= 0; --i)
+        {
+            if (key[i] == best) at = i * 32 + lane;
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+        {
+            if (at == i * 32 + lane) key[i] = 0;
+        }
+        const float w = expf(__uint_as_float((best >> 31) != 0 ? best & 0x7fffffffu : ~best) - top);
+        sum += w;
+        if (lane == j)
+        {
+            mine = at;
+            own  = w;
+        }
+    }
+    weight = mine >= 0 ? own / (p.renormalize != 0 ? sum : all) : 0.f;
+    return mine;
+}
+template <typename T>
+__device__ __forceinline__ int route_any(const RouteParams &p, int t, int lane, float &weight)
+{
+    if (p.experts <= 64) return route_token<T, 2>(p, t, lane, weight);
+    if (p.experts <= 128) return route_token<T, 4>(p, t, lane, weight);
+    return route_token<T, kMaxExperts / 32>(p, t, lane, weight);
+}
+
+struct RouteShared
+{
+    uint32_t mask[kMaxExperts][kMaskWords]; // tokens of the chunk that chose an expert
+    int      start[kMaxExperts];            // the group's first row, then the chunk's first row of it
+    int      scan[kMaxExperts];
+    int      before[kMaxExperts];
+};
+// Starts of the groups from the choices per expert in `scan` (which is left as it is): every group takes whole slabs.  By warp 0.
+__device__ __forceinline__ void group_starts(const RouteParams &p, RouteShared &s, int lane)
+{
+    const int per = (p.experts + 31) / 32, first = lane * per, last = min(first + per, p.experts);
+    int       sum = 0;
+    for (int e = first; e < last; ++e) sum += (s.scan[e] + kSlab - 1) / kSlab * kSlab;
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    int at = incl - sum;
+    for (int e = first; e < last; ++e)
+    {
+        s.start[e] = at;
+        at += (s.scan[e] + kSlab - 1) / kSlab * kSlab;
+    }
+}
+// rows of the choices of a chunk's tokens, from the mask and the chunk's first rows
+__device__ __forceinline__ void place_choices(const RouteParams &p, const RouteShared &s, int t0, int tokens)
+{
+    for (int i = threadIdx.x; i < tokens * p.top_k; i += static_cast<int>(blockDim.x))
+    {
+        const int t = i / p.top_k, e = p.ids[static_cast<int64_t>(t0) * p.top_k + i];
+        int       row = -1;
+        if (e >= 0)
+        {
+            row = s.start[e];
+            for (int w = 0; w < (t >> 5); ++w) row += __popc(s.mask[e][w]);
+            row += __popc(s.mask[e][t >> 5] & ((1u << (t & 31)) - 1u));
+        }
+        p.slots[static_cast<int64_t>(t0) * p.top_k + i] = row;
+    }
+}
+
+// kStep 0: all of it in one block; 1: choices of a chunk; 2: their rows
+template <typename T, int kStep>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p)
+{
+    __shared__ RouteShared s;
+    dependent_prologue();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
+    const int t0 = static_cast<int>(blockIdx.x) * p.chunk, tokens = min(p.chunk, p.tokens - t0);
+    for (int i = threadIdx.x; i < p.experts * kMaskWords; i += static_cast<int>(blockDim.x)) (&s.mask[0][0])[i] = 0;
+    __syncthreads();
+    if constexpr (kStep != 2)
+    {
+        for (int t = warp; t < tokens; t += warps)
+        {
+            float     weight;
+            const int e = route_any<T>(p, t0 + t, lane, weight);
+            if (lane < p.top_k)
+            {
+                const int64_t at = static_cast<int64_t>(t0 + t) * p.top_k + lane;
+                p.ids[at]        = e;
+                p.weights[at]    = weight;
+                if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
+            }
+        }
+    }
+    else
+    {
+        for (int i = threadIdx.x; i < tokens * p.top_k; i += static_cast<int>(blockDim.x))
+        {
+            const int e = p.ids[static_cast<int64_t>(t0) * p.top_k + i], t = i / p.top_k;
+            if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
+        }
+    }
+    __syncthreads();
+    if constexpr (kStep != 2)
+    {
+        for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
+        {
+            int n = 0;
+            for (int w = 0; w < kMaskWords; ++w) n += __popc(s.mask[e][w]);
+            if constexpr (kStep == 1) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = n;
+            s.scan[e]   = n;
+            s.before[e] = 0;
+        }
+    }
+    else
+    {
+        // choices of all chunks and of those before this one: slices of chunks per expert, several loads in flight per thread
+        for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] = s.before[e] = 0;
+        __syncthreads();
+        const int slices = max(1, static_cast<int>(blockDim.x) / p.experts);
+        for (int i = threadIdx.x; i < slices * p.experts; i += static_cast<int>(blockDim.x))
+        {
+            const int e = i % p.experts, slice = i / p.experts;
+            int       all = 0, own = 0;
+#pragma unroll 8
+            for (int c = slice; c < p.chunks; c += slices)
+            {
+                const int n = __ldg(p.counts + static_cast<int64_t>(c) * p.experts + e);
+                all += n;
+                own += c < static_cast<int>(blockIdx.x) ? n : 0;
+            }
+            atomicAdd(&s.scan[e], all); // whole numbers: the same sum in any order
+            atomicAdd(&s.before[e], own);
+        }
+    }
+    if constexpr (kStep == 1)
+    {
+        return;
+    }
+    __syncthreads();
+    if (warp == 0) group_starts(p, s, lane);
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
+    {
+        if (blockIdx.x == 0) p.groups[e] = make_int2(s.start[e], s.scan[e]);
+        s.start[e] += s.before[e];
+    }
+    __syncthreads();
+    place_choices(p, s, t0, tokens);
+}
+
+// ---- combination ---------------------------------------------------------------------------------------------
+// dst[t] = sum_j weights[t][j] * src[slots[t][j]], in the order of j, in float, rounded once.  Eight columns of a token per thread, all
+// its rows asked for before the first is used; the bytes bound it.
+struct CombineParams
+{
+    const uint8_t *src;
+    const int32_t *slots;
+    const float   *weights;
+    uint8_t       *dst;
+    int64_t        ld_src, ld_dst;
+    int            tokens, top_k, cols, rows, units; // units of eight columns of a row
+};
+
+template <typename TS>
+__device__ __forceinline__ void widen8(const uint4 *raw, float (&v)[8])
+{
+    TS e[8];
+    memcpy(e, raw, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+}
+
+template <typename TS, typename TD, bool kVec>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p)
+{
+    dependent_prologue();
+    const int64_t total = static_cast<int64_t>(p.tokens) * p.units;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256)
+    {
+        const int t = static_cast<int>(i / p.units), c0 = static_cast<int>(i - static_cast<int64_t>(t) * p.units) * 8, n = min(8, p.cols - c0);
+        const int32_t *slots   = p.slots + static_cast<int64_t>(t) * p.top_k;
+        const float   *weights = p.weights + static_cast<int64_t>(t) * p.top_k;
+        float          sum[8] = {};
+        constexpr int  kBatch = sizeof(TS) == 4 ? 4 : 8, kLoads = sizeof(TS) / 2;
+        for (int j0 = 0; j0 < p.top_k; j0 += kBatch)
+        {
+            uint4 raw[kBatch][kLoads];
+            float w[kBatch];
+            bool  has[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+            {
+                has[j] = false;
+                if (j0 + j < p.top_k)
+                {
+                    const int row = __ldg(slots + j0 + j);
+                    has[j]        = row >= 0 && row < p.rows;
+                    if (has[j])
+                    {
+                        w[j]          = __ldg(weights + j0 + j);
+                        const TS *src = reinterpret_cast<const TS *>(p.src + row * p.ld_src) + c0;
+                        if constexpr (kVec)
+                        {
+#pragma unroll
+                            for (int l = 0; l < kLoads; ++l) raw[j][l] = __ldg(reinterpret_cast<const uint4 *>(src) + l);
+                        }
+                        else
+                        {
+                            TS e[8] = {};
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                            {
+                                if (k < n) e[k] = src[k];
+                            }
+                            memcpy(raw[j], e, sizeof(e));
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+            {
+                if (has[j])
+                {
+                    float v[8];
+                    widen8<TS>(raw[j], v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum[k] = fmaf(w[j], v[k], sum[k]);
+                }
+            }
+        }
+        TD  out[8];
+        TD *dst = reinterpret_cast<TD *>(p.dst + t * p.ld_dst) + c0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out[k] = from_float<TD>(sum[k]);
+        if constexpr (kVec)
+        {
+            uint4 q[sizeof(TD) / 2];
+            memcpy(q, out, sizeof(out));
+#pragma unroll
+            for (int l = 0; l < static_cast<int>(sizeof(TD)) / 2; ++l) reinterpret_cast<uint4 *>(dst)[l] = q[l];
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+            {
+                if (k < n) dst[k] = out[k];
+            }
+        }
+    }
+}
+
+template <typename TS, typename TD>
+cudaError_t launch_combine(cugl_context *ctx, const CombineParams &p, bool vec)
+{
+    const int64_t blocks = (static_cast<int64_t>(p.tokens) * p.units + 255) / 256, most = static_cast<int64_t>(ctx->sm_count) * 64;
+    const unsigned grid  = static_cast<unsigned>(blocks < most ? blocks : most);
+    return vec ? launch_dependent(ctx, combine_kernel<TS, TD, true>, dim3(grid), 256, 0, blocks, p)
+               : launch_dependent(ctx, combine_kernel<TS, TD, false>, dim3(grid), 256, 0, blocks, p);
+}
+template <typename TS>
+cudaError_t launch_combine(cugl_context *ctx, int dst_dtype, const CombineParams &p, bool vec)
+{
+    return dst_dtype == CUGL_F32 ? launch_combine<TS, float>(ctx, p, vec)
+           : dst_dtype == CUGL_F16 ? launch_combine<TS, __half>(ctx, p, vec)
+                                   : launch_combine<TS, __nv_bfloat16>(ctx, p, vec);
+}
+
+bool aligned(const void *p, uintptr_t n)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+const char *validate_route(const cugl_moe_route_desc *d)
+{
+    if (d == nullptr) return "descriptor is NULL";
+    if (d->tokens < 0) return "tokens must not be negative";
+    if (d->experts < 1 || d->experts > kMaxExperts) return "experts must lie within 1 .. 512";
+    if (d->top_k < 1 || d->top_k > kMaxTopK || d->top_k > d->experts) return "top_k must lie within 1 .. 16 and not exceed experts";
+    if (!is_float_dtype(d->dtype)) return "dtype must be CUGL_F32, CUGL_F16 or CUGL_BF16";
+    if (d->ld_logits < static_cast<int64_t>(d->experts) * dtype_size(d->dtype) || d->ld_logits % dtype_size(d->dtype) != 0)
+        return "ld_logits must hold a row and be a multiple of the element size";
+    if (static_cast<int64_t>(d->tokens) * d->top_k + static_cast<int64_t>(kSlab) * d->experts > INT32_MAX - 1024) return "more rows than 32 bits count";
+    return nullptr;
+}
+int route_chunks(int tokens)
+{
+    return tokens <= kRouteSingle ? 1 : (tokens + kRouteChunk - 1) / kRouteChunk;
+}
+
+const char *validate_combine(const cugl_moe_combine_desc *d)
+{
+    if (d == nullptr) return "descriptor is NULL";
+    if (d->tokens < 0 || d->cols < 1 || d->rows < 0) return "tokens and rows must not be negative, cols must be positive";
+    if (d->cols > INT32_MAX - 1024) return "cols is too large";
+    if (d->top_k < 1 || d->top_k > kMaxTopK) return "top_k must lie within 1 .. 16";
+    if (!is_float_dtype(d->src_dtype) || !is_float_dtype(d->dst_dtype)) return "dtypes must be CUGL_F32, CUGL_F16 or CUGL_BF16";
+    const int ss = dtype_size(d->src_dtype), ds = dtype_size(d->dst_dtype);
+    if (d->ld_src < static_cast<int64_t>(d->cols) * ss || d->ld_src % ss != 0 || d->ld_dst < static_cast<int64_t>(d->cols) * ds || d->ld_dst % ds != 0)
+        return "ld_src and ld_dst must hold a row and be multiples of their element sizes";
+    return nullptr;
+}
+
+cugl_status told(const char *why, const char **reason)
+{
+    if (reason != nullptr)
+    {
+        *reason = why != nullptr ? why : "";
+    }
+    return why == nullptr ? CUGL_SUCCESS : CUGL_INVALID_ARGUMENT;
+}
+} // namespace
+} // namespace cugl
+
+using namespace cugl;
+
+extern "C"
+{
+    cugl_status cugl_moe_route_validate(const cugl_moe_route_desc *desc, const char **reason)
+    {
+        return told(validate_route(desc), reason);
+    }
+
+    size_t cugl_moe_route_workspace_bytes(const cugl_moe_route_desc *desc)
+    {
+        if (validate_route(desc) != nullptr)
+        {
+            return 0;
+        }
+        const int chunks = route_chunks(desc->tokens);
+        return chunks == 1 ? 16 : static_cast<size_t>(chunks) * static_cast<size_t>(desc->experts) * 4;
+    }
+
+    cugl_status cugl_moe_route(cugl_context *ctx, const cugl_moe_route_desc *desc, const void *d_logits, int32_t *d_ids, float *d_weights,
+                               int32_t *d_slots, int32_t *d_groups, void *d_workspace, size_t workspace_bytes)
+    {
+        if (ctx == nullptr)
+        {
+            return fail(nullptr, CUGL_INVALID_ARGUMENT, "context is NULL");
+        }
+        const char *why = validate_route(desc);
+        if (why == nullptr)
+        {
+            const bool some = desc->tokens > 0;
+            if (d_groups == nullptr || (some && (d_logits == nullptr || d_ids == nullptr || d_weights == nullptr || d_slots == nullptr || d_workspace == nullptr)))
+                why = "NULL pointer";
+            else if (!aligned(d_groups, 8)) why = "groups must be 8-byte aligned";
+            else if (some && (!aligned(d_logits, static_cast<uintptr_t>(dtype_size(desc->dtype))) || !aligned(d_ids, 4) || !aligned(d_weights, 4) || !aligned(d_slots, 4) ||
+                              !aligned(d_workspace, 16)))
+                why = "a buffer is not aligned to its elements (the workspace: 16 bytes)";
+            else if (some && workspace_bytes < cugl_moe_route_workspace_bytes(desc)) why = "the workspace is too small";
+        }
+        if (why != nullptr)
+        {
+            return fail(ctx, CUGL_INVALID_ARGUMENT, std::string("cugl_moe_route: ") + why);
+        }
+        const DeviceScope device(ctx);
+        RouteParams       p{};
+        p.logits      = static_cast<const uint8_t *>(d_logits);
+        p.ids         = d_ids;
+        p.slots       = d_slots;
+        p.weights     = d_weights;
+        p.groups      = reinterpret_cast<int2 *>(d_groups);
+        p.counts      = static_cast<int32_t *>(d_workspace);
+        p.ld          = desc->ld_logits;
+        p.tokens      = desc->tokens;
+        p.experts     = desc->experts;
+        p.top_k       = desc->top_k;
+        p.renormalize = desc->renormalize;
+        p.chunks      = route_chunks(desc->tokens);
+        p.chunk       = p.chunks == 1 ? kRouteSingle : kRouteChunk;
+        auto run      = [&](auto element) -> cugl_status {
+            using T = decltype(element);
+            if (p.chunks == 1)
+            {
+                const int threads = 32 * std::min(kRouteWarps, std::max(4, p.tokens));
+                CUGL_CUDA_TRY(ctx, launch_dependent(ctx, route_kernel<T, 0>, dim3(1), threads, 0, 1, p));
+                return CUGL_SUCCESS;
+            }
+            const dim3 grid(static_cast<unsigned>(p.chunks));
+            CUGL_CUDA_TRY(ctx, launch_dependent(ctx, route_kernel<T, 1>, grid, kRouteWarps * 32, 0, p.chunks, p));
+            CUGL_CUDA_TRY(ctx, launch_dependent(ctx, route_kernel<T, 2>, grid, kRouteWarps * 32, 0, p.chunks, p));
+            return CUGL_SUCCESS;
+        };
+        return desc->dtype == CUGL_F32 ? run(float{}) : desc->dtype == CUGL_F16 ? run(__half{}) : run(__nv_bfloat16{});
+    }
+
+    cugl_status cugl_moe_combine_validate(const cugl_moe_combine_desc *desc, const char **reason)
+    {
+        return told(validate_combine(desc), reason);
+    }
+
+    cugl_status cugl_moe_combine(cugl_context *ctx, const cugl_moe_combine_desc *desc, const void *d_src, const int32_t *d_slots, const float *d_weights,
+                                 void *d_dst)
+    {
+        if (ctx == nullptr)
+        {
+            return fail(nullptr, CUGL_INVALID_ARGUMENT, "context is NULL");
+        }
+        const char *why = validate_combine(desc);
+        if (why == nullptr && desc->tokens > 0)
+        {
+            if ((d_src == nullptr && desc->rows > 0) || d_slots == nullptr || d_weights == nullptr || d_dst == nullptr) why = "NULL pointer";
+            else if (!aligned(d_src, static_cast<uintptr_t>(dtype_size(desc->src_dtype))) || !aligned(d_dst, static_cast<uintptr_t>(dtype_size(desc->dst_dtype))) ||
+                     !aligned(d_slots, 4) || !aligned(d_weights, 4))
+                why = "a buffer is not aligned to its elements";
+        }
+        if (why != nullptr)
+        {
+            return fail(ctx, CUGL_INVALID_ARGUMENT, std::string("cugl_moe_combine: ") + why);
+        }
+        if (desc->tokens == 0) return CUGL_SUCCESS;
+        const DeviceScope device(ctx);
+        CombineParams     p{};
+        p.src     = static_cast<const uint8_t *>(d_src);
+        p.slots   = d_slots;
+        p.weights = d_weights;
+        p.dst     = static_cast<uint8_t *>(d_dst);
+        p.ld_src  = desc->ld_src;
+        p.ld_dst  = desc->ld_dst;
+        p.tokens  = desc->tokens;
+        p.top_k   = desc->top_k;
+        p.cols    = desc->cols;
+        p.rows    = desc->rows;
+        p.units   = (desc->cols + 7) / 8;
+        const bool vec = desc->cols % 8 == 0 && aligned(d_src, 16) && aligned(d_dst, 16) && desc->ld_src % 16 == 0 && desc->ld_dst % 16 == 0;
+        CUGL_CUDA_TRY(ctx, desc->src_dtype == CUGL_F32 ? launch_combine<float>(ctx, desc->dst_dtype, p, vec)
+                           : desc->src_dtype == CUGL_F16 ? launch_combine<__half>(ctx, desc->dst_dtype, p, vec)
+                                                         : launch_combine<__nv_bfloat16>(ctx, desc->dst_dtype, p, vec));
+        return CUGL_SUCCESS;
+    }
+}

@@ -467,31 +467,6 @@ __device__ __forceinline__ void stage_block(uint32_t s_out, int lane, const uint
     }
 }
 
-// drain_stages of an SM pair, by its leader, whose barriers count the copies of both CTAs: the producers may have stopped at different
-// stages, so what the barrier of a stage that only one of them has filled still expects, or does not expect yet, is put right first.
-// bytes: of one CTA's copies of a stage.  (The counts are at most STAGES apart: both wait for the same MMAs.)
-template <int STAGES, typename Bytes>
-__device__ __forceinline__ void drain_pair_stages(uint32_t bars, int issued, int peer, int withheld, long long limit, Bytes bytes)
-{
-    const int end = max(issued, peer);
-    for (int i = max(0, end - STAGES); i < end; ++i)
-    {
-        const uint32_t bar = bars + 8u * (i % STAGES);
-        const bool     own = i < issued && i != withheld, other = i < peer;
-        if (own != other && elect_one())
-        {
-            if (own) mbar_complete_tx(bar, bytes(i)); // expected, but the peer never asked for it
-            else mbar_expect_tx(bar, bytes(i));       // the other way round
-        }
-        __syncwarp();
-        const long long t0 = clock64(), bound = limit + 2000000;
-        while ((own || other) && !mbar_try_wait(bar, static_cast<uint32_t>(i / STAGES) & 1u) && clock64() - t0 <= bound)
-        {
-        }
-    }
-    __syncwarp();
-}
-
 template <int kFormat, int kBulk>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t,

@@ -27,7 +27,32 @@ struct QuantParams
     int            lane_shift;           // 2^lane_shift lanes of a warp share a row
     float          exponent_mul;
     int            vec_plain, vec_packed; // the plain matrix is 16-byte aligned, the packed one 4-byte
+    const int32_t *slots;                 // rows of groups (see Rows), within 0 .. group_rows - 1
+    int            top_k, group_rows;
 };
+
+// Which rows a row of the launch stands for.
+//   kSame     row r of the plain matrix, row r of the packed one
+//   kChoices  row r of the plain matrix, rows slots[r * top_k] and following of the packed one: a token's choices
+//   kSlots    row slots[r] of both: rows of groups, choice by choice
+// A slot outside the groups' rows stands for none.
+enum Rows
+{
+    kSame,
+    kChoices,
+    kSlots
+};
+__device__ __forceinline__ int slot_of(const QuantParams &p, int64_t i)
+{
+    const int r = __ldg(p.slots + i);
+    return static_cast<unsigned>(r) < static_cast<unsigned>(p.group_rows) ? r : -1;
+}
+template <int kWhich>
+__device__ __forceinline__ int source_row(const QuantParams &p, int row) // -1: none
+{
+    if (row >= p.rows) return -1;
+    return kWhich == kSlots ? slot_of(p, row) : row;
+}
 
 // What a warp takes: kRows rows (or groups of narrow rows) of kSegs segments of 256 columns.  Segments lie 256 columns apart at
 // addresses that differ by constants, so that a row's address is computed once.
@@ -48,13 +73,14 @@ __device__ __forceinline__ Place place_of(const QuantParams &p, int group, int l
 
 // Rows that start anywhere: a warp moves its 256 values as consecutive elements and turns them over in shared memory, where a
 // lane's eight lie in a row.  row: of lane 0's columns; c0: the segment's first column.
-template <typename T>
+template <typename T, int kWhich>
 __device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c0, int lane, T (&v)[kLaneCols])
 {
     if (p.lane_shift == 5) // the warp's values lie in one row
     {
-        const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + c0 + lane;
-        const int n   = row < p.rows ? p.cols - c0 - lane : 0;
+        const int from = source_row<kWhich>(p, row);
+        const T  *src  = reinterpret_cast<const T *>(p.src + from * p.ld) + c0 + lane;
+        const int n    = from >= 0 ? p.cols - c0 - lane : 0;
 #pragma unroll
         for (int i = 0; i < kLaneCols; ++i) v[i] = i * 32 < n ? src[i * 32] : from_float<T>(0.f);
         return;
@@ -64,8 +90,9 @@ __device__ __forceinline__ void load_ragged(const QuantParams &p, int row, int c
     {
         const int at = i * 32 + lane, l = at / kLaneCols, r = row + (l >> p.lane_shift);
         const int c  = c0 + (l & ((1 << p.lane_shift) - 1)) * kLaneCols + at % kLaneCols;
-        v[i]         = from_float<T>(0.f);
-        if (r < p.rows && c < p.cols) v[i] = reinterpret_cast<const T *>(p.src + r * p.ld)[c];
+        const int from = source_row<kWhich>(p, r);
+        v[i]           = from_float<T>(0.f);
+        if (from >= 0 && c < p.cols) v[i] = reinterpret_cast<const T *>(p.src + from * p.ld)[c];
     }
 }
 template <typename T>
@@ -152,7 +179,7 @@ __device__ __forceinline__ void swap_units(uint4 &a, uint4 &b, int lane) // the 
 }
 
 // kWhole: every segment lies inside the matrix and all rows are aligned; nothing to test.
-template <typename T, int kFormat, bool kVec, bool kWhole, int kSegs, int kRows>
+template <typename T, int kFormat, bool kVec, bool kWhole, int kSegs, int kRows, int kWhich>
 __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, T *area)
 {
     constexpr int kBlock = kFormat == CUGL_NVFP4 ? 16 : 32;
@@ -171,7 +198,7 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
 #pragma unroll
             for (int g = 0; g < kSegs; ++g)
             {
-                load_ragged(p, at.row + u * at.step - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, loose[u][g]);
+                load_ragged<T, kWhich>(p, at.row + u * at.step - (lane >> p.lane_shift), (static_cast<int>(blockIdx.x) * kSegs + g) * kItemCols, lane, loose[u][g]);
             }
         }
     }
@@ -180,8 +207,9 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
 #pragma unroll
         for (int u = 0; u < kRows; ++u)
         {
-            const int row = at.row + u * at.step;
-            const T  *src = reinterpret_cast<const T *>(p.src + row * p.ld) + at.c0;
+            const int  row  = at.row + u * at.step, from = kWhich == kSlots ? source_row<kWhich>(p, row) : row;
+            const bool in   = kWhich == kSlots ? from >= 0 : row < p.rows;
+            const T   *src  = reinterpret_cast<const T *>(p.src + (kWhich == kSlots ? max(from, 0) : from) * p.ld) + at.c0; // none: row 0, not stored
 #pragma unroll
             for (int g = 0; g < kSegs; ++g)
             {
@@ -192,7 +220,7 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
                     raw[u][g][1]      = __ldg(unit + 2);
                     continue;
                 }
-                const int n = kWhole || row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
+                const int n = kWhole || in ? p.cols - at.c0 - g * kItemCols : 0;
 #pragma unroll
                 for (int l = 0; l < kLoads; ++l)
                 {
@@ -236,14 +264,13 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
             word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
             scale_to_codes<kFormat, sizeof(T) == 4>(v, s);
             const uint32_t w = pack_e2m1x8(v);
-            if (kWhole || row < p.rows)
-            {
+            auto store = [&](uint8_t *row_scales, uint8_t *row_dst) {
                 if ((lane & (4 * kLanes - 1)) == 0 && (kWhole || block + g * 4 * kTiles < 4 * p.tiles))
                 {
-                    *reinterpret_cast<uint32_t *>(scales + g * kTiles * kMxTileBytes) = word; // blocks behind the row: 0
+                    *reinterpret_cast<uint32_t *>(row_scales + g * kTiles * kMxTileBytes) = word; // blocks behind the row: 0
                 }
                 const int n = p.cols - at.c0 - g * kItemCols;
-                uint8_t  *d = dst + g * kItemCols / 2;
+                uint8_t  *d = row_dst + g * kItemCols / 2;
                 if (kWhole || (n >= kLaneCols && p.vec_packed != 0))
                 {
                     *reinterpret_cast<uint32_t *>(d) = w;
@@ -251,6 +278,19 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
                 else
                 {
                     for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) d[i] = static_cast<uint8_t>(w >> (8 * i)); // the half byte behind an odd row is 0
+                }
+            };
+            if constexpr (kWhich == kSame)
+            {
+                if (kWhole || row < p.rows) store(scales, dst);
+            }
+            else if (kWhole || row < p.rows)
+            {
+                const int copies = kWhich == kChoices ? p.top_k : 1;
+                for (int j = 0; j < copies; ++j)
+                {
+                    const int to = slot_of(p, static_cast<int64_t>(row) * copies + j);
+                    if (to >= 0) store(p.scales + mx_scale_offset(to, block, p.tiles), p.dst + to * p.ld_packed + at.c0 / 2);
                 }
             }
         }
@@ -342,7 +382,7 @@ __device__ __forceinline__ void dequantize_group(const QuantParams &p, int group
     }
 }
 
-template <typename T, int kFormat, bool kVec, int kSegs, int kRows, bool kBack>
+template <typename T, int kFormat, bool kVec, int kSegs, int kRows, bool kBack, int kWhich = kSame>
 __global__ void __launch_bounds__(kWarps * 32) mx_rows_kernel(const __grid_constant__ QuantParams p)
 {
     __shared__ __align__(16) T areas[kVec ? 1 : kWarps][kVec ? 8 : kItemCols];
@@ -359,8 +399,8 @@ __global__ void __launch_bounds__(kWarps * 32) mx_rows_kernel(const __grid_const
         }
         else
         {
-            if (whole) quantize_group<T, kFormat, kVec, kVec, kSegs, kRows>(p, group, area);
-            else quantize_group<T, kFormat, kVec, false, kSegs, kRows>(p, group, area);
+            if (whole) quantize_group<T, kFormat, kVec, kVec, kSegs, kRows, kWhich>(p, group, area);
+            else quantize_group<T, kFormat, kVec, false, kSegs, kRows, kWhich>(p, group, area);
         }
     }
 }
@@ -424,28 +464,28 @@ bool wide(const cugl_context *ctx, const QuantParams &p)
 {
     return p.cols >= 4 * kItemCols && static_cast<int64_t>(p.rows) * (p.cols / (4 * kItemCols)) >= 24ll * ctx->sm_count;
 }
-template <typename T, int kFormat, bool kBack>
+template <typename T, int kFormat, bool kBack, int kWhich>
 cudaError_t launch_matrix(cugl_context *ctx, const QuantParams &p)
 {
     if (p.vec_plain == 0)
     {
-        return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 4, 1, kBack>, p, 4, 1)
-                            : launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 1, 1, kBack>, p, 1, 1);
+        return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 4, 1, kBack, kWhich>, p, 4, 1)
+                            : launch_rows(ctx, mx_rows_kernel<T, kFormat, false, 1, 1, kBack, kWhich>, p, 1, 1);
     }
-    return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 4, 1, kBack>, p, 4, 1)
-                        : launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 1, 1, kBack>, p, 1, 1);
+    return wide(ctx, p) ? launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 4, 1, kBack, kWhich>, p, 4, 1)
+                        : launch_rows(ctx, mx_rows_kernel<T, kFormat, true, 1, 1, kBack, kWhich>, p, 1, 1);
 }
-template <typename T, bool kBack>
+template <typename T, bool kBack, int kWhich>
 cudaError_t launch_matrix(cugl_context *ctx, int format, const QuantParams &p)
 {
-    return format == CUGL_NVFP4 ? launch_matrix<T, CUGL_NVFP4, kBack>(ctx, p) : launch_matrix<T, CUGL_MXFP4, kBack>(ctx, p);
+    return format == CUGL_NVFP4 ? launch_matrix<T, CUGL_NVFP4, kBack, kWhich>(ctx, p) : launch_matrix<T, CUGL_MXFP4, kBack, kWhich>(ctx, p);
 }
-template <bool kBack>
+template <bool kBack, int kWhich = kSame>
 cudaError_t launch_matrix(cugl_context *ctx, const cugl_mx_desc &d, const QuantParams &p)
 {
-    return d.dtype == CUGL_F32 ? launch_matrix<float, kBack>(ctx, d.format, p)
-           : d.dtype == CUGL_F16 ? launch_matrix<__half, kBack>(ctx, d.format, p)
-                                 : launch_matrix<__nv_bfloat16, kBack>(ctx, d.format, p);
+    return d.dtype == CUGL_F32 ? launch_matrix<float, kBack, kWhich>(ctx, d.format, p)
+           : d.dtype == CUGL_F16 ? launch_matrix<__half, kBack, kWhich>(ctx, d.format, p)
+                                 : launch_matrix<__nv_bfloat16, kBack, kWhich>(ctx, d.format, p);
 }
 
 const char *validate_mx(const cugl_mx_desc *d, cugl_status *code)
@@ -464,6 +504,25 @@ const char *validate_mx(const cugl_mx_desc *d, cugl_status *code)
     if (d->tensor_exponent < -64 || d->tensor_exponent > 64) return "tensor_exponent must lie within -64 .. 64";
     *code = CUGL_SUCCESS;
     return nullptr;
+}
+
+// the descriptor of the matrix whose rows the launch goes through, or the reason why it cannot
+const char *validate_group(const cugl_mx_group_desc *d, cugl_mx_desc *m)
+{
+    if (d == nullptr) return "descriptor is NULL";
+    if (d->tokens < 0 || d->rows < 0) return "tokens and rows must not be negative";
+    if (d->top_k < 1 || d->top_k > 16) return "top_k must lie within 1 .. 16";
+    if (static_cast<int64_t>(d->tokens) * d->top_k > INT32_MAX - (1 << 20)) return "tokens is too large";
+    *m                 = cugl_mx_desc{};
+    m->rows            = d->src_grouped != 0 ? d->tokens * d->top_k : d->tokens;
+    m->cols            = d->cols;
+    m->format          = d->format;
+    m->dtype           = d->dtype;
+    m->ld              = d->ld;
+    m->ld_packed       = d->ld_packed;
+    m->tensor_exponent = d->tensor_exponent;
+    cugl_status code;
+    return validate_mx(m, &code);
 }
 
 cugl_status check_mx(cugl_context *ctx, const char *name, const cugl_mx_desc *d, const void *plain, const void *packed, const void *scales)
@@ -535,6 +594,46 @@ extern "C"
         p.scales       = const_cast<uint8_t *>(static_cast<const uint8_t *>(d_scales));
         p.exponent_mul = std::ldexp(1.f, desc->tensor_exponent);
         CUGL_CUDA_TRY(ctx, launch_matrix<true>(ctx, *desc, p));
+        return CUGL_SUCCESS;
+    }
+
+    cugl_status cugl_mx_group_validate(const cugl_mx_group_desc *desc, const char **reason)
+    {
+        cugl_mx_desc m;
+        const char  *why = validate_group(desc, &m);
+        if (reason != nullptr)
+        {
+            *reason = why != nullptr ? why : "";
+        }
+        return why == nullptr ? CUGL_SUCCESS : CUGL_INVALID_ARGUMENT;
+    }
+
+    cugl_status cugl_mx_quantize_grouped(cugl_context *ctx, const cugl_mx_group_desc *desc, const void *d_src, const int32_t *d_slots, void *d_dst,
+                                         void *d_scales)
+    {
+        if (ctx == nullptr)
+        {
+            return fail(nullptr, CUGL_INVALID_ARGUMENT, "context is NULL");
+        }
+        cugl_mx_desc m;
+        const char  *why = validate_group(desc, &m);
+        if (why == nullptr && desc->tokens > 0 && desc->rows > 0 && (d_slots == nullptr || !aligned(d_slots, 4))) why = "d_slots must be given, aligned to its elements";
+        if (why != nullptr)
+        {
+            return fail(ctx, CUGL_INVALID_ARGUMENT, std::string("cugl_mx_quantize_grouped: ") + why);
+        }
+        if (desc->tokens == 0 || desc->rows == 0) return CUGL_SUCCESS;
+        CUGL_TRY(check_mx(ctx, "cugl_mx_quantize_grouped", &m, d_src, d_dst, d_scales));
+        const DeviceScope device(ctx);
+        QuantParams       p = make_params(m, d_src, d_dst);
+        p.src          = static_cast<const uint8_t *>(d_src);
+        p.dst          = static_cast<uint8_t *>(d_dst);
+        p.scales       = static_cast<uint8_t *>(d_scales);
+        p.exponent_mul = std::ldexp(1.f, -desc->tensor_exponent);
+        p.slots        = d_slots;
+        p.top_k        = desc->top_k;
+        p.group_rows   = desc->rows;
+        CUGL_CUDA_TRY(ctx, (desc->src_grouped != 0 ? launch_matrix<false, kSlots>(ctx, m, p) : launch_matrix<false, kChoices>(ctx, m, p)));
         return CUGL_SUCCESS;
     }
 

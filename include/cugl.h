@@ -641,6 +641,103 @@ CUGL_API cugl_status cugl_mx_moe(cugl_context *ctx, const cugl_mx_moe_desc *desc
                                  const void *d_down, const void *d_down_scales, void *d_dst, void *d_workspace,
                                  size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------------------------------
+ * Expert layers of any number of tokens, step by step: the rows of an expert's tokens lie together, as a group of the rows of one
+ * matrix.  Groups are (start, count) pairs on the device, int32 [groups][2]; a group starts at a multiple of 128 rows, so that its
+ * scale tiles are its own.  Groups do not overlap.  No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------------- */
+/* Rows of a matrix that holds any `rows` rows in `groups` groups (a multiple of 128; 0: bad argument). */
+CUGL_API int64_t     cugl_mx_group_rows(int32_t groups, int64_t rows);
+
+/* The gate: the top_k largest logits of every token, equal ones by index (NaN and -infinity are never chosen), and a row for every
+ * choice.
+ *   ids      [tokens][top_k]  chosen experts, the largest logit first; -1: fewer than top_k could be chosen
+ *   weights  [tokens][top_k]  exp(logit) over its sum, over the chosen ones (renormalize) or over all; 0 where there is no choice
+ *   slots    [tokens][top_k]  the choice's row: the rows of an expert follow each other in the order of the tokens; -1: no choice
+ *   groups   [experts][2]     (start, count) of every expert's rows: whole multiples of 128 rows each, one behind the other, within the
+ *                             first cugl_mx_group_rows(experts, tokens * top_k) */
+typedef struct cugl_moe_route_desc
+{
+    int32_t tokens;
+    int32_t experts, top_k; /* 1 .. 512, 1 .. 16 */
+    int32_t dtype;          /* of the logits: CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int32_t renormalize;
+    int64_t ld_logits;      /* bytes between rows */
+} cugl_moe_route_desc;
+
+CUGL_API cugl_status cugl_moe_route_validate(const cugl_moe_route_desc *desc, const char **reason);
+/* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU need one each. */
+CUGL_API size_t      cugl_moe_route_workspace_bytes(const cugl_moe_route_desc *desc);
+/* One launch for up to 128 tokens, else two.  d_workspace: 16-byte aligned; groups: 8-byte aligned.  tokens == 0: groups of no rows. */
+CUGL_API cugl_status cugl_moe_route(cugl_context *ctx, const cugl_moe_route_desc *desc, const void *d_logits, int32_t *d_ids,
+                                    float *d_weights, int32_t *d_slots, int32_t *d_groups, void *d_workspace,
+                                    size_t workspace_bytes);
+
+/* Plain rows -> packed rows of groups, as cugl_mx_quantize stores them.
+ *   src_grouped == 0  row t of src to the rows slots[t][0 .. top_k): a token to all its experts, quantised once
+ *   src_grouped != 0  row slots[t][j] of src to the same row of dst: what the groups' products left
+ * Slots outside 0 .. rows - 1 (-1) are skipped; rows that no slot names are left as they are. */
+typedef struct cugl_mx_group_desc
+{
+    int32_t tokens, top_k;   /* of the slots; top_k 1 .. 16 */
+    int32_t rows, cols;      /* rows of the grouped matrix; columns */
+    int32_t format;          /* cugl_mx_format */
+    int32_t dtype;           /* of the plain matrix: CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int32_t src_grouped;
+    int32_t tensor_exponent; /* as in cugl_mx_desc */
+    int64_t ld, ld_packed;   /* bytes between rows of the plain and of the packed matrix */
+} cugl_mx_group_desc;
+
+CUGL_API cugl_status cugl_mx_group_validate(const cugl_mx_group_desc *desc, const char **reason);
+/* d_scales: the tiles of a matrix of `rows` rows (cugl_mx_scale_bytes).  No buffer overlaps another. */
+CUGL_API cugl_status cugl_mx_quantize_grouped(cugl_context *ctx, const cugl_mx_group_desc *desc, const void *d_src,
+                                              const int32_t *d_slots, void *d_dst, void *d_scales);
+
+/* The way back from the groups: dst[t] = sum over j of weights[t][j] * src[slots[t][j]], added up in float in the order of j, rounded
+ * once.  Slots outside 0 .. rows - 1 (-1) count nothing; a token without any gets zeros. */
+typedef struct cugl_moe_combine_desc
+{
+    int32_t tokens, top_k;        /* top_k 1 .. 16 */
+    int32_t rows, cols;           /* rows of src; columns */
+    int32_t src_dtype, dst_dtype; /* CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int64_t ld_src, ld_dst;       /* bytes between rows */
+} cugl_moe_combine_desc;
+
+CUGL_API cugl_status cugl_moe_combine_validate(const cugl_moe_combine_desc *desc, const char **reason);
+/* dst overlaps none of the others. */
+CUGL_API cugl_status cugl_moe_combine(cugl_context *ctx, const cugl_moe_combine_desc *desc, const void *d_src,
+                                      const int32_t *d_slots, const float *d_weights, void *d_dst);
+
+/* Products of every group with weights of its own, r a row of group g:
+ *   dst[r][n] = alpha * d_b_alpha[g] * sum_k a[r][k] * b[g][n][k] + bias[g][n]
+ *   dst[r][n] = silu(alpha * d_b_alpha[g] * a[r] . b[g][n]) * (up_alpha * d_up_alpha[g] * a[r] . up[g][n])      (swiglu)
+ * a: packed rows with scale tiles; b and up: [groups * N] packed rows of K elements, the scale tiles of every group those of an N x K
+ * matrix of its own (cugl_mx_scale_bytes); the layout of cugl_mx_moe's weights.  Float accumulation, rounded once to dst_dtype.  Rows of dst
+ * that belong to no group are left as they were; those of a may hold anything. */
+typedef struct cugl_mx_grouped_gemm_desc
+{
+    int32_t groups;        /* 1 .. 512 */
+    int32_t rows;          /* of a and dst */
+    int32_t expected_rows; /* about how many of them belong to groups (chooses the kernel only; 0: all) */
+    int32_t N, K;
+    int32_t format;        /* cugl_mx_format, of a, b and up */
+    int32_t dst_dtype;     /* CUGL_F32, CUGL_F16 or CUGL_BF16 */
+    int32_t swiglu;        /* two products */
+    int32_t has_bias;      /* float bias [groups][N]; not with swiglu */
+    float   alpha, up_alpha;
+    int64_t lda, ldb, ldd; /* bytes between rows (ldb: of b and up); lda and ldb multiples of 16 */
+} cugl_mx_grouped_gemm_desc;
+
+CUGL_API cugl_status cugl_mx_grouped_gemm_validate(const cugl_mx_grouped_gemm_desc *desc, const char **reason);
+/* One launch, no workspace, nothing kept between calls.  d_b_alpha, d_up_alpha: float [groups] or NULL (1).  Operands and scale tiles
+ * are 16-byte aligned, dst overlaps none of them.  Equal calls give equal bits.  A group that does not start at a multiple of 128 or does not
+ * lie within the rows is left out; the next cugl_sync() reports it as CUGL_RUNTIME_ERROR.  rows == 0: nothing to do. */
+CUGL_API cugl_status cugl_mx_grouped_gemm(cugl_context *ctx, const cugl_mx_grouped_gemm_desc *desc, const void *d_a,
+                                          const void *d_a_scales, const int32_t *d_groups, const void *d_b,
+                                          const void *d_b_scales, const float *d_b_alpha, const void *d_up,
+                                          const void *d_up_scales, const float *d_up_alpha, const float *d_bias,
+                                          void *d_dst);
+
 #ifdef __cplusplus
 }
 #endif
