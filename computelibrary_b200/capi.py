@@ -133,6 +133,15 @@ class MoeCombineDesc(C.Structure):
     ]
 
 
+class LoraDesc(C.Structure):
+    """cugl_lora_desc"""
+    _fields_ = [
+        ("tokens", _i32), ("requests", _i32), ("adapters", _i32), ("max_rank", _i32), ("K", _i32), ("N", _i32),
+        ("dtype", _i32), ("dst_dtype", _i32),
+        ("ld_x", _i64), ("ld_a", _i64), ("ld_b", _i64), ("ld_base", _i64), ("ld_dst", _i64),
+    ]
+
+
 POOL_MAX, POOL_AVG = 0, 1
 ACT_NONE, ACT_RELU, ACT_BOUNDED_RELU, ACT_LU_BOUNDED_RELU = -1, 0, 1, 2
 
@@ -248,6 +257,9 @@ _SIGNATURES = {
     "cugl_mx_quantize_grouped": (C.c_int, [_vp, C.POINTER(MxGroupDesc)] + [_vp] * 4),
     "cugl_moe_combine_validate": (C.c_int, [C.POINTER(MoeCombineDesc), C.POINTER(C.c_char_p)]),
     "cugl_moe_combine": (C.c_int, [_vp, C.POINTER(MoeCombineDesc)] + [_vp] * 4),
+    "cugl_lora_validate": (C.c_int, [C.POINTER(LoraDesc), C.POINTER(C.c_char_p)]),
+    "cugl_lora_workspace_bytes": (C.c_size_t, [C.POINTER(LoraDesc)]),
+    "cugl_lora": (C.c_int, [_vp, C.POINTER(LoraDesc)] + [_vp] * 10 + [C.c_size_t]),
     "cugl_mx_group_rows": (_i64, [_i32, _i64]),
     "cugl_mx_grouped_gemm_validate": (C.c_int, [C.POINTER(MxGroupedGemmDesc), C.POINTER(C.c_char_p)]),
     "cugl_mx_grouped_gemm": (C.c_int, [_vp, C.POINTER(MxGroupedGemmDesc)] + [_vp] * 11),
@@ -507,6 +519,14 @@ class Context:
         self.check(self.lib.cugl_mx_grouped_gemm(self.handle, C.byref(desc), _dptr(a), _dptr(a_scales), _dptr(groups), *parts(b),
                                                  *parts(up), _dptr(bias), _dptr(dst)))
 
+    def lora(self, desc: "LoraDesc", x, starts, request_adapters, ranks, scales, a, b, base, dst, workspace, workspace_bytes=None):
+        """dst = base + the adapters' products; workspace: lora_workspace_bytes(desc) bytes (workspace_bytes: its size where it is a
+        raw pointer)."""
+        if workspace_bytes is None:
+            workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        self.check(self.lib.cugl_lora(self.handle, C.byref(desc), _dptr(x), _dptr(starts), _dptr(request_adapters), _dptr(ranks),
+                                      _dptr(scales), _dptr(a), _dptr(b), _dptr(base), _dptr(dst), _dptr(workspace), workspace_bytes))
+
     def weights_reshape_nhwc(self, w, dst, K, OFM):
         self.check(self.lib.cugl_weights_reshape_nhwc(self.handle, _dptr(w), _dptr(dst), K, OFM))
 
@@ -698,6 +718,30 @@ def make_moe_combine_desc(tokens, top_k, cols, rows, src_dtype, dst_dtype, ld_sr
 def moe_combine_validate(desc: MoeCombineDesc):
     """Returns (status, reason)."""
     return _validated(load_library().cugl_moe_combine_validate, desc)
+
+
+def make_lora_desc(tokens, requests, adapters, max_rank, K, N, dtype, dst_dtype, ld_x=None, ld_a=None, ld_b=None, ld_base=None,
+                   ld_dst=None) -> LoraDesc:
+    """cugl_lora_desc; dense matrices (rows of B at the next multiple of 16 bytes) unless strides (bytes) are given."""
+    d = LoraDesc()
+    d.tokens, d.requests, d.adapters, d.max_rank, d.K, d.N = tokens, requests, adapters, max_rank, K, N
+    d.dtype, d.dst_dtype = dtype, dst_dtype
+    size = 4 if dst_dtype == F32 else 2
+    d.ld_x = 2 * K if ld_x is None else ld_x
+    d.ld_a = 2 * K if ld_a is None else ld_a
+    d.ld_b = (2 * max_rank + 15) // 16 * 16 if ld_b is None else ld_b
+    d.ld_base = N * size if ld_base is None else ld_base
+    d.ld_dst = N * size if ld_dst is None else ld_dst
+    return d
+
+
+def lora_validate(desc: LoraDesc):
+    """Returns (status, reason)."""
+    return _validated(load_library().cugl_lora_validate, desc)
+
+
+def lora_workspace_bytes(desc: LoraDesc) -> int:
+    return int(load_library().cugl_lora_workspace_bytes(C.byref(desc)))
 
 
 def make_mx_grouped_gemm_desc(groups, rows, N, K, format, dst_dtype, expected_rows=0, swiglu=False, has_bias=False, alpha=1.0,

@@ -738,6 +738,39 @@ CUGL_API cugl_status cugl_mx_grouped_gemm(cugl_context *ctx, const cugl_mx_group
                                           const void *d_up_scales, const float *d_up_alpha, const float *d_bias,
                                           void *d_dst);
 
+/* ------------------------------------------------------------------------------------------------
+ * Low-rank adapters of many requests at once beside a projection that all of them share (cugl_mx_gemm's, for instance):
+ *   dst[t] = base[t] + scales[a] * (x[t] . A[a]^T) . B[a]^T,    a the adapter of the request that token t belongs to
+ * The tokens of request i are [starts[i], starts[i + 1]); its adapter is request_adapters[i], any index outside 0 .. adapters - 1 for
+ * none (dst[t] = base[t]).  Adapter a has ranks[a] ranks, at most max_rank; what lies behind them in A and B counts nothing.  Float sums;
+ * x . A^T is kept to 16 bits or more (22 for CUGL_F16, 24 where bf16 adapters add to 32-bit results), the sum is rounded once.  Tokens of
+ * no request are left as they were.  No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct cugl_lora_desc
+{
+    int32_t tokens, requests;
+    int32_t adapters, max_rank; /* max_rank 1 .. 128 */
+    int32_t K, N;               /* columns of x; of base and dst */
+    int32_t dtype;              /* of x, A and B: CUGL_F16 or CUGL_BF16 */
+    int32_t dst_dtype;          /* of base and dst: dtype or CUGL_F32 */
+    int64_t ld_x;               /* bytes between rows */
+    int64_t ld_a;               /* A: [adapters][max_rank] rows of K elements */
+    int64_t ld_b;               /* B: [adapters][N] rows of max_rank elements, a multiple of 16 */
+    int64_t ld_base, ld_dst;
+} cugl_lora_desc;
+
+CUGL_API cugl_status cugl_lora_validate(const cugl_lora_desc *desc, const char **reason);
+/* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU, and captured graphs
+ * that are replayed at the same time, need one each. */
+CUGL_API size_t      cugl_lora_workspace_bytes(const cugl_lora_desc *desc);
+/* starts: int32 [requests + 1], in order; request_adapters: int32 [requests]; ranks: int32 [adapters] or NULL (max_rank); scales: float
+ * [adapters].  B and the workspace are 16-byte aligned, B's rows are read in whole units of 8 bytes.  dst may be base (then ld_dst == ld_base), else it overlaps nothing.  Two
+ * launches; equal calls give equal bits.  tokens == 0 or requests == 0: nothing to do. */
+CUGL_API cugl_status cugl_lora(cugl_context *ctx, const cugl_lora_desc *desc, const void *d_x, const int32_t *d_starts,
+                               const int32_t *d_request_adapters, const int32_t *d_ranks, const float *d_scales,
+                               const void *d_a, const void *d_b, const void *d_base, void *d_dst, void *d_workspace,
+                               size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif
