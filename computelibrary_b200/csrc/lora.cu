@@ -10,10 +10,9 @@
 // work (4096 tokens, 4096 -> 4096, rank 64: 2 x 2.1 GFLOP beside 170 MB).  Hence mma.sync, whose accumulators are the registers that
 // base is added to: nothing of a matrix unit's rate is missing, and no operand waits in shared memory.
 //
-// Fragments.  Sums do not care in which order their terms come, as long as both operands agree: a lane takes 8 consecutive elements of
-// K (16 bytes) as the four pairs that two steps of the matrix instruction want from it, and 4 consecutive ranks as the two pairs of
-// one step.  Channels likewise: the four 8-column tiles of a warp's 32 channels are dealt out so that a lane's results are 8 consecutive
-// channels of a row.
+// Fragments.  Sums do not care in which order their terms come, as long as both operands agree: a lane of the second launch takes 4
+// consecutive ranks as the two pairs that a step of the matrix instruction wants from it.  Channels likewise: the four 8-column tiles
+// of a warp's 32 channels are dealt out so that a lane's results are whole 16-byte pieces of a row.
 //
 // v is kept as two 16-bit parts, v = high + low (three where bf16 adapters add to 32-bit results): 16 (bf16) or 22 (f16) bits of it
 // count, 24 with three parts, so rounding v costs less than rounding the result.  f16 parts would leave that type's range: a token's
@@ -21,6 +20,7 @@
 #include "mx.cuh"
 #include "sm100.cuh"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstring>
@@ -31,7 +31,6 @@ namespace
 {
 constexpr int kThreads  = 256;
 constexpr int kWarps    = kThreads / 32;
-constexpr int kChannels = 32 * kWarps; // of a CTA of the second launch
 constexpr int kMaxRank  = 128;
 constexpr int kMaxSplit = 8;
 
@@ -41,10 +40,10 @@ struct LoraParams
     uint8_t       *dst;
     const int32_t *starts, *adapters, *ranks;
     const float   *scales;
-    uint16_t      *v;      // [parts][tokens][padded rank]
-    float         *factor; // [tokens]
+    uint16_t      *v; // [parts][tokens][padded rank + 8]: the first part's last eight elements hold the token's factor (a float)
     int64_t        ld_x, ld_a, ld_b, ld_base, ld_dst; // bytes
     int            tokens, requests, n_adapters, max_rank, K, N, parts, tile;
+    int            tiles; // at most
 };
 
 // ---- which tokens a tile holds -------------------------------------------------------------------------------
@@ -60,51 +59,69 @@ __device__ __forceinline__ int load_l2(const int32_t *p)
 {
     return __ldcg(p);
 }
-// A request's tokens are [starts[i], starts[i + 1]), cut to those there are.  Called by all threads.
+// A request's tokens are [starts[i], starts[i + 1]), cut to those there are.
+struct Request
+{
+    int begin, end, adapter, rank;
+};
+__device__ __forceinline__ Request load_request(const LoraParams &p, int r)
+{
+    Request q{0, 0, -1, 0};
+    if (r < p.requests)
+    {
+        const int begin = load_l2(p.starts + r), end = load_l2(p.starts + r + 1), a = load_l2(p.adapters + r);
+        q.begin         = min(max(begin, 0), p.tokens);
+        q.end           = min(max(end, q.begin), p.tokens);
+        if (a >= 0 && a < p.n_adapters)
+        {
+            q.rank    = p.ranks != nullptr ? min(max(load_l2(p.ranks + a), 0), p.max_rank) : p.max_rank;
+            q.adapter = q.rank > 0 ? a : -1;
+        }
+    }
+    return q;
+}
+struct ScanShared
+{
+    int sums[2][kWarps];
+};
+// The tiles of kThreads requests: a thread's own come behind `at` others, `all` are there.  By all threads; turn: alternately 0 and 1.
+__device__ __forceinline__ void scan_tiles(ScanShared &s, int turn, int tiles, int &at, int &all)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int       incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int n = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += n;
+    }
+    if (lane == 31) s.sums[turn][warp] = incl;
+    __syncthreads();
+    at = incl - tiles;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+    {
+        if (w < warp) at += s.sums[turn][w];
+        all += s.sums[turn][w];
+    }
+}
+// Tile number `wanted`.  By all threads.
 __device__ __forceinline__ Tile find_tile(const LoraParams &p, int wanted)
 {
-    __shared__ Tile found;
-    __shared__ int  sums[kWarps];
-    const int       lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ Tile       found;
+    __shared__ ScanShared scan;
     if (threadIdx.x == 0) found = Tile{0, 0, -1, 0};
-    int before = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreads)
+    int before = 0, turn = 0;
+    for (int r0 = 0; r0 < p.requests && before <= wanted; r0 += kThreads, turn ^= 1)
     {
-        const int r = r0 + static_cast<int>(threadIdx.x);
-        int       begin = 0, end = 0;
-        if (r < p.requests)
-        {
-            begin = min(max(load_l2(p.starts + r), 0), p.tokens);
-            end   = min(max(load_l2(p.starts + r + 1), begin), p.tokens);
-        }
-        const int tiles = (end - begin + p.tile - 1) / p.tile;
-        int       incl  = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-        {
-            const int n = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += n;
-        }
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        int at = before, all = before;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-        {
-            if (w < warp) at += sums[w];
-            all += sums[w];
-        }
-        at += incl - tiles;
-        if (wanted >= at && wanted < at + tiles)
-        {
-            const int first = begin + (wanted - at) * p.tile;
-            int       a     = load_l2(p.adapters + r), rank = 0;
-            if (a >= 0 && a < p.n_adapters) rank = p.ranks != nullptr ? min(max(load_l2(p.ranks + a), 0), p.max_rank) : p.max_rank;
-            found = Tile{first, min(p.tile, end - first), rank > 0 ? a : -1, rank};
-        }
-        before = all;
-        __syncthreads();
-        if (wanted < before) break; // the same for all
+        const Request q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
+        const int     tiles = (q.end - q.begin + p.tile - 1) / p.tile;
+        int           at, all;
+        scan_tiles(scan, turn, tiles, at, all);
+        const int i = wanted - before - at;
+        if (i >= 0 && i < tiles) found = Tile{q.begin + i * p.tile, min(p.tile, q.end - q.begin - i * p.tile), q.adapter, q.rank};
+        before += all;
     }
     __syncthreads();
     return found;
@@ -129,32 +146,63 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     }
 }
 
-// eight 16-bit elements of a row from column k on, zeros behind `cols`
+// ---- asynchronous copies -------------------------------------------------------------------------------------
+// 16 bytes to shared memory, those from `valid` on as zeros; past L1
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int valid)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
+__device__ __forceinline__ void copy_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void copy_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// eight 16-bit elements of a row from column k on to shared memory, zeros behind `cols`; kVec: rows are 16-byte aligned
 template <bool kVec>
-__device__ __forceinline__ uint4 load_eight(const uint8_t *row, int k, int cols)
+__device__ __forceinline__ void stage_eight(uint32_t dst, const uint8_t *row, int k, int cols)
 {
     const uint16_t *src = reinterpret_cast<const uint16_t *>(row) + k;
-    if (kVec && k + 8 <= cols) return __ldg(reinterpret_cast<const uint4 *>(src));
-    uint16_t e[8];
+    if constexpr (kVec)
+    {
+        const int valid = min(max(cols - k, 0) * 2, 16);
+        copy16(dst, valid > 0 ? src : reinterpret_cast<const uint16_t *>(row), valid);
+    }
+    else
+    {
+        uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = k + i < cols ? __ldg(src + i) : static_cast<uint16_t>(0);
-    uint4 v;
-    memcpy(&v, e, 16);
-    return v;
+        for (int i = 0; i < 4; ++i)
+        {
+            const uint32_t lo = k + 2 * i < cols ? __ldg(src + 2 * i) : 0u, hi = k + 2 * i + 1 < cols ? __ldg(src + 2 * i + 1) : 0u;
+            w[i]              = lo | (hi << 16);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
 }
 
 // ---- first launch: v = x . A^T -------------------------------------------------------------------------------
-// A warp multiplies 16 kMt tokens with all ranks over a share of K; tiles of more tokens take two warps side by side.  The loads of two
-// blocks of 32 columns are in flight per warp.
+// A ring of stages of 64 columns of K: up to 64 (32) tokens and all ranks, rows of 128 bytes whose 16-byte units are exchanged by row, so
+// that ldmatrix reads eight rows from different banks.  A warp takes 16 columns of a stage and 32 (16) tokens; tiles of few tokens
+// leave every other stage to the other half of the warps.
 template <int kRank>
 struct Shrink
 {
     static constexpr int kMt     = kRank == 128 ? 1 : 2; // 16-row tiles of a warp
     static constexpr int kRows   = 16 * kMt;
     static constexpr int kTile   = 2 * kRows;
-    static constexpr int kPitch  = kRank + 8; // floats: rows in different banks
-    static constexpr int kSmem   = kWarps * kRows * kPitch * 4;
-    static_assert(kTile * kPitch <= kWarps * kRows * kPitch, "sums fit where the warps' shares were");
+    static constexpr int kStages = kRank == 128 ? 5 : 6;
+    static constexpr int kStage  = (kTile + kRank) * 128; // bytes
+    static constexpr int kPitch  = kRank + 8;             // floats: rows in different banks
+    static constexpr int kSmem   = kStages * kStage;
+    static_assert(kWarps * kRows * kPitch * 4 <= kSmem, "the warps' sums fit where the stages were");
 };
 __device__ __forceinline__ float load_cluster(uint32_t addr)
 {
@@ -168,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 {
     using S = Shrink<kRank>;
     constexpr int kNt = kRank / 8;
-    extern __shared__ __align__(16) float share[]; // [warp][row][rank], then [token][rank]
+    extern __shared__ __align__(128) float share[]; // stages, then sums [warp][row][rank], then [token][rank]
     griddep_wait();
     griddep_launch_dependents(); // whatever ran before has completed: the second launch may read it
     const int ranks = static_cast<int>(gridDim.x / num_clusters_x());
@@ -181,49 +229,79 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int halves = t.count > S::kRows ? 2 : 1, subs = kWarps / halves;
     const int half = warp & (halves - 1), sub = halves == 2 ? warp >> 1 : warp;
-    // blocks of 32 columns, shared by the CTAs of the cluster and their warps
-    const int blocks = (p.K + 31) / 32, parts = ranks * subs, part = rank * subs + sub;
-    const int k_begin = static_cast<int>(static_cast<int64_t>(blocks) * part / parts), k_end = static_cast<int>(static_cast<int64_t>(blocks) * (part + 1) / parts);
-    const int row0 = half * S::kRows, left = t.count - row0; // tokens of this warp
-    const uint8_t *x = p.x + static_cast<int64_t>(t.first + row0) * p.ld_x;
+    const int blocks = (p.K + 63) / 64; // of 64 columns, shared by the CTAs of the cluster
+    const int first  = static_cast<int>(static_cast<int64_t>(blocks) * rank / ranks), n_blocks = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / ranks) - first;
+    const int x_rows = (t.count + 15) & ~15, a_rows = (t.rank + 15) & ~15; // those that the matrix instructions read
+    const uint8_t *x = p.x + static_cast<int64_t>(t.first) * p.ld_x;
     const uint8_t *a = p.a + static_cast<int64_t>(t.adapter) * p.max_rank * p.ld_a;
-    float          acc[S::kMt][kNt][4] = {};
-    const uint4    zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
-    for (int kb = k_begin; kb < k_end; ++kb)
+    const uint32_t s_base = smem_u32(share);
+    // what a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows (rows behind the last: zeros)
+    constexpr int  kCopies = (S::kTile + kRank + kThreads / 8 - 1) / (kThreads / 8);
+    const int      c8      = (static_cast<int>(threadIdx.x) & 7) * 8;
+    const uint8_t *from[kCopies];
+    uint32_t       to[kCopies];
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j)
     {
-        const int k = kb * 32 + c * 8;
-        uint4     xv[S::kMt][2];
+        const int  i = (static_cast<int>(threadIdx.x) >> 3) + j * (kThreads / 8), row = i < x_rows ? i : i - x_rows;
+        const bool is_x = i < x_rows;
+        from[j] = is_x ? (row < t.count ? x + row * p.ld_x : nullptr) : (row < t.rank ? a + row * p.ld_a : nullptr);
+        to[j]   = row < (is_x ? x_rows : a_rows) ? static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4)) : 0xffffffffu;
+    }
+    auto load = [&](int block) {
+        if (block < n_blocks)
+        {
+            const uint32_t st = s_base + static_cast<uint32_t>(block % S::kStages) * S::kStage;
+            const int      k  = (first + block) * 64 + c8;
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j)
+            {
+                if (to[j] != 0xffffffffu) stage_eight<kVec>(st + to[j], from[j] != nullptr ? from[j] : x, k, from[j] != nullptr ? p.K : 0);
+            }
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) load(i);
+    float     acc[S::kMt][kNt][4] = {};
+    const int step = halves == 2 ? sub : sub & 3; // 16 columns of a stage
+    for (int i = 0; i < n_blocks; ++i)
+    {
+        copy_wait<S::kStages - 2>();
+        __syncthreads();
+        load(i + S::kStages - 1); // to the stage that all warps have left
+        if (halves == 1 && (i & 1) != (sub >> 2)) continue;
+        const uint32_t st = s_base + static_cast<uint32_t>(i % S::kStages) * S::kStage;
+        uint32_t       xv[S::kMt][4];
 #pragma unroll
         for (int m = 0; m < S::kMt; ++m)
         {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-            {
-                const int r = m * 16 + h * 8 + g;
-                xv[m][h]    = r < left ? load_eight<kVec>(x + r * p.ld_x, k, p.K) : zero;
-            }
+            const int row = half * S::kRows + m * 16 + (lane & 15), unit = 2 * step + (lane >> 4);
+            if (half * S::kRows + m * 16 < t.count) ldmatrix_x4(st + static_cast<uint32_t>(row * 128 + ((unit ^ (row & 7)) << 4)), xv[m]);
         }
 #pragma unroll
-        for (int n = 0; n < kNt; ++n)
+        for (int n = 0; n < kNt; n += 2)
         {
             if (n * 8 < t.rank)
             {
-                const int   r  = n * 8 + g;
-                const uint4 av = r < t.rank ? load_eight<kVec>(a + r * p.ld_a, k, p.K) : zero;
+                const int row = n * 8 + (lane & 7) + ((lane >> 4) << 3), unit = 2 * step + ((lane >> 3) & 1);
+                uint32_t  av[4];
+                ldmatrix_x4(st + static_cast<uint32_t>((S::kTile + row) * 128 + ((unit ^ (row & 7)) << 4)), av);
 #pragma unroll
                 for (int m = 0; m < S::kMt; ++m)
                 {
-                    if (m * 16 < left)
+                    if (half * S::kRows + m * 16 < t.count)
                     {
-                        mma<T>(acc[m][n], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av.x, av.y);
-                        mma<T>(acc[m][n], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av.z, av.w);
+                        mma<T>(acc[m][n], xv[m][0], xv[m][1], xv[m][2], xv[m][3], av[0], av[1]);
+                        mma<T>(acc[m][n + 1], xv[m][0], xv[m][1], xv[m][2], xv[m][3], av[2], av[3]);
                     }
                 }
             }
         }
     }
-    float *mine = share + static_cast<int>(warp) * S::kRows * S::kPitch;
+    copy_wait<0>();
+    __syncthreads(); // the stages are free
+    float *mine = share + warp * S::kRows * S::kPitch;
 #pragma unroll
     for (int m = 0; m < S::kMt; ++m)
     {
@@ -236,12 +314,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
         }
     }
     __syncthreads();
-    // the warps' shares, in their order, to where the first of them was (a thread adds up what it writes to; with two halves the second
+    // the warps' sums, in their order, to where the first of them was (a thread adds up what it writes to; with two halves the second
     // half's sums go to the second warp's place)
     for (int i = threadIdx.x; i < t.count * kRank; i += kThreads)
     {
-        const int tok = i / kRank, r = i % kRank, h = tok / S::kRows, row = tok % S::kRows;
-        float    *at = share + (h * S::kRows + row) * S::kPitch + r;
+        const int tok = i / kRank, r = i % kRank;
+        float    *at = share + tok * S::kPitch + r; // rows of both halves follow each other
         float     sum = *at;
         for (int s = 1; s < subs; ++s) sum += at[s * halves * S::kRows * S::kPitch];
         *at = sum;
@@ -252,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     for (int tok = rank * kWarps + warp; tok < t.count; tok += ranks * kWarps)
     {
         constexpr int  kPer = (kRank + 31) / 32;
-        const uint32_t at   = smem_u32(share + tok * S::kPitch); // rows of both halves follow each other
+        const uint32_t at   = smem_u32(share + tok * S::kPitch);
         float          v[kPer];
         float          top = 0.f;
 #pragma unroll
@@ -279,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
                 factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             }
         }
-        uint16_t *out = p.v + static_cast<int64_t>(t.first + tok) * kRank;
+        uint16_t *out = p.v + static_cast<int64_t>(t.first + tok) * (kRank + 8);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
         {
@@ -292,161 +370,344 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
                     const T part = from_float<T>(rest);
                     uint16_t bits;
                     memcpy(&bits, &part, 2);
-                    out[static_cast<int64_t>(q) * p.tokens * kRank + r] = bits;
+                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + r] = bits;
                     const float f = to_float(part);
                     rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
                 }
             }
         }
-        if (lane == 0) p.factor[t.first + tok] = factor;
+        if (lane == 0) *reinterpret_cast<float *>(out + kRank) = factor;
     }
     if (ranks > 1) cluster_sync(); // nobody leaves while others read its sums
 }
 
 // ---- second launch: dst = base + factor * v . B^T --------------------------------------------------------------
-template <typename TD, bool kVec>
-__device__ __forceinline__ void load_base(const uint8_t *row, int n, int cols, float (&v)[8])
+// Every CTA works through an equal share of the items, an item being 256 channels of a tile; consecutive items are consecutive channels.  A
+// warp has 32 channels, the tokens of the tile sixteen at a time.  What it needs next is under way while it works: units of 16 tokens
+// x 32 channels of base pass through a ring of four slots of its own, the next item's B waits in registers, the next tile's v in the other
+// half of its buffer.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
+//   two-byte results  8 c .. 8 c + 7
+//   floats            4 c .. 4 c + 3 and 16 + 4 c .. 16 + 4 c + 3, so that a store of four lanes covers whole sectors
+constexpr int kListTiles = 256; // tiles of a CTA's share
+template <typename T, typename TD, int kRank>
+struct Expand
 {
-    TD        e[8];
-    const TD *src = reinterpret_cast<const TD *>(row) + n;
-    if constexpr (kVec)
-    {
-        uint4 q[sizeof(TD) / 2];
+    static constexpr int kSteps   = kRank / 16;
+    static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM: two items' B take 128 registers there
+    static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
+    static constexpr int kTile    = Shrink<kRank>::kTile;
+    static constexpr int kPitch   = kRank == 16 ? 48 : kRank * 2 + 32; // bytes of a row of v: four rows in different banks
+    static constexpr int kV       = kParts * kTile * kPitch;
+    static constexpr int kRow     = 32 * static_cast<int>(sizeof(TD)); // bytes of a row of a unit
+    static constexpr int kSlots   = 4;
+    static constexpr int kOffBase = 2 * kV;
+    static constexpr int kSmem    = kOffBase + kWarps * kSlots * 16 * kRow;
+};
+// the first channel of a lane's piece of 16 bytes
+template <typename TD>
+__device__ __forceinline__ int piece_channel(int piece, int c)
+{
+    return sizeof(TD) == 4 ? piece * 16 + 4 * c : 8 * c;
+}
+
+// B of an item, as fragments; what lies behind the adapter's rank counts nothing, whatever it is
+template <typename TD, int kSteps>
+__device__ __forceinline__ void load_b(const LoraParams &p, const Tile &t, int n, int lane, uint2 (&b)[4][kSteps])
+{
+    constexpr int  kPer = 16 / static_cast<int>(sizeof(TD));
+    const int      g = lane >> 2, c = lane & 3;
+    const uint8_t *rows = p.b + static_cast<int64_t>(t.adapter) * p.N * p.ld_b;
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(TD)) / 2; ++i) q[i] = __ldcg(reinterpret_cast<const uint4 *>(src) + i);
-        memcpy(e, q, sizeof(e));
-    }
-    else
+    for (int i = 0; i < 4; ++i)
     {
+        // column j = g of the i-th tile of eight: the lane that gets its results has c = j / 2, as its elements 2 i + j % 2
+        const int el = 2 * i + (g & 1), ch = n + piece_channel<TD>(el / kPer, g >> 1) + el % kPer;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int s = 0; s < kSteps; ++s)
         {
-            e[i] = from_float<TD>(0.f);
-            if (n + i < cols) e[i] = __ldcg(src + i);
+            const int r = s * 16 + 4 * c;
+            b[i][s]     = make_uint2(0, 0);
+            if (t.adapter >= 0 && ch < p.N && r < t.rank) b[i][s] = __ldcg(reinterpret_cast<const uint2 *>(rows + ch * p.ld_b + r * 2));
         }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
 }
-template <typename TD, bool kVec>
-__device__ __forceinline__ void store_row(uint8_t *row, int n, int cols, const float (&v)[8])
+template <int kSteps>
+__device__ __forceinline__ void cut_b(int rank, int c, uint2 (&b)[4][kSteps])
 {
-    TD  e[8];
-    TD *dst = reinterpret_cast<TD *>(row) + n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_float<TD>(v[i]);
-    if constexpr (kVec)
+    for (int s = 0; s < kSteps; ++s)
     {
-        uint4 q[sizeof(TD) / 2];
-        memcpy(q, e, sizeof(e));
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(TD)) / 2; ++i) reinterpret_cast<uint4 *>(dst)[i] = q[i];
-    }
-    else
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
+        const int left = rank - s * 16 - 4 * c; // (nothing to cut where ranks are multiples of 4)
+        if (left > 0 && left < 4)
         {
-            if (n + i < cols) dst[i] = e[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                b[i][s].y = left == 3 ? b[i][s].y & 0xffffu : 0u;
+                if (left == 1) b[i][s].x &= 0xffffu;
+            }
         }
     }
 }
 
-// A warp: 32 channels, the tokens of a tile sixteen at a time.  Lane (g, c) of the results: rows g and g + 8, channels 8 c .. 8 c + 7.
 template <typename T, typename TD, int kRank, bool kVec>
-__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(const __grid_constant__ LoraParams p)
+__global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_expand_kernel(const __grid_constant__ LoraParams p)
 {
-    constexpr int kSteps = kRank / 16;
-    constexpr int kParts = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
+    using E = Expand<T, TD, kRank>;
+    constexpr int kPieces = static_cast<int>(sizeof(TD)) / 2, kPer = 8 / kPieces; // 16-byte pieces of a lane's row, elements of one
+    extern __shared__ __align__(128) uint8_t smem[]; // v of two tiles, then the slots
+    __shared__ Tile       list[kListTiles];
+    __shared__ ScanShared scan;
     griddep_launch_dependents();
     // the launch ahead let this one start after its own wait: all but v is as it will be
-    const Tile t = find_tile(p, static_cast<int>(blockIdx.y));
-    if (t.count == 0)
+    const int blocks = (p.N + 32 * kWarps - 1) / (32 * kWarps); // of channels
+    int       lo = 0, hi = 0, tile_lo = 0;                      // this CTA's items, the first one's tile
     {
-        griddep_wait();
-        return;
+        Request q     = load_request(p, static_cast<int>(threadIdx.x));
+        int     tiles = (q.end - q.begin + p.tile - 1) / p.tile, at, all, turn = 0;
+        scan_tiles(scan, turn, tiles, at, all);
+        int total = all;
+        for (int r0 = kThreads; r0 < p.requests; r0 += kThreads)
+        {
+            const Request more = load_request(p, r0 + static_cast<int>(threadIdx.x));
+            int           unused;
+            scan_tiles(scan, turn ^= 1, (more.end - more.begin + p.tile - 1) / p.tile, unused, all);
+            total += all;
+        }
+        total            = min(total, p.tiles);
+        const int64_t items = static_cast<int64_t>(total) * blocks;
+        lo                  = static_cast<int>(items * blockIdx.x / gridDim.x);
+        hi                  = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+        if (lo >= hi)
+        {
+            griddep_wait();
+            return;
+        }
+        tile_lo           = lo / blocks;
+        const int tile_hi = min((hi - 1) / blocks, tile_lo + kListTiles - 1); // the grid has so many CTAs that the list is long enough
+        int       before  = 0;
+        for (int r0 = 0; r0 < p.requests && before <= tile_hi; r0 += kThreads)
+        {
+            if (p.requests > kThreads)
+            {
+                q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
+                tiles = (q.end - q.begin + p.tile - 1) / p.tile;
+                scan_tiles(scan, turn ^= 1, tiles, at, all);
+            }
+            for (int i = max(tile_lo - before - at, 0); i < min(tiles, tile_hi + 1 - before - at); ++i)
+            {
+                list[before + at + i - tile_lo] = Tile{q.begin + i * p.tile, min(p.tile, q.end - q.begin - i * p.tile), q.adapter, q.rank};
+            }
+            before += all;
+        }
+        __syncthreads();
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int n0 = static_cast<int>(blockIdx.x) * kChannels + warp * 32, n = n0 + 8 * c;
-    uint2     b[4][kSteps];
-    if (t.adapter >= 0)
+    const uint32_t slots = smem_u32(smem) + E::kOffBase + static_cast<uint32_t>(warp) * E::kSlots * 16 * E::kRow;
+    const int warp_n = warp * 32; // the warp's channels of an item
+    // A place in the CTA's share: an item's tile and block of channels.
+    struct Place
     {
-        const uint8_t *rows = p.b + static_cast<int64_t>(t.adapter) * p.N * p.ld_b;
+        int at, block; // tile of the list, block of channels
+    };
+    auto advance = [&](Place &q) {
+        if (++q.block == blocks)
+        {
+            q.block = 0;
+            ++q.at;
+        }
+    };
+    // The ring: units in the order in which they are worked on.  16-byte pieces are exchanged by row where a row has eight of them
+    // (reading two rows side by side hits all banks once).  A lane copies one piece of every kStep-th row.
+    constexpr int  kUnit = E::kRow / 16, kStep = 32 / kUnit; // pieces of a row, rows that the warp copies at a time
+    const int      copy_row = lane / kUnit, copy_ch = warp_n + lane % kUnit * (16 / static_cast<int>(sizeof(TD)));
+    const uint32_t copy_to  = slots + static_cast<uint32_t>(copy_row * E::kRow + ((kUnit == 8 ? (lane % kUnit) ^ ((copy_row & 1) << 2) : lane % kUnit) << 4));
+    Place          ahead{0, lo - tile_lo * blocks};
+    int            ahead_left = hi - lo, ahead_m = 0, ahead_slot = 0;
+    const uint8_t *ahead_src = nullptr;
+    auto           load_unit = [&]() {
+        if (ahead_m == 0)
+        {
+            while (ahead_left > 0 && ahead.block * 32 * kWarps + warp_n >= p.N) // nothing for this warp there
+            {
+                --ahead_left;
+                advance(ahead);
+            }
+        }
+        if (ahead_left > 0)
+        {
+            const int count = list[ahead.at].count;
+            if constexpr (kVec)
+            {
+                const int ch = ahead.block * 32 * kWarps + copy_ch;
+                if (ahead_m == 0)
+                {
+                    ahead_src = p.base + static_cast<int64_t>(list[ahead.at].first + copy_row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
+                }
+                const uint8_t *src = ahead_src;
+#pragma unroll
+                for (int j = 0; j < 16 / kStep; ++j, src += kStep * p.ld_base)
+                {
+                    const bool in = ahead_m + copy_row + j * kStep < count && ch < p.N; // N is a multiple of 8
+                    copy16(copy_to + static_cast<uint32_t>(ahead_slot * 16 * E::kRow + j * kStep * E::kRow), in ? src : p.base, in ? 16 : 0);
+                }
+                ahead_src += 16 * p.ld_base;
+            }
+            ahead_slot = (ahead_slot + 1) % E::kSlots;
+            ahead_m += 16;
+            if (ahead_m >= count)
+            {
+                ahead_m = 0;
+                --ahead_left;
+                advance(ahead);
+            }
+        }
+        copy_commit();
+    };
+    // v of a tile to one half of its buffer, by all threads
+    auto load_v = [&](const Tile &t, int half) {
+        if (t.adapter < 0) return;
+        constexpr int kUnits = kRank / 8 + 1; // 16-byte units of a row
+        const int     rows   = (t.count + 15) & ~15;
+        for (int i = threadIdx.x; i < E::kParts * rows * kUnits; i += kThreads)
+        {
+            const int  row = (i / kUnits) % rows, part = i / (kUnits * rows), unit = i % kUnits;
+            const bool in  = row < t.count;
+            copy16(smem_u32(smem) + static_cast<uint32_t>(half * E::kV + (part * E::kTile + row) * E::kPitch + unit * 16),
+                   p.v + (in ? (static_cast<int64_t>(part) * p.tokens + t.first + row) * (kRank + 8) + unit * 8 : 0), in ? 16 : 0);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < E::kSlots; ++u) load_unit();
+    Place place{0, lo - tile_lo * blocks};
+    uint2 b[4][E::kSteps], next[4][E::kSteps];
+    load_b<TD>(p, list[0], place.block * 32 * kWarps + warp_n, lane, next);
+    griddep_wait();
+    load_v(list[0], 0);
+    int  slot = 0, half = 1; // of the ring; of the buffer: the other one is the current tile's
+    bool begins = true;
+    for (int item = lo; item < hi; ++item)
+    {
+        const Tile t = list[place.at];
+        const int  n = place.block * 32 * kWarps + warp_n;
+        if (begins) // a tile: its v has been asked for
+        {
+            copy_commit();
+            copy_wait<0>();
+            __syncthreads();
+            half ^= 1;
+            if (hi - item > blocks - place.block) load_v(list[place.at + 1], half ^ 1);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-            // column g of the i-th tile of eight: the lane that gets its results has c = g / 2, as its elements 2 i and 2 i + 1
-            const int ch = n0 + 8 * (g >> 1) + 2 * i + (g & 1);
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+            for (int s = 0; s < E::kSteps; ++s) b[i][s] = next[i][s];
+        }
+        if ((t.rank & 3) != 0) cut_b(t.rank, c, b);
+        advance(place);
+        begins = place.block == 0;
+        if (item + 1 < hi) load_b<TD>(p, list[place.at], place.block * 32 * kWarps + warp_n, lane, next);
+        if (n >= p.N) continue; // the same for the warp
+        uint8_t       *dst_row = p.dst + static_cast<int64_t>(t.first + g) * p.ld_dst + static_cast<int64_t>(n) * static_cast<int>(sizeof(TD));
+        const uint8_t *v_row   = smem + half * E::kV + g * E::kPitch;
+        for (int m = 0; m < t.count; m += 16, dst_row += 16 * p.ld_dst, v_row += 16 * E::kPitch)
+        {
+            copy_wait<E::kSlots - 1>();
+            __syncwarp();
+            float base[2][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
             {
-                const int r = s * 16 + 4 * c;
-                b[i][s]     = make_uint2(0, 0);
-                if (ch < p.N && r < t.rank)
+                const int row = h * 8 + g;
+                if constexpr (kVec)
                 {
-                    b[i][s] = __ldcg(reinterpret_cast<const uint2 *>(rows + ch * p.ld_b + r * 2));
-                    // what lies behind the adapter's rank counts nothing, whatever it is
-                    if (t.rank - r < 4) b[i][s].y = t.rank - r == 3 ? b[i][s].y & 0xffffu : 0u;
-                    if (t.rank - r == 1) b[i][s].x &= 0xffffu;
+                    const uint8_t *from = smem + E::kOffBase + (warp * E::kSlots + slot) * 16 * E::kRow + row * E::kRow;
+                    TD             e[8];
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i)
+                    {
+                        const int   piece = kPieces == 2 ? (4 * i + c) ^ ((row & 1) << 2) : c;
+                        const uint4 v     = *reinterpret_cast<const uint4 *>(from + piece * 16);
+                        memcpy(e + i * kPer, &v, 16);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) base[h][i] = to_float(e[i]);
+                }
+                else
+                {
+                    const TD *src = reinterpret_cast<const TD *>(p.base + static_cast<int64_t>(t.first + m + row) * p.ld_base);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        const int ch = n + piece_channel<TD>(i / kPer, c) + i % kPer;
+                        base[h][i]   = 0.f;
+                        if (m + row < t.count && ch < p.N) base[h][i] = to_float(__ldcg(src + ch));
+                    }
                 }
             }
-        }
-    }
-    bool waited = false;
-    for (int m = 0; m < t.count; m += 16)
-    {
-        float base[2][8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-        {
-            const int row = m + h * 8 + g;
-            if (row < t.count && n < p.N) load_base<TD, kVec>(p.base + static_cast<int64_t>(t.first + row) * p.ld_base, n, p.N, base[h]);
-        }
-        if (!waited)
-        {
-            griddep_wait();
-            waited = true;
-        }
-        if (t.adapter >= 0)
-        {
-            float acc[4][4] = {};
-#pragma unroll
-            for (int q = kParts - 1; q >= 0; --q) // small parts first
+            __syncwarp();
+            load_unit(); // to the slot that the warp has read
+            slot = (slot + 1) % E::kSlots;
+            if (t.adapter >= 0)
             {
-                const uint16_t *v = p.v + (static_cast<int64_t>(q) * p.tokens + t.first + m) * kRank;
+                float acc[4][4] = {};
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+                for (int part = E::kParts - 1; part >= 0; --part) // small parts first
                 {
-                    if (s * 16 < t.rank)
-                    {
-                        uint2 lo = make_uint2(0, 0), hi = make_uint2(0, 0);
-                        if (m + g < t.count) lo = *reinterpret_cast<const uint2 *>(v + g * kRank + s * 16 + 4 * c);
-                        if (m + g + 8 < t.count) hi = *reinterpret_cast<const uint2 *>(v + (g + 8) * kRank + s * 16 + 4 * c);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma<T>(acc[i], lo.x, hi.x, lo.y, hi.y, b[i][s].x, b[i][s].y);
+                    for (int s = 0; s < E::kSteps; ++s)
+                    {
+                        if (s * 16 < t.rank)
+                        {
+                            const uint8_t *v   = v_row + part * E::kTile * E::kPitch + s * 32 + 8 * c;
+                            const uint2    top = *reinterpret_cast<const uint2 *>(v), low = *reinterpret_cast<const uint2 *>(v + 8 * E::kPitch);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma<T>(acc[i], top.x, low.x, top.y, low.y, b[i][s].x, b[i][s].y);
+                        }
                     }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                {
+                    const float f = *reinterpret_cast<const float *>(v_row + h * 8 * E::kPitch + kRank * 2);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) base[h][i] = fmaf(acc[i >> 1][2 * h + (i & 1)], f, base[h][i]);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
-                const int   row = m + h * 8 + g;
-                const float f   = row < t.count ? p.factor[t.first + row] : 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                if (m + h * 8 + g < t.count)
                 {
-                    base[h][2 * i]     = fmaf(acc[i][2 * h], f, base[h][2 * i]);
-                    base[h][2 * i + 1] = fmaf(acc[i][2 * h + 1], f, base[h][2 * i + 1]);
+                    TD *dst = reinterpret_cast<TD *>(dst_row + h * 8 * p.ld_dst);
+                    TD  e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = from_float<TD>(base[h][i]);
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i)
+                    {
+                        const int ch = piece_channel<TD>(i, c);
+                        if constexpr (kVec)
+                        {
+                            uint4 v;
+                            memcpy(&v, e + i * kPer, 16);
+                            if (n + ch < p.N) *reinterpret_cast<uint4 *>(dst + ch) = v;
+                        }
+                        else
+                        {
+#pragma unroll
+                            for (int k = 0; k < kPer; ++k)
+                            {
+                                if (n + ch + k < p.N) dst[ch + k] = e[i * kPer + k];
+                            }
+                        }
+                    }
                 }
             }
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-        {
-            const int row = m + h * 8 + g;
-            if (row < t.count && n < p.N) store_row<TD, kVec>(p.dst + static_cast<int64_t>(t.first + row) * p.ld_dst, n, p.N, base[h]);
-        }
     }
+    copy_wait<0>();
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -479,21 +740,34 @@ cugl_status launch_shrink(cugl_context *ctx, const LoraParams &p, int64_t tiles)
         CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         set[ctx->device & 63].store(true, std::memory_order_release);
     }
-    // CTAs that share a tile's K: until there are two for every SM, each with a block of 32 columns per warp at least
+    // CTAs that share a tile's K: as many as run at once, two to an SM, with two stages each at least
     int split = 1;
-    while (split < kMaxSplit && tiles * split < 2 * ctx->sm_count && p.K >= 2 * split * 32 * kWarps) split *= 2;
+    while (split < kMaxSplit && tiles * split * 2 <= 2 * ctx->sm_count && p.K >= 2 * split * 128) split *= 2;
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, p));
+    return CUGL_SUCCESS;
+}
+template <typename T, typename TD, int kRank, bool kVec>
+cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
+{
+    using E                          = Expand<T, TD, kRank>;
+    auto                     kernel  = lora_expand_kernel<T, TD, kRank, kVec>;
+    static std::atomic<bool> set[64] = {};
+    if (!set[ctx->device & 63].load(std::memory_order_acquire))
+    {
+        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, E::kSmem));
+        set[ctx->device & 63].store(true, std::memory_order_release);
+    }
+    // one CTA or two to an SM; more only where a share would be longer than a CTA's list of tiles
+    const int64_t items = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps) * tiles, most = std::max<int64_t>(E::kCtas * ctx->sm_count, tiles / (kListTiles - 2) + 1);
+    const int64_t grid  = items < most ? items : most;
+    CUGL_CUDA_TRY(ctx, launch_dependent(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, E::kSmem, grid, p));
     return CUGL_SUCCESS;
 }
 template <typename T, typename TD, int kRank>
 cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, bool vec_in, bool vec_out)
 {
     CUGL_TRY((vec_in ? launch_shrink<T, kRank, true>(ctx, p, tiles) : launch_shrink<T, kRank, false>(ctx, p, tiles)));
-    const dim3 grid(static_cast<unsigned>((p.N + kChannels - 1) / kChannels), static_cast<unsigned>(tiles));
-    const long long units = static_cast<long long>(grid.x) * grid.y;
-    CUGL_CUDA_TRY(ctx, vec_out ? launch_dependent(ctx, lora_expand_kernel<T, TD, kRank, true>, grid, kThreads, 0, units, p)
-                               : launch_dependent(ctx, lora_expand_kernel<T, TD, kRank, false>, grid, kThreads, 0, units, p));
-    return CUGL_SUCCESS;
+    return vec_out ? launch_expand<T, TD, kRank, true>(ctx, p, tiles) : launch_expand<T, TD, kRank, false>(ctx, p, tiles);
 }
 template <typename T, typename TD>
 cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, bool vec_in, bool vec_out)
@@ -548,7 +822,7 @@ extern "C"
         {
             return 0;
         }
-        return 16 + static_cast<size_t>(desc->tokens) * (static_cast<size_t>(padded_rank(desc->max_rank)) * 2 * static_cast<size_t>(v_parts(*desc)) + 4);
+        return static_cast<size_t>(desc->tokens) * static_cast<size_t>(padded_rank(desc->max_rank) + 8) * 2 * static_cast<size_t>(v_parts(*desc)) + 16;
     }
 
     cugl_status cugl_lora(cugl_context *ctx, const cugl_lora_desc *desc, const void *d_x, const int32_t *d_starts, const int32_t *d_request_adapters,
@@ -604,11 +878,11 @@ extern "C"
         p.parts      = v_parts(*desc);
         p.tile       = tile_tokens(desc->max_rank);
         p.v          = static_cast<uint16_t *>(d_workspace);
-        p.factor     = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + static_cast<size_t>(p.tokens) * padded_rank(p.max_rank) * 2 * p.parts);
         auto       even = [](const void *q, int64_t ld) { return ((reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ld)) & 15) == 0; };
         const bool vec_in  = even(d_x, desc->ld_x) && even(d_a, desc->ld_a);
         const bool vec_out = even(d_base, desc->ld_base) && even(d_dst, desc->ld_dst) && desc->N % 8 == 0;
         const int64_t tiles = most_tiles(*desc);
+        p.tiles             = static_cast<int>(tiles);
         if (desc->dtype == CUGL_F16)
         {
             return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, vec_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, vec_in, vec_out);
