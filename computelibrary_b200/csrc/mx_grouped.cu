@@ -22,8 +22,10 @@ namespace
 {
 constexpr int kMmaWarp   = 1;
 constexpr int kFirstEpi  = 2;
-constexpr int kEpi       = 8; // epilogue warps, two per tensor-memory lane quarter
-constexpr int kThreads   = 32 * (kFirstEpi + kEpi);
+constexpr int kFewEpi      = 8;  // epilogue warps, two per tensor-memory lane quarter
+constexpr int kFewThreads  = 32 * (kFirstEpi + kFewEpi);
+constexpr int kPairEpi     = 16; // four
+constexpr int kPairThreads = 32 * (kFirstEpi + kPairEpi);
 constexpr int kMaxGroups = 512;
 constexpr int kSlab      = 128; // rows at whose multiples groups start
 
@@ -60,7 +62,7 @@ __device__ __forceinline__ int2 load_group(const GroupedParams &p, int g, bool &
 template <int kTile>
 __device__ __forceinline__ int scan_groups(const GroupedParams &p, int *before)
 {
-    for (int g = threadIdx.x; g < p.n_groups; g += kThreads)
+    for (int g = threadIdx.x; g < p.n_groups; g += static_cast<int>(blockDim.x))
     {
         bool       bad;
         const int2 v  = load_group(p, g, bad);
@@ -122,6 +124,33 @@ __device__ __forceinline__ Item find_item(const GroupedParams &p, const int *bef
     it.row           = v.x + tb * kTile;
     it.count         = min(kTile, v.y - tb * kTile);
     return it;
+}
+
+// The first items of a CTA, found once, side by side, at the start: a search is a thousand clocks of dependent instructions, which every
+// role would otherwise run through at every item (and the MMAs wait for).  Later ones, of a CTA with many items, are searched for.
+constexpr int kListed = 128;
+struct ListedItem
+{
+    uint32_t group_count; // count << 16 | group
+    int      wb, row;
+};
+template <int kTile>
+__device__ __forceinline__ void list_items(const GroupedParams &p, const int *before, ListedItem *list, int w_blocks, int first, int stride, int items)
+{
+    const int i = static_cast<int>(threadIdx.x);
+    if (i < kListed && static_cast<int64_t>(i) * stride + first < items)
+    {
+        const Item it = find_item<kTile>(p, before, w_blocks, first + i * stride);
+        list[i]       = ListedItem{static_cast<uint32_t>(it.count) << 16 | static_cast<uint32_t>(it.group), it.wb, it.row};
+    }
+    __syncthreads();
+}
+template <int kTile>
+__device__ __forceinline__ Item get_item(const GroupedParams &p, const int *before, const ListedItem *list, int w_blocks, int i, int item)
+{
+    if (i >= kListed) return find_item<kTile>(p, before, w_blocks, item);
+    const ListedItem l = list[i];
+    return Item{static_cast<int>(l.group_count & 0xffffu), l.wb, l.row, static_cast<int>(l.group_count >> 16)};
 }
 
 // ---- what happens to sums ------------------------------------------------------------------------------------
@@ -214,7 +243,8 @@ struct FewPlan
     static constexpr int OFF_BAR   = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_MISC  = OFF_BAR + (2 * STAGES + 5) * 8;
     static constexpr int OFF_SCAN  = OFF_MISC + 16;
-    static constexpr int DYN_BYTES = OFF_SCAN + (kMaxGroups + 1) * 4 + 1024;
+    static constexpr int OFF_LIST  = OFF_SCAN + (kMaxGroups + 1) * 4;
+    static constexpr int DYN_BYTES = OFF_LIST + kListed * static_cast<int>(sizeof(ListedItem)) + 1024;
     static constexpr int SF_COL    = 256;
     static_assert(SF_COL + STAGES * SF_COLS <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
 };
@@ -248,7 +278,7 @@ struct Halves
 };
 
 template <int kFormat, bool kSwiglu>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kFewThreads, 1)
     mx_grouped_few_kernel(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_up, const __grid_constant__ TokenMaps tmap_a,
                           const __grid_constant__ GroupedParams p)
 {
@@ -268,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC);
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     int           *before    = reinterpret_cast<int *>(smem + P::OFF_SCAN);
+    ListedItem    *list      = reinterpret_cast<ListedItem *>(smem + P::OFF_LIST);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int      w_blocks = (p.channels + kMxRows - 1) / kMxRows;
     const int      chunks   = (p.K + kMxChunk - 1) / kMxChunk;
@@ -282,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = 0; h < 2; ++h)
         {
             mbar_init(tfull_bar(h), 1);
-            mbar_init(tempty_bar(h), kEpi);
+            mbar_init(tempty_bar(h), kFewEpi);
         }
         mbar_init(gone_bar, 1);
         *s_abort = 0;
@@ -299,15 +330,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_launch_dependents();
     griddep_wait(); // the groups come from a kernel ahead
     const int items = scan_groups<kSlab>(p, before) * w_blocks;
+    list_items<kSlab>(p, before, list, w_blocks, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), items);
 
     int issued = 0; // stages that the producer has filled
     if (warp == 0)
     {
         const bool el = elect_one();
-        int        g  = 0;
-        for (int v = blockIdx.x; v < items; v += gridDim.x)
+        int        g = 0, n = 0;
+        for (int v = blockIdx.x; v < items; v += gridDim.x, ++n)
         {
-            const Item     it   = find_item<kSlab>(p, before, w_blocks, v);
+            const Item     it   = get_item<kSlab>(p, before, list, w_blocks, n, v);
             const int      box  = token_box(it.count);
             const int      w_row = it.group * p.channels + it.wb * kMxRows;
             const int64_t  w_sf = it.group * p.group_tiles + it.wb * p.k_tiles, a_sf = it.row / kSlab * p.k_tiles;
@@ -347,12 +379,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     else if (warp == kMmaWarp)
     {
         const bool      el = elect_one();
-        int             g  = 0;
+        int             g = 0, n_item = 0;
         bool            ok = true;
         Halves<kSwiglu> half;
-        for (int v = blockIdx.x; v < items && ok; v += gridDim.x)
+        for (int v = blockIdx.x; v < items && ok; v += gridDim.x, ++n_item)
         {
-            const Item     it    = find_item<kSlab>(p, before, w_blocks, v);
+            const Item     it    = get_item<kSlab>(p, before, list, w_blocks, n_item, v);
             const int      cols  = (it.count + 15) & ~15;
             const uint32_t idesc = p.idesc | (static_cast<uint32_t>(cols >> 3) << 17);
             half.take(it.count);
@@ -399,9 +431,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int       q = warp & 3, turn = (warp - kFirstEpi) >> 2;
         Halves<kSwiglu> half;
         bool            ok = true;
-        for (int v = blockIdx.x; v < items && ok; v += gridDim.x)
+        int             n_item = 0;
+        for (int v = blockIdx.x; v < items && ok; v += gridDim.x, ++n_item)
         {
-            const Item    it = find_item<kSlab>(p, before, w_blocks, v);
+            const Item    it = get_item<kSlab>(p, before, list, w_blocks, n_item, v);
             const int     n  = it.wb * kMxRows + q * 32 + lane;
             const Factors f  = group_factors(p, it.group);
             const float   b  = group_bias(p, it.group, n);
@@ -467,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // epilogue drains the shared columns first.
 constexpr int kPairCols   = 256;
 constexpr int kPairShared = 64;
+constexpr int kStaging    = 2048;
 template <int kFormat, bool kSwiglu>
 struct PairPlan
 {
@@ -478,36 +512,37 @@ struct PairPlan
     static constexpr int STAGE     = WEIGHTS * kMxWBytes + T_BYTES;
     static constexpr int SF_PARTS  = WEIGHTS + TILE / 128;
     static constexpr int SF_STAGE  = SF_PARTS * F::kChunkScale;
-    static constexpr int OFF_OUT   = STAGES * STAGE; // staging: 4 KB per epilogue warp
-    static constexpr int OFF_SF    = OFF_OUT + kEpi * 4096;
+    static constexpr int OFF_OUT   = STAGES * STAGE; // staging: 2 KB per epilogue warp
+    static constexpr int OFF_SF    = OFF_OUT + kPairEpi * kStaging;
     static constexpr int OFF_BAR   = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_MISC  = OFF_BAR + (2 * STAGES + 4) * 8;
     static constexpr int OFF_SCAN  = OFF_MISC + 16;
-    static constexpr int DYN_BYTES = OFF_SCAN + (kMaxGroups + 1) * 4 + 1024;
+    static constexpr int OFF_LIST  = OFF_SCAN + (kMaxGroups + 1) * 4;
+    static constexpr int DYN_BYTES = OFF_LIST + kListed * static_cast<int>(sizeof(ListedItem)) + 1024;
     static constexpr int SF_COL    = 2 * kPairCols - kPairShared;
     static_assert(SF_COL + SF_PARTS * F::kChunkCols <= 512 && DYN_BYTES <= 232448, "tensor and shared memory of an SM");
     static_assert(STAGE % 1024 == 0, "operands start at multiples of the swizzle's period");
 };
 
 // 32 channels x 32 tokens of results (two halves of 16 lanes as fragments) to a staging area of 32 rows of 64 bytes in the 64-byte
-// swizzle.
-template <typename T>
-__device__ __forceinline__ void stage_results(uint32_t s_out, int lane, const float (&lo)[16], const float (&hi)[16])
+// swizzle; r: neighbours of a row as words, the lower half's eight first.
+__device__ __forceinline__ void stage_results(uint32_t s_out, int lane, const uint32_t (&r)[2][8])
 {
-    auto pack = [](float a, float b) {
-        const T  two[2] = {from_float<T>(a), from_float<T>(b)};
-        uint32_t w;
-        memcpy(&w, two, 4);
-        return w;
-    };
 #pragma unroll
     for (int i = 0; i < 4; ++i) // eight tokens: matrix m holds channels 8 m .. 8 m + 7
     {
         const int      row  = 8 * i + (lane & 7), chunk = lane >> 3;
         const uint32_t addr = s_out + static_cast<uint32_t>(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
-        stmatrix_x4_trans(addr, pack(lo[4 * i], lo[4 * i + 1]), pack(lo[4 * i + 2], lo[4 * i + 3]), pack(hi[4 * i], hi[4 * i + 1]),
-                          pack(hi[4 * i + 2], hi[4 * i + 3]));
+        stmatrix_x4_trans(addr, r[0][2 * i], r[0][2 * i + 1], r[1][2 * i], r[1][2 * i + 1]);
     }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_two(float a, float b)
+{
+    const T  two[2] = {from_float<T>(a), from_float<T>(b)};
+    uint32_t w;
+    memcpy(&w, two, 4);
+    return w;
 }
 // The first `cols` rows of a staging area (kUnits 16-byte units each) to rows m and up of dst, channels n0 and up.  Bulk stores write
 // whole boxes: this is for the one that a group's end cuts.
@@ -529,7 +564,7 @@ __device__ __forceinline__ void store_staged(const GroupedParams &p, const uint8
 }
 
 template <int kFormat, int kBulk, bool kSwiglu>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     mx_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_up, const __grid_constant__ CUtensorMap tmap_a,
                            const __grid_constant__ CUtensorMap tmap_bsf, const __grid_constant__ CUtensorMap tmap_upsf,
                            const __grid_constant__ CUtensorMap tmap_asf, const __grid_constant__ CUtensorMap tmap_out,
@@ -552,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int  *s_abort   = reinterpret_cast<volatile int *>(smem + P::OFF_MISC + 4);
     uint32_t      *s_peer    = reinterpret_cast<uint32_t *>(smem + P::OFF_MISC + 8); // stages the peer has filled; bit 31: it has given up
     int           *before    = reinterpret_cast<int *>(smem + P::OFF_SCAN);
+    ListedItem    *list      = reinterpret_cast<ListedItem *>(smem + P::OFF_LIST);
     const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int      rank     = static_cast<int>(cluster_ctarank());
     const int      w_blocks = (p.channels + 2 * kMxRows - 1) / (2 * kMxRows);
@@ -568,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(tfull_bar(0), 1);
         mbar_init(tfull_bar(1), 1);
-        mbar_init(tempty, 2 * kEpi);
+        mbar_init(tempty, 2 * kPairEpi);
         mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -585,16 +621,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_launch_dependents();
     griddep_wait(); // the groups come from a kernel ahead
     const int items = scan_groups<TILE>(p, before) * w_blocks;
+    list_items<TILE>(p, before, list, w_blocks, first, stride, items);
 
     int issued = 0; // stages that the producer has filled
     if (warp == 0)
     {
         const bool el = elect_one();
-        int        g  = 0;
+        int        g = 0, n_item = 0;
         const int  kt = static_cast<int>(p.k_tiles);
-        for (int v = first; v < items; v += stride)
+        for (int v = first; v < items; v += stride, ++n_item)
         {
-            const Item it    = find_item<TILE>(p, before, w_blocks, v);
+            const Item it    = get_item<TILE>(p, before, list, w_blocks, n_item, v);
             const int  w_row = it.group * p.channels + (it.wb * 2 + rank) * kMxRows;
             const int  w_sf  = static_cast<int>(it.group * p.group_tiles) + (it.wb * 2 + rank) * kt, a_sf = it.row / kSlab * kt;
             const int  a_row = it.row + rank * (((it.count + 31) & ~31) >> 1); // this CTA's half of the MMAs' columns
@@ -644,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int  kStepCols = 4 * (TILE / 128); // scale columns of a step's tokens
             for (int v = first; v < items && ok; v += stride, ++it)
             {
-                const Item     item  = find_item<TILE>(p, before, w_blocks, v);
+                const Item     item  = get_item<TILE>(p, before, list, w_blocks, it, v);
                 const int      cols  = (item.count + 31) & ~31;
                 const uint32_t idesc = p.idesc | (static_cast<uint32_t>(cols >> 3) << 17);
                 ok = warp_wait(tempty, (static_cast<uint32_t>(it) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
@@ -698,13 +735,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     else
     {
-        // Two warps per lane quarter, which take turns with groups of 32 tokens; those in the shared columns are the first two groups.
+        // Four warps per lane quarter, which take turns with groups of 32 tokens; those in the shared columns are the first two groups.  One
+        // waits for its own instructions most of the time: with eight warps the drain of 128 x 128 SwiGLU results took 11000 clocks, 2.7
+        // times the MMAs of K = 2048 (768 channels, 512 rows a group: 72 us against 50).
         const int      q = warp & 3, turn = (warp - kFirstEpi) >> 2;
         const uint32_t release = map_to_cta(tempty, 0);
-        int            it = 0, staged = 0;
+        uint8_t       *out     = smem + P::OFF_OUT + (warp - kFirstEpi) * kStaging;
+        const uint32_t s_out   = s_stage + P::OFF_OUT + (warp - kFirstEpi) * kStaging;
+        int            it = 0;
         for (int v = first; v < items; v += stride, ++it)
         {
-            const Item    item = find_item<TILE>(p, before, w_blocks, v);
+            const Item    item = get_item<TILE>(p, before, list, w_blocks, it, v);
             const int     as = it & 1, n0 = (item.wb * 2 + rank) * kMxRows + q * 32;
             const Factors f  = group_factors(p, item.group);
             float         bias[4] = {}; // kBulk = 2: of the fragments' rows, else of this lane's channel
@@ -720,74 +761,63 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t acc = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
-            for (int i = 0; i < TILE / 64; ++i)
+            for (int i = 0; i < TILE / 128; ++i)
             {
-                const int  group = 2 * i + turn;
+                const int  group = 4 * i + turn;
                 const int  j     = as == 0 ? (group * 32 + TILE - kPairShared) % TILE : group * 32;
-                const bool any   = j < item.count; // the same for the warp
-                uint32_t   r[2][16], u[2][16];
-                if (any)
-                {
-                    if constexpr (kBulk == 2)
+                const bool any   = j < item.count && n0 < p.channels; // the same for the warp
+                auto       drained = [&]() { // the shared columns have been read
+                    if (i == 0)
                     {
-                        tmem_ld_frag32(acc + j, r[0]);
-                        tmem_ld_frag32(acc + j + (16u << 16), r[1]);
-                        if constexpr (kSwiglu)
-                        {
-                            tmem_ld_frag32(acc + 128 + j, u[0]);
-                            tmem_ld_frag32(acc + 128 + j + (16u << 16), u[1]);
-                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_no_writes(release);
                     }
-                    else
-                    {
-                        tmem_ld_x16(acc + j, r[0]);
-                        tmem_ld_x16(acc + j + 16, r[1]);
-                        if constexpr (kSwiglu)
-                        {
-                            tmem_ld_x16(acc + 128 + j, u[0]);
-                            tmem_ld_x16(acc + 128 + j + 16, u[1]);
-                        }
-                    }
-                    tmem_ld_wait();
-                }
-                if (i == 0)
+                };
+                if (!any)
                 {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(release);
+                    drained();
+                    continue;
                 }
-                if (!any || n0 >= p.channels) continue;
-                float x[2][16];
+                const int m = item.row + j, cols = item.count - j;
+                uint32_t  r[2][16], u[2][16]; // all of it first: the next tile's MMAs wait for the shared columns
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                 {
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) // of a fragment, elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
+                    if constexpr (kBulk == 2)
                     {
-                        x[h][k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[kBulk == 2 ? 2 * h + ((k >> 1) & 1) : 0]);
+                        tmem_ld_frag32(acc + j + (static_cast<uint32_t>(16 * h) << 16), r[h]);
+                        if constexpr (kSwiglu) tmem_ld_frag32(acc + 128 + j + (static_cast<uint32_t>(16 * h) << 16), u[h]);
+                    }
+                    else
+                    {
+                        tmem_ld_x16(acc + j + 16 * h, r[h]);
+                        if constexpr (kSwiglu) tmem_ld_x16(acc + 128 + j + 16 * h, u[h]);
                     }
                 }
-                const int m = item.row + j, cols = item.count - j;
-                if constexpr (kBulk != 0)
+                tmem_ld_wait();
+                drained();
+                if constexpr (kBulk == 2)
                 {
-                    // two-byte results: two areas in turn; floats: one
-                    const int      area  = (warp - kFirstEpi) * 4096 + (kBulk == 2 ? (staged & 1) * 2048 : 0);
-                    uint8_t       *out   = smem + P::OFF_OUT + area;
-                    const uint32_t s_out = s_stage + P::OFF_OUT + area;
-                    ++staged;
-                    if (lane == 0) // the store that reads this area has done so
-                    {
-                        if (kBulk == 2) tma_store_wait_read_but_one();
-                        else tma_store_wait_read();
-                    }
-                    __syncwarp();
-                    if constexpr (kBulk == 4)
-                    {
+                    uint32_t packed[2][8];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) reinterpret_cast<float *>(out)[32 * k + lane] = x[k / 16][k % 16];
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        float x[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) // elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
+                        {
+                            x[k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[2 * h + ((k >> 1) & 1)]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                        {
+                            packed[h][k] = p.dtype == CUGL_F16 ? pack_two<__half>(x[2 * k], x[2 * k + 1]) : pack_two<__nv_bfloat16>(x[2 * k], x[2 * k + 1]);
+                        }
                     }
-                    else if (p.dtype == CUGL_F16) stage_results<__half>(s_out, lane, x[0], x[1]);
-                    else stage_results<__nv_bfloat16>(s_out, lane, x[0], x[1]);
+                    if (lane == 0) tma_store_wait_read(); // the store that reads this area has done so
+                    __syncwarp();
+                    stage_results(s_out, lane, packed);
                     if (cols >= 32)
                     {
                         fence_proxy_async_smem();
@@ -797,15 +827,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                     else
                     {
                         __syncwarp();
-                        store_staged<kBulk == 2 ? 4 : 8, kBulk == 2>(p, out, lane, m, n0, cols);
+                        store_staged<4, true>(p, out, lane, m, n0, cols);
                     }
                     if (lane == 0) tma_store_commit();
                     __syncwarp();
                 }
                 else
                 {
-                    store_tokens(p, m, n0 + lane, x[0], cols);
-                    store_tokens(p, m + 16, n0 + lane, x[1], cols - 16);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) // sixteen tokens
+                    {
+                        float x[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) x[k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[0]);
+                        const int left = cols - 16 * h;
+                        if constexpr (kBulk == 4)
+                        {
+                            if (lane == 0) tma_store_wait_read();
+                            __syncwarp();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) reinterpret_cast<float *>(out)[32 * k + lane] = x[k];
+                            if (left >= 16)
+                            {
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                                if (lane == 0) tma_store_2d(&tmap_out, s_out, n0, m + 16 * h);
+                            }
+                            else if (left > 0)
+                            {
+                                __syncwarp();
+                                store_staged<8, false>(p, out, lane, m + 16 * h, n0, left);
+                            }
+                            if (lane == 0) tma_store_commit();
+                            __syncwarp();
+                        }
+                        else
+                        {
+                            store_tokens(p, m + 16 * h, n0 + lane, x, left);
+                        }
+                    }
                 }
             }
             tc_fence_before();
@@ -874,19 +934,19 @@ cugl_status launch_few(cugl_context *ctx, const GroupedOperands &op, GroupedPara
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc        = mx_idesc(kFormat, kMxRows, 0);
     const int grid = static_cast<int>(items < ctx->sm_count ? items : ctx->sm_count);
-    CUGL_CUDA_TRY(ctx, launch_dependent(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, items, map_b, map_up, map_a, p));
+    CUGL_CUDA_TRY(ctx, launch_dependent(ctx, kernel, dim3(static_cast<unsigned>(grid)), kFewThreads, P::DYN_BYTES, items, map_b, map_up, map_a, p));
     return CUGL_SUCCESS;
 }
 
-// dst in boxes of 32 rows x 32 channels: rows of 64 bytes in the 64-byte swizzle, or of 128 bytes
+// dst in boxes of 2 KB: 32 rows x 32 channels of two bytes in the 64-byte swizzle, or 16 rows of floats
 bool encode_results_map(CUtensorMap *map, const GroupedParams &p)
 {
     EncodeTiledFn    fn         = get_encode_fn();
     const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(p.channels), static_cast<cuuint64_t>(p.rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ldd)};
-    const cuuint32_t box[2]     = {32, 32};
-    const cuuint32_t estr[2]    = {1, 1};
     const bool       wide       = p.dtype == CUGL_F32;
+    const cuuint32_t box[2]     = {32, wide ? 16u : 32u};
+    const cuuint32_t estr[2]    = {1, 1};
     return fn != nullptr && fn(map, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, wide ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B,
                                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -912,7 +972,7 @@ cugl_status launch_pair(cugl_context *ctx, const GroupedOperands &op, GroupedPar
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc         = mx_idesc(kFormat, 2 * kMxRows, 0);
     const int pairs = ctx->sm_count / 2, grid = 2 * static_cast<int>(items < pairs ? items : pairs);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, P::DYN_BYTES, 2, 2 * items, map_b, map_up, map_a, map_bsf,
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kPairThreads, P::DYN_BYTES, 2, 2 * items, map_b, map_up, map_a, map_bsf,
                                                 map_upsf, map_asf, map_out, p));
     return CUGL_SUCCESS;
 }

@@ -307,6 +307,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same for a thread that has written nothing the waiting one reads (it hands back tensor memory, ordered by tcgen05.fence): a release
+// at cluster scope waits until all of the thread's stores are performed, one to two thousand clocks beside stores of results.
+__device__ __forceinline__ void mbar_arrive_cluster_no_writes(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // mbar_wait on a barrier that other CTAs of the cluster arrive on after writing to this CTA's shared memory
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
 {
