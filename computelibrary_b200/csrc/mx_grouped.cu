@@ -154,8 +154,18 @@ __device__ __forceinline__ Item get_item(const GroupedParams &p, const int *befo
 }
 
 // ---- what happens to sums ------------------------------------------------------------------------------------
+// silu(g) * u.  16-bit results take 2^x of the rounded product -g log2(e): off by 2^-20 + |g| 2^-23 of the result, where half a step of
+// theirs is 2^-11 or 2^-8; eight instructions instead of seventeen (768 channels, K = 2048, 512 rows a group: 67 -> 64 us).
+template <bool kShort>
 __device__ __forceinline__ float swiglu(float g, float u)
 {
+    if constexpr (kShort)
+    {
+        float e, q;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.442695041f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+        return g * q * u;
+    }
     return __fdividef(g, 1.f + expf(-g)) * u;
 }
 struct Factors
@@ -173,10 +183,10 @@ __device__ __forceinline__ float group_bias(const GroupedParams &p, int g, int n
 {
     return p.bias != nullptr && n < p.channels ? __ldg(p.bias + static_cast<int64_t>(g) * p.channels + n) : 0.f;
 }
-template <bool kSwiglu>
+template <bool kSwiglu, bool kShort = false>
 __device__ __forceinline__ float finish(uint32_t a, uint32_t u, const Factors &f, float bias)
 {
-    if constexpr (kSwiglu) return swiglu(__uint_as_float(a) * f.alpha, __uint_as_float(u) * f.up);
+    if constexpr (kSwiglu) return swiglu<kShort>(__uint_as_float(a) * f.alpha, __uint_as_float(u) * f.up);
     return __fmaf_rn(__uint_as_float(a), f.alpha, bias);
 }
 
@@ -807,7 +817,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 16; ++k) // elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
                         {
-                            x[k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[2 * h + ((k >> 1) & 1)]);
+                            x[k] = finish<kSwiglu, true>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[2 * h + ((k >> 1) & 1)]);
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k)

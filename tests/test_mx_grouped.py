@@ -2,7 +2,8 @@
 
 Tolerance of a sum as for the plain product: ceil(K / 64) + 10 steps of 2^-23 of its magnitudes (its MMAs, the factors, one fused
 multiply-add).  SwiGLU: the slope of silu is below 1.1; the exponential, the division and the products are off by 2^-20 of the result
-at most.  Half a step of the destination type on top."""
+at most; 16-bit results take 2^(-g log2 e) of a product that is off by two half steps (the constant's and its own), 2^-23 |g| log2 e, which
+makes 2^-23 |g| of the exponential.  Half a step of the destination type on top."""
 import ctypes as C
 
 import numpy as np
@@ -135,7 +136,8 @@ def check(ctx, counts, N, K, fmt, dtype, swiglu=False, bias=False, factors=False
             with np.errstate(over="ignore"):
                 silu = g / (1 + np.exp(-g))
             want = silu * u
-            tol = (1.1 * eg + 2.0 ** -20 * np.abs(silu)) * (np.abs(u) + eu) + np.abs(silu) * eu
+            rel = 2.0 ** -20 + (2.0 ** -23 * np.abs(g) if dtype != capi.F32 else 0)
+            tol = (1.1 * eg + rel * np.abs(silu)) * (np.abs(u) + eu) + np.abs(silu) * eu
         else:
             want = sums[0] + (vbias[e].astype(np.float64) if bias else 0)
             tol = steps * (sizes[0] + (np.abs(vbias[e]) if bias else 0))
