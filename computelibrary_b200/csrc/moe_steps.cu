@@ -35,74 +35,121 @@ struct RouteParams
     int32_t       *counts; // [chunks][experts]
     int64_t        ld;
     int            tokens, experts, top_k, renormalize, chunk, chunks;
+    int            vec; // rows of the logits are 16-byte aligned
 };
 
-template <typename T>
-__device__ __forceinline__ float load_logit(const T *p)
+// Logits become unsigned keys in their order (0: not to be chosen: NaN and -infinity, or chosen already).  A lane holds kPer experts that
+// follow each other, and knows its largest key, the first among equal ones: up to four are sorted at the start and move up when one is
+// taken, more are searched through.  A choice is the lowest lane with the largest key of all.  All lanes run the same instructions: the
+// winner's part under a branch cost twice as many.  Lane j returns the j-th choice (-1: none) and its weight.
+__device__ __forceinline__ uint32_t logit_key(float v)
 {
-    return to_float(*p);
+    const uint32_t b = __float_as_uint(v + 0.f); // -0 and 0 are equal logits
+    return v > -INFINITY ? ((b >> 31) != 0 ? ~b : b | 0x80000000u) : 0u;
 }
-
-// Logits become unsigned keys in their order (0: not to be chosen: NaN and -infinity, or chosen already); a choice is the largest key,
-// the lowest index among equal ones.  Lane j returns the j-th choice (-1: none) and its weight.
+__device__ __forceinline__ float key_logit(uint32_t key)
+{
+    return __uint_as_float((key >> 31) != 0 ? key & 0x7fffffffu : ~key);
+}
 template <typename T, int kPer> // experts per lane
 __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane, float &weight)
 {
-    const T *row = reinterpret_cast<const T *>(p.logits + t * p.ld);
+    const T *row = reinterpret_cast<const T *>(p.logits + t * p.ld) + lane * kPer;
     uint32_t key[kPer];
-    float    top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    constexpr int kBytes = kPer * static_cast<int>(sizeof(T)), kUnit = kBytes >= 16 ? 16 : kBytes;
+    if (p.vec != 0 && (lane + 1) * kPer <= p.experts)
     {
-        const int      e = i * 32 + lane;
-        const float    v = e < p.experts ? load_logit(row + e) : -INFINITY;
-        const uint32_t b = __float_as_uint(v + 0.f); // -0 and 0 are equal logits
-        key[i] = v > -INFINITY ? ((b >> 31) != 0 ? ~b : b | 0x80000000u) : 0u;
-        if (v > top) top = v;
-    }
+        T e[kPer];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float all = 0.f;
-    if (p.renormalize == 0)
-    {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
+        for (int i = 0; i < kBytes / kUnit; ++i)
         {
-            if (key[i] != 0) all += expf(__uint_as_float((key[i] >> 31) != 0 ? key[i] & 0x7fffffffu : ~key[i]) - top);
+            if constexpr (kUnit == 16) reinterpret_cast<uint4 *>(e)[i] = __ldg(reinterpret_cast<const uint4 *>(row) + i);
+            else if constexpr (kUnit == 8) reinterpret_cast<uint2 *>(e)[i] = __ldg(reinterpret_cast<const uint2 *>(row) + i);
+            else reinterpret_cast<uint32_t *>(e)[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + i);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        for (int i = 0; i < kPer; ++i) key[i] = logit_key(to_float(e[i]));
     }
-    int   mine = -1;
-    float own = 0.f, sum = 0.f;
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) key[i] = lane * kPer + i < p.experts ? logit_key(to_float(row[i])) : 0u;
+    }
+    float    top = 0.f, all = 0.f;
+    uint32_t own = 0;
+    int      mine = -1, index[kPer];
+    constexpr bool kSorted = kPer <= 4;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) index[i] = lane * kPer + i;
+    if constexpr (kSorted)
+    {
+        // neighbours change places, equal ones do not: stable
+#pragma unroll
+        for (int round = 0; round < kPer; ++round)
+        {
+#pragma unroll
+            for (int i = round & 1; i + 1 < kPer; i += 2)
+            {
+                const bool     swap = key[i + 1] > key[i];
+                const uint32_t k    = key[i];
+                const int      n    = index[i];
+                key[i]              = swap ? key[i + 1] : k;
+                key[i + 1]          = swap ? k : key[i + 1];
+                index[i]            = swap ? index[i + 1] : n;
+                index[i + 1]        = swap ? n : index[i + 1];
+            }
+        }
+    }
     for (int j = 0; j < p.top_k; ++j)
     {
-        uint32_t best = 0;
+        uint32_t head = key[0];
+        int      at   = index[0];
+        if constexpr (!kSorted)
+        {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-        best = __reduce_max_sync(0xffffffffu, best);
+            for (int i = 1; i < kPer; ++i)
+            {
+                const bool more = key[i] > head;
+                head            = more ? key[i] : head;
+                at              = more ? index[i] : at;
+            }
+        }
+        const uint32_t best = __reduce_max_sync(0xffffffffu, head);
         if (best == 0) break;
-        int at = kMaxExperts;
+        const int winner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
+        const int e      = __shfl_sync(0xffffffffu, at, winner);
+        mine             = lane == j ? e : mine;
+        own              = lane == j ? best : own;
+        if (j == 0)
+        {
+            top = key_logit(best);
+            if (p.renormalize == 0)
+            {
 #pragma unroll
-        for (int i = kPer - 1; i >= 0; --i)
-        {
-            if (key[i] == best) at = i * 32 + lane;
+                for (int i = 0; i < kPer; ++i) all += key[i] != 0 ? expf(key_logit(key[i]) - top) : 0.f;
+            }
         }
-        at = __reduce_min_sync(0xffffffffu, at);
+        const bool won = lane == winner;
+        if constexpr (kSorted)
+        {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-        {
-            if (at == i * 32 + lane) key[i] = 0;
+            for (int i = 0; i < kPer; ++i)
+            {
+                key[i]   = won ? (i + 1 < kPer ? key[i + 1] : 0u) : key[i];
+                index[i] = won && i + 1 < kPer ? index[i + 1] : index[i];
+            }
         }
-        const float w = expf(__uint_as_float((best >> 31) != 0 ? best & 0x7fffffffu : ~best) - top);
-        sum += w;
-        if (lane == j)
+        else
         {
-            mine = at;
-            own  = w;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) key[i] = index[i] == e ? 0u : key[i];
         }
     }
-    weight = mine >= 0 ? own / (p.renormalize != 0 ? sum : all) : 0.f;
+    const float w = mine >= 0 ? expf(key_logit(own) - top) : 0.f;
+    if (p.renormalize != 0) all = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    weight = mine >= 0 ? w / all : 0.f;
     return mine;
 }
 template <typename T>
@@ -110,6 +157,7 @@ __device__ __forceinline__ int route_any(const RouteParams &p, int t, int lane, 
 {
     if (p.experts <= 64) return route_token<T, 2>(p, t, lane, weight);
     if (p.experts <= 128) return route_token<T, 4>(p, t, lane, weight);
+    if (p.experts <= 256) return route_token<T, 8>(p, t, lane, weight);
     return route_token<T, kMaxExperts / 32>(p, t, lane, weight);
 }
 
@@ -119,25 +167,34 @@ struct RouteShared
     int      start[kMaxExperts];            // the group's first row, then the chunk's first row of it
     int      scan[kMaxExperts];
     int      before[kMaxExperts];
+    int      total[kMaxExperts / 32];
 };
-// Starts of the groups from the choices per expert in `scan` (which is left as it is): every group takes whole slabs.  By warp 0.
-__device__ __forceinline__ void group_starts(const RouteParams &p, RouteShared &s, int lane)
+// Starts of the groups from the choices per expert in `scan` (which is left as it is): every group takes whole slabs.  By all threads; warp w
+// adds up the experts from 32 w on.
+__device__ __forceinline__ void group_starts(const RouteParams &p, RouteShared &s)
 {
-    const int per = (p.experts + 31) / 32, first = lane * per, last = min(first + per, p.experts);
-    int       sum = 0;
-    for (int e = first; e < last; ++e) sum += (s.scan[e] + kSlab - 1) / kSlab * kSlab;
-    int incl = sum;
+    const int lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
+    for (int w = static_cast<int>(threadIdx.x) >> 5; w < (p.experts + 31) / 32; w += warps)
+    {
+        const int e    = w * 32 + lane;
+        const int room = e < p.experts ? (s.scan[e] + kSlab - 1) / kSlab * kSlab : 0;
+        int       incl = room;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
-    {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (e < p.experts) s.start[e] = incl - room;
+        if (lane == 31) s.total[w] = incl;
     }
-    int at = incl - sum;
-    for (int e = first; e < last; ++e)
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
     {
-        s.start[e] = at;
-        at += (s.scan[e] + kSlab - 1) / kSlab * kSlab;
+        int start = s.start[e];
+        for (int w = 0; w < (e >> 5); ++w) start += s.total[w];
+        if (blockIdx.x == 0) p.groups[e] = make_int2(start, s.scan[e]);
+        s.start[e] = start + s.before[e];
     }
 }
 // rows of the choices of a chunk's tokens, from the mask and the chunk's first rows
@@ -162,10 +219,11 @@ template <typename T, int kStep>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p)
 {
     __shared__ RouteShared s;
-    dependent_prologue();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
     const int t0 = static_cast<int>(blockIdx.x) * p.chunk, tokens = min(p.chunk, p.tokens - t0);
     for (int i = threadIdx.x; i < p.experts * kMaskWords; i += static_cast<int>(blockDim.x)) (&s.mask[0][0])[i] = 0;
+    for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] = s.before[e] = 0;
+    dependent_prologue();
     __syncthreads();
     if constexpr (kStep != 2)
     {
@@ -181,46 +239,45 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
                 if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
             }
         }
-    }
-    else
-    {
-        for (int i = threadIdx.x; i < tokens * p.top_k; i += static_cast<int>(blockDim.x))
-        {
-            const int e = p.ids[static_cast<int64_t>(t0) * p.top_k + i], t = i / p.top_k;
-            if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
-        }
-    }
-    __syncthreads();
-    if constexpr (kStep != 2)
-    {
+        __syncthreads();
         for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
         {
             int n = 0;
             for (int w = 0; w < kMaskWords; ++w) n += __popc(s.mask[e][w]);
             if constexpr (kStep == 1) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = n;
-            s.scan[e]   = n;
-            s.before[e] = 0;
+            s.scan[e] = n;
         }
     }
     else
     {
-        // choices of all chunks and of those before this one: slices of chunks per expert, several loads in flight per thread
-        for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] = s.before[e] = 0;
-        __syncthreads();
+        // choices of all chunks and of those before this one: slices of chunks per expert, eight loads in flight per thread beside those of
+        // this chunk's choices
+        const int first = static_cast<int>(threadIdx.x), choices = tokens * p.top_k;
+        const int e0 = first < choices ? p.ids[static_cast<int64_t>(t0) * p.top_k + first] : -1;
         const int slices = max(1, static_cast<int>(blockDim.x) / p.experts);
         for (int i = threadIdx.x; i < slices * p.experts; i += static_cast<int>(blockDim.x))
         {
             const int e = i % p.experts, slice = i / p.experts;
             int       all = 0, own = 0;
-#pragma unroll 8
-            for (int c = slice; c < p.chunks; c += slices)
+            for (int c = slice; c < p.chunks; c += 8 * slices)
             {
-                const int n = __ldg(p.counts + static_cast<int64_t>(c) * p.experts + e);
-                all += n;
-                own += c < static_cast<int>(blockIdx.x) ? n : 0;
+                int n[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) n[k] = c + k * slices < p.chunks ? p.counts[static_cast<int64_t>(c + k * slices) * p.experts + e] : 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                {
+                    all += n[k];
+                    own += c + k * slices < static_cast<int>(blockIdx.x) ? n[k] : 0;
+                }
             }
             atomicAdd(&s.scan[e], all); // whole numbers: the same sum in any order
             atomicAdd(&s.before[e], own);
+        }
+        for (int i = first; i < choices; i += static_cast<int>(blockDim.x))
+        {
+            const int e = i == first ? e0 : p.ids[static_cast<int64_t>(t0) * p.top_k + i], t = i / p.top_k;
+            if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
         }
     }
     if constexpr (kStep == 1)
@@ -228,13 +285,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
         return;
     }
     __syncthreads();
-    if (warp == 0) group_starts(p, s, lane);
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
-    {
-        if (blockIdx.x == 0) p.groups[e] = make_int2(s.start[e], s.scan[e]);
-        s.start[e] += s.before[e];
-    }
+    group_starts(p, s);
     __syncthreads();
     place_choices(p, s, t0, tokens);
 }
@@ -461,6 +512,7 @@ extern "C"
         p.renormalize = desc->renormalize;
         p.chunks      = route_chunks(desc->tokens);
         p.chunk       = p.chunks == 1 ? kRouteSingle : kRouteChunk;
+        p.vec         = aligned(d_logits, 16) && desc->ld_logits % 16 == 0;
         auto run      = [&](auto element) -> cugl_status {
             using T = decltype(element);
             if (p.chunks == 1)

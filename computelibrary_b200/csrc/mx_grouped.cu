@@ -554,26 +554,23 @@ __device__ __forceinline__ uint32_t pack_two(float a, float b)
     memcpy(&w, two, 4);
     return w;
 }
-// The first `cols` rows of a staging area (kUnits 16-byte units each) to rows m and up of dst, channels n0 and up.  Bulk stores write
-// whole boxes: this is for the one that a group's end cuts.
-template <int kUnits, bool kSwizzled>
+// The first `cols` rows of a staging area to rows m and up of dst, channels n0 and up.  Bulk stores write whole boxes: this is for the one
+// that a group's end cuts.
 __device__ __forceinline__ void store_staged(const GroupedParams &p, const uint8_t *area, int lane, int m, int n0, int cols)
 {
-    constexpr int kSize = kUnits == 4 ? 2 : 4;
-    const int     units = min(kUnits, (p.channels - n0) * kSize / 16); // rows are whole units long
-    for (int i = lane; i < cols * kUnits; i += 32)
+    const int units = min(4, (p.channels - n0) / 8); // of 16 bytes; rows are whole units long
+    for (int i = lane; i < cols * 4; i += 32)
     {
-        const int row = i / kUnits, unit = i % kUnits;
+        const int row = i / 4, unit = i % 4;
         if (unit < units)
         {
-            const int at = kSwizzled ? unit ^ ((row >> 1) & 3) : unit;
-            *reinterpret_cast<uint4 *>(p.dst + static_cast<int64_t>(m + row) * p.ldd + static_cast<int64_t>(n0) * kSize + unit * 16) =
-                *reinterpret_cast<const uint4 *>(area + row * kUnits * 16 + at * 16);
+            *reinterpret_cast<uint4 *>(p.dst + static_cast<int64_t>(m + row) * p.ldd + static_cast<int64_t>(n0) * 2 + unit * 16) =
+                *reinterpret_cast<const uint4 *>(area + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
         }
     }
 }
 
-template <int kFormat, int kBulk, bool kSwiglu>
+template <int kFormat, bool kBulk, bool kSwiglu>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mx_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_up, const __grid_constant__ CUtensorMap tmap_a,
                            const __grid_constant__ CUtensorMap tmap_bsf, const __grid_constant__ CUtensorMap tmap_upsf,
@@ -758,11 +755,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const Item    item = get_item<TILE>(p, before, list, w_blocks, it, v);
             const int     as = it & 1, n0 = (item.wb * 2 + rank) * kMxRows + q * 32;
             const Factors f  = group_factors(p, item.group);
-            float         bias[4] = {}; // kBulk = 2: of the fragments' rows, else of this lane's channel
+            float         bias[4] = {}; // kBulk: of the fragments' rows, else of this lane's channel
             if (!kSwiglu && p.bias != nullptr)
             {
 #pragma unroll
-                for (int i = 0; i < (kBulk == 2 ? 4 : 1); ++i) bias[i] = group_bias(p, item.group, n0 + (kBulk == 2 ? lane / 4 + 8 * i : lane));
+                for (int i = 0; i < (kBulk ? 4 : 1); ++i) bias[i] = group_bias(p, item.group, n0 + (kBulk ? lane / 4 + 8 * i : lane));
             }
             if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it >> 1) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
@@ -794,7 +791,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                 {
-                    if constexpr (kBulk == 2)
+                    if constexpr (kBulk)
                     {
                         tmem_ld_frag32(acc + j + (static_cast<uint32_t>(16 * h) << 16), r[h]);
                         if constexpr (kSwiglu) tmem_ld_frag32(acc + 128 + j + (static_cast<uint32_t>(16 * h) << 16), u[h]);
@@ -807,7 +804,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 }
                 tmem_ld_wait();
                 drained();
-                if constexpr (kBulk == 2)
+                if constexpr (kBulk)
                 {
                     uint32_t packed[2][8];
 #pragma unroll
@@ -837,7 +834,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     else
                     {
                         __syncwarp();
-                        store_staged<4, true>(p, out, lane, m, n0, cols);
+                        store_staged(p, out, lane, m, n0, cols);
                     }
                     if (lane == 0) tma_store_commit();
                     __syncwarp();
@@ -851,36 +848,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 16; ++k) x[k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[0]);
                         const int left = cols - 16 * h;
-                        if constexpr (kBulk == 4)
-                        {
-                            if (lane == 0) tma_store_wait_read();
-                            __syncwarp();
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) reinterpret_cast<float *>(out)[32 * k + lane] = x[k];
-                            if (left >= 16)
-                            {
-                                fence_proxy_async_smem();
-                                __syncwarp();
-                                if (lane == 0) tma_store_2d(&tmap_out, s_out, n0, m + 16 * h);
-                            }
-                            else if (left > 0)
-                            {
-                                __syncwarp();
-                                store_staged<8, false>(p, out, lane, m + 16 * h, n0, left);
-                            }
-                            if (lane == 0) tma_store_commit();
-                            __syncwarp();
-                        }
-                        else
-                        {
-                            store_tokens(p, m + 16 * h, n0 + lane, x, left);
-                        }
+                        store_tokens(p, m + 16 * h, n0 + lane, x, left);
                     }
                 }
             }
             tc_fence_before();
         }
-        if (kBulk != 0 && lane == 0)
+        if (kBulk && lane == 0)
         {
             tma_store_wait_all(); // shared memory stays valid until the stores have read it
         }
@@ -948,21 +922,19 @@ cugl_status launch_few(cugl_context *ctx, const GroupedOperands &op, GroupedPara
     return CUGL_SUCCESS;
 }
 
-// dst in boxes of 2 KB: 32 rows x 32 channels of two bytes in the 64-byte swizzle, or 16 rows of floats
+// 16-bit dst in boxes of 32 rows x 32 channels, in the 64-byte swizzle
 bool encode_results_map(CUtensorMap *map, const GroupedParams &p)
 {
     EncodeTiledFn    fn         = get_encode_fn();
     const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(p.channels), static_cast<cuuint64_t>(p.rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ldd)};
-    const bool       wide       = p.dtype == CUGL_F32;
-    const cuuint32_t box[2]     = {32, wide ? 16u : 32u};
+    const cuuint32_t box[2]     = {32, 32};
     const cuuint32_t estr[2]    = {1, 1};
-    return fn != nullptr && fn(map, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, wide ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B,
+    return fn != nullptr && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.dst, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kFormat, int kBulk, bool kSwiglu>
+template <int kFormat, bool kBulk, bool kSwiglu>
 cugl_status launch_pair(cugl_context *ctx, const GroupedOperands &op, GroupedParams p, long long items)
 {
     using P = PairPlan<kFormat, kSwiglu>;
@@ -973,7 +945,7 @@ cugl_status launch_pair(cugl_context *ctx, const GroupedOperands &op, GroupedPar
     if (!encode_packed_map(&map_b, op.b, weights, inner, op.d->ldb, kMxRows) || !encode_packed_map(&map_a, op.a, p.rows, inner, op.d->lda, P::TILE / 2) ||
         !encode_scale_map(&map_bsf, p.b_scales, w_tiles, F::kChunkTiles) || !encode_scale_map(&map_asf, p.a_scales, a_tiles, F::kChunkTiles) ||
         (kSwiglu && (!encode_packed_map(&map_up, op.up, weights, inner, op.d->ldb, kMxRows) || !encode_scale_map(&map_upsf, p.up_scales, w_tiles, F::kChunkTiles))) ||
-        (kBulk != 0 && !encode_results_map(&map_out, p)))
+        (kBulk && !encode_results_map(&map_out, p)))
     {
         return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for an operand");
     }
@@ -996,16 +968,16 @@ cugl_status launch_grouped(cugl_context *ctx, const GroupedOperands &op, const G
         const long long tiles = (expected + rows - 1) / rows + (expected < p.n_groups ? expected : p.n_groups);
         return tiles * ((p.channels + channels - 1) / channels);
     };
-    if (expected < 48ll * p.n_groups)
+    // us on one CTA per SM / SM pairs at 48, 64, 96, 128 rows a group, NVFP4.  64 groups, 2048 -> 768 SwiGLU to BF16 25.0 / 26.4, 25.4 / 26.9,
+    // 30.3 / 27.6, 33.0 / 29.0; 64 groups, 768 -> 2048 to BF16 14.9 / 15.4, 15.3 / 15.3, 17.7 / 16.2, 21.0 / 17.8; 8 groups, 4096 -> 4096 to BF16
+    // 16.0 / 16.4, 16.2 / 16.4, 17.2 / 16.6, 17.6 / 17.5.  Floats leave from registers either way: at 96, 128, 160, 256 rows 8 groups, 4096 -> 4096
+    // 17.4 / 17.6, 18.3 / 18.7, 27.5 / 21.1, 30.2 / 26.5; 64 groups, 1024 -> 1024 14.4 / 15.5, 15.3 / 16.6, 21.3 / 19.6, 24.8 / 25.6.
+    if (expected < (p.dtype == CUGL_F32 ? 130ll : 72ll) * p.n_groups)
     {
         return launch_few<kFormat, kSwiglu>(ctx, op, p, items(kSlab, kMxRows));
     }
     const long long n = items(PairPlan<kFormat, kSwiglu>::TILE, 2 * kMxRows);
-    if (p.vec_out != 0)
-    {
-        return p.dtype == CUGL_F32 ? launch_pair<kFormat, 4, kSwiglu>(ctx, op, p, n) : launch_pair<kFormat, 2, kSwiglu>(ctx, op, p, n);
-    }
-    return launch_pair<kFormat, 0, kSwiglu>(ctx, op, p, n);
+    return p.vec_out != 0 && p.dtype != CUGL_F32 ? launch_pair<kFormat, true, kSwiglu>(ctx, op, p, n) : launch_pair<kFormat, false, kSwiglu>(ctx, op, p, n);
 }
 
 const char *validate_grouped(const cugl_mx_grouped_gemm_desc *d)
