@@ -165,6 +165,16 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void store_zeros(uint32_t dst)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+}
+// where the share of part i of n equal ones begins
+__device__ __forceinline__ int share_begin(int total, int i, int n)
+{
+    const int each = total / n;
+    return i * each + min(i, total - each * n);
+}
 // eight 16-bit elements of a row from column k on to shared memory, zeros behind `cols`; kVec: rows are 16-byte aligned
 template <bool kVec>
 __device__ __forceinline__ void stage_eight(uint32_t dst, const uint8_t *row, int k, int cols)
@@ -211,6 +221,13 @@ __device__ __forceinline__ float load_cluster(uint32_t addr)
     return v;
 }
 
+// Where rank r stands in a row of v: of sixteen, lane c of the second launch wants 4 c and the next as the matrix instruction's columns 2 c
+// and the next, 4 c + 2 and the next as 2 c + 8 and the next.
+__device__ __forceinline__ int v_place(int r)
+{
+    return (r & ~15) + ((r >> 1) & 6) + ((r & 2) << 2) + (r & 1);
+}
+
 template <typename T, int kRank, bool kVec>
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p)
 {
@@ -230,15 +247,16 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const int halves = t.count > S::kRows ? 2 : 1, subs = kWarps / halves;
     const int half = warp & (halves - 1), sub = halves == 2 ? warp >> 1 : warp;
     const int blocks = (p.K + 63) / 64; // of 64 columns, shared by the CTAs of the cluster
-    const int first  = static_cast<int>(static_cast<int64_t>(blocks) * rank / ranks), n_blocks = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / ranks) - first;
+    const int first = share_begin(blocks, rank, ranks), n_blocks = share_begin(blocks, rank + 1, ranks) - first;
     const int x_rows = (t.count + 15) & ~15, a_rows = (t.rank + 15) & ~15; // those that the matrix instructions read
     const uint8_t *x = p.x + static_cast<int64_t>(t.first) * p.ld_x;
     const uint8_t *a = p.a + static_cast<int64_t>(t.adapter) * p.max_rank * p.ld_a;
     const uint32_t s_base = smem_u32(share);
-    // what a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows (rows behind the last: zeros)
+    // What a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows.  Rows behind the last are zeros,
+    // written once.
     constexpr int  kCopies = (S::kTile + kRank + kThreads / 8 - 1) / (kThreads / 8);
     const int      c8      = (static_cast<int>(threadIdx.x) & 7) * 8;
-    const uint8_t *from[kCopies];
+    const uint8_t *from[kCopies]; // nullptr: nothing to copy
     uint32_t       to[kCopies];
 #pragma unroll
     for (int j = 0; j < kCopies; ++j)
@@ -246,47 +264,66 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
         const int  i = (static_cast<int>(threadIdx.x) >> 3) + j * (kThreads / 8), row = i < x_rows ? i : i - x_rows;
         const bool is_x = i < x_rows;
         from[j] = is_x ? (row < t.count ? x + row * p.ld_x : nullptr) : (row < t.rank ? a + row * p.ld_a : nullptr);
-        to[j]   = row < (is_x ? x_rows : a_rows) ? static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4)) : 0xffffffffu;
-    }
-    auto load = [&](int block) {
-        if (block < n_blocks)
+        to[j]   = s_base + static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4));
+        if (from[j] == nullptr && row < (is_x ? x_rows : a_rows))
         {
-            const uint32_t st = s_base + static_cast<uint32_t>(block % S::kStages) * S::kStage;
-            const int      k  = (first + block) * 64 + c8;
-#pragma unroll
-            for (int j = 0; j < kCopies; ++j)
+            for (int s = 0; s < S::kStages; ++s) store_zeros(to[j] + static_cast<uint32_t>(s) * S::kStage);
+        }
+    }
+    int      loading = 0, load_k = first * 64 + c8; // the next block to load; its first column of this thread
+    uint32_t load_at = 0;                           // its stage
+    auto     load    = [&]() {
+        if (loading < n_blocks)
+        {
+            if (kVec && load_k + 64 - c8 <= p.K)
             {
-                if (to[j] != 0xffffffffu) stage_eight<kVec>(st + to[j], from[j] != nullptr ? from[j] : x, k, from[j] != nullptr ? p.K : 0);
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j)
+                {
+                    if (from[j] != nullptr) copy16(to[j] + load_at, from[j] + static_cast<int64_t>(load_k) * 2, 16);
+                }
             }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j)
+                {
+                    if (from[j] != nullptr) stage_eight<kVec>(to[j] + load_at, from[j], load_k, p.K);
+                }
+            }
+            load_k += 64;
+            ++loading;
+            load_at = load_at + S::kStage == S::kStages * S::kStage ? 0u : load_at + S::kStage;
         }
         copy_commit();
     };
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) load(i);
+    for (int i = 0; i < S::kStages - 1; ++i) load();
     float     acc[S::kMt][kNt][4] = {};
     const int step = halves == 2 ? sub : sub & 3; // 16 columns of a stage
-    for (int i = 0; i < n_blocks; ++i)
+    // rows 16 m + lane % 16 of x, rows 8 n + .. of A: their numbers modulo 8, and so the places of their units, do not depend on m and n
+    const uint32_t x_at = s_base + static_cast<uint32_t>((half * S::kRows + (lane & 15)) * 128 + (((2 * step + (lane >> 4)) ^ (lane & 7)) << 4));
+    const uint32_t a_at = s_base + static_cast<uint32_t>((S::kTile + (lane & 7) + ((lane >> 4) << 3)) * 128 + (((2 * step + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+    uint32_t       st = 0;
+    for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
     {
         copy_wait<S::kStages - 2>();
         __syncthreads();
-        load(i + S::kStages - 1); // to the stage that all warps have left
+        load(); // to the stage that all warps have left
         if (halves == 1 && (i & 1) != (sub >> 2)) continue;
-        const uint32_t st = s_base + static_cast<uint32_t>(i % S::kStages) * S::kStage;
-        uint32_t       xv[S::kMt][4];
+        uint32_t xv[S::kMt][4];
 #pragma unroll
         for (int m = 0; m < S::kMt; ++m)
         {
-            const int row = half * S::kRows + m * 16 + (lane & 15), unit = 2 * step + (lane >> 4);
-            if (half * S::kRows + m * 16 < t.count) ldmatrix_x4(st + static_cast<uint32_t>(row * 128 + ((unit ^ (row & 7)) << 4)), xv[m]);
+            if (half * S::kRows + m * 16 < t.count) ldmatrix_x4(x_at + st + m * 16 * 128, xv[m]);
         }
 #pragma unroll
         for (int n = 0; n < kNt; n += 2)
         {
             if (n * 8 < t.rank)
             {
-                const int row = n * 8 + (lane & 7) + ((lane >> 4) << 3), unit = 2 * step + ((lane >> 3) & 1);
-                uint32_t  av[4];
-                ldmatrix_x4(st + static_cast<uint32_t>((S::kTile + row) * 128 + ((unit ^ (row & 7)) << 4)), av);
+                uint32_t av[4];
+                ldmatrix_x4(a_at + st + n * 8 * 128, av);
 #pragma unroll
                 for (int m = 0; m < S::kMt; ++m)
                 {
@@ -370,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
                     const T part = from_float<T>(rest);
                     uint16_t bits;
                     memcpy(&bits, &part, 2);
-                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + r] = bits;
+                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + v_place(r)] = bits;
                     const float f = to_float(part);
                     rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
                 }
@@ -396,7 +433,7 @@ struct Expand
     static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM: two items' B take 128 registers there
     static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
     static constexpr int kTile    = Shrink<kRank>::kTile;
-    static constexpr int kPitch   = kRank == 16 ? 48 : kRank * 2 + 32; // bytes of a row of v: four rows in different banks
+    static constexpr int kPitch   = kRank * 2 + 16; // bytes of a row of v, its factor included: eight rows in different banks
     static constexpr int kV       = kParts * kTile * kPitch;
     static constexpr int kRow     = 32 * static_cast<int>(sizeof(TD)); // bytes of a row of a unit
     static constexpr int kSlots   = 4;
@@ -475,9 +512,8 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
             total += all;
         }
         total            = min(total, p.tiles);
-        const int64_t items = static_cast<int64_t>(total) * blocks;
-        lo                  = static_cast<int>(items * blockIdx.x / gridDim.x);
-        hi                  = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+        lo               = share_begin(total * blocks, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+        hi               = share_begin(total * blocks, static_cast<int>(blockIdx.x) + 1, static_cast<int>(gridDim.x));
         if (lo >= hi)
         {
             griddep_wait();
@@ -549,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                 for (int j = 0; j < 16 / kStep; ++j, src += kStep * p.ld_base)
                 {
                     const bool in = ahead_m + copy_row + j * kStep < count && ch < p.N; // N is a multiple of 8
-                    copy16(copy_to + static_cast<uint32_t>(ahead_slot * 16 * E::kRow + j * kStep * E::kRow), in ? src : p.base, in ? 16 : 0);
+                    copy16(copy_to + static_cast<uint32_t>(ahead_slot * 16 * E::kRow + j * kStep * E::kRow), src, in ? 16 : 0); // (of none, nothing is read)
                 }
                 ahead_src += 16 * p.ld_base;
             }
@@ -569,12 +605,16 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
         if (t.adapter < 0) return;
         constexpr int kUnits = kRank / 8 + 1; // 16-byte units of a row
         const int     rows   = (t.count + 15) & ~15;
-        for (int i = threadIdx.x; i < E::kParts * rows * kUnits; i += kThreads)
+        for (int i = threadIdx.x; i < rows * kUnits; i += kThreads)
         {
-            const int  row = (i / kUnits) % rows, part = i / (kUnits * rows), unit = i % kUnits;
-            const bool in  = row < t.count;
-            copy16(smem_u32(smem) + static_cast<uint32_t>(half * E::kV + (part * E::kTile + row) * E::kPitch + unit * 16),
-                   p.v + (in ? (static_cast<int64_t>(part) * p.tokens + t.first + row) * (kRank + 8) + unit * 8 : 0), in ? 16 : 0);
+            const int       row = i / kUnits, unit = i % kUnits;
+            const uint16_t *src = p.v + static_cast<int64_t>(t.first + min(row, t.count - 1)) * (kRank + 8) + unit * 8;
+            const uint32_t  dst = smem_u32(smem) + static_cast<uint32_t>(half * E::kV + row * E::kPitch + unit * 16);
+#pragma unroll
+            for (int part = 0; part < E::kParts; ++part)
+            {
+                copy16(dst + part * E::kTile * E::kPitch, src + static_cast<int64_t>(part) * p.tokens * (kRank + 8), row < t.count ? 16 : 0);
+            }
         }
     };
 #pragma unroll
@@ -609,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
         begins = place.block == 0;
         if (item + 1 < hi) load_b<TD>(p, list[place.at], place.block * 32 * kWarps + warp_n, lane, next);
         if (n >= p.N) continue; // the same for the warp
+        const uint32_t v_at    = smem_u32(smem) + static_cast<uint32_t>(half * E::kV + (lane & 15) * E::kPitch + (lane >> 4) * 16);
         uint8_t       *dst_row = p.dst + static_cast<int64_t>(t.first + g) * p.ld_dst + static_cast<int64_t>(n) * static_cast<int>(sizeof(TD));
         const uint8_t *v_row   = smem + half * E::kV + g * E::kPitch;
         for (int m = 0; m < t.count; m += 16, dst_row += 16 * p.ld_dst, v_row += 16 * E::kPitch)
@@ -660,10 +701,10 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                     {
                         if (s * 16 < t.rank)
                         {
-                            const uint8_t *v   = v_row + part * E::kTile * E::kPitch + s * 32 + 8 * c;
-                            const uint2    top = *reinterpret_cast<const uint2 *>(v), low = *reinterpret_cast<const uint2 *>(v + 8 * E::kPitch);
+                            uint32_t v[4];
+                            ldmatrix_x4(v_at + static_cast<uint32_t>(m * E::kPitch + part * E::kTile * E::kPitch + s * 32), v);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) mma<T>(acc[i], top.x, low.x, top.y, low.y, b[i][s].x, b[i][s].y);
+                            for (int i = 0; i < 4; ++i) mma<T>(acc[i], v[0], v[1], v[2], v[3], b[i][s].x, b[i][s].y);
                         }
                     }
                 }
@@ -797,6 +838,7 @@ const char *validate_lora(const cugl_lora_desc *d)
     if (d->ld_base < static_cast<int64_t>(d->N) * size || d->ld_base % size != 0 || d->ld_dst < static_cast<int64_t>(d->N) * size || d->ld_dst % size != 0)
         return "ld_base and ld_dst must hold a row and be multiples of the element size";
     if (most_tiles(*d) > 65535) return "more than 65535 tiles of tokens";
+    if (most_tiles(*d) * ((static_cast<int64_t>(d->N) + 32 * kWarps - 1) / (32 * kWarps)) > INT32_MAX / 2) return "more than 2^30 tiles of tokens and channels";
     return nullptr;
 }
 } // namespace
