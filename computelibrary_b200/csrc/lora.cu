@@ -129,20 +129,21 @@ __device__ __forceinline__ Tile find_tile(const LoraParams &p, int wanted)
 
 // ---- matrix instruction --------------------------------------------------------------------------------------
 // D (+)= A . B, 16 x 8 x 16: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) and the next
-template <typename T>
+template <typename T, bool kFirst = false>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
+    if constexpr (kFirst) d[0] = d[1] = d[2] = d[3] = 0.f;
     if constexpr (std::is_same<T, __half>::value)
     {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     else
     {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
 }
 
@@ -357,8 +358,12 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     {
         const int tok = i / kRank, r = i % kRank;
         float    *at = share + tok * S::kPitch + r; // rows of both halves follow each other
-        float     sum = *at;
-        for (int s = 1; s < subs; ++s) sum += at[s * halves * S::kRows * S::kPitch];
+        float     part[kWarps];
+#pragma unroll
+        for (int s = 0; s < kWarps; ++s) part[s] = s < subs ? at[s * halves * S::kRows * S::kPitch] : 0.f;
+        float sum = part[0];
+#pragma unroll
+        for (int s = 1; s < kWarps; ++s) sum += part[s];
         *at = sum;
     }
     if (ranks > 1) cluster_sync();
@@ -368,17 +373,25 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     {
         constexpr int  kPer = (kRank + 31) / 32;
         const uint32_t at   = smem_u32(share + tok * S::kPitch);
-        float          v[kPer];
+        float          v[kPer], parts[kPer][kMaxSplit];
         float          top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) // all of them under way before the first is added
+        {
+            const int r = min(i * 32 + lane, kRank - 1);
+#pragma unroll
+            for (int q = 0; q < kMaxSplit; ++q)
+            {
+                parts[i][q] = 0.f;
+                if (q < ranks) parts[i][q] = load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
         {
-            const int r = i * 32 + lane;
-            v[i]        = 0.f;
-            if (r < kRank)
-            {
-                for (int q = 0; q < ranks; ++q) v[i] += load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
-            }
+            v[i] = parts[i][0];
+#pragma unroll
+            for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
             if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
         }
         float factor = __ldg(p.scales + t.adapter);
@@ -421,8 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 // ---- second launch: dst = base + factor * v . B^T --------------------------------------------------------------
 // Every CTA works through an equal share of the items, an item being 256 channels of a tile; consecutive items are consecutive channels.  A
 // warp has 32 channels, the tokens of the tile sixteen at a time.  What it needs next is under way while it works: units of 16 tokens
-// x 32 channels of base pass through a ring of four slots of its own, the next item's B waits in registers, the next tile's v in the other
-// half of its buffer.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
+// x 32 channels of base pass through a ring of four slots of its own, the next tile's v waits in the other half of its buffer.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
 //   two-byte results  8 c .. 8 c + 7
 //   floats            4 c .. 4 c + 3 and 16 + 4 c .. 16 + 4 c + 3, so that a store of four lanes covers whole sectors
 constexpr int kListTiles = 256; // tiles of a CTA's share
@@ -430,7 +442,7 @@ template <typename T, typename TD, int kRank>
 struct Expand
 {
     static constexpr int kSteps   = kRank / 16;
-    static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM: two items' B take 128 registers there
+    static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM
     static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
     static constexpr int kTile    = Shrink<kRank>::kTile;
     static constexpr int kPitch   = kRank * 2 + 16; // bytes of a row of v, its factor included: eight rows in different banks
@@ -447,41 +459,49 @@ __device__ __forceinline__ int piece_channel(int piece, int c)
     return sizeof(TD) == 4 ? piece * 16 + 4 * c : 8 * c;
 }
 
-// B of an item, as fragments; what lies behind the adapter's rank counts nothing, whatever it is
+// B of an item, as fragments; what lies behind the adapter's rank counts nothing, whatever it is.  Channels behind the last one are read
+// as the last one: nobody stores their results.
 template <typename TD, int kSteps>
 __device__ __forceinline__ void load_b(const LoraParams &p, const Tile &t, int n, int lane, uint2 (&b)[4][kSteps])
 {
     constexpr int  kPer = 16 / static_cast<int>(sizeof(TD));
     const int      g = lane >> 2, c = lane & 3;
-    const uint8_t *rows = p.b + static_cast<int64_t>(t.adapter) * p.N * p.ld_b;
+    const uint8_t *row[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
         // column j = g of the i-th tile of eight: the lane that gets its results has c = j / 2, as its elements 2 i + j % 2
         const int el = 2 * i + (g & 1), ch = n + piece_channel<TD>(el / kPer, g >> 1) + el % kPer;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-        {
-            const int r = s * 16 + 4 * c;
-            b[i][s]     = make_uint2(0, 0);
-            if (t.adapter >= 0 && ch < p.N && r < t.rank) b[i][s] = __ldcg(reinterpret_cast<const uint2 *>(rows + ch * p.ld_b + r * 2));
-        }
+        row[i]       = p.b + (static_cast<int64_t>(t.adapter) * p.N + min(ch, p.N - 1)) * p.ld_b + 8 * c;
     }
-}
-template <int kSteps>
-__device__ __forceinline__ void cut_b(int rank, int c, uint2 (&b)[4][kSteps])
-{
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
     {
-        const int left = rank - s * 16 - 4 * c; // (nothing to cut where ranks are multiples of 4)
-        if (left > 0 && left < 4)
+        if (s * 16 < t.rank)
         {
+            const int left = t.rank - s * 16 - 4 * c; // ranks of this lane's four
 #pragma unroll
             for (int i = 0; i < 4; ++i)
             {
-                b[i][s].y = left == 3 ? b[i][s].y & 0xffffu : 0u;
-                if (left == 1) b[i][s].x &= 0xffffu;
+                b[i][s] = make_uint2(0, 0);
+                if (left > 0) b[i][s] = __ldcg(reinterpret_cast<const uint2 *>(row[i] + s * 32));
+            }
+        }
+    }
+    if ((t.rank & 3) != 0)
+    {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+        {
+            const int left = t.rank - s * 16 - 4 * c;
+            if (left > 0 && left < 4)
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    b[i][s].y = left == 3 ? b[i][s].y & 0xffffu : 0u;
+                    if (left == 1) b[i][s].x &= 0xffffu;
+                }
             }
         }
     }
@@ -559,44 +579,42 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     const int      copy_row = lane / kUnit, copy_ch = warp_n + lane % kUnit * (16 / static_cast<int>(sizeof(TD)));
     const uint32_t copy_to  = slots + static_cast<uint32_t>(copy_row * E::kRow + ((kUnit == 8 ? (lane % kUnit) ^ ((copy_row & 1) << 2) : lane % kUnit) << 4));
     Place          ahead{0, lo - tile_lo * blocks};
-    int            ahead_left = hi - lo, ahead_m = 0, ahead_slot = 0;
-    const uint8_t *ahead_src = nullptr;
-    auto           load_unit = [&]() {
-        if (ahead_m == 0)
+    int            ahead_left = hi - lo, ahead_rows = 0, ahead_units = 0; // items; rows of this lane and units of the item that are still to come
+    uint32_t       ahead_slot = 0;
+    const uint8_t *ahead_src  = nullptr;
+    const int64_t  copy_step  = kStep * p.ld_base;
+    auto           load_unit  = [&]() {
+        if (ahead_units == 0 && ahead_left > 0)
         {
-            while (ahead_left > 0 && ahead.block * 32 * kWarps + warp_n >= p.N) // nothing for this warp there
+            while (ahead.block * 32 * kWarps + warp_n >= p.N) // nothing for this warp there
             {
-                --ahead_left;
                 advance(ahead);
+                if (--ahead_left == 0) break;
+            }
+            if (ahead_left > 0)
+            {
+                const Tile &t  = list[ahead.at];
+                const int   ch = ahead.block * 32 * kWarps + copy_ch;
+                ahead_units    = (t.count + 15) >> 4;
+                ahead_rows     = ch < p.N ? t.count - copy_row : 0; // N is a multiple of 8
+                ahead_src      = p.base + static_cast<int64_t>(t.first + copy_row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
+                advance(ahead);
+                --ahead_left;
             }
         }
-        if (ahead_left > 0)
+        if (ahead_units > 0)
         {
-            const int count = list[ahead.at].count;
             if constexpr (kVec)
             {
-                const int ch = ahead.block * 32 * kWarps + copy_ch;
-                if (ahead_m == 0)
-                {
-                    ahead_src = p.base + static_cast<int64_t>(list[ahead.at].first + copy_row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
-                }
-                const uint8_t *src = ahead_src;
 #pragma unroll
-                for (int j = 0; j < 16 / kStep; ++j, src += kStep * p.ld_base)
+                for (int j = 0; j < 16 / kStep; ++j, ahead_src += copy_step)
                 {
-                    const bool in = ahead_m + copy_row + j * kStep < count && ch < p.N; // N is a multiple of 8
-                    copy16(copy_to + static_cast<uint32_t>(ahead_slot * 16 * E::kRow + j * kStep * E::kRow), src, in ? 16 : 0); // (of none, nothing is read)
+                    if (j * kStep < ahead_rows) copy16(copy_to + ahead_slot + j * kStep * E::kRow, ahead_src, 16); // rows behind the last: never stored
                 }
-                ahead_src += 16 * p.ld_base;
             }
-            ahead_slot = (ahead_slot + 1) % E::kSlots;
-            ahead_m += 16;
-            if (ahead_m >= count)
-            {
-                ahead_m = 0;
-                --ahead_left;
-                advance(ahead);
-            }
+            ahead_rows -= 16;
+            --ahead_units;
+            ahead_slot = ahead_slot == (E::kSlots - 1) * 16 * E::kRow ? 0u : ahead_slot + 16 * E::kRow;
         }
         copy_commit();
     };
@@ -620,16 +638,22 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
 #pragma unroll
     for (int u = 0; u < E::kSlots; ++u) load_unit();
     Place place{0, lo - tile_lo * blocks};
-    uint2 b[4][E::kSteps], next[4][E::kSteps];
-    load_b<TD>(p, list[0], place.block * 32 * kWarps + warp_n, lane, next);
     griddep_wait();
     load_v(list[0], 0);
-    int  slot = 0, half = 1; // of the ring; of the buffer: the other one is the current tile's
-    bool begins = true;
+    int      half   = 1; // of the buffer of v: the other one is the current tile's
+    bool     begins = true;
+    // a lane's pieces of a unit, in the slot that is next
+    const uint8_t *piece[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+        piece[i] = smem + E::kOffBase + warp * E::kSlots * 16 * E::kRow + g * E::kRow + 16 * (kPieces == 2 ? (4 * i + c) ^ ((g & 1) << 2) : c);
+    int slot = 0;
     for (int item = lo; item < hi; ++item)
     {
         const Tile t = list[place.at];
         const int  n = place.block * 32 * kWarps + warp_n;
+        uint2      b[4][E::kSteps];
+        if (t.adapter >= 0) load_b<TD>(p, t, min(n, p.N - 1), lane, b);
         if (begins) // a tile: its v has been asked for
         {
             copy_commit();
@@ -638,21 +662,14 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
             half ^= 1;
             if (hi - item > blocks - place.block) load_v(list[place.at + 1], half ^ 1);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-#pragma unroll
-            for (int s = 0; s < E::kSteps; ++s) b[i][s] = next[i][s];
-        }
-        if ((t.rank & 3) != 0) cut_b(t.rank, c, b);
         advance(place);
         begins = place.block == 0;
-        if (item + 1 < hi) load_b<TD>(p, list[place.at], place.block * 32 * kWarps + warp_n, lane, next);
         if (n >= p.N) continue; // the same for the warp
         const uint32_t v_at    = smem_u32(smem) + static_cast<uint32_t>(half * E::kV + (lane & 15) * E::kPitch + (lane >> 4) * 16);
         uint8_t       *dst_row = p.dst + static_cast<int64_t>(t.first + g) * p.ld_dst + static_cast<int64_t>(n) * static_cast<int>(sizeof(TD));
         const uint8_t *v_row   = smem + half * E::kV + g * E::kPitch;
-        for (int m = 0; m < t.count; m += 16, dst_row += 16 * p.ld_dst, v_row += 16 * E::kPitch)
+        const int64_t  low_row = 8 * p.ld_dst;
+        for (int m = 0; m < t.count; m += 16, dst_row += 2 * low_row, v_row += 16 * E::kPitch)
         {
             copy_wait<E::kSlots - 1>();
             __syncwarp();
@@ -663,13 +680,11 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                 const int row = h * 8 + g;
                 if constexpr (kVec)
                 {
-                    const uint8_t *from = smem + E::kOffBase + (warp * E::kSlots + slot) * 16 * E::kRow + row * E::kRow;
-                    TD             e[8];
+                    TD e[8];
 #pragma unroll
                     for (int i = 0; i < kPieces; ++i)
                     {
-                        const int   piece = kPieces == 2 ? (4 * i + c) ^ ((row & 1) << 2) : c;
-                        const uint4 v     = *reinterpret_cast<const uint4 *>(from + piece * 16);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(piece[i] + slot + h * 8 * E::kRow);
                         memcpy(e + i * kPer, &v, 16);
                     }
 #pragma unroll
@@ -689,10 +704,10 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
             }
             __syncwarp();
             load_unit(); // to the slot that the warp has read
-            slot = (slot + 1) % E::kSlots;
+            slot = slot == (E::kSlots - 1) * 16 * E::kRow ? 0 : slot + 16 * E::kRow;
             if (t.adapter >= 0)
             {
-                float acc[4][4] = {};
+                float acc[4][4];
 #pragma unroll
                 for (int part = E::kParts - 1; part >= 0; --part) // small parts first
                 {
@@ -704,7 +719,11 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                             uint32_t v[4];
                             ldmatrix_x4(v_at + static_cast<uint32_t>(m * E::kPitch + part * E::kTile * E::kPitch + s * 32), v);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) mma<T>(acc[i], v[0], v[1], v[2], v[3], b[i][s].x, b[i][s].y);
+                            for (int i = 0; i < 4; ++i)
+                            {
+                                if (part == E::kParts - 1 && s == 0) mma<T, true>(acc[i], v[0], v[1], v[2], v[3], b[i][s].x, b[i][s].y);
+                                else mma<T>(acc[i], v[0], v[1], v[2], v[3], b[i][s].x, b[i][s].y);
+                            }
                         }
                     }
                 }
@@ -721,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
             {
                 if (m + h * 8 + g < t.count)
                 {
-                    TD *dst = reinterpret_cast<TD *>(dst_row + h * 8 * p.ld_dst);
+                    TD *dst = reinterpret_cast<TD *>(h == 0 ? dst_row : dst_row + low_row);
                     TD  e[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) e[i] = from_float<TD>(base[h][i]);
