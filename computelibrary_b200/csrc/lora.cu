@@ -209,7 +209,7 @@ struct Shrink
     static constexpr int kMt     = kRank == 128 ? 1 : 2; // 16-row tiles of a warp
     static constexpr int kRows   = 16 * kMt;
     static constexpr int kTile   = 2 * kRows;
-    static constexpr int kStages = kRank == 128 ? 5 : 6;
+    static constexpr int kStages = kRank == 128 ? 5 : kRank == 64 ? 6 : 9; // as many as leave room for two CTAs on an SM
     static constexpr int kStage  = (kTile + kRank) * 128; // bytes
     static constexpr int kPitch  = kRank + 8;             // floats: rows in different banks
     static constexpr int kSmem   = kStages * kStage;
@@ -306,11 +306,20 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const uint32_t x_at = s_base + static_cast<uint32_t>((half * S::kRows + (lane & 15)) * 128 + (((2 * step + (lane >> 4)) ^ (lane & 7)) << 4));
     const uint32_t a_at = s_base + static_cast<uint32_t>((S::kTile + (lane & 7) + ((lane >> 4) << 3)) * 128 + (((2 * step + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
     uint32_t       st = 0;
+    const bool     all = n_blocks < S::kStages; // every stage is under way: one wait
+    if (all)
+    {
+        copy_wait<0>();
+        __syncthreads();
+    }
     for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
     {
-        copy_wait<S::kStages - 2>();
-        __syncthreads();
-        load(); // to the stage that all warps have left
+        if (!all)
+        {
+            copy_wait<S::kStages - 2>();
+            __syncthreads();
+            load(); // to the stage that all warps have left
+        }
         if (halves == 1 && (i & 1) != (sub >> 2)) continue;
         uint32_t xv[S::kMt][4];
 #pragma unroll
@@ -432,17 +441,25 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 }
 
 // ---- second launch: dst = base + factor * v . B^T --------------------------------------------------------------
-// Every CTA works through an equal share of the items, an item being 256 channels of a tile; consecutive items are consecutive channels.  A
+// An item is 256 channels of a tile.  Every CTA takes every gridDim.x-th of them, so that tiles of high and of low rank, which are not
+// equally much work, are spread over all (consecutive shares: prompts of 4096 tokens with ranks of 16 to 64 47 us, this 41).  A
 // warp has 32 channels, the tokens of the tile sixteen at a time.  What it needs next is under way while it works: units of 16 tokens
-// x 32 channels of base pass through a ring of four slots of its own, the next tile's v waits in the other half of its buffer.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
+// x 32 channels of base pass through a ring of four slots of its own, the next item's v waits in the other half of its buffer, and its B
+// in registers where there are enough of them.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
 //   two-byte results  8 c .. 8 c + 7
 //   floats            4 c .. 4 c + 3 and 16 + 4 c .. 16 + 4 c + 3, so that a store of four lanes covers whole sectors
-constexpr int kListTiles = 256; // tiles of a CTA's share
+constexpr int kListed = 256; // items of a CTA at most
+struct Item
+{
+    Tile tile;
+    int  n; // first channel
+};
 template <typename T, typename TD, int kRank>
 struct Expand
 {
     static constexpr int kSteps   = kRank / 16;
     static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM
+    static constexpr bool kAhead  = kRank <= 32;          // the next item's B in registers
     static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
     static constexpr int kTile    = Shrink<kRank>::kTile;
     static constexpr int kPitch   = kRank * 2 + 16; // bytes of a row of v, its factor included: eight rows in different banks
@@ -472,12 +489,12 @@ __device__ __forceinline__ void load_b(const LoraParams &p, const Tile &t, int n
     {
         // column j = g of the i-th tile of eight: the lane that gets its results has c = j / 2, as its elements 2 i + j % 2
         const int el = 2 * i + (g & 1), ch = n + piece_channel<TD>(el / kPer, g >> 1) + el % kPer;
-        row[i]       = p.b + (static_cast<int64_t>(t.adapter) * p.N + min(ch, p.N - 1)) * p.ld_b + 8 * c;
+        row[i]       = p.b + (static_cast<int64_t>(max(t.adapter, 0)) * p.N + min(ch, p.N - 1)) * p.ld_b + 8 * c;
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
     {
-        if (s * 16 < t.rank)
+        if (t.adapter >= 0 && s * 16 < t.rank)
         {
             const int left = t.rank - s * 16 - 4 * c; // ranks of this lane's four
 #pragma unroll
@@ -513,93 +530,61 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     using E = Expand<T, TD, kRank>;
     constexpr int kPieces = static_cast<int>(sizeof(TD)) / 2, kPer = 8 / kPieces; // 16-byte pieces of a lane's row, elements of one
     extern __shared__ __align__(128) uint8_t smem[]; // v of two tiles, then the slots
-    __shared__ Tile       list[kListTiles];
+    __shared__ Item       list[kListed];
     __shared__ ScanShared scan;
     griddep_launch_dependents();
     // the launch ahead let this one start after its own wait: all but v is as it will be
     const int blocks = (p.N + 32 * kWarps - 1) / (32 * kWarps); // of channels
-    int       lo = 0, hi = 0, tile_lo = 0;                      // this CTA's items, the first one's tile
+    const int grid = static_cast<int>(gridDim.x), own = static_cast<int>(blockIdx.x);
+    int       before = 0, turn = 0; // tiles of the requests so far
+    for (int r0 = 0; r0 < p.requests; r0 += kThreads, turn ^= 1)
     {
-        Request q     = load_request(p, static_cast<int>(threadIdx.x));
-        int     tiles = (q.end - q.begin + p.tile - 1) / p.tile, at, all, turn = 0;
+        const Request q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
+        const int     tiles = (q.end - q.begin + p.tile - 1) / p.tile;
+        int           at, all;
         scan_tiles(scan, turn, tiles, at, all);
-        int total = all;
-        for (int r0 = kThreads; r0 < p.requests; r0 += kThreads)
+        const int first = (before + at) * blocks, end = first + tiles * blocks; // the request's items
+        if (tiles > 0)
         {
-            const Request more = load_request(p, r0 + static_cast<int>(threadIdx.x));
-            int           unused;
-            scan_tiles(scan, turn ^= 1, (more.end - more.begin + p.tile - 1) / p.tile, unused, all);
-            total += all;
-        }
-        total            = min(total, p.tiles);
-        lo               = share_begin(total * blocks, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-        hi               = share_begin(total * blocks, static_cast<int>(blockIdx.x) + 1, static_cast<int>(gridDim.x));
-        if (lo >= hi)
-        {
-            griddep_wait();
-            return;
-        }
-        tile_lo           = lo / blocks;
-        const int tile_hi = min((hi - 1) / blocks, tile_lo + kListTiles - 1); // the grid has so many CTAs that the list is long enough
-        int       before  = 0;
-        for (int r0 = 0; r0 < p.requests && before <= tile_hi; r0 += kThreads)
-        {
-            if (p.requests > kThreads)
+            for (int i = max(first - own + grid - 1, 0) / grid; i < kListed && own + i * grid < end; ++i)
             {
-                q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
-                tiles = (q.end - q.begin + p.tile - 1) / p.tile;
-                scan_tiles(scan, turn ^= 1, tiles, at, all);
+                const int in = (own + i * grid - first) / blocks * p.tile; // tokens before the tile
+                list[i]      = Item{Tile{q.begin + in, min(p.tile, q.end - q.begin - in), q.adapter, q.rank}, (own + i * grid - first) % blocks * 32 * kWarps};
             }
-            for (int i = max(tile_lo - before - at, 0); i < min(tiles, tile_hi + 1 - before - at); ++i)
-            {
-                list[before + at + i - tile_lo] = Tile{q.begin + i * p.tile, min(p.tile, q.end - q.begin - i * p.tile), q.adapter, q.rank};
-            }
-            before += all;
         }
-        __syncthreads();
+        before += all;
     }
+    const int items = min(max(min(before, p.tiles) * blocks - own + grid - 1, 0) / grid, kListed);
+    if (items == 0)
+    {
+        griddep_wait();
+        return;
+    }
+    __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t slots = smem_u32(smem) + E::kOffBase + static_cast<uint32_t>(warp) * E::kSlots * 16 * E::kRow;
     const int warp_n = warp * 32; // the warp's channels of an item
-    // A place in the CTA's share: an item's tile and block of channels.
-    struct Place
-    {
-        int at, block; // tile of the list, block of channels
-    };
-    auto advance = [&](Place &q) {
-        if (++q.block == blocks)
-        {
-            q.block = 0;
-            ++q.at;
-        }
-    };
     // The ring: units in the order in which they are worked on.  16-byte pieces are exchanged by row where a row has eight of them
     // (reading two rows side by side hits all banks once).  A lane copies one piece of every kStep-th row.
     constexpr int  kUnit = E::kRow / 16, kStep = 32 / kUnit; // pieces of a row, rows that the warp copies at a time
     const int      copy_row = lane / kUnit, copy_ch = warp_n + lane % kUnit * (16 / static_cast<int>(sizeof(TD)));
     const uint32_t copy_to  = slots + static_cast<uint32_t>(copy_row * E::kRow + ((kUnit == 8 ? (lane % kUnit) ^ ((copy_row & 1) << 2) : lane % kUnit) << 4));
-    Place          ahead{0, lo - tile_lo * blocks};
-    int            ahead_left = hi - lo, ahead_rows = 0, ahead_units = 0; // items; rows of this lane and units of the item that are still to come
+    int            ahead = 0, ahead_rows = 0, ahead_units = 0; // the next item; rows of this lane and units of the present one that are still to come
     uint32_t       ahead_slot = 0;
     const uint8_t *ahead_src  = nullptr;
     const int64_t  copy_step  = kStep * p.ld_base;
     auto           load_unit  = [&]() {
-        if (ahead_units == 0 && ahead_left > 0)
+        if (ahead_units == 0)
         {
-            while (ahead.block * 32 * kWarps + warp_n >= p.N) // nothing for this warp there
+            while (ahead < items && list[ahead].n + warp_n >= p.N) ++ahead; // nothing for this warp there
+            if (ahead < items)
             {
-                advance(ahead);
-                if (--ahead_left == 0) break;
-            }
-            if (ahead_left > 0)
-            {
-                const Tile &t  = list[ahead.at];
-                const int   ch = ahead.block * 32 * kWarps + copy_ch;
+                const Tile &t  = list[ahead].tile;
+                const int   ch = list[ahead].n + copy_ch;
                 ahead_units    = (t.count + 15) >> 4;
                 ahead_rows     = ch < p.N ? t.count - copy_row : 0; // N is a multiple of 8
                 ahead_src      = p.base + static_cast<int64_t>(t.first + copy_row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
-                advance(ahead);
-                --ahead_left;
+                ++ahead;
             }
         }
         if (ahead_units > 0)
@@ -637,34 +622,46 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     };
 #pragma unroll
     for (int u = 0; u < E::kSlots; ++u) load_unit();
-    Place place{0, lo - tile_lo * blocks};
+    uint2 b[4][E::kSteps], next[E::kAhead ? 4 : 1][E::kSteps];
+    if constexpr (E::kAhead) load_b<TD>(p, list[0].tile, list[0].n + warp_n, lane, next);
     griddep_wait();
-    load_v(list[0], 0);
-    int      half   = 1; // of the buffer of v: the other one is the current tile's
-    bool     begins = true;
+    load_v(list[0].tile, 0);
+    copy_commit();
     // a lane's pieces of a unit, in the slot that is next
     const uint8_t *piece[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
         piece[i] = smem + E::kOffBase + warp * E::kSlots * 16 * E::kRow + g * E::kRow + 16 * (kPieces == 2 ? (4 * i + c) ^ ((g & 1) << 2) : c);
-    int slot = 0;
-    for (int item = lo; item < hi; ++item)
+    int slot = 0, units = 0; // units: groups of copies since the one that brought this item's v
+    for (int item = 0; item < items; ++item)
     {
-        const Tile t = list[place.at];
-        const int  n = place.block * 32 * kWarps + warp_n;
-        uint2      b[4][E::kSteps];
-        if (t.adapter >= 0) load_b<TD>(p, t, min(n, p.N - 1), lane, b);
-        if (begins) // a tile: its v has been asked for
+        const Tile t    = list[item].tile;
+        const int  n    = list[item].n + warp_n, half = item & 1;
+        if constexpr (E::kAhead)
         {
-            copy_commit();
-            copy_wait<0>();
-            __syncthreads();
-            half ^= 1;
-            if (hi - item > blocks - place.block) load_v(list[place.at + 1], half ^ 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+#pragma unroll
+                for (int s = 0; s < E::kSteps; ++s) b[i][s] = next[i][s];
+            }
+            if (item + 1 < items) load_b<TD>(p, list[item + 1].tile, list[item + 1].n + warp_n, lane, next);
         }
-        advance(place);
-        begins = place.block == 0;
+        else
+        {
+            load_b<TD>(p, t, n, lane, b);
+        }
+        if (units == 0) copy_wait<0>();
+        else if (units == 1) copy_wait<1>();
+        else if (units == 2) copy_wait<2>();
+        else if (units == 3) copy_wait<3>();
+        else copy_wait<4>();
+        __syncthreads(); // v is there, and all warps have done with the item before
+        if (item + 1 < items) load_v(list[item + 1].tile, half ^ 1);
+        copy_commit();
+        units = 0;
         if (n >= p.N) continue; // the same for the warp
+        units = (t.count + 15) >> 4;
         const uint32_t v_at    = smem_u32(smem) + static_cast<uint32_t>(half * E::kV + (lane & 15) * E::kPitch + (lane >> 4) * 16);
         uint8_t       *dst_row = p.dst + static_cast<int64_t>(t.first + g) * p.ld_dst + static_cast<int64_t>(n) * static_cast<int>(sizeof(TD));
         const uint8_t *v_row   = smem + half * E::kV + g * E::kPitch;
@@ -817,8 +814,8 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
         CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, E::kSmem));
         set[ctx->device & 63].store(true, std::memory_order_release);
     }
-    // one CTA or two to an SM; more only where a share would be longer than a CTA's list of tiles
-    const int64_t items = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps) * tiles, most = std::max<int64_t>(E::kCtas * ctx->sm_count, tiles / (kListTiles - 2) + 1);
+    // one CTA or two to an SM; more only where there are more items than these list
+    const int64_t items = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps) * tiles, most = std::max<int64_t>(E::kCtas * ctx->sm_count, (items + kListed - 1) / kListed);
     const int64_t grid  = items < most ? items : most;
     CUGL_CUDA_TRY(ctx, launch_dependent(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, E::kSmem, grid, p));
     return CUGL_SUCCESS;
