@@ -62,23 +62,27 @@ __device__ __forceinline__ int load_l2(const int32_t *p)
 // A request's tokens are [starts[i], starts[i + 1]), cut to those there are.
 struct Request
 {
-    int begin, end, adapter, rank;
+    int begin, end, adapter, rank; // adapter and rank as they were read
 };
 __device__ __forceinline__ Request load_request(const LoraParams &p, int r)
 {
     Request q{0, 0, -1, 0};
     if (r < p.requests)
     {
-        const int begin = load_l2(p.starts + r), end = load_l2(p.starts + r + 1), a = load_l2(p.adapters + r);
-        q.begin         = min(max(begin, 0), p.tokens);
-        q.end           = min(max(end, q.begin), p.tokens);
-        if (a >= 0 && a < p.n_adapters)
-        {
-            q.rank    = p.ranks != nullptr ? min(max(load_l2(p.ranks + a), 0), p.max_rank) : p.max_rank;
-            q.adapter = q.rank > 0 ? a : -1;
-        }
+        const int begin = load_l2(p.starts + r), end = load_l2(p.starts + r + 1);
+        q.adapter       = load_l2(p.adapters + r);
+        q.rank          = p.max_rank;
+        if (p.ranks != nullptr && q.adapter >= 0 && q.adapter < p.n_adapters) q.rank = load_l2(p.ranks + q.adapter); // on its way during the scan
+        q.begin = min(max(begin, 0), p.tokens);
+        q.end   = min(max(end, q.begin), p.tokens);
     }
     return q;
+}
+// tile `i` of a request
+__device__ __forceinline__ Tile request_tile(const LoraParams &p, const Request &q, int i)
+{
+    const int first = q.begin + i * p.tile, rank = min(max(q.rank, 0), p.max_rank);
+    return Tile{first, min(p.tile, q.end - first), q.adapter >= 0 && q.adapter < p.n_adapters && rank > 0 ? q.adapter : -1, rank};
 }
 struct ScanShared
 {
@@ -120,7 +124,7 @@ __device__ __forceinline__ Tile find_tile(const LoraParams &p, int wanted)
         int           at, all;
         scan_tiles(scan, turn, tiles, at, all);
         const int i = wanted - before - at;
-        if (i >= 0 && i < tiles) found = Tile{q.begin + i * p.tile, min(p.tile, q.end - q.begin - i * p.tile), q.adapter, q.rank};
+        if (i >= 0 && i < tiles) found = request_tile(p, q, i);
         before += all;
     }
     __syncthreads();
@@ -209,7 +213,7 @@ struct Shrink
     static constexpr int kMt     = kRank == 128 ? 1 : 2; // 16-row tiles of a warp
     static constexpr int kRows   = 16 * kMt;
     static constexpr int kTile   = 2 * kRows;
-    static constexpr int kStages = kRank == 128 ? 5 : kRank == 64 ? 6 : 9; // as many as leave room for two CTAs on an SM
+    static constexpr int kStages = kRank == 128 ? 4 : kRank == 64 ? 6 : 8; // as many pairs as leave room for two CTAs on an SM
     static constexpr int kStage  = (kTile + kRank) * 128; // bytes
     static constexpr int kPitch  = kRank + 8;             // floats: rows in different banks
     static constexpr int kSmem   = kStages * kStage;
@@ -299,26 +303,21 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
         copy_commit();
     };
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) load();
+    for (int i = 0; i < S::kStages - 2; ++i) load();
     float     acc[S::kMt][kNt][4] = {};
     const int step = halves == 2 ? sub : sub & 3; // 16 columns of a stage
     // rows 16 m + lane % 16 of x, rows 8 n + .. of A: their numbers modulo 8, and so the places of their units, do not depend on m and n
     const uint32_t x_at = s_base + static_cast<uint32_t>((half * S::kRows + (lane & 15)) * 128 + (((2 * step + (lane >> 4)) ^ (lane & 7)) << 4));
     const uint32_t a_at = s_base + static_cast<uint32_t>((S::kTile + (lane & 7) + ((lane >> 4) << 3)) * 128 + (((2 * step + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
     uint32_t       st = 0;
-    const bool     all = n_blocks < S::kStages; // every stage is under way: one wait
-    if (all)
-    {
-        copy_wait<0>();
-        __syncthreads();
-    }
     for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
     {
-        if (!all)
+        if ((i & 1) == 0) // two stages at a time
         {
-            copy_wait<S::kStages - 2>();
+            copy_wait<S::kStages - 4>();
             __syncthreads();
-            load(); // to the stage that all warps have left
+            load(); // to the stages that all warps have left
+            load();
         }
         if (halves == 1 && (i & 1) != (sub >> 2)) continue;
         uint32_t xv[S::kMt][4];
@@ -548,8 +547,8 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
         {
             for (int i = max(first - own + grid - 1, 0) / grid; i < kListed && own + i * grid < end; ++i)
             {
-                const int in = (own + i * grid - first) / blocks * p.tile; // tokens before the tile
-                list[i]      = Item{Tile{q.begin + in, min(p.tile, q.end - q.begin - in), q.adapter, q.rank}, (own + i * grid - first) % blocks * 32 * kWarps};
+                const int in = own + i * grid - first;
+                list[i]      = Item{request_tile(p, q, in / blocks), in % blocks * 32 * kWarps};
             }
         }
         before += all;
