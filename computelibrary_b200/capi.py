@@ -9,7 +9,7 @@ import re
 
 from . import build as _build
 
-U8, S8, S32, S16, F32, F16, BF16 = 0, 1, 2, 3, 4, 5, 6  # F16, BF16: mx_* only. S16: QSYMM16 (stand-alone stage only); F32: dequantized GEMM output
+U8, S8, S32, S16, F32, F16, BF16 = 0, 1, 2, 3, 4, 5, 6  # F16, BF16: mx_*, moe_*, lora only. S16: QSYMM16 (stand-alone stage only); F32: dequantized GEMM output
 STAGE_NONE, STAGE_QUANTIZE_DOWN, STAGE_FIXEDPOINT = 0, 1, 2
 # cugl_status values the tests name
 SUCCESS, RUNTIME_ERROR, INVALID_ARGUMENT = 0, 1, 6

@@ -78,6 +78,12 @@ __device__ __forceinline__ Request load_request(const LoraParams &p, int r)
     }
     return q;
 }
+// Tiles of a request.  Starts that are not in order may give more of them than there can be: none of it runs out of range, and nothing
+// behind p.tiles is worked on.
+__device__ __forceinline__ int request_tiles(const LoraParams &p, const Request &q)
+{
+    return min((q.end - q.begin + p.tile - 1) / p.tile, p.tiles);
+}
 // tile `i` of a request
 __device__ __forceinline__ Tile request_tile(const LoraParams &p, const Request &q, int i)
 {
@@ -120,12 +126,12 @@ __device__ __forceinline__ Tile find_tile(const LoraParams &p, int wanted)
     for (int r0 = 0; r0 < p.requests && before <= wanted; r0 += kThreads, turn ^= 1)
     {
         const Request q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
-        const int     tiles = (q.end - q.begin + p.tile - 1) / p.tile;
+        const int     tiles = request_tiles(p, q);
         int           at, all;
         scan_tiles(scan, turn, tiles, at, all);
         const int i = wanted - before - at;
         if (i >= 0 && i < tiles) found = request_tile(p, q, i);
-        before += all;
+        before = min(before + all, p.tiles);
     }
     __syncthreads();
     return found;
@@ -539,11 +545,11 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     for (int r0 = 0; r0 < p.requests; r0 += kThreads, turn ^= 1)
     {
         const Request q     = load_request(p, r0 + static_cast<int>(threadIdx.x));
-        const int     tiles = (q.end - q.begin + p.tile - 1) / p.tile;
+        const int     tiles = request_tiles(p, q);
         int           at, all;
         scan_tiles(scan, turn, tiles, at, all);
-        const int first = (before + at) * blocks, end = first + tiles * blocks; // the request's items
-        if (tiles > 0)
+        const int first = min(before + at, p.tiles) * blocks, end = min(before + at + tiles, p.tiles) * blocks; // the request's items
+        if (first < end)
         {
             for (int i = max(first - own + grid - 1, 0) / grid; i < kListed && own + i * grid < end; ++i)
             {
@@ -551,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                 list[i]      = Item{request_tile(p, q, in / blocks), in % blocks * 32 * kWarps};
             }
         }
-        before += all;
+        before = min(before + all, p.tiles);
     }
-    const int items = min(max(min(before, p.tiles) * blocks - own + grid - 1, 0) / grid, kListed);
+    const int items = min(max(before * blocks - own + grid - 1, 0) / grid, kListed);
     if (items == 0)
     {
         griddep_wait();

@@ -16,15 +16,17 @@ constexpr int kSlab = 128; // rows at whose multiples groups start
 // ---- the gate ------------------------------------------------------------------------------------------------
 // A warp chooses for a token; a block takes a chunk of consecutive tokens.  The rows of a group are in the order of the tokens, so a
 // choice's row is its group's start, the choices of that expert in the chunks before, and those of the tokens before it in its own
-// chunk (bits of a mask per expert).  One chunk: one launch.  Several: the first launch leaves the number of choices per chunk and expert,
-// the second adds up those of the chunks before (no block waits for another one, nothing depends on the order of atomics).
+// chunk (bits of a mask per expert, 128 tokens at a time).  One chunk: one launch.  Several: the first launch leaves the number of
+// choices per chunk and expert, the second adds up those of the chunks before (no block waits for another one, nothing depends on the
+// order of atomics).  There are at most 256 chunks, which every block of the second launch reads.
 //
-// What bounds it: latency.  64 tokens a chunk, two per warp: a choice is a dozen dependent instructions, top_k of them follow each
-// other.
+// What bounds it: the instructions of the choices, top_k of which follow each other, and two launches.  8192 tokens, 128 experts, top 8:
+// 13 us, 0.5 at the copy rate.
 constexpr int kRouteWarps  = 32;
-constexpr int kRouteChunk  = 64;  // tokens of a block, where there are several
-constexpr int kRouteSingle = 128; // tokens of a single block
-constexpr int kMaskWords   = kRouteSingle / 32;
+constexpr int kRouteChunk  = 64;  // tokens of a block at least, where there are several
+constexpr int kRouteChunks = 256; // at most
+constexpr int kRoutePart   = 128; // tokens at a time
+constexpr int kMaskWords   = kRoutePart / 32;
 
 struct RouteParams
 {
@@ -197,7 +199,27 @@ __device__ __forceinline__ void group_starts(const RouteParams &p, RouteShared &
         s.start[e] = start + s.before[e];
     }
 }
-// rows of the choices of a chunk's tokens, from the mask and the chunk's first rows
+// The mask of a part's choices: read back where another launch made them.
+__device__ __forceinline__ void clear_mask(const RouteParams &p, RouteShared &s)
+{
+    for (int i = threadIdx.x; i < p.experts * kMaskWords; i += static_cast<int>(blockDim.x)) (&s.mask[0][0])[i] = 0;
+}
+__device__ __forceinline__ void set_mask(const RouteParams &p, RouteShared &s, int t0, int tokens)
+{
+    for (int i = threadIdx.x; i < tokens * p.top_k; i += static_cast<int>(blockDim.x))
+    {
+        const int e = p.ids[static_cast<int64_t>(t0) * p.top_k + i], t = i / p.top_k;
+        if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
+    }
+}
+__device__ __forceinline__ int mask_count(const RouteShared &s, int e)
+{
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < kMaskWords; ++w) n += __popc(s.mask[e][w]);
+    return n;
+}
+// rows of the choices of a part's tokens, from the mask and the part's first rows
 __device__ __forceinline__ void place_choices(const RouteParams &p, const RouteShared &s, int t0, int tokens)
 {
     for (int i = threadIdx.x; i < tokens * p.top_k; i += static_cast<int>(blockDim.x))
@@ -220,40 +242,49 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
 {
     __shared__ RouteShared s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
-    const int t0 = static_cast<int>(blockIdx.x) * p.chunk, tokens = min(p.chunk, p.tokens - t0);
-    for (int i = threadIdx.x; i < p.experts * kMaskWords; i += static_cast<int>(blockDim.x)) (&s.mask[0][0])[i] = 0;
+    const int t0 = static_cast<int>(blockIdx.x) * p.chunk, end = min(t0 + p.chunk, p.tokens);
+    clear_mask(p, s);
     for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] = s.before[e] = 0;
     dependent_prologue();
     __syncthreads();
     if constexpr (kStep != 2)
     {
-        for (int t = warp; t < tokens; t += warps)
+        for (int part = t0; part < end; part += kRoutePart)
         {
-            float     weight;
-            const int e = route_any<T>(p, t0 + t, lane, weight);
-            if (lane < p.top_k)
+            const int tokens = min(kRoutePart, end - part);
+            for (int t = warp; t < tokens; t += warps)
             {
-                const int64_t at = static_cast<int64_t>(t0 + t) * p.top_k + lane;
-                p.ids[at]        = e;
-                p.weights[at]    = weight;
-                if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
+                float     weight;
+                const int e = route_any<T>(p, part + t, lane, weight);
+                if (lane < p.top_k)
+                {
+                    const int64_t at = static_cast<int64_t>(part + t) * p.top_k + lane;
+                    p.ids[at]        = e;
+                    p.weights[at]    = weight;
+                    if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
+                }
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] += mask_count(s, e);
+            if (part + kRoutePart < end)
+            {
+                __syncthreads();
+                clear_mask(p, s);
+                __syncthreads();
             }
         }
-        __syncthreads();
-        for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x))
+        if constexpr (kStep == 1)
         {
-            int n = 0;
-            for (int w = 0; w < kMaskWords; ++w) n += __popc(s.mask[e][w]);
-            if constexpr (kStep == 1) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = n;
-            s.scan[e] = n;
+            for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) // (written by the same thread)
+            {
+                p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = s.scan[e];
+            }
+            return;
         }
     }
     else
     {
-        // choices of all chunks and of those before this one: slices of chunks per expert, eight loads in flight per thread beside those of
-        // this chunk's choices
-        const int first = static_cast<int>(threadIdx.x), choices = tokens * p.top_k;
-        const int e0 = first < choices ? p.ids[static_cast<int64_t>(t0) * p.top_k + first] : -1;
+        // choices of all chunks and of those before this one: slices of chunks per expert, eight loads in flight per thread
         const int slices = max(1, static_cast<int>(blockDim.x) / p.experts);
         for (int i = threadIdx.x; i < slices * p.experts; i += static_cast<int>(blockDim.x))
         {
@@ -274,20 +305,25 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             atomicAdd(&s.scan[e], all); // whole numbers: the same sum in any order
             atomicAdd(&s.before[e], own);
         }
-        for (int i = first; i < choices; i += static_cast<int>(blockDim.x))
-        {
-            const int e = i == first ? e0 : p.ids[static_cast<int64_t>(t0) * p.top_k + i], t = i / p.top_k;
-            if (e >= 0) atomicOr(&s.mask[e][t >> 5], 1u << (t & 31));
-        }
-    }
-    if constexpr (kStep == 1)
-    {
-        return;
+        set_mask(p, s, t0, min(kRoutePart, end - t0));
     }
     __syncthreads();
     group_starts(p, s);
     __syncthreads();
-    place_choices(p, s, t0, tokens);
+    for (int part = t0; part < end; part += kRoutePart)
+    {
+        place_choices(p, s, part, min(kRoutePart, end - part));
+        if (part + kRoutePart < end)
+        {
+            __syncthreads();
+            for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.start[e] += mask_count(s, e);
+            __syncthreads();
+            clear_mask(p, s);
+            __syncthreads();
+            set_mask(p, s, part + kRoutePart, min(kRoutePart, end - part - kRoutePart));
+            __syncthreads();
+        }
+    }
 }
 
 // ---- combination ---------------------------------------------------------------------------------------------
@@ -426,9 +462,16 @@ const char *validate_route(const cugl_moe_route_desc *d)
     if (static_cast<int64_t>(d->tokens) * d->top_k + static_cast<int64_t>(kSlab) * d->experts > INT32_MAX - 1024) return "more rows than 32 bits count";
     return nullptr;
 }
+int route_chunk(int tokens) // tokens of a block
+{
+    if (tokens <= kRoutePart) return kRoutePart;
+    const int least = (tokens + kRouteChunks - 1) / kRouteChunks;
+    return least <= kRouteChunk ? kRouteChunk : (least + kRoutePart - 1) / kRoutePart * kRoutePart;
+}
 int route_chunks(int tokens)
 {
-    return tokens <= kRouteSingle ? 1 : (tokens + kRouteChunk - 1) / kRouteChunk;
+    const int chunk = route_chunk(tokens);
+    return tokens <= chunk ? 1 : (tokens + chunk - 1) / chunk;
 }
 
 const char *validate_combine(const cugl_moe_combine_desc *d)
@@ -511,7 +554,7 @@ extern "C"
         p.top_k       = desc->top_k;
         p.renormalize = desc->renormalize;
         p.chunks      = route_chunks(desc->tokens);
-        p.chunk       = p.chunks == 1 ? kRouteSingle : kRouteChunk;
+        p.chunk       = route_chunk(desc->tokens);
         p.vec         = aligned(d_logits, 16) && desc->ld_logits % 16 == 0;
         auto run      = [&](auto element) -> cugl_status {
             using T = decltype(element);

@@ -54,9 +54,9 @@ typedef enum cugl_dtype
     CUGL_S8  = 1,
     CUGL_S32 = 2,
     CUGL_S16 = 3, /* QSYMM16: destination of the stand-alone fixed-point output stage only */
-    CUGL_F32 = 4, /* destination of the GEMM with stage NONE: the int32 result times dequantize_scale; cugl_mx_* */
-    CUGL_F16 = 5, /* cugl_mx_* only */
-    CUGL_BF16 = 6 /* cugl_mx_* only */
+    CUGL_F32 = 4, /* destination of the GEMM with stage NONE: the int32 result times dequantize_scale; cugl_mx_*, cugl_moe_*, cugl_lora */
+    CUGL_F16 = 5, /* cugl_mx_*, cugl_moe_* and cugl_lora only */
+    CUGL_BF16 = 6 /* cugl_mx_*, cugl_moe_* and cugl_lora only */
 } cugl_dtype;
 
 /* GEMMLowpOutputStageType (arm_compute/function_info/GEMMInfo.h:40-46).  Only NONE and
@@ -666,7 +666,8 @@ typedef struct cugl_moe_route_desc
 } cugl_moe_route_desc;
 
 CUGL_API cugl_status cugl_moe_route_validate(const cugl_moe_route_desc *desc, const char **reason);
-/* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU need one each. */
+/* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU, and captured graphs
+ * that are replayed at the same time, need one each. */
 CUGL_API size_t      cugl_moe_route_workspace_bytes(const cugl_moe_route_desc *desc);
 /* One launch for up to 128 tokens, else two.  d_workspace: 16-byte aligned; groups: 8-byte aligned.  tokens == 0: groups of no rows. */
 CUGL_API cugl_status cugl_moe_route(cugl_context *ctx, const cugl_moe_route_desc *desc, const void *d_logits, int32_t *d_ids,
@@ -676,7 +677,7 @@ CUGL_API cugl_status cugl_moe_route(cugl_context *ctx, const cugl_moe_route_desc
 /* Plain rows -> packed rows of groups, as cugl_mx_quantize stores them.
  *   src_grouped == 0  row t of src to the rows slots[t][0 .. top_k): a token to all its experts, quantised once
  *   src_grouped != 0  row slots[t][j] of src to the same row of dst: what the groups' products left
- * Slots outside 0 .. rows - 1 (-1) are skipped; rows that no slot names are left as they are. */
+ * Slots outside 0 .. rows - 1 (-1) are skipped; rows that no slot names are left as they are.  No two tokens share a row. */
 typedef struct cugl_mx_group_desc
 {
     int32_t tokens, top_k;   /* of the slots; top_k 1 .. 16 */

@@ -210,6 +210,28 @@ def test_equal_calls_give_equal_bits(ctx, lengths):
 
 
 @pytest.mark.gpu
+def test_starts_out_of_order(ctx):
+    """Requests that overlap, lie outside or end before they begin are cut to the tokens there are; nothing else is written."""
+    import torch
+    M, R, N = 300, 600, 72
+    d = capi.make_lora_desc(M, R, 2, 16, 128, N, capi.F16, capi.F16)
+    x = torch.ones((M, 128), dtype=torch.float16, device="cuda")
+    a, b = torch.ones((2, 16, 128), dtype=torch.float16, device="cuda"), torch.ones((2, N, 16), dtype=torch.float16, device="cuda")
+    base = torch.zeros((M, N), dtype=torch.float16, device="cuda")
+    out = torch.full((M + 4, N), 7.0, dtype=torch.float16, device="cuda")
+    ws = torch.full((capi.lora_workspace_bytes(d) + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(0)
+    for starts in (rng.integers(-2 ** 31, 2 ** 31 - 1, R + 1), np.where(np.arange(R + 1) % 2, 10 ** 9, -5), rng.integers(-400, 700, R + 1), np.arange(R, -1, -1)):
+        picks = rng.integers(-3, 5, R)
+        ctx.lora(d, x, torch.tensor(starts, dtype=torch.int32, device="cuda"), torch.tensor(picks, dtype=torch.int32, device="cuda"), None,
+                 torch.ones(2, device="cuda"), a, b, base, out, ws[:capi.lora_workspace_bytes(d)])
+        ctx.sync()
+        assert (out[M:] == 7).all() and (ws[-64:] == 0xFF).all()
+        got = out[:M].double().cpu().numpy()  # a token is left alone, copied, or given its adapter's 16 * 128
+        assert np.isin(got, [7.0, 0.0, 2048.0]).all()
+
+
+@pytest.mark.gpu
 def test_nothing_to_do(ctx):
     for M, R in ((0, 3), (3, 0)):
         ctx.lora(capi.make_lora_desc(M, R, 2, 8, 64, 64, capi.F16, capi.F16), *[None] * 10)

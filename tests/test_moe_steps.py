@@ -114,7 +114,8 @@ def check_route(ctx, logits, top_k, dtype=capi.F32, renormalize=True, pad=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("renormalize", [True, False])
 @pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 64, 8), (2, 3, 3), (33, 8, 2), (128, 64, 8), (129, 64, 8), (200, 500, 16), (1000, 128, 6), (64, 512, 16),
-                                   (4097, 60, 4), (3, 33, 1), (700, 5, 5), (20000, 7, 2)])
+                                   (4097, 60, 4), (3, 33, 1), (700, 5, 5), (20000, 7, 2), (16384, 3, 1),
+                                   (16385, 4, 2), (40000, 40, 3)])
 def test_route(ctx, T, E, k, renormalize):
     rng = np.random.default_rng(T + E)
     logits = (rng.standard_normal((T, E)) * 3 + rng.standard_normal(E)).astype(np.float32)
