@@ -180,34 +180,29 @@ __device__ __forceinline__ void store_zeros(uint32_t dst)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
 }
+__device__ __forceinline__ void store_word(uint32_t dst, uint32_t v)
+{
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+}
 // where the share of part i of n equal ones begins
 __device__ __forceinline__ int share_begin(int total, int i, int n)
 {
     const int each = total / n;
     return i * each + min(i, total - each * n);
 }
-// eight 16-bit elements of a row from column k on to shared memory, zeros behind `cols`; kVec: rows are 16-byte aligned
-template <bool kVec>
+// eight 16-bit elements of a 16-byte aligned row from column k on to shared memory, zeros behind `cols`
 __device__ __forceinline__ void stage_eight(uint32_t dst, const uint8_t *row, int k, int cols)
 {
-    const uint16_t *src = reinterpret_cast<const uint16_t *>(row) + k;
-    if constexpr (kVec)
-    {
-        const int valid = min(max(cols - k, 0) * 2, 16);
-        copy16(dst, valid > 0 ? src : reinterpret_cast<const uint16_t *>(row), valid);
-    }
-    else
-    {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-            const uint32_t lo = k + 2 * i < cols ? __ldg(src + 2 * i) : 0u, hi = k + 2 * i + 1 < cols ? __ldg(src + 2 * i + 1) : 0u;
-            w[i]              = lo | (hi << 16);
-        }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-    }
+    const int valid = min(max(cols - k, 0) * 2, 16);
+    copy16(dst, valid > 0 ? row + static_cast<int64_t>(k) * 2 : row, valid);
 }
+// How rows of x and A start: at multiples of 16 bytes, of 4 (and K is even), or anywhere.
+enum RowsIn
+{
+    kUnits16,
+    kWords,
+    kAnywhere
+};
 
 // ---- first launch: v = x . A^T -------------------------------------------------------------------------------
 // A ring of stages of 64 columns of K: up to 64 (32) tokens and all ranks, rows of 128 bytes whose 16-byte units are exchanged by row, so
@@ -239,7 +234,7 @@ __device__ __forceinline__ int v_place(int r)
     return (r & ~15) + ((r >> 1) & 6) + ((r & 2) << 2) + (r & 1);
 }
 
-template <typename T, int kRank, bool kVec>
+template <typename T, int kRank, int kIn>
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p)
 {
     using S = Shrink<kRank>;
@@ -263,69 +258,13 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
     const uint8_t *x = p.x + static_cast<int64_t>(t.first) * p.ld_x;
     const uint8_t *a = p.a + static_cast<int64_t>(t.adapter) * p.max_rank * p.ld_a;
     const uint32_t s_base = smem_u32(share);
-    // What a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows.  Rows behind the last are zeros,
-    // written once.
-    constexpr int  kCopies = (S::kTile + kRank + kThreads / 8 - 1) / (kThreads / 8);
-    const int      c8      = (static_cast<int>(threadIdx.x) & 7) * 8;
-    const uint8_t *from[kCopies]; // nullptr: nothing to copy
-    uint32_t       to[kCopies];
-#pragma unroll
-    for (int j = 0; j < kCopies; ++j)
-    {
-        const int  i = (static_cast<int>(threadIdx.x) >> 3) + j * (kThreads / 8), row = i < x_rows ? i : i - x_rows;
-        const bool is_x = i < x_rows;
-        from[j] = is_x ? (row < t.count ? x + row * p.ld_x : nullptr) : (row < t.rank ? a + row * p.ld_a : nullptr);
-        to[j]   = s_base + static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4));
-        if (from[j] == nullptr && row < (is_x ? x_rows : a_rows))
-        {
-            for (int s = 0; s < S::kStages; ++s) store_zeros(to[j] + static_cast<uint32_t>(s) * S::kStage);
-        }
-    }
-    int      loading = 0, load_k = first * 64 + c8; // the next block to load; its first column of this thread
-    uint32_t load_at = 0;                           // its stage
-    auto     load    = [&]() {
-        if (loading < n_blocks)
-        {
-            if (kVec && load_k + 64 - c8 <= p.K)
-            {
-#pragma unroll
-                for (int j = 0; j < kCopies; ++j)
-                {
-                    if (from[j] != nullptr) copy16(to[j] + load_at, from[j] + static_cast<int64_t>(load_k) * 2, 16);
-                }
-            }
-            else
-            {
-#pragma unroll
-                for (int j = 0; j < kCopies; ++j)
-                {
-                    if (from[j] != nullptr) stage_eight<kVec>(to[j] + load_at, from[j], load_k, p.K);
-                }
-            }
-            load_k += 64;
-            ++loading;
-            load_at = load_at + S::kStage == S::kStages * S::kStage ? 0u : load_at + S::kStage;
-        }
-        copy_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < S::kStages - 2; ++i) load();
     float     acc[S::kMt][kNt][4] = {};
     const int step = halves == 2 ? sub : sub & 3; // 16 columns of a stage
     // rows 16 m + lane % 16 of x, rows 8 n + .. of A: their numbers modulo 8, and so the places of their units, do not depend on m and n
     const uint32_t x_at = s_base + static_cast<uint32_t>((half * S::kRows + (lane & 15)) * 128 + (((2 * step + (lane >> 4)) ^ (lane & 7)) << 4));
     const uint32_t a_at = s_base + static_cast<uint32_t>((S::kTile + (lane & 7) + ((lane >> 4) << 3)) * 128 + (((2 * step + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-    uint32_t       st = 0;
-    for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
-    {
-        if ((i & 1) == 0) // two stages at a time
-        {
-            copy_wait<S::kStages - 4>();
-            __syncthreads();
-            load(); // to the stages that all warps have left
-            load();
-        }
-        if (halves == 1 && (i & 1) != (sub >> 2)) continue;
+    auto           multiply = [&](int i, uint32_t st) { // block i, in the stage at st
+        if (halves == 1 && (i & 1) != (sub >> 2)) return;
         uint32_t xv[S::kMt][4];
 #pragma unroll
         for (int m = 0; m < S::kMt; ++m)
@@ -349,6 +288,107 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
                     }
                 }
             }
+        }
+    };
+    if constexpr (kIn == kUnits16)
+    {
+        // What a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows.  Rows behind the last are
+        // zeros, written once.
+        constexpr int  kCopies = (S::kTile + kRank + kThreads / 8 - 1) / (kThreads / 8);
+        const int      c8      = (static_cast<int>(threadIdx.x) & 7) * 8;
+        const uint8_t *from[kCopies]; // nullptr: nothing to copy
+        uint32_t       to[kCopies];
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j)
+        {
+            const int  i = (static_cast<int>(threadIdx.x) >> 3) + j * (kThreads / 8), row = i < x_rows ? i : i - x_rows;
+            const bool is_x = i < x_rows;
+            from[j] = is_x ? (row < t.count ? x + row * p.ld_x : nullptr) : (row < t.rank ? a + row * p.ld_a : nullptr);
+            to[j]   = s_base + static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4));
+            if (from[j] == nullptr && row < (is_x ? x_rows : a_rows))
+            {
+                for (int s = 0; s < S::kStages; ++s) store_zeros(to[j] + static_cast<uint32_t>(s) * S::kStage);
+            }
+        }
+        int      loading = 0, load_k = first * 64 + c8; // the next block to load; its first column of this thread
+        uint32_t load_at = 0, st = 0;                   // its stage; that of the block worked on
+        auto     load    = [&]() {
+            if (loading < n_blocks)
+            {
+                const bool whole = load_k + 64 - c8 <= p.K;
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j)
+                {
+                    if (from[j] == nullptr) continue;
+                    if (whole) copy16(to[j] + load_at, from[j] + static_cast<int64_t>(load_k) * 2, 16);
+                    else stage_eight(to[j] + load_at, from[j], load_k, p.K);
+                }
+                load_k += 64;
+                ++loading;
+                load_at = load_at + S::kStage == S::kStages * S::kStage ? 0u : load_at + S::kStage;
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < S::kStages - 2; ++i) load();
+        for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
+        {
+            if ((i & 1) == 0) // two stages at a time
+            {
+                copy_wait<S::kStages - 4>();
+                __syncthreads();
+                load(); // to the stages that all warps have left
+                load();
+            }
+            multiply(i, st);
+        }
+    }
+    else
+    {
+        // Rows that are not 16-byte aligned: a warp takes a row, a lane two of its columns.  A block passes through registers, asked for
+        // before the one ahead of it is multiplied.  (Nothing here may use a value between the loads: each would then wait for its own.)
+        constexpr int  kEach = (S::kTile + kRank) / kWarps;
+        constexpr bool kWord = kIn == kWords;
+        uint32_t       low[kEach], high[kWord ? 1 : kEach];
+        auto           fetch = [&](int block) {
+            const int k = (first + block) * 64 + 2 * lane, k0 = min(k, kWord ? p.K - 2 : p.K - 1), k1 = min(k + 1, p.K - 1);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+            {
+                const int i = warp + j * kWarps, row = i < S::kTile ? i : i - S::kTile; // (whole groups of eight rows lie before A's)
+                if (row < (i < S::kTile ? t.count : t.rank))
+                {
+                    const uint8_t *src = i < S::kTile ? x + row * p.ld_x : a + row * p.ld_a;
+                    if constexpr (kWord) low[j] = __ldg(reinterpret_cast<const uint32_t *>(src + static_cast<int64_t>(k0) * 2));
+                    else
+                    {
+                        low[j]  = __ldg(reinterpret_cast<const uint16_t *>(src) + k0);
+                        high[j] = __ldg(reinterpret_cast<const uint16_t *>(src) + k1);
+                    }
+                }
+            }
+        };
+        fetch(0);
+        for (int i = 0; i < n_blocks; ++i)
+        {
+            const uint32_t st = (i & 1) != 0 ? S::kStage : 0u;
+            const int      k  = (first + i) * 64 + 2 * lane;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+            {
+                const int at = warp + j * kWarps, row = at < S::kTile ? at : at - S::kTile;
+                uint32_t  w = 0; // rows behind the last and columns behind K: zeros
+                if (row < (at < S::kTile ? t.count : t.rank))
+                {
+                    if constexpr (kWord) w = k < p.K ? low[j] : 0u;
+                    else w = (k < p.K ? low[j] : 0u) | (k + 1 < p.K ? high[j] << 16 : 0u);
+                }
+                if (row < (at < S::kTile ? x_rows : a_rows))
+                    store_word(s_base + st + static_cast<uint32_t>(at * 128 + (((lane >> 2) ^ (at & 7)) << 4) + (lane & 3) * 4), w);
+            }
+            __syncthreads(); // (the stage of the block before is the other one)
+            if (i + 1 < n_blocks) fetch(i + 1);
+            multiply(i, st);
         }
     }
     copy_wait<0>();
@@ -578,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     uint32_t       ahead_slot = 0;
     const uint8_t *ahead_src  = nullptr;
     const int64_t  copy_step  = kStep * p.ld_base;
+    TD             held[kVec ? 1 : 16]; // rows that start anywhere: the next unit's values of this lane's channel, on their way
     auto           load_unit  = [&]() {
         if (ahead_units == 0)
         {
@@ -585,10 +626,10 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
             if (ahead < items)
             {
                 const Tile &t  = list[ahead].tile;
-                const int   ch = list[ahead].n + copy_ch;
+                const int   ch = list[ahead].n + (kVec ? copy_ch : warp_n + lane), row = kVec ? copy_row : 0;
                 ahead_units    = (t.count + 15) >> 4;
-                ahead_rows     = ch < p.N ? t.count - copy_row : 0; // N is a multiple of 8
-                ahead_src      = p.base + static_cast<int64_t>(t.first + copy_row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
+                ahead_rows     = ch < p.N ? t.count - row : 0; // pieces lie before the last channel or behind it
+                ahead_src      = p.base + static_cast<int64_t>(t.first + row) * p.ld_base + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD));
                 ++ahead;
             }
         }
@@ -600,6 +641,15 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
                 for (int j = 0; j < 16 / kStep; ++j, ahead_src += copy_step)
                 {
                     if (j * kStep < ahead_rows) copy16(copy_to + ahead_slot + j * kStep * E::kRow, ahead_src, 16); // rows behind the last: never stored
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 16; ++j, ahead_src += p.ld_base)
+                {
+                    held[j] = from_float<TD>(0.f);
+                    if (j < ahead_rows) held[j] = __ldcg(reinterpret_cast<const TD *>(ahead_src));
                 }
             }
             ahead_rows -= 16;
@@ -626,7 +676,13 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
         }
     };
 #pragma unroll
-    for (int u = 0; u < E::kSlots; ++u) load_unit();
+    for (int u = 0; u < (kVec ? E::kSlots : 1); ++u) load_unit();
+    // Rows that start anywhere pass through one slot, in and out: a lane's channel of all rows on the one side, its pieces on the other.
+    TD *const column = reinterpret_cast<TD *>(smem + E::kOffBase + warp * E::kSlots * 16 * E::kRow);
+    auto      place  = [&](int row) {
+        const int at = lane * static_cast<int>(sizeof(TD)), unit = at >> 4;
+        return (row * E::kRow + ((kUnit == 8 ? unit ^ ((row & 1) << 2) : unit) << 4) + (at & 15)) / static_cast<int>(sizeof(TD));
+    };
     uint2 b[4][E::kSteps], next[E::kAhead ? 4 : 1][E::kSteps];
     if constexpr (E::kAhead) load_b<TD>(p, list[0].tile, list[0].n + warp_n, lane, next);
     griddep_wait();
@@ -673,40 +729,30 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
         const int64_t  low_row = 8 * p.ld_dst;
         for (int m = 0; m < t.count; m += 16, dst_row += 2 * low_row, v_row += 16 * E::kPitch)
         {
-            copy_wait<E::kSlots - 1>();
+            if constexpr (kVec) copy_wait<E::kSlots - 1>();
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) column[place(j)] = held[j];
+            }
             __syncwarp();
             float base[2][8];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
-                const int row = h * 8 + g;
-                if constexpr (kVec)
+                TD e[8];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i)
                 {
-                    TD e[8];
-#pragma unroll
-                    for (int i = 0; i < kPieces; ++i)
-                    {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(piece[i] + slot + h * 8 * E::kRow);
-                        memcpy(e + i * kPer, &v, 16);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) base[h][i] = to_float(e[i]);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(piece[i] + slot + h * 8 * E::kRow);
+                    memcpy(e + i * kPer, &v, 16);
                 }
-                else
-                {
-                    const TD *src = reinterpret_cast<const TD *>(p.base + static_cast<int64_t>(t.first + m + row) * p.ld_base);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                    {
-                        const int ch = n + piece_channel<TD>(i / kPer, c) + i % kPer;
-                        base[h][i]   = 0.f;
-                        if (m + row < t.count && ch < p.N) base[h][i] = to_float(__ldcg(src + ch));
-                    }
-                }
+                for (int i = 0; i < 8; ++i) base[h][i] = to_float(e[i]);
             }
             __syncwarp();
             load_unit(); // to the slot that the warp has read
-            slot = slot == (E::kSlots - 1) * 16 * E::kRow ? 0 : slot + 16 * E::kRow;
+            if constexpr (kVec) slot = slot == (E::kSlots - 1) * 16 * E::kRow ? 0 : slot + 16 * E::kRow;
             if (t.adapter >= 0)
             {
                 float acc[4][4];
@@ -740,32 +786,39 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
-                if (m + h * 8 + g < t.count)
+                TD  e[8];
+                TD *dst = reinterpret_cast<TD *>(h == 0 ? dst_row : dst_row + low_row);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = from_float<TD>(base[h][i]);
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i)
                 {
-                    TD *dst = reinterpret_cast<TD *>(h == 0 ? dst_row : dst_row + low_row);
-                    TD  e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = from_float<TD>(base[h][i]);
-#pragma unroll
-                    for (int i = 0; i < kPieces; ++i)
+                    uint4 v;
+                    memcpy(&v, e + i * kPer, 16);
+                    if constexpr (kVec)
                     {
                         const int ch = piece_channel<TD>(i, c);
-                        if constexpr (kVec)
-                        {
-                            uint4 v;
-                            memcpy(&v, e + i * kPer, 16);
-                            if (n + ch < p.N) *reinterpret_cast<uint4 *>(dst + ch) = v;
-                        }
-                        else
-                        {
-#pragma unroll
-                            for (int k = 0; k < kPer; ++k)
-                            {
-                                if (n + ch + k < p.N) dst[ch + k] = e[i * kPer + k];
-                            }
-                        }
+                        if (m + h * 8 + g < t.count && n + ch < p.N) *reinterpret_cast<uint4 *>(dst + ch) = v;
+                    }
+                    else
+                    {
+                        *reinterpret_cast<uint4 *>(const_cast<uint8_t *>(piece[i]) + h * 8 * E::kRow) = v;
                     }
                 }
+            }
+            if constexpr (!kVec)
+            {
+                __syncwarp();
+                TD *dst = reinterpret_cast<TD *>(dst_row - g * p.ld_dst) + lane;
+                if (n + lane < p.N)
+                {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                    {
+                        if (m + j < t.count) *reinterpret_cast<TD *>(reinterpret_cast<uint8_t *>(dst) + j * p.ld_dst) = column[place(j)];
+                    }
+                }
+                __syncwarp();
             }
         }
     }
@@ -791,11 +844,11 @@ int64_t most_tiles(const cugl_lora_desc &d) // of a request, all but the last ar
     return (d.tokens - some) / tile + some;
 }
 
-template <typename T, int kRank, bool kVec>
+template <typename T, int kRank, int kIn>
 cugl_status launch_shrink(cugl_context *ctx, const LoraParams &p, int64_t tiles)
 {
     using S                          = Shrink<kRank>;
-    auto                     kernel  = lora_shrink_kernel<T, kRank, kVec>;
+    auto                     kernel  = lora_shrink_kernel<T, kRank, kIn>;
     static std::atomic<bool> set[64] = {};
     if (!set[ctx->device & 63].load(std::memory_order_acquire))
     {
@@ -826,20 +879,22 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
     return CUGL_SUCCESS;
 }
 template <typename T, typename TD, int kRank>
-cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, bool vec_in, bool vec_out)
+cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int rows_in, bool vec_out)
 {
-    CUGL_TRY((vec_in ? launch_shrink<T, kRank, true>(ctx, p, tiles) : launch_shrink<T, kRank, false>(ctx, p, tiles)));
+    CUGL_TRY((rows_in == kUnits16 ? launch_shrink<T, kRank, kUnits16>(ctx, p, tiles)
+              : rows_in == kWords ? launch_shrink<T, kRank, kWords>(ctx, p, tiles)
+                                  : launch_shrink<T, kRank, kAnywhere>(ctx, p, tiles)));
     return vec_out ? launch_expand<T, TD, kRank, true>(ctx, p, tiles) : launch_expand<T, TD, kRank, false>(ctx, p, tiles);
 }
 template <typename T, typename TD>
-cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, bool vec_in, bool vec_out)
+cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int rows_in, bool vec_out)
 {
     switch (padded_rank(p.max_rank))
     {
-        case 16: return launch_lora<T, TD, 16>(ctx, p, tiles, vec_in, vec_out);
-        case 32: return launch_lora<T, TD, 32>(ctx, p, tiles, vec_in, vec_out);
-        case 64: return launch_lora<T, TD, 64>(ctx, p, tiles, vec_in, vec_out);
-        default: return launch_lora<T, TD, 128>(ctx, p, tiles, vec_in, vec_out);
+        case 16: return launch_lora<T, TD, 16>(ctx, p, tiles, rows_in, vec_out);
+        case 32: return launch_lora<T, TD, 32>(ctx, p, tiles, rows_in, vec_out);
+        case 64: return launch_lora<T, TD, 64>(ctx, p, tiles, rows_in, vec_out);
+        default: return launch_lora<T, TD, 128>(ctx, p, tiles, rows_in, vec_out);
     }
 }
 
@@ -942,15 +997,16 @@ extern "C"
         p.tile       = tile_tokens(desc->max_rank);
         p.v          = static_cast<uint16_t *>(d_workspace);
         auto       even = [](const void *q, int64_t ld) { return ((reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ld)) & 15) == 0; };
-        const bool vec_in  = even(d_x, desc->ld_x) && even(d_a, desc->ld_a);
+        const bool words = ((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_a) | static_cast<uintptr_t>(desc->ld_x) | static_cast<uintptr_t>(desc->ld_a)) & 3) == 0;
+        const int  rows_in = even(d_x, desc->ld_x) && even(d_a, desc->ld_a) ? kUnits16 : words && desc->K % 2 == 0 ? kWords : kAnywhere;
         const bool vec_out = even(d_base, desc->ld_base) && even(d_dst, desc->ld_dst) && desc->N % 8 == 0;
         const int64_t tiles = most_tiles(*desc);
         p.tiles             = static_cast<int>(tiles);
         if (desc->dtype == CUGL_F16)
         {
-            return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, vec_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, vec_in, vec_out);
+            return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, rows_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, rows_in, vec_out);
         }
-        return desc->dst_dtype == CUGL_F32 ? launch_lora<__nv_bfloat16, float>(ctx, p, tiles, vec_in, vec_out)
-                                           : launch_lora<__nv_bfloat16, __nv_bfloat16>(ctx, p, tiles, vec_in, vec_out);
+        return desc->dst_dtype == CUGL_F32 ? launch_lora<__nv_bfloat16, float>(ctx, p, tiles, rows_in, vec_out)
+                                           : launch_lora<__nv_bfloat16, __nv_bfloat16>(ctx, p, tiles, rows_in, vec_out);
     }
 }

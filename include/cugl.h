@@ -669,7 +669,7 @@ CUGL_API cugl_status cugl_moe_route_validate(const cugl_moe_route_desc *desc, co
 /* Device bytes a call needs (0: bad descriptor).  They hold nothing between calls; calls that overlap on the GPU, and captured graphs
  * that are replayed at the same time, need one each. */
 CUGL_API size_t      cugl_moe_route_workspace_bytes(const cugl_moe_route_desc *desc);
-/* One launch for up to 128 tokens, else two.  d_workspace: 16-byte aligned; groups: 8-byte aligned.  tokens == 0: groups of no rows. */
+/* One launch for up to 32 tokens, else two.  d_workspace: 16-byte aligned; groups: 8-byte aligned.  tokens == 0: groups of no rows. */
 CUGL_API cugl_status cugl_moe_route(cugl_context *ctx, const cugl_moe_route_desc *desc, const void *d_logits, int32_t *d_ids,
                                     float *d_weights, int32_t *d_slots, int32_t *d_groups, void *d_workspace,
                                     size_t workspace_bytes);
