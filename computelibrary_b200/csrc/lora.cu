@@ -6,9 +6,9 @@
 // CTA.  Which tiles there are is known on the device only (the requests' lengths): every CTA counts them (a scan over the requests)
 // and takes the one with its number; the grid is the most that there can be.
 //
-// What bounds it: bytes.  x, base and dst pass once, the adapters once per tile of tokens; with ranks up to 128 the products are short
-// work (4096 tokens, 4096 -> 4096, rank 64: 2 x 2.1 GFLOP beside 170 MB).  Hence mma.sync, whose accumulators are the registers that
-// base is added to: nothing of a matrix unit's rate is missing, and no operand waits in shared memory.
+// What bounds it: bytes.  x, base and dst pass once, the adapters once per tile of tokens.  The first product is one for tcgen05.mma (K is
+// long, its sums few); the second has K of at most 128 ranks, and all the rest of its time goes to base and dst, hence mma.sync, whose
+// accumulators are the registers that base is added to.
 //
 // Fragments.  Sums do not care in which order their terms come, as long as both operands agree: a lane of the second launch takes 4
 // consecutive ranks as the two pairs that a step of the matrix instruction wants from it.  Channels likewise: the four 8-column tiles
@@ -17,11 +17,9 @@
 // v is kept as two 16-bit parts, v = high + low (three where bf16 adapters add to 32-bit results): 16 (bf16) or 22 (f16) bits of it
 // count, 24 with three parts, so rounding v costs less than rounding the result.  f16 parts would leave that type's range: a token's
 // v is first divided by a power of two that brings its largest rank into [1, 2).
-#include "mx.cuh"
-#include "sm100.cuh"
+#include "mx_mma.cuh"
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -44,6 +42,10 @@ struct LoraParams
     int64_t        ld_x, ld_a, ld_b, ld_base, ld_dst; // bytes
     int            tokens, requests, n_adapters, max_rank, K, N, parts, tile;
     int            tiles; // at most
+    uint32_t       idesc; // of no columns
+    int32_t       *status;
+    long long      spin_limit;
+    int            withhold; // see cugl_context_withhold_copy_once
 };
 
 // ---- which tokens a tile holds -------------------------------------------------------------------------------
@@ -176,10 +178,6 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void store_zeros(uint32_t dst)
-{
-    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
-}
 __device__ __forceinline__ void store_word(uint32_t dst, uint32_t v)
 {
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
@@ -190,12 +188,6 @@ __device__ __forceinline__ int share_begin(int total, int i, int n)
     const int each = total / n;
     return i * each + min(i, total - each * n);
 }
-// eight 16-bit elements of a 16-byte aligned row from column k on to shared memory, zeros behind `cols`
-__device__ __forceinline__ void stage_eight(uint32_t dst, const uint8_t *row, int k, int cols)
-{
-    const int valid = min(max(cols - k, 0) * 2, 16);
-    copy16(dst, valid > 0 ? row + static_cast<int64_t>(k) * 2 : row, valid);
-}
 // How rows of x and A start: at multiples of 16 bytes, of 4 (and K is even), or anywhere.
 enum RowsIn
 {
@@ -205,20 +197,17 @@ enum RowsIn
 };
 
 // ---- first launch: v = x . A^T -------------------------------------------------------------------------------
-// A ring of stages of 64 columns of K: up to 64 (32) tokens and all ranks, rows of 128 bytes whose 16-byte units are exchanged by row, so
-// that ldmatrix reads eight rows from different banks.  A warp takes 16 columns of a stage and 32 (16) tokens; tiles of few tokens
-// leave every other stage to the other half of the warps.
+// A CTA takes a share of K of a tile, in blocks of 64 columns; rows of 128 bytes whose 16-byte units are exchanged by row.
 template <int kRank>
 struct Shrink
 {
-    static constexpr int kMt     = kRank == 128 ? 1 : 2; // 16-row tiles of a warp
-    static constexpr int kRows   = 16 * kMt;
-    static constexpr int kTile   = 2 * kRows;
-    static constexpr int kStages = kRank == 128 ? 4 : kRank == 64 ? 6 : 8; // as many pairs as leave room for two CTAs on an SM
-    static constexpr int kStage  = (kTile + kRank) * 128; // bytes
-    static constexpr int kPitch  = kRank + 8;             // floats: rows in different banks
-    static constexpr int kSmem   = kStages * kStage;
-    static_assert(kWarps * kRows * kPitch * 4 <= kSmem, "the warps' sums fit where the stages were");
+    static constexpr int kMt    = kRank == 128 ? 1 : 2; // 16-row tiles of a warp
+    static constexpr int kRows  = 16 * kMt;
+    static constexpr int kTile  = 2 * kRows;
+    static constexpr int kStage = (kTile + kRank) * 128; // bytes; two of them
+    static constexpr int kPitch = kRank + 8;             // floats: rows in different banks
+    static constexpr int kSums  = kWarps * kRows * kPitch * 4;
+    static constexpr int kSmem  = 2 * kStage > kSums ? 2 * kStage : kSums;
 };
 __device__ __forceinline__ float load_cluster(uint32_t addr)
 {
@@ -234,6 +223,248 @@ __device__ __forceinline__ int v_place(int r)
     return (r & ~15) + ((r >> 1) & 6) + ((r & 2) << 2) + (r & 1);
 }
 
+// The CTAs' sums of x . A^T ([token][rank] in the shared memory of each), added up in the order of the CTAs, to the parts of v: a warp per
+// token.  By all threads of the cluster.
+template <typename T, int kRank>
+__device__ __forceinline__ void finish_v(const LoraParams &p, const Tile &t, const float *share, int pitch, int rank, int ranks)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+    for (int tok = rank * kWarps + warp; tok < t.count; tok += ranks * kWarps)
+    {
+        constexpr int  kPer = (kRank + 31) / 32;
+        const uint32_t at   = smem_u32(share + tok * pitch);
+        float          v[kPer], parts[kPer][kMaxSplit];
+        float          top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) // all of them under way before the first is added
+        {
+            const int r = min(i * 32 + lane, kRank - 1);
+#pragma unroll
+            for (int q = 0; q < kMaxSplit; ++q)
+            {
+                parts[i][q] = 0.f;
+                if (q < ranks) parts[i][q] = load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+        {
+            v[i] = parts[i][0];
+#pragma unroll
+            for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
+            if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
+        }
+        float factor = __ldg(p.scales + t.adapter);
+        float mul    = 1.f;
+        if constexpr (std::is_same<T, __half>::value)
+        {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+            if (e > -126 && e < 127) // zero and subnormal sums stay as they are
+            {
+                mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+        }
+        uint16_t *out = p.v + static_cast<int64_t>(t.first + tok) * (kRank + 8);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+        {
+            const int r = i * 32 + lane;
+            if (r < kRank)
+            {
+                float rest = v[i] * mul;
+                for (int q = 0; q < p.parts; ++q)
+                {
+                    const T part = from_float<T>(rest);
+                    uint16_t bits;
+                    memcpy(&bits, &part, 2);
+                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + v_place(r)] = bits;
+                    const float f = to_float(part);
+                    rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
+                }
+            }
+        }
+        if (lane == 0) *reinterpret_cast<float *>(out + kRank) = factor;
+    }
+    // Nobody leaves while others read its sums: they have what they read.  (A releasing arrival would wait for the stores of v.)
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- first launch, rows of x and A at multiples of 16 bytes --------------------------------------------------
+// Ranks are the rows of a tcgen05.mma, tokens its columns, blocks of 64 columns of K come by TMA.  A CTA's sums stay in tensor memory
+// until its share of K is done: no adding up of warps, and the stream of blocks from L2 bounds it, where the warps' own matrix
+// instructions took twice as long (prompts of 4096 tokens, K = 4096, ranks up to 64: 20.6 -> 14.2 us under ncu).  Of the 128 rows of an MMA only
+// the adapter's count; the others are whatever shared memory holds behind them.  Rows of x behind the tile belong to other requests:
+// columns that nobody reads.
+template <int kRank>
+struct ShrinkMma
+{
+    static constexpr int kTile   = Shrink<kRank>::kTile;
+    static constexpr int kStages = kRank == 128 ? 4 : kRank == 64 ? 6 : 8;
+    static constexpr int kA      = kRank * 128, kX = kTile * 128, kStage = kA + kX; // bytes
+    static constexpr int kPitch  = kRank + 1;                                       // floats of a token's sums
+    static constexpr int kOffBar = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384); // an MMA reads 16 KB from a stage's start on
+    static constexpr int kSmem   = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
+    static constexpr int kColumns = 64;
+    static_assert(kTile * kPitch * 4 <= kOffBar && kTile <= kColumns, "sums fit where the stages were, and in tensor memory");
+};
+inline uint32_t f16_idesc(bool bf16) // float sums, 128 rows; add columns / 8 << 17
+{
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((128u >> 4) << 24);
+}
+// D[tmem] (+)= sum over 16 elements
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t"
+                 ".reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                 "}"
+                 :
+                 : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+template <typename T, int kRank>
+__global__ void __launch_bounds__(kThreads, 2)
+    lora_shrink_mma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_few,
+                           const __grid_constant__ LoraParams p)
+{
+    using S = ShrinkMma<kRank>;
+    constexpr int STAGES = S::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t       *smem      = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t s_stage   = smem_u32(smem), bar_base = smem_u32(smem + S::kOffBar);
+    auto           full_bar  = [&](int s) { return bar_base + 8u * s; };
+    auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    const uint32_t done_bar  = bar_base + 8u * (2 * STAGES), gone_bar = done_bar + 8;
+    uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + S::kOffBar + (2 * STAGES + 2) * 8);
+    volatile int  *s_abort   = reinterpret_cast<volatile int *>(s_tmem + 1);
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0)
+    {
+        for (int s = 0; s < STAGES; ++s)
+        {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        mbar_init(gone_bar, 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1)
+    {
+        tmem_alloc(smem_u32(s_tmem), S::kColumns);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    griddep_wait();
+    griddep_launch_dependents(); // whatever ran before has completed: the second launch may read it
+    const int  ranks = static_cast<int>(gridDim.x / num_clusters_x()), rank = static_cast<int>(cluster_ctarank());
+    const Tile t     = find_tile(p, static_cast<int>(cluster_id_x()));
+    if (t.count == 0 || t.adapter < 0) // the same for the cluster
+    {
+        if (warp == 1) tmem_dealloc(tmem, S::kColumns);
+        return;
+    }
+    const int blocks = (p.K + 63) / 64; // of 64 columns, shared by the CTAs of the cluster
+    const int first  = share_begin(blocks, rank, ranks), n_blocks = share_begin(blocks, rank + 1, ranks) - first;
+    int       issued = 0; // stages that the producer has filled
+    if (warp == 0)
+    {
+        const bool el  = elect_one(), few = t.count <= 16;
+        const int  a_row = t.adapter * p.max_rank;
+        int        g = 0;
+        for (; g < n_blocks; ++g)
+        {
+            const int s = g % STAGES;
+            if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(g / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit)) break;
+            if (g == p.withhold && blockIdx.x == 0) continue;
+            if (el)
+            {
+                const uint32_t dst = s_stage + s * S::kStage;
+                mbar_expect_tx(full_bar(s), static_cast<uint32_t>(S::kA + (few ? 16 * 128 : S::kX)));
+                tma_load_2d(dst, &tmap_a, (first + g) * 64, a_row, full_bar(s));
+                tma_load_2d(dst + S::kA, few ? &tmap_few : &tmap_x, (first + g) * 64, t.first, full_bar(s));
+            }
+            __syncwarp();
+        }
+        issued = g;
+    }
+    else if (warp == 1)
+    {
+        const bool     el    = elect_one();
+        const uint32_t idesc = p.idesc | (static_cast<uint32_t>((t.count + 15) >> 4) << 18); // columns / 8
+        bool           ok    = true;
+        for (int g = 0; g < n_blocks && ok; ++g)
+        {
+            const int s = g % STAGES;
+            ok = warp_wait(full_bar(s), static_cast<uint32_t>(g / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t a_desc = make_kmajor_sw128_desc(s_stage + s * S::kStage), b_desc = make_kmajor_sw128_desc(s_stage + s * S::kStage + S::kA);
+            if (el)
+            {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16(tmem, a_desc + 2u * k, b_desc + 2u * k, idesc, (g | k) != 0 ? 1u : 0u);
+                umma_commit(empty_bar(s));
+            }
+            __syncwarp();
+        }
+        if (ok && el) umma_commit(done_bar);
+        __syncwarp();
+    }
+    // sums to shared memory, [token][rank]: a lane has a rank, warps 4 .. 7 the upper half of the tokens
+    const bool ok    = warp_wait(done_bar, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
+    float     *share = reinterpret_cast<float *>(smem);
+    const int  r = (warp & 3) * 32 + lane, c0 = (warp >> 2) * 32;
+    __syncthreads(); // every warp's waits are over; the MMAs have read the stages
+    if (ok && *s_abort == 0 && (warp & 3) * 32 < kRank && c0 < t.count)
+    {
+        tc_fence_after();
+        uint32_t v[32];
+        tmem_ld_x32(tmem + c0 + (static_cast<uint32_t>((warp & 3) * 32) << 16), v);
+        tmem_ld_wait();
+        if (r < kRank)
+        {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+            {
+                if (c0 + i < t.count) share[(c0 + i) * S::kPitch + r] = n_blocks > 0 && r < t.rank ? __uint_as_float(v[i]) : 0.f; // behind the adapter's ranks: zeros
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    const bool gone = *s_abort != 0;
+    if (warp == 0 && gone)
+    {
+        drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit);
+    }
+    if (warp == 1)
+    {
+        if (gone) drain_mmas<false>(gone_bar, p.spin_limit);
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kColumns);
+    }
+    if (threadIdx.x == 0 && gone)
+    {
+        atomicCAS(p.status, 0, *s_abort);
+    }
+    finish_v<T, kRank>(p, t, share, S::kPitch, rank, ranks); // (of a CTA that has given up: nothing of use)
+}
+
+// ---- first launch, other rows ----------------------------------------------------------------------------------
+// Rows that are not 16-byte aligned: a warp takes a row, a lane two of its columns.  A block passes through registers, asked for before
+// the one ahead of it is multiplied by the warps' own matrix instructions: a warp takes 16 columns of a block and 32 (16) tokens; tiles of
+// few tokens leave every other block to the other half of the warps.
 template <typename T, int kRank, int kIn>
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p)
 {
@@ -290,108 +521,50 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
             }
         }
     };
-    if constexpr (kIn == kUnits16)
+    // (Nothing may use a value between the loads: each would then wait for its own.)
+    constexpr int  kEach = (S::kTile + kRank) / kWarps;
+    constexpr bool kWord = kIn == kWords;
+    uint32_t       low[kEach], high[kWord ? 1 : kEach];
+    auto           fetch = [&](int block) {
+        const int k = (first + block) * 64 + 2 * lane, k0 = min(k, kWord ? p.K - 2 : p.K - 1), k1 = min(k + 1, p.K - 1);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+        {
+            const int i = warp + j * kWarps, row = i < S::kTile ? i : i - S::kTile; // (whole groups of eight rows lie before A's)
+            if (row < (i < S::kTile ? t.count : t.rank))
+            {
+                const uint8_t *src = i < S::kTile ? x + row * p.ld_x : a + row * p.ld_a;
+                if constexpr (kWord) low[j] = __ldg(reinterpret_cast<const uint32_t *>(src + static_cast<int64_t>(k0) * 2));
+                else
+                {
+                    low[j]  = __ldg(reinterpret_cast<const uint16_t *>(src) + k0);
+                    high[j] = __ldg(reinterpret_cast<const uint16_t *>(src) + k1);
+                }
+            }
+        }
+    };
+    fetch(0);
+    for (int i = 0; i < n_blocks; ++i)
     {
-        // What a thread copies of every stage: eight columns of a row of x or A, of at most kCopies rows.  Rows behind the last are
-        // zeros, written once.
-        constexpr int  kCopies = (S::kTile + kRank + kThreads / 8 - 1) / (kThreads / 8);
-        const int      c8      = (static_cast<int>(threadIdx.x) & 7) * 8;
-        const uint8_t *from[kCopies]; // nullptr: nothing to copy
-        uint32_t       to[kCopies];
+        const uint32_t st = (i & 1) != 0 ? S::kStage : 0u;
+        const int      k  = (first + i) * 64 + 2 * lane;
 #pragma unroll
-        for (int j = 0; j < kCopies; ++j)
+        for (int j = 0; j < kEach; ++j)
         {
-            const int  i = (static_cast<int>(threadIdx.x) >> 3) + j * (kThreads / 8), row = i < x_rows ? i : i - x_rows;
-            const bool is_x = i < x_rows;
-            from[j] = is_x ? (row < t.count ? x + row * p.ld_x : nullptr) : (row < t.rank ? a + row * p.ld_a : nullptr);
-            to[j]   = s_base + static_cast<uint32_t>((is_x ? row : S::kTile + row) * 128 + (((c8 >> 3) ^ (row & 7)) << 4));
-            if (from[j] == nullptr && row < (is_x ? x_rows : a_rows))
+            const int at = warp + j * kWarps, row = at < S::kTile ? at : at - S::kTile;
+            uint32_t  w = 0; // rows behind the last and columns behind K: zeros
+            if (row < (at < S::kTile ? t.count : t.rank))
             {
-                for (int s = 0; s < S::kStages; ++s) store_zeros(to[j] + static_cast<uint32_t>(s) * S::kStage);
+                if constexpr (kWord) w = k < p.K ? low[j] : 0u;
+                else w = (k < p.K ? low[j] : 0u) | (k + 1 < p.K ? high[j] << 16 : 0u);
             }
+            if (row < (at < S::kTile ? x_rows : a_rows))
+                store_word(s_base + st + static_cast<uint32_t>(at * 128 + (((lane >> 2) ^ (at & 7)) << 4) + (lane & 3) * 4), w);
         }
-        int      loading = 0, load_k = first * 64 + c8; // the next block to load; its first column of this thread
-        uint32_t load_at = 0, st = 0;                   // its stage; that of the block worked on
-        auto     load    = [&]() {
-            if (loading < n_blocks)
-            {
-                const bool whole = load_k + 64 - c8 <= p.K;
-#pragma unroll
-                for (int j = 0; j < kCopies; ++j)
-                {
-                    if (from[j] == nullptr) continue;
-                    if (whole) copy16(to[j] + load_at, from[j] + static_cast<int64_t>(load_k) * 2, 16);
-                    else stage_eight(to[j] + load_at, from[j], load_k, p.K);
-                }
-                load_k += 64;
-                ++loading;
-                load_at = load_at + S::kStage == S::kStages * S::kStage ? 0u : load_at + S::kStage;
-            }
-            copy_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < S::kStages - 2; ++i) load();
-        for (int i = 0; i < n_blocks; ++i, st = st + S::kStage == S::kStages * S::kStage ? 0u : st + S::kStage)
-        {
-            if ((i & 1) == 0) // two stages at a time
-            {
-                copy_wait<S::kStages - 4>();
-                __syncthreads();
-                load(); // to the stages that all warps have left
-                load();
-            }
-            multiply(i, st);
-        }
+        __syncthreads(); // (the stage of the block before is the other one)
+        if (i + 1 < n_blocks) fetch(i + 1);
+        multiply(i, st);
     }
-    else
-    {
-        // Rows that are not 16-byte aligned: a warp takes a row, a lane two of its columns.  A block passes through registers, asked for
-        // before the one ahead of it is multiplied.  (Nothing here may use a value between the loads: each would then wait for its own.)
-        constexpr int  kEach = (S::kTile + kRank) / kWarps;
-        constexpr bool kWord = kIn == kWords;
-        uint32_t       low[kEach], high[kWord ? 1 : kEach];
-        auto           fetch = [&](int block) {
-            const int k = (first + block) * 64 + 2 * lane, k0 = min(k, kWord ? p.K - 2 : p.K - 1), k1 = min(k + 1, p.K - 1);
-#pragma unroll
-            for (int j = 0; j < kEach; ++j)
-            {
-                const int i = warp + j * kWarps, row = i < S::kTile ? i : i - S::kTile; // (whole groups of eight rows lie before A's)
-                if (row < (i < S::kTile ? t.count : t.rank))
-                {
-                    const uint8_t *src = i < S::kTile ? x + row * p.ld_x : a + row * p.ld_a;
-                    if constexpr (kWord) low[j] = __ldg(reinterpret_cast<const uint32_t *>(src + static_cast<int64_t>(k0) * 2));
-                    else
-                    {
-                        low[j]  = __ldg(reinterpret_cast<const uint16_t *>(src) + k0);
-                        high[j] = __ldg(reinterpret_cast<const uint16_t *>(src) + k1);
-                    }
-                }
-            }
-        };
-        fetch(0);
-        for (int i = 0; i < n_blocks; ++i)
-        {
-            const uint32_t st = (i & 1) != 0 ? S::kStage : 0u;
-            const int      k  = (first + i) * 64 + 2 * lane;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j)
-            {
-                const int at = warp + j * kWarps, row = at < S::kTile ? at : at - S::kTile;
-                uint32_t  w = 0; // rows behind the last and columns behind K: zeros
-                if (row < (at < S::kTile ? t.count : t.rank))
-                {
-                    if constexpr (kWord) w = k < p.K ? low[j] : 0u;
-                    else w = (k < p.K ? low[j] : 0u) | (k + 1 < p.K ? high[j] << 16 : 0u);
-                }
-                if (row < (at < S::kTile ? x_rows : a_rows))
-                    store_word(s_base + st + static_cast<uint32_t>(at * 128 + (((lane >> 2) ^ (at & 7)) << 4) + (lane & 3) * 4), w);
-            }
-            __syncthreads(); // (the stage of the block before is the other one)
-            if (i + 1 < n_blocks) fetch(i + 1);
-            multiply(i, st);
-        }
-    }
-    copy_wait<0>();
     __syncthreads(); // the stages are free
     float *mine = share + warp * S::kRows * S::kPitch;
 #pragma unroll
@@ -420,69 +593,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
         for (int s = 1; s < kWarps; ++s) sum += part[s];
         *at = sum;
     }
-    if (ranks > 1) cluster_sync();
-    else __syncthreads();
-    // the CTAs' sums, in their order: a warp per token
-    for (int tok = rank * kWarps + warp; tok < t.count; tok += ranks * kWarps)
-    {
-        constexpr int  kPer = (kRank + 31) / 32;
-        const uint32_t at   = smem_u32(share + tok * S::kPitch);
-        float          v[kPer], parts[kPer][kMaxSplit];
-        float          top = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) // all of them under way before the first is added
-        {
-            const int r = min(i * 32 + lane, kRank - 1);
-#pragma unroll
-            for (int q = 0; q < kMaxSplit; ++q)
-            {
-                parts[i][q] = 0.f;
-                if (q < ranks) parts[i][q] = load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-        {
-            v[i] = parts[i][0];
-#pragma unroll
-            for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
-            if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
-        }
-        float factor = __ldg(p.scales + t.adapter);
-        float mul    = 1.f;
-        if constexpr (std::is_same<T, __half>::value)
-        {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-            if (e > -126 && e < 127) // zero and subnormal sums stay as they are
-            {
-                mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            }
-        }
-        uint16_t *out = p.v + static_cast<int64_t>(t.first + tok) * (kRank + 8);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-        {
-            const int r = i * 32 + lane;
-            if (r < kRank)
-            {
-                float rest = v[i] * mul;
-                for (int q = 0; q < p.parts; ++q)
-                {
-                    const T part = from_float<T>(rest);
-                    uint16_t bits;
-                    memcpy(&bits, &part, 2);
-                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + v_place(r)] = bits;
-                    const float f = to_float(part);
-                    rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
-                }
-            }
-        }
-        if (lane == 0) *reinterpret_cast<float *>(out + kRank) = factor;
-    }
-    if (ranks > 1) cluster_sync(); // nobody leaves while others read its sums
+    finish_v<T, kRank>(p, t, share, S::kPitch, rank, ranks);
 }
 
 // ---- second launch: dst = base + factor * v . B^T --------------------------------------------------------------
@@ -844,20 +955,49 @@ int64_t most_tiles(const cugl_lora_desc &d) // of a request, all but the last ar
     return (d.tokens - some) / tile + some;
 }
 
+// CTAs that share a tile's K: as many as run at once, two to an SM, with four blocks of 64 columns each at least
+int shrink_split(const cugl_context *ctx, const LoraParams &p, int64_t tiles)
+{
+    int split = 1;
+    while (split < kMaxSplit && tiles * split * 2 <= 2 * ctx->sm_count && p.K >= 2 * split * 128) split *= 2;
+    return split;
+}
+// rows of 16-bit elements; box = 64 columns x box_rows in the 128-byte swizzle, what lies outside reads as 0
+bool encode_rows_map(CUtensorMap *map, const void *base, int64_t rows, int cols, int64_t ld, int box_rows)
+{
+    EncodeTiledFn    fn         = get_encode_fn();
+    const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2]     = {64, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2]    = {1, 1};
+    return fn != nullptr && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+template <typename T, int kRank>
+cugl_status launch_shrink_mma(cugl_context *ctx, const LoraParams &p, int64_t tiles)
+{
+    using S = ShrinkMma<kRank>;
+    CUtensorMap map_a, map_x, map_few;
+    if (!encode_rows_map(&map_a, p.a, static_cast<int64_t>(p.n_adapters) * p.max_rank, p.K, p.ld_a, kRank) || !encode_rows_map(&map_x, p.x, p.tokens, p.K, p.ld_x, S::kTile) ||
+        !encode_rows_map(&map_few, p.x, p.tokens, p.K, p.ld_x, 16))
+    {
+        return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for x or A");
+    }
+    auto                     kernel  = lora_shrink_mma_kernel<T, kRank>;
+    static std::atomic<bool> set[64] = {};
+    CUGL_TRY(allow_smem(ctx, kernel, S::kSmem, set));
+    const int split = shrink_split(ctx, p, tiles);
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, map_a, map_x, map_few, p));
+    return CUGL_SUCCESS;
+}
 template <typename T, int kRank, int kIn>
 cugl_status launch_shrink(cugl_context *ctx, const LoraParams &p, int64_t tiles)
 {
     using S                          = Shrink<kRank>;
     auto                     kernel  = lora_shrink_kernel<T, kRank, kIn>;
     static std::atomic<bool> set[64] = {};
-    if (!set[ctx->device & 63].load(std::memory_order_acquire))
-    {
-        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-        set[ctx->device & 63].store(true, std::memory_order_release);
-    }
-    // CTAs that share a tile's K: as many as run at once, two to an SM, with two stages each at least
-    int split = 1;
-    while (split < kMaxSplit && tiles * split * 2 <= 2 * ctx->sm_count && p.K >= 2 * split * 128) split *= 2;
+    CUGL_TRY(allow_smem(ctx, kernel, S::kSmem, set));
+    const int split = shrink_split(ctx, p, tiles);
     CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, p));
     return CUGL_SUCCESS;
 }
@@ -867,11 +1007,7 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
     using E                          = Expand<T, TD, kRank>;
     auto                     kernel  = lora_expand_kernel<T, TD, kRank, kVec>;
     static std::atomic<bool> set[64] = {};
-    if (!set[ctx->device & 63].load(std::memory_order_acquire))
-    {
-        CUGL_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, E::kSmem));
-        set[ctx->device & 63].store(true, std::memory_order_release);
-    }
+    CUGL_TRY(allow_smem(ctx, kernel, E::kSmem, set));
     // one CTA or two to an SM; more only where there are more items than these list
     const int64_t items = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps) * tiles, most = std::max<int64_t>(E::kCtas * ctx->sm_count, (items + kListed - 1) / kListed);
     const int64_t grid  = items < most ? items : most;
@@ -881,7 +1017,7 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
 template <typename T, typename TD, int kRank>
 cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int rows_in, bool vec_out)
 {
-    CUGL_TRY((rows_in == kUnits16 ? launch_shrink<T, kRank, kUnits16>(ctx, p, tiles)
+    CUGL_TRY((rows_in == kUnits16 ? launch_shrink_mma<T, kRank>(ctx, p, tiles)
               : rows_in == kWords ? launch_shrink<T, kRank, kWords>(ctx, p, tiles)
                                   : launch_shrink<T, kRank, kAnywhere>(ctx, p, tiles)));
     return vec_out ? launch_expand<T, TD, kRank, true>(ctx, p, tiles) : launch_expand<T, TD, kRank, false>(ctx, p, tiles);
@@ -998,10 +1134,16 @@ extern "C"
         p.v          = static_cast<uint16_t *>(d_workspace);
         auto       even = [](const void *q, int64_t ld) { return ((reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ld)) & 15) == 0; };
         const bool words = ((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_a) | static_cast<uintptr_t>(desc->ld_x) | static_cast<uintptr_t>(desc->ld_a)) & 3) == 0;
-        const int  rows_in = even(d_x, desc->ld_x) && even(d_a, desc->ld_a) ? kUnits16 : words && desc->K % 2 == 0 ? kWords : kAnywhere;
+        const bool mapped  = desc->ld_x < (1ll << 40) && desc->ld_a < (1ll << 40) && static_cast<int64_t>(desc->adapters) * desc->max_rank < (1ll << 31);
+        const int  rows_in = even(d_x, desc->ld_x) && even(d_a, desc->ld_a) && mapped ? kUnits16 : words && desc->K % 2 == 0 ? kWords : kAnywhere;
         const bool vec_out = even(d_base, desc->ld_base) && even(d_dst, desc->ld_dst) && desc->N % 8 == 0;
         const int64_t tiles = most_tiles(*desc);
         p.tiles             = static_cast<int>(tiles);
+        p.idesc             = f16_idesc(desc->dtype == CUGL_BF16);
+        p.status            = ctx->d_status;
+        p.spin_limit        = ctx->spin_limit;
+        p.withhold          = ctx->withhold_kb;
+        ctx->withhold_kb    = -1;
         if (desc->dtype == CUGL_F16)
         {
             return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, rows_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, rows_in, vec_out);

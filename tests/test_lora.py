@@ -210,6 +210,47 @@ def test_equal_calls_give_equal_bits(ctx, lengths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,rank,k_block", [([1] * 24, 16, 0), ([1] * 24, 16, 3), ([200, 70], 64, 5), ([200, 70], 128, 2)])
+def test_wait_limit(ctx, lengths, rank, k_block):
+    """Operand copies that never come: the call ends by its wait limit and says so; the next one is as always."""
+    import torch
+    out, args = check(ctx, lengths, [i % 3 for i in range(len(lengths))], rank, 4096, 264, capi.BF16, capi.F32)
+    want = out.clone()
+    ctx.set_wait_limit_us(20000)
+    try:
+        ctx.withhold_copy_once(k_block)
+        ctx.lora(*args)
+        with pytest.raises(capi.CuglError) as e:
+            ctx.sync()
+        assert e.value.status == capi.RUNTIME_ERROR and "wait ran out" in e.value.message
+    finally:
+        ctx.set_wait_limit_us(0)
+    out[:sum(lengths)] = 7
+    ctx.lora(*args)
+    ctx.sync()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,rank", [(10, 16), (64, 32), (64, 64), (32, 128)])
+def test_gives_up_in_flight(ctx, tokens, rank):
+    """A limit far below the time of a tile: the kernel gives up with copies and products under way."""
+    import torch
+    from test_mx_give_up import check as give_up
+    K, N = 2 ** 23, 64
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    x = torch.randint(-8, 8, (tokens, K), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    a = torch.randint(-8, 8, (1, rank, K), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    b = torch.randn((1, N, rank), generator=g, device="cuda").to(torch.bfloat16)
+    base, out = torch.randn((tokens, N), generator=g, device="cuda"), torch.zeros((tokens, N), device="cuda")
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    d = capi.make_lora_desc(tokens, 1, 1, rank, K, N, capi.BF16, capi.F32)
+    ws = torch.zeros(capi.lora_workspace_bytes(d), dtype=torch.uint8, device="cuda")
+    starts, picks, scales = i(0, tokens), i(0), torch.full((1,), 2.0 ** -20, device="cuda")
+    give_up(ctx, lambda: ctx.lora(d, x, starts, picks, None, scales, a, b, base, out, ws), out)
+
+
+@pytest.mark.gpu
 def test_starts_out_of_order(ctx):
     """Requests that overlap, lie outside or end before they begin are cut to the tokens there are; nothing else is written."""
     import torch
