@@ -24,8 +24,6 @@ constexpr int kMmaWarp   = 1;
 constexpr int kFirstEpi  = 2;
 constexpr int kFewEpi      = 8;  // epilogue warps, two per tensor-memory lane quarter
 constexpr int kFewThreads  = 32 * (kFirstEpi + kFewEpi);
-constexpr int kPairEpi     = 16; // four
-constexpr int kPairThreads = 32 * (kFirstEpi + kPairEpi);
 constexpr int kMaxGroups = 512;
 constexpr int kSlab      = 128; // rows at whose multiples groups start
 
@@ -517,13 +515,17 @@ struct PairPlan
     using F                        = MxTraits<kFormat>;
     static constexpr int WEIGHTS   = kSwiglu ? 2 : 1;
     static constexpr int TILE      = kSwiglu ? 128 : 256; // tokens
+    // Epilogue warps, two or four per tensor-memory lane quarter.  us sustained with eight / sixteen, 4096 tokens, top 8 of 64, NVFP4 to BF16:
+    // SwiGLU 2048 -> 768 72.1 / 74.9 (power is what bounds it), 768 -> 2048 52.8 / 51.6.
+    static constexpr int EPI       = kSwiglu ? 8 : 16;
+    static constexpr int THREADS   = 32 * (kFirstEpi + EPI);
     static constexpr int STAGES    = kSwiglu ? 4 : 5;
     static constexpr int T_BYTES   = TILE / 2 * kMxChunkBytes;
     static constexpr int STAGE     = WEIGHTS * kMxWBytes + T_BYTES;
     static constexpr int SF_PARTS  = WEIGHTS + TILE / 128;
     static constexpr int SF_STAGE  = SF_PARTS * F::kChunkScale;
     static constexpr int OFF_OUT   = STAGES * STAGE; // staging: 2 KB per epilogue warp
-    static constexpr int OFF_SF    = OFF_OUT + kPairEpi * kStaging;
+    static constexpr int OFF_SF    = OFF_OUT + EPI * kStaging;
     static constexpr int OFF_BAR   = OFF_SF + STAGES * SF_STAGE;
     static constexpr int OFF_MISC  = OFF_BAR + (2 * STAGES + 4) * 8;
     static constexpr int OFF_SCAN  = OFF_MISC + 16;
@@ -571,7 +573,7 @@ __device__ __forceinline__ void store_staged(const GroupedParams &p, const uint8
 }
 
 template <int kFormat, bool kBulk, bool kSwiglu>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
     mx_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_up, const __grid_constant__ CUtensorMap tmap_a,
                            const __grid_constant__ CUtensorMap tmap_bsf, const __grid_constant__ CUtensorMap tmap_upsf,
                            const __grid_constant__ CUtensorMap tmap_asf, const __grid_constant__ CUtensorMap tmap_out,
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         mbar_init(tfull_bar(0), 1);
         mbar_init(tfull_bar(1), 1);
-        mbar_init(tempty, 2 * kPairEpi);
+        mbar_init(tempty, 2 * P::EPI);
         mbar_init(gone_bar, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -742,9 +744,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     else
     {
-        // Four warps per lane quarter, which take turns with groups of 32 tokens; those in the shared columns are the first two groups.  One
-        // waits for its own instructions most of the time: with eight warps the drain of 128 x 128 SwiGLU results took 11000 clocks, 2.7
-        // times the MMAs of K = 2048 (768 channels, 512 rows a group: 72 us against 50).
+        // Two or four warps per lane quarter, which take turns with groups of 32 tokens; those in the shared columns are the first two groups.
+        constexpr int  kTurns = P::EPI / 4;
         const int      q = warp & 3, turn = (warp - kFirstEpi) >> 2;
         const uint32_t release = map_to_cta(tempty, 0);
         uint8_t       *out     = smem + P::OFF_OUT + (warp - kFirstEpi) * kStaging;
@@ -768,9 +769,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const uint32_t acc = tmem_base + as * (kPairCols - kPairShared) + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
-            for (int i = 0; i < TILE / 128; ++i)
+            for (int i = 0; i < TILE / (32 * kTurns); ++i)
             {
-                const int  group = 4 * i + turn;
+                const int  group = kTurns * i + turn;
                 const int  j     = as == 0 ? (group * 32 + TILE - kPairShared) % TILE : group * 32;
                 const bool any   = j < item.count && n0 < p.channels; // the same for the warp
                 auto       drained = [&]() { // the shared columns have been read
@@ -954,7 +955,7 @@ cugl_status launch_pair(cugl_context *ctx, const GroupedOperands &op, GroupedPar
     CUGL_TRY(allow_smem(ctx, kernel, P::DYN_BYTES, set));
     p.idesc         = mx_idesc(kFormat, 2 * kMxRows, 0);
     const int pairs = ctx->sm_count / 2, grid = 2 * static_cast<int>(items < pairs ? items : pairs);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), kPairThreads, P::DYN_BYTES, 2, 2 * items, map_b, map_up, map_a, map_bsf,
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(grid)), P::THREADS, P::DYN_BYTES, 2, 2 * items, map_b, map_up, map_a, map_bsf,
                                                 map_upsf, map_asf, map_out, p));
     return CUGL_SUCCESS;
 }
