@@ -42,20 +42,29 @@ struct RouteParams
 
 // Logits become unsigned keys in their order (0: not to be chosen: NaN and -infinity, or chosen already).  A lane holds kPer experts that
 // follow each other, and knows its largest key, the first among equal ones: up to four are sorted at the start and move up when one is
-// taken, more are searched through.  A choice is the lowest lane with the largest key of all.  All lanes run the same instructions: the
-// winner's part under a branch cost twice as many.  Lane j returns the j-th choice (-1: none) and its weight.
-__device__ __forceinline__ uint32_t logit_key(float v)
+// taken, more are searched through.  A choice is the lowest lane with the largest key of all.  16-bit logits leave the lowest 13 bits of a
+// 32-bit key alone: nine of them hold the expert's number, the lowest one largest, and the largest key is the choice, with nothing to
+// look up.  All lanes run the same instructions: the winner's part under a branch cost twice as many.  Lane j returns the j-th choice
+// (-1: none) and its weight.
+constexpr uint32_t kNumberBits = kMaxExperts - 1;
+template <bool kPacked>
+__device__ __forceinline__ uint32_t logit_key(float v, int e)
 {
     const uint32_t b = __float_as_uint(v + 0.f); // -0 and 0 are equal logits
-    return v > -INFINITY ? ((b >> 31) != 0 ? ~b : b | 0x80000000u) : 0u;
+    uint32_t       k = (b >> 31) != 0 ? ~b : b | 0x80000000u;
+    if constexpr (kPacked) k = (k & ~kNumberBits) | (kNumberBits - static_cast<uint32_t>(e));
+    return v > -INFINITY ? k : 0u;
 }
+template <bool kPacked>
 __device__ __forceinline__ float key_logit(uint32_t key)
 {
+    if constexpr (kPacked) key = (key >> 31) != 0 ? key & ~kNumberBits : key | kNumberBits;
     return __uint_as_float((key >> 31) != 0 ? key & 0x7fffffffu : ~key);
 }
 template <typename T, int kPer> // experts per lane
 __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane, float &weight)
 {
+    constexpr bool kPacked = sizeof(T) == 2;
     const T *row = reinterpret_cast<const T *>(p.logits + t * p.ld) + lane * kPer;
     uint32_t key[kPer];
     constexpr int kBytes = kPer * static_cast<int>(sizeof(T)), kUnit = kBytes >= 16 ? 16 : kBytes;
@@ -70,19 +79,22 @@ __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane
             else reinterpret_cast<uint32_t *>(e)[i] = __ldg(reinterpret_cast<const uint32_t *>(row) + i);
         }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) key[i] = logit_key(to_float(e[i]));
+        for (int i = 0; i < kPer; ++i) key[i] = logit_key<kPacked>(to_float(e[i]), lane * kPer + i);
     }
     else
     {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) key[i] = lane * kPer + i < p.experts ? logit_key(to_float(row[i])) : 0u;
+        for (int i = 0; i < kPer; ++i) key[i] = lane * kPer + i < p.experts ? logit_key<kPacked>(to_float(row[i]), lane * kPer + i) : 0u;
     }
     float    top = 0.f, all = 0.f;
     uint32_t own = 0;
-    int      mine = -1, index[kPer];
+    int      mine = -1, index[kPacked ? 1 : kPer];
     constexpr bool kSorted = kPer <= 4;
+    if constexpr (!kPacked)
+    {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) index[i] = lane * kPer + i;
+        for (int i = 0; i < kPer; ++i) index[i] = lane * kPer + i;
+    }
     if constexpr (kSorted)
     {
         // neighbours change places, equal ones do not: stable
@@ -94,18 +106,21 @@ __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane
             {
                 const bool     swap = key[i + 1] > key[i];
                 const uint32_t k    = key[i];
-                const int      n    = index[i];
                 key[i]              = swap ? key[i + 1] : k;
                 key[i + 1]          = swap ? k : key[i + 1];
-                index[i]            = swap ? index[i + 1] : n;
-                index[i + 1]        = swap ? n : index[i + 1];
+                if constexpr (!kPacked)
+                {
+                    const int n  = index[i];
+                    index[i]     = swap ? index[i + 1] : n;
+                    index[i + 1] = swap ? n : index[i + 1];
+                }
             }
         }
     }
     for (int j = 0; j < p.top_k; ++j)
     {
         uint32_t head = key[0];
-        int      at   = index[0];
+        int      at   = kPacked ? 0 : index[0];
         if constexpr (!kSorted)
         {
 #pragma unroll
@@ -113,41 +128,46 @@ __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane
             {
                 const bool more = key[i] > head;
                 head            = more ? key[i] : head;
-                at              = more ? index[i] : at;
+                if constexpr (!kPacked) at = more ? index[i] : at;
             }
         }
         const uint32_t best = __reduce_max_sync(0xffffffffu, head);
         if (best == 0) break;
-        const int winner = __ffs(__ballot_sync(0xffffffffu, head == best)) - 1;
-        const int e      = __shfl_sync(0xffffffffu, at, winner);
-        mine             = lane == j ? e : mine;
-        own              = lane == j ? best : own;
+        own      = lane == j ? best : own;
+        bool won = head == best;
+        if constexpr (!kPacked) // several lanes may hold it
+        {
+            const int winner = __ffs(__ballot_sync(0xffffffffu, won)) - 1;
+            const int e      = __shfl_sync(0xffffffffu, at, winner);
+            mine             = lane == j ? e : mine;
+            won              = lane == winner;
+        }
         if (j == 0)
         {
-            top = key_logit(best);
+            top = key_logit<kPacked>(best);
             if (p.renormalize == 0)
             {
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) all += key[i] != 0 ? expf(key_logit(key[i]) - top) : 0.f;
+                for (int i = 0; i < kPer; ++i) all += key[i] != 0 ? expf(key_logit<kPacked>(key[i]) - top) : 0.f;
             }
         }
-        const bool won = lane == winner;
         if constexpr (kSorted)
         {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
             {
-                key[i]   = won ? (i + 1 < kPer ? key[i + 1] : 0u) : key[i];
-                index[i] = won && i + 1 < kPer ? index[i + 1] : index[i];
+                key[i] = won ? (i + 1 < kPer ? key[i + 1] : 0u) : key[i];
+                if constexpr (!kPacked) index[i] = won && i + 1 < kPer ? index[i + 1] : index[i];
             }
         }
         else
         {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) key[i] = index[i] == e ? 0u : key[i];
+            for (int i = 0; i < kPer; ++i) key[i] = won && (kPacked ? key[i] == best : index[kPacked ? 0 : i] == at) ? 0u : key[i];
         }
     }
-    const float w = mine >= 0 ? expf(key_logit(own) - top) : 0.f;
+    if constexpr (kPacked) mine = own != 0 ? static_cast<int>(kNumberBits - (own & kNumberBits)) : -1;
+    const float w = mine >= 0 ? expf(key_logit<kPacked>(own) - top) : 0.f;
     if (p.renormalize != 0) all = w;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
