@@ -381,7 +381,7 @@ extern "C"
             cudaStreamSynchronize(ctx->stream);
             if (code == cugl::DEV_BAD_GROUP)
             {
-                return fail(ctx, CUGL_RUNTIME_ERROR, "cugl_mx_grouped_gemm: a group did not start at a multiple of 128 or did not lie within the rows; it was left out");
+                return fail(ctx, CUGL_RUNTIME_ERROR, "cugl_mx_grouped_gemm: a group did not start at a multiple of 128 or did not lie within the rows, or groups overlapped; it was left out");
             }
             return fail(ctx, CUGL_RUNTIME_ERROR,
                         "device-side bounded wait ran out (code " + std::to_string(code) +

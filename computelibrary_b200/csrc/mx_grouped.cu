@@ -51,12 +51,14 @@ struct GroupedParams
 // A group that does not start at a multiple of 128 or does not lie within the rows counts as empty and is reported.
 __device__ __forceinline__ int2 load_group(const GroupedParams &p, int g, bool &bad)
 {
-    int2 v = __ldg(p.groups + g);
+    int2 v = p.groups[g];
     bad    = v.y < 0 || (v.y > 0 && (v.x < 0 || v.x % kSlab != 0 || v.x > p.rows || v.y > p.rows - v.x));
     if (bad || v.y <= 0) v = make_int2(0, 0);
     return v;
 }
-// before[g]: tiles of kTile rows of the groups before g; returns those of all.  Called by all threads.
+// before[g]: tiles of kTile rows of the groups before g; returns those of all.  Called by all threads.  Groups that do not overlap have no
+// more tiles than the rows have slabs; more are reported and none of them is worked on, so that items stay countable.  Sums stop at kMostTiles.
+constexpr int kMostTiles = 1 << 28;
 template <int kTile>
 __device__ __forceinline__ int scan_groups(const GroupedParams &p, int *before)
 {
@@ -79,17 +81,23 @@ __device__ __forceinline__ int scan_groups(const GroupedParams &p, int *before)
         for (int o = 1; o < 32; o <<= 1)
         {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (static_cast<int>(threadIdx.x) >= o) incl += v;
+            if (static_cast<int>(threadIdx.x) >= o) incl = min(incl + v, kMostTiles);
         }
         int at = incl - sum;
         for (int i = first; i < min(first + per, p.n_groups + 1); ++i)
         {
-            at += before[i];
+            at        = min(at + before[i], kMostTiles);
             before[i] = at;
         }
     }
     __syncthreads();
-    return before[p.n_groups];
+    const int tiles = before[p.n_groups];
+    if (tiles > (p.rows + kSlab - 1) / kSlab)
+    {
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.status, 0, DEV_BAD_GROUP);
+        return 0;
+    }
+    return tiles;
 }
 
 // An item: 128 (or 256) channels of a tile of tokens of a group.
@@ -118,7 +126,7 @@ __device__ __forceinline__ Item find_item(const GroupedParams &p, const int *bef
     const int width  = min(kStrip, w_blocks - strip * kStrip);
     const int tb     = at / width;
     it.wb            = strip * kStrip + at - tb * width;
-    const int2 v     = __ldg(p.groups + lo);
+    const int2 v     = p.groups[lo];
     it.row           = v.x + tb * kTile;
     it.count         = min(kTile, v.y - tb * kTile);
     return it;
@@ -475,6 +483,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 if (half.both || half.first == 0) mbar_arrive(tempty_bar(0));
                 if (half.both || half.first == 1) mbar_arrive(tempty_bar(1));
             }
+            __syncwarp();
             half.done();
         }
     }
@@ -780,6 +789,7 @@ __global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster_no_writes(release);
+                        __syncwarp(); // aligned loads of tensor memory may be next
                     }
                 };
                 if (!any)

@@ -260,6 +260,32 @@ def test_groups_outside_are_left_out(ctx, group, expected):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("expected", [FEW, MANY])
+def test_groups_that_overlap(ctx, expected):
+    """512 groups of the same 512 rows have more tiles than the rows.  Nothing is computed, the next sync reports it, and the call after
+    that is as ever."""
+    import torch
+    rng = np.random.default_rng(5)
+    E, N, K, rows = 512, 8, 64, 512
+    a, sa, _ = operand(rng, rows, K, capi.NVFP4)
+    b, sb, _ = operand(rng, N, K, capi.NVFP4, matrices=E)
+    groups = torch.zeros((E, 2), dtype=torch.int32, device="cuda")
+    groups[:, 1] = rows
+    out = torch.full((rows, N), 7.0, device="cuda")
+    d = capi.make_mx_grouped_gemm_desc(E, rows, N, K, capi.NVFP4, capi.F32, expected_rows=expected)
+    ctx.mx_grouped_gemm(d, a, sa, groups, (b, sb, None), out)
+    with pytest.raises(capi.CuglError) as e:
+        ctx.sync()
+    assert e.value.status == capi.RUNTIME_ERROR and "overlap" in e.value.message
+    assert bool((out == 7).all())
+    groups[1:] = 0
+    groups[0, 1] = rows
+    ctx.mx_grouped_gemm(d, a, sa, groups, (b, sb, None), out)
+    ctx.sync()
+    assert bool((out != 7).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("expected", [FEW, MANY])
 @pytest.mark.parametrize("swiglu", [False, True])
 @pytest.mark.parametrize("k_block", [0, 3, 7])
 def test_wait_limit(ctx, expected, swiglu, k_block):
