@@ -534,11 +534,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
             if (row < (i < S::kTile ? t.count : t.rank))
             {
                 const uint8_t *src = i < S::kTile ? x + row * p.ld_x : a + row * p.ld_a;
-                if constexpr (kWord) low[j] = __ldg(reinterpret_cast<const uint32_t *>(src + static_cast<int64_t>(k0) * 2));
+                if constexpr (kWord) low[j] = *reinterpret_cast<const uint32_t *>(src + static_cast<int64_t>(k0) * 2);
                 else
                 {
-                    low[j]  = __ldg(reinterpret_cast<const uint16_t *>(src) + k0);
-                    high[j] = __ldg(reinterpret_cast<const uint16_t *>(src) + k1);
+                    low[j]  = reinterpret_cast<const uint16_t *>(src)[k0];
+                    high[j] = reinterpret_cast<const uint16_t *>(src)[k1];
                 }
             }
         }
@@ -599,8 +599,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_c
 // ---- second launch: dst = base + factor * v . B^T --------------------------------------------------------------
 // An item is 256 channels of a tile.  Every CTA takes every gridDim.x-th of them, so that tiles of high and of low rank, which are not
 // equally much work, are spread over all (prompts of 4096 tokens with ranks of 16 to 64, both launches: consecutive shares 46.8 us,
-// this 45.5 when it was taken).  A warp has 32 channels, the tokens of the tile sixteen at a time.  What it needs next is under way while it works: units of 16 tokens
-// x 32 channels of base pass through a ring of four slots of its own, the next item's v waits in the other half of its buffer, and its B
+// this 45.5 when it was taken).  A warp has 32 channels, the tokens of the tile sixteen at a time.  What it needs next is under way
+// while it works: units of 16 tokens x 32 channels of base pass through a ring of four slots of its own, the next item's v waits in the other half of its buffer, and its B
 // in registers where there are enough of them.  Of a unit's results lane (g, c) has rows g and g + 8, and of each the channels that it stores as 16-byte pieces:
 //   two-byte results  8 c .. 8 c + 7
 //   floats            4 c .. 4 c + 3 and 16 + 4 c .. 16 + 4 c + 3, so that a store of four lanes covers whole sectors

@@ -45,7 +45,7 @@ enum Rows
 };
 __device__ __forceinline__ int slot_of(const QuantParams &p, int64_t i)
 {
-    const int r = __ldg(p.slots + i);
+    const int r = p.slots[i];
     return static_cast<unsigned>(r) < static_cast<unsigned>(p.group_rows) ? r : -1;
 }
 template <int kWhich>
@@ -255,8 +255,8 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
                 if constexpr (kWhole && kLoads == 2)
                 {
                     const uint4 *unit = reinterpret_cast<const uint4 *>(src + g * kItemCols) - (lane & 1); // of the pair's first lane: + 2 per lane before it
-                    raw[u][g][0]      = __ldg(unit);
-                    raw[u][g][1]      = __ldg(unit + 2);
+                    raw[u][g][0]      = unit[0];
+                    raw[u][g][1]      = unit[2];
                     continue;
                 }
                 const int n = kWhole || in ? p.cols - at.c0 - g * kItemCols : 0;
@@ -264,7 +264,7 @@ __device__ __forceinline__ void quantize_group(const QuantParams &p, int group, 
                 for (int l = 0; l < kLoads; ++l)
                 {
                     raw[u][g][l] = make_uint4(0, 0, 0, 0);
-                    if (kWhole || n >= kLaneCols) raw[u][g][l] = __ldg(reinterpret_cast<const uint4 *>(src + g * kItemCols) + l);
+                    if (kWhole || n >= kLaneCols) raw[u][g][l] = reinterpret_cast<const uint4 *>(src + g * kItemCols)[l];
                 }
                 if (!kWhole && n > 0 && n < kLaneCols)
                 {
@@ -364,14 +364,14 @@ __device__ __forceinline__ void dequantize_group(const QuantParams &p, int group
         {
             const int n = kWhole ? kLaneCols : row < p.rows ? p.cols - at.c0 - g * kItemCols : 0;
             w[u][g] = byte[u][g] = 0;
-            if (n > 0) byte[u][g] = __ldg(scales + g * kTiles * kMxTileBytes);
+            if (n > 0) byte[u][g] = scales[g * kTiles * kMxTileBytes];
             if (kWhole || (n >= kLaneCols && p.vec_packed != 0))
             {
-                w[u][g] = __ldg(reinterpret_cast<const uint32_t *>(src + g * kItemCols / 2));
+                w[u][g] = *reinterpret_cast<const uint32_t *>(src + g * kItemCols / 2);
             }
             else
             {
-                for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) w[u][g] |= static_cast<uint32_t>(__ldg(src + g * kItemCols / 2 + i)) << (8 * i);
+                for (int i = 0; i < (min(n, kLaneCols) + 1) / 2; ++i) w[u][g] |= static_cast<uint32_t>(src[g * kItemCols / 2 + i]) << (8 * i);
             }
         }
     }
