@@ -1,7 +1,8 @@
 // Low-rank adapters of many requests at once, beside a projection that all of them share:
 //   dst[t] = base[t] + scale_a * (x[t] . A_a^T) . B_a^T          a: the adapter of the request that token t belongs to
 //
-// Two launches.  The first makes v = x . A^T: a tile of up to 64 tokens of one request per cluster, whose CTAs share K; their sums are added
+// Long requests take two launches, short ones have one that does the same for tiles of 16 tokens (lora_few_kernel: 24 requests of a token,
+// 4096 -> 14336, rank 16, BF16 9.3 us, in two launches 13.3).  The first makes v = x . A^T: a tile of up to 64 tokens of one request per cluster, whose CTAs share K; their sums are added
 // up in a fixed order through distributed shared memory.  The second adds scale * v . B^T to base, 256 channels x a tile of tokens per
 // CTA.  Which tiles there are is known on the device only (the requests' lengths): every CTA counts them (a scan over the requests)
 // and takes the one with its number; the grid is the most that there can be.
@@ -31,6 +32,7 @@ constexpr int kThreads  = 256;
 constexpr int kWarps    = kThreads / 32;
 constexpr int kMaxRank  = 128;
 constexpr int kMaxSplit = 8;
+constexpr int kFewRank  = 64; // largest padded rank of the single launch
 
 struct LoraParams
 {
@@ -144,18 +146,18 @@ __device__ __forceinline__ Tile find_tile(const LoraParams &p, int wanted)
 template <typename T, bool kFirst = false>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    if constexpr (kFirst) d[0] = d[1] = d[2] = d[3] = 0.f;
+    const float c0 = kFirst ? 0.f : d[0], c1 = kFirst ? 0.f : d[1], c2 = kFirst ? 0.f : d[2], c3 = kFirst ? 0.f : d[3];
     if constexpr (std::is_same<T, __half>::value)
     {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     }
     else
     {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     }
 }
 
@@ -223,8 +225,69 @@ __device__ __forceinline__ int v_place(int r)
     return (r & ~15) + ((r >> 1) & 6) + ((r & 2) << 2) + (r & 1);
 }
 
-// The CTAs' sums of x . A^T ([token][rank] in the shared memory of each), added up in the order of the CTAs, to the parts of v: a warp per
-// token.  By all threads of the cluster.
+// v of a token: the CTAs' sums of x . A^T ([token][rank] in the shared memory of each), added up in the order of the CTAs, its parts to
+// put(part, place, bits); returns the token's factor.  By a warp.
+template <typename T, int kRank, typename Put>
+__device__ __forceinline__ float token_v(const LoraParams &p, const Tile &t, const float *share, int pitch, int ranks, int tok, Put put)
+{
+    constexpr int  kPer = (kRank + 31) / 32;
+    const int      lane = threadIdx.x & 31;
+    const uint32_t at   = smem_u32(share + tok * pitch);
+    float          v[kPer], parts[kPer][kMaxSplit];
+    float          top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) // all of them under way before the first is added
+    {
+        const int r = min(i * 32 + lane, kRank - 1);
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+        {
+            parts[i][q] = 0.f;
+            if (q < ranks) parts[i][q] = load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+    {
+        v[i] = parts[i][0];
+#pragma unroll
+        for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
+        if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
+    }
+    float factor = __ldg(p.scales + t.adapter);
+    float mul    = 1.f;
+    if constexpr (std::is_same<T, __half>::value)
+    {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+        if (e > -126 && e < 127) // zero and subnormal sums stay as they are
+        {
+            mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+    {
+        const int r = i * 32 + lane;
+        if (r < kRank)
+        {
+            float rest = v[i] * mul;
+            for (int q = 0; q < p.parts; ++q)
+            {
+                const T  part = from_float<T>(rest);
+                uint16_t bits;
+                memcpy(&bits, &part, 2);
+                put(q, v_place(r), bits);
+                const float f = to_float(part);
+                rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
+            }
+        }
+    }
+    return factor;
+}
+// v of a tile's tokens to memory, shared by the CTAs of the cluster: a warp per token.  By all threads of the cluster.
 template <typename T, int kRank>
 __device__ __forceinline__ void finish_v(const LoraParams &p, const Tile &t, const float *share, int pitch, int rank, int ranks)
 {
@@ -233,64 +296,14 @@ __device__ __forceinline__ void finish_v(const LoraParams &p, const Tile &t, con
     else __syncthreads();
     for (int tok = rank * kWarps + warp; tok < t.count; tok += ranks * kWarps)
     {
-        constexpr int  kPer = (kRank + 31) / 32;
-        const uint32_t at   = smem_u32(share + tok * pitch);
-        float          v[kPer], parts[kPer][kMaxSplit];
-        float          top = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) // all of them under way before the first is added
-        {
-            const int r = min(i * 32 + lane, kRank - 1);
-#pragma unroll
-            for (int q = 0; q < kMaxSplit; ++q)
-            {
-                parts[i][q] = 0.f;
-                if (q < ranks) parts[i][q] = load_cluster(map_to_cta(at + 4u * r, static_cast<uint32_t>(q)));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-        {
-            v[i] = parts[i][0];
-#pragma unroll
-            for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
-            if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
-        }
-        float factor = __ldg(p.scales + t.adapter);
-        float mul    = 1.f;
-        if constexpr (std::is_same<T, __half>::value)
-        {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-            if (e > -126 && e < 127) // zero and subnormal sums stay as they are
-            {
-                mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            }
-        }
-        uint16_t *out = p.v + static_cast<int64_t>(t.first + tok) * (kRank + 8);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-        {
-            const int r = i * 32 + lane;
-            if (r < kRank)
-            {
-                float rest = v[i] * mul;
-                for (int q = 0; q < p.parts; ++q)
-                {
-                    const T part = from_float<T>(rest);
-                    uint16_t bits;
-                    memcpy(&bits, &part, 2);
-                    out[static_cast<int64_t>(q) * p.tokens * (kRank + 8) + v_place(r)] = bits;
-                    const float f = to_float(part);
-                    rest          = fabsf(f) < INFINITY ? rest - f : 0.f; // an infinity or NaN is whole in the first part
-                }
-            }
-        }
+        uint16_t   *out    = p.v + static_cast<int64_t>(t.first + tok) * (kRank + 8);
+        const float factor = token_v<T, kRank>(p, t, share, pitch, ranks, tok, [&](int part, int place, uint16_t bits) {
+            out[static_cast<int64_t>(part) * p.tokens * (kRank + 8) + place] = bits;
+        });
         if (lane == 0) *reinterpret_cast<float *>(out + kRank) = factor;
     }
     // Nobody leaves while others read its sums: they have what they read.  (A releasing arrival would wait for the stores of v.)
+    __syncwarp();
     if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -936,6 +949,356 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
     copy_wait<0>();
 }
 
+// ---- few tiles: both products in one launch ---------------------------------------------------------------------
+// Tiles of up to 16 tokens, a cluster each.  Its CTAs share K as above, every one of them adds up all of v for itself, and takes every
+// ranks-th block of 256 channels.  What bounds it is the chain requests -> tile (2 us) -> x and A -> sums (4 us) -> results (3 us, 24 requests
+// of a token, 14336 channels), and in the last part its instructions: addresses that are kept, v in registers at 16 ranks and no work for
+// rows that are not there took 10.8 to 9.3 us.  B and base of a warp's first blocks are on their way before the sums are there, those of the
+// blocks to come while others are multiplied.
+template <typename T, typename TD, int kRank>
+struct Few
+{
+    static constexpr int kTile    = 16;
+    static constexpr int kSteps   = kRank / 16;
+    static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
+    static constexpr int kDepth   = kRank == 16 ? 3 : kRank == 32 ? 2 : 1; // blocks whose B and base a warp has in registers
+    static constexpr bool kKept   = kRank == 16;                           // v in registers
+    static constexpr int kStages  = kRank == 64 ? 6 : 8;
+    static constexpr int kA       = kRank * 128, kX = kTile * 128, kStage = kA + kX;
+    static constexpr int kSums    = kRank + 1;                                                   // floats of a token's sums
+    static constexpr int kOffV    = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384);  // an MMA reads 16 KB from a stage's start on
+    static constexpr int kPitch   = kRank * 2 + 16;                                              // bytes of a row of v, its factor included
+    static constexpr int kOffBar  = kOffV + kParts * kTile * kPitch;
+    static constexpr int kSmem    = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
+    static constexpr int kColumns = 32;
+    static_assert(kTile * kSums * 4 <= kOffV && kStage % 1024 == 0, "sums fit where the stages were");
+};
+template <typename T, typename TD, int kRank, bool kVec>
+__global__ void __launch_bounds__(kThreads, 2)
+    lora_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ LoraParams p)
+{
+    using S = Few<T, TD, kRank>;
+    constexpr int STAGES = S::kStages, kPieces = static_cast<int>(sizeof(TD)) / 2, kPer = 8 / kPieces; // 16-byte pieces of a lane's row, elements of one
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t       *smem      = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t s_stage   = smem_u32(smem), bar_base = smem_u32(smem + S::kOffBar);
+    auto           full_bar  = [&](int s) { return bar_base + 8u * s; };
+    auto           empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    const uint32_t done_bar  = bar_base + 8u * (2 * STAGES), gone_bar = done_bar + 8;
+    uint32_t      *s_tmem    = reinterpret_cast<uint32_t *>(smem + S::kOffBar + (2 * STAGES + 2) * 8);
+    volatile int  *s_abort   = reinterpret_cast<volatile int *>(s_tmem + 1);
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    if (threadIdx.x == 0)
+    {
+        for (int s = 0; s < STAGES; ++s)
+        {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        mbar_init(gone_bar, 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1)
+    {
+        tmem_alloc(smem_u32(s_tmem), S::kColumns);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    griddep_launch_dependents();
+    griddep_wait();
+    const int  ranks = static_cast<int>(gridDim.x / num_clusters_x()), rank = static_cast<int>(cluster_ctarank());
+    const Tile t     = find_tile(p, static_cast<int>(cluster_id_x()));
+    if (t.count == 0) // the same for the cluster, as is whether there is an adapter
+    {
+        if (warp == 1) tmem_dealloc(tmem, S::kColumns);
+        return;
+    }
+    const bool adds   = t.adapter >= 0;
+    const int  blocks = (p.K + 63) / 64; // of 64 columns, shared by the CTAs of the cluster
+    const int  first  = share_begin(blocks, rank, ranks), n_blocks = adds ? share_begin(blocks, rank + 1, ranks) - first : 0;
+    int        issued = 0; // stages that the producer has filled
+    auto       produce = [&](int end) { // by warp 0
+        const bool el    = elect_one();
+        const int  a_row = max(t.adapter, 0) * p.max_rank;
+        for (; issued < end; ++issued)
+        {
+            const int s = issued % STAGES;
+            if (!warp_wait(empty_bar(s), (static_cast<uint32_t>(issued / STAGES) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_PRODUCER, p.spin_limit)) break;
+            if (issued == p.withhold && blockIdx.x == 0) continue;
+            if (el)
+            {
+                const uint32_t dst = s_stage + s * S::kStage;
+                mbar_expect_tx(full_bar(s), static_cast<uint32_t>(S::kStage));
+                tma_load_2d(dst, &tmap_a, (first + issued) * 64, a_row, full_bar(s));
+                tma_load_2d(dst + S::kA, &tmap_x, (first + issued) * 64, t.first, full_bar(s));
+            }
+            __syncwarp();
+        }
+    };
+    if (warp == 0) produce(min(n_blocks, STAGES));
+    // B and base of the warp's first blocks of channels, ahead of its part in the sums
+    const int wide = (p.N + 32 * kWarps - 1) / (32 * kWarps);
+    uint2     b[S::kDepth][4][S::kSteps] = {};
+    uint4     base[S::kDepth][2][kPieces];
+    // A lane's places in the warp's next block to load and to store: row of B of its first column (see load_b), piece of rows g of base and dst.
+    const int      n_first   = rank * 32 * kWarps + warp * 32;
+    const uint8_t *b_lane    = p.b + (static_cast<int64_t>(max(t.adapter, 0)) * p.N + n_first + piece_channel<TD>(0, g >> 1) + (g & 1)) * p.ld_b + 8 * c;
+    const uint8_t *base_lane = p.base + static_cast<int64_t>(t.first + g) * p.ld_base + static_cast<int64_t>(n_first) * static_cast<int>(sizeof(TD)) + 16 * c;
+    uint8_t       *dst_lane  = p.dst + static_cast<int64_t>(t.first + g) * p.ld_dst + static_cast<int64_t>(n_first) * static_cast<int>(sizeof(TD)) + 16 * c;
+    const int64_t  b_step    = static_cast<int64_t>(ranks) * 32 * kWarps * p.ld_b, step = static_cast<int64_t>(ranks) * 32 * kWarps * static_cast<int>(sizeof(TD));
+    const bool     plain     = kVec && adds && (t.rank & 3) == 0; // whole blocks need no tests
+    auto load_block = [&](int block, uint2 (&to)[4][S::kSteps], uint4 (&rows)[2][kPieces]) { // blocks one after the other
+        if (block >= wide) return;
+        const int n = block * 32 * kWarps + warp * 32;
+        if (n >= p.N) return; // the same for the warp
+        if (plain && n + 32 <= p.N)
+        {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                const int ch = sizeof(TD) == 2 ? 2 * i : 16 * (i >> 1) + 2 * (i & 1);
+#pragma unroll
+                for (int s = 0; s < S::kSteps; ++s)
+                {
+                    if (s * 16 + 4 * c < t.rank) to[i][s] = __ldcg(reinterpret_cast<const uint2 *>(b_lane + ch * p.ld_b + s * 32)); // else: zeros, as they were
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+            {
+                if (h * 8 + g < t.count)
+                {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) rows[h][i] = __ldcg(reinterpret_cast<const uint4 *>(base_lane + h * 8 * p.ld_base + 64 * i));
+                }
+            }
+            b_lane += b_step;
+            base_lane += step;
+            return;
+        }
+        load_b<TD>(p, t, n, lane, to);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+        {
+            const int row = h * 8 + g;
+            if (row >= t.count) continue;
+            const uint8_t *src = p.base + static_cast<int64_t>(t.first + row) * p.ld_base;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+            {
+                const int ch = n + piece_channel<TD>(i, c);
+                if constexpr (kVec)
+                {
+                    if (ch < p.N) rows[h][i] = __ldcg(reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(ch) * static_cast<int>(sizeof(TD))));
+                }
+                else
+                {
+                    TD e[kPer];
+#pragma unroll
+                    for (int k = 0; k < kPer; ++k)
+                    {
+                        e[k] = from_float<TD>(0.f);
+                        if (ch + k < p.N) e[k] = __ldcg(reinterpret_cast<const TD *>(src) + ch + k);
+                    }
+                    memcpy(&rows[h][i], e, 16);
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < S::kDepth; ++d) load_block(rank + d * ranks, b[d], base[d]);
+    __syncwarp();
+    if (warp == 0)
+    {
+        produce(n_blocks);
+    }
+    else if (warp == 1)
+    {
+        const bool     el    = elect_one();
+        const uint32_t idesc = p.idesc | (2u << 17); // 16 columns
+        bool           ok    = true;
+        for (int i = 0; i < n_blocks && ok; ++i)
+        {
+            const int s = i % STAGES;
+            ok = warp_wait(full_bar(s), static_cast<uint32_t>(i / STAGES) & 1u, s_abort, DEV_TIMEOUT_MMA, p.spin_limit);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t a_desc = make_kmajor_sw128_desc(s_stage + s * S::kStage), b_desc = make_kmajor_sw128_desc(s_stage + s * S::kStage + S::kA);
+            if (el)
+            {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_f16(tmem, a_desc + 2u * k, b_desc + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
+                umma_commit(empty_bar(s));
+            }
+            __syncwarp();
+        }
+        if (ok && el && adds) umma_commit(done_bar);
+        __syncwarp();
+    }
+    uint8_t *const area = smem + S::kOffV; // v: [part][token][rank], the factor behind a token's first part
+    if (adds)
+    {
+        const bool ok    = warp_wait(done_bar, 0, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit);
+        float     *share = reinterpret_cast<float *>(smem);
+        const int  r     = warp * 32 + lane;
+        __syncthreads(); // every warp's waits are over; the MMAs have read the stages
+        if (ok && *s_abort == 0 && warp * 32 < kRank) // sums to shared memory, [token][rank]: a lane has a rank
+        {
+            tc_fence_after();
+            uint32_t v[16];
+            tmem_ld_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16), v);
+            tmem_ld_wait();
+            if (r < kRank)
+            {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    if (i < t.count) share[i * S::kSums + r] = n_blocks > 0 && r < t.rank ? __uint_as_float(v[i]) : 0.f; // behind the adapter's ranks: zeros
+                }
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+        const bool gone = *s_abort != 0;
+        if (warp == 0 && gone)
+        {
+            drain_stages<STAGES>(bar_base, issued, blockIdx.x == 0 ? p.withhold : -1, p.spin_limit);
+        }
+        if (warp == 1 && gone)
+        {
+            drain_mmas<false>(gone_bar, p.spin_limit);
+        }
+        if (threadIdx.x == 0 && gone)
+        {
+            atomicCAS(p.status, 0, *s_abort);
+        }
+        __syncwarp();
+        if (ranks > 1) cluster_sync();
+        else __syncthreads();
+        for (int tok = warp; tok < t.count; tok += kWarps) // (of a CTA that has given up: nothing of use)
+        {
+            uint8_t *const row    = area + tok * S::kPitch;
+            const float    factor = token_v<T, kRank>(p, t, share, S::kSums, ranks, tok, [&](int part, int place, uint16_t bits) {
+                *reinterpret_cast<uint16_t *>(row + part * S::kTile * S::kPitch + place * 2) = bits;
+            });
+            if (lane == 0) *reinterpret_cast<float *>(row + kRank * 2) = factor;
+        }
+        __syncwarp();
+        if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // this warp has read the others' sums
+        __syncthreads();
+    }
+    if (warp == 1)
+    {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kColumns);
+    }
+    float f[2] = {};
+    if (adds)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) f[h] = *reinterpret_cast<const float *>(area + (h * 8 + g) * S::kPitch + kRank * 2); // rows behind the last: not stored
+    }
+    const uint32_t v_at = smem_u32(area) + static_cast<uint32_t>((lane & 15) * S::kPitch + (lane >> 4) * 16);
+    auto           load_v = [&](int part, int s, uint32_t (&v)[4]) { ldmatrix_x4(v_at + static_cast<uint32_t>(part * S::kTile * S::kPitch + s * 32), v); };
+    uint32_t       kept[S::kKept ? S::kParts : 1][4];
+    if (S::kKept && adds)
+    {
+#pragma unroll
+        for (int part = 0; part < S::kParts; ++part) load_v(part, 0, kept[S::kKept ? part : 0]);
+    }
+    for (int block = rank; block < wide; block += S::kDepth * ranks)
+    {
+#pragma unroll
+        for (int d = 0; d < S::kDepth; ++d)
+        {
+            const int at = block + d * ranks, n = at < wide ? at * 32 * kWarps + warp * 32 : p.N;
+            if (n < p.N) // the same for the warp
+            {
+                float acc[4][4];
+                __syncwarp();
+                if (adds)
+                {
+#pragma unroll
+                    for (int part = S::kParts - 1; part >= 0; --part) // small parts first
+                    {
+#pragma unroll
+                        for (int s = 0; s < S::kSteps; ++s)
+                        {
+                            if (s * 16 < t.rank)
+                            {
+                                uint32_t own[4];
+                                if (!S::kKept) load_v(part, s, own);
+                                const uint32_t(&v)[4] = S::kKept ? kept[S::kKept ? part : 0] : own;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                {
+                                    if (part == S::kParts - 1 && s == 0) mma<T, true>(acc[i], v[0], v[1], v[2], v[3], b[d][i][s].x, b[d][i][s].y);
+                                    else mma<T>(acc[i], v[0], v[1], v[2], v[3], b[d][i][s].x, b[d][i][s].y);
+                                }
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                {
+                    if (h * 8 >= t.count) break; // the same for the block
+                    TD e[8];
+                    memcpy(e, base[d][h], 16 * kPieces);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        if (adds) e[i] = from_float<TD>(fmaf(acc[i >> 1][2 * h + (i & 1)], f[h], to_float(e[i])));
+                    }
+                    const int row = h * 8 + g;
+                    if (plain && n + 32 <= p.N)
+                    {
+                        uint4 v[kPieces];
+                        memcpy(v, e, sizeof(v));
+                        if (row < t.count)
+                        {
+#pragma unroll
+                            for (int i = 0; i < kPieces; ++i)
+                                *reinterpret_cast<uint4 *>(dst_lane + h * 8 * p.ld_dst + 64 * i) = v[i];
+                        }
+                    }
+                    else if (row < t.count)
+                    {
+                        TD *dst = reinterpret_cast<TD *>(p.dst + static_cast<int64_t>(t.first + row) * p.ld_dst);
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i)
+                        {
+                            const int ch = n + piece_channel<TD>(i, c);
+                            if constexpr (kVec)
+                            {
+                                uint4 v;
+                                memcpy(&v, e + i * kPer, 16);
+                                if (ch < p.N) *reinterpret_cast<uint4 *>(dst + ch) = v;
+                            }
+                            else
+                            {
+#pragma unroll
+                                for (int k = 0; k < kPer; ++k)
+                                {
+                                    if (ch + k < p.N) dst[ch + k] = e[i * kPer + k];
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            dst_lane += step;
+            load_block(at + S::kDepth * ranks, b[d], base[d]);
+        }
+    }
+    __syncwarp();
+    if (adds && ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // nobody leaves while others read its sums
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------
 int padded_rank(int r)
 {
@@ -949,9 +1312,9 @@ int v_parts(const cugl_lora_desc &d)
 {
     return d.dtype == CUGL_BF16 && d.dst_dtype == CUGL_F32 ? 3 : 2;
 }
-int64_t most_tiles(const cugl_lora_desc &d) // of a request, all but the last are full
+int64_t most_tiles(const cugl_lora_desc &d, int64_t tile) // of a request, all but the last are full
 {
-    const int64_t tile = tile_tokens(d.max_rank), some = d.requests < d.tokens ? d.requests : d.tokens;
+    const int64_t some = d.requests < d.tokens ? d.requests : d.tokens;
     return (d.tokens - some) / tile + some;
 }
 
@@ -1014,23 +1377,58 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
     CUGL_CUDA_TRY(ctx, launch_dependent(ctx, kernel, dim3(static_cast<unsigned>(grid)), kThreads, E::kSmem, grid, p));
     return CUGL_SUCCESS;
 }
-template <typename T, typename TD, int kRank>
-cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int rows_in, bool vec_out)
+// CTAs of a cluster that works on both products in one launch; 0: two launches.  One launch where requests are short, and are eight at least or
+// have little to add (few channels, low ranks).  us in two / in one, K = 4096, requests x tokens.  Rank 16, N = 14336, BF16: 1 x 1 6.8 / 7.9,
+// 8 x 1 8.5 / 8.4, 24 x 1 13.3 / 9.3, 148 x 1 47 / 26, 24 x 8 14.4 / 10.8, 24 x 16 15.7 / 19.2, 256 x 4 78 / 49.  Rank 64, N = 4096, BF16: 1 x 1
+// 7.4 / 7.8, 8 x 1 8.9 / 8.4, 24 x 8 14.0 / 12.2, 8 x 16 9.3 / 11.8.  Rank 16, N = 4096, F16 to F32: 1 x 1 6.7 / 6.1, 24 x 8 9.2 / 7.5.  Rank 128,
+// N = 4096, BF16: 1 x 1 8.7 / 11.6, 24 x 1 20.4 / 20.3.
+int few_split(const cugl_context *ctx, const LoraParams &p, int padded)
 {
+    const int64_t some = std::min(p.requests, p.tokens), wide = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps);
+    if (padded > kFewRank || p.tokens > 8 * some || (some < 8 && wide * padded > 256)) return 0;
+    int split = kMaxSplit; // clusters that run at once: 28 of eight CTAs 9.2 us, of four 13.7; 37 16.9 and 14.1
+    while (split > 1 && some * split * 5 > 8ll * ctx->sm_count) split /= 2;
+    return split;
+}
+template <typename T, typename TD, int kRank>
+cugl_status launch_few(cugl_context *ctx, LoraParams p, int64_t tiles, int split, bool vec_out)
+{
+    using S = Few<T, TD, kRank>;
+    CUtensorMap map_a, map_x;
+    if (!encode_rows_map(&map_a, p.a, static_cast<int64_t>(p.n_adapters) * p.max_rank, p.K, p.ld_a, kRank) || !encode_rows_map(&map_x, p.x, p.tokens, p.K, p.ld_x, S::kTile))
+    {
+        return fail(ctx, CUGL_RUNTIME_ERROR, "cuTensorMapEncodeTiled failed for x or A");
+    }
+    p.tile  = S::kTile;
+    p.tiles = static_cast<int>(tiles);
+    static std::atomic<bool> set[2][64] = {};
+    auto                     kernel     = vec_out ? lora_few_kernel<T, TD, kRank, true> : lora_few_kernel<T, TD, kRank, false>;
+    CUGL_TRY(allow_smem(ctx, kernel, S::kSmem, set[vec_out ? 1 : 0]));
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, map_a, map_x, p));
+    return CUGL_SUCCESS;
+}
+template <typename T, typename TD, int kRank>
+cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int64_t few_tiles, int rows_in, bool vec_out)
+{
+    if constexpr (kRank <= kFewRank)
+    {
+        const int split = rows_in == kUnits16 ? few_split(ctx, p, kRank) : 0;
+        if (split > 0) return launch_few<T, TD, kRank>(ctx, p, few_tiles, split, vec_out);
+    }
     CUGL_TRY((rows_in == kUnits16 ? launch_shrink_mma<T, kRank>(ctx, p, tiles)
               : rows_in == kWords ? launch_shrink<T, kRank, kWords>(ctx, p, tiles)
                                   : launch_shrink<T, kRank, kAnywhere>(ctx, p, tiles)));
     return vec_out ? launch_expand<T, TD, kRank, true>(ctx, p, tiles) : launch_expand<T, TD, kRank, false>(ctx, p, tiles);
 }
 template <typename T, typename TD>
-cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int rows_in, bool vec_out)
+cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, int64_t few_tiles, int rows_in, bool vec_out)
 {
     switch (padded_rank(p.max_rank))
     {
-        case 16: return launch_lora<T, TD, 16>(ctx, p, tiles, rows_in, vec_out);
-        case 32: return launch_lora<T, TD, 32>(ctx, p, tiles, rows_in, vec_out);
-        case 64: return launch_lora<T, TD, 64>(ctx, p, tiles, rows_in, vec_out);
-        default: return launch_lora<T, TD, 128>(ctx, p, tiles, rows_in, vec_out);
+        case 16: return launch_lora<T, TD, 16>(ctx, p, tiles, few_tiles, rows_in, vec_out);
+        case 32: return launch_lora<T, TD, 32>(ctx, p, tiles, few_tiles, rows_in, vec_out);
+        case 64: return launch_lora<T, TD, 64>(ctx, p, tiles, few_tiles, rows_in, vec_out);
+        default: return launch_lora<T, TD, 128>(ctx, p, tiles, few_tiles, rows_in, vec_out);
     }
 }
 
@@ -1049,8 +1447,9 @@ const char *validate_lora(const cugl_lora_desc *d)
     if (d->ld_b < 2ll * d->max_rank || d->ld_b % 16 != 0) return "ld_b must hold a row and be a multiple of 16";
     if (d->ld_base < static_cast<int64_t>(d->N) * size || d->ld_base % size != 0 || d->ld_dst < static_cast<int64_t>(d->N) * size || d->ld_dst % size != 0)
         return "ld_base and ld_dst must hold a row and be multiples of the element size";
-    if (most_tiles(*d) > 65535) return "more than 65535 tiles of tokens";
-    if (most_tiles(*d) * ((static_cast<int64_t>(d->N) + 32 * kWarps - 1) / (32 * kWarps)) > INT32_MAX / 2) return "more than 2^30 tiles of tokens and channels";
+    const int64_t tiles = most_tiles(*d, tile_tokens(d->max_rank));
+    if (tiles > 65535) return "more than 65535 tiles of tokens";
+    if (tiles * ((static_cast<int64_t>(d->N) + 32 * kWarps - 1) / (32 * kWarps)) > INT32_MAX / 2) return "more than 2^30 tiles of tokens and channels";
     return nullptr;
 }
 } // namespace
@@ -1137,7 +1536,7 @@ extern "C"
         const bool mapped  = desc->ld_x < (1ll << 40) && desc->ld_a < (1ll << 40) && static_cast<int64_t>(desc->adapters) * desc->max_rank < (1ll << 31);
         const int  rows_in = even(d_x, desc->ld_x) && even(d_a, desc->ld_a) && mapped ? kUnits16 : words && desc->K % 2 == 0 ? kWords : kAnywhere;
         const bool vec_out = even(d_base, desc->ld_base) && even(d_dst, desc->ld_dst) && desc->N % 8 == 0;
-        const int64_t tiles = most_tiles(*desc);
+        const int64_t tiles = most_tiles(*desc, p.tile), few_tiles = most_tiles(*desc, 16);
         p.tiles             = static_cast<int>(tiles);
         p.idesc             = f16_idesc(desc->dtype == CUGL_BF16);
         p.status            = ctx->d_status;
@@ -1146,9 +1545,9 @@ extern "C"
         ctx->withhold_kb    = -1;
         if (desc->dtype == CUGL_F16)
         {
-            return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, rows_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, rows_in, vec_out);
+            return desc->dst_dtype == CUGL_F32 ? launch_lora<__half, float>(ctx, p, tiles, few_tiles, rows_in, vec_out) : launch_lora<__half, __half>(ctx, p, tiles, few_tiles, rows_in, vec_out);
         }
-        return desc->dst_dtype == CUGL_F32 ? launch_lora<__nv_bfloat16, float>(ctx, p, tiles, rows_in, vec_out)
-                                           : launch_lora<__nv_bfloat16, __nv_bfloat16>(ctx, p, tiles, rows_in, vec_out);
+        return desc->dst_dtype == CUGL_F32 ? launch_lora<__nv_bfloat16, float>(ctx, p, tiles, few_tiles, rows_in, vec_out)
+                                           : launch_lora<__nv_bfloat16, __nv_bfloat16>(ctx, p, tiles, few_tiles, rows_in, vec_out);
     }
 }

@@ -766,8 +766,9 @@ CUGL_API cugl_status cugl_lora_validate(const cugl_lora_desc *desc, const char *
  * that are replayed at the same time, need one each. */
 CUGL_API size_t      cugl_lora_workspace_bytes(const cugl_lora_desc *desc);
 /* starts: int32 [requests + 1], in order; request_adapters: int32 [requests]; ranks: int32 [adapters] or NULL (max_rank); scales: float
- * [adapters].  B and the workspace are 16-byte aligned, B's rows are read in whole units of 8 bytes.  dst may be base (then ld_dst == ld_base), else it overlaps nothing.  Two
- * launches; equal calls give equal bits.  tokens == 0 or requests == 0: nothing to do. */
+ * [adapters].  B and the workspace are 16-byte aligned, B's rows are read in whole units of 8 bytes.  dst may be base (then ld_dst ==
+ * ld_base), else it overlaps nothing.  One launch where requests are short (eight tokens or fewer on average), rows of x and A are 16-byte
+ * aligned and ranks at most 64, two otherwise; equal calls give equal bits.  tokens == 0 or requests == 0: nothing to do. */
 CUGL_API cugl_status cugl_lora(cugl_context *ctx, const cugl_lora_desc *desc, const void *d_x, const int32_t *d_starts,
                                const int32_t *d_request_adapters, const int32_t *d_ranks, const float *d_scales,
                                const void *d_a, const void *d_b, const void *d_base, void *d_dst, void *d_workspace,

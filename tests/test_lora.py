@@ -291,3 +291,103 @@ def test_call_refuses(ctx, change, word):
         ctx.lora(d, f.view(torch.uint8)[1:] if change == "x" else f, i, i, None, None if change == "null" else s, f, f[4:] if change == "b" else f, f, f, f,
                  workspace_bytes=100 if change == "workspace" else None)
     assert e.value.status == capi.INVALID_ARGUMENT and word in e.value.message
+
+
+# ---- short requests: both products in one launch; long ones in two -----------------------------------------------
+SHORT = [1, 2, 0, 17, 1, 33, 1, 1, 16, 1, 0, 1, 1, 3, 1, 15]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dst", TYPES)
+@pytest.mark.parametrize("max_rank", [1, 4, 8, 16, 20, 30, 32, 48, 64])
+def test_short_requests(ctx, max_rank, dtype, dst):
+    picks = [i % 4 - (i % 7 == 3) for i in range(len(SHORT))]
+    check(ctx, SHORT, picks, max_rank, 200, 520, dtype, dst, adapters=4)
+    check(ctx, SHORT, picks, max_rank, 72, 7000, dtype, dst, adapters=4, ranks=[max_rank, 0, max(1, max_rank // 3), max_rank - 1])
+    check(ctx, SHORT, picks, max_rank, 1032, 1001, dtype, dst, adapters=4, before=2)  # rows of base and dst start anywhere
+    check(ctx, SHORT, picks, max_rank, 64, 296, dtype, dst, adapters=4, in_place=True, pad=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [8, 60, 150, 300, 700])
+@pytest.mark.parametrize("max_rank", [16, 64])
+def test_many_short_requests(ctx, R, max_rank):
+    """Clusters of eight CTAs down to single ones, more blocks of channels than a CTA has asked for ahead."""
+    rng = np.random.default_rng(R)
+    check(ctx, rng.integers(0, 4, R).tolist(), rng.integers(-1, 3, R).tolist(), max_rank, 136, 2056, capi.BF16, capi.BF16, adapters=3)
+    check(ctx, [1] * R, rng.integers(-1, 3, R).tolist(), max_rank, 64, 1288, capi.F16, capi.F32, adapters=3, in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [1, 8, 63, 64, 65, 130, 4096])
+def test_short_requests_k(ctx, K):
+    """Fewer blocks of K than CTAs of a cluster, and more than stages."""
+    check(ctx, [1] * 9, [i % 3 for i in range(9)], 16, K, 264, capi.BF16, capi.F32, pad=-K % 8)
+    check(ctx, [2], [0], 32, K, 256, capi.F16, capi.F16, pad=-K % 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_rank", [16, 128])
+def test_many_long_requests(ctx, max_rank):
+    rng = np.random.default_rng(max_rank)
+    lengths = rng.integers(9, 21, 300).tolist()
+    check(ctx, lengths, rng.integers(-1, 3, 300).tolist(), max_rank, 64, 264, capi.BF16, capi.BF16, adapters=3)
+    check(ctx, lengths, rng.integers(-1, 3, 300).tolist(), max_rank, 36, 259, capi.F16, capi.F32, adapters=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank,k_block", [(16, 1), (64, 0), (64, 7)])
+def test_wait_limit_of_short_requests(ctx, rank, k_block):
+    test_wait_limit(ctx, [1] * 24, rank, k_block)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,rank", [(1, 16), (8, 32), (5, 64)])
+def test_short_requests_give_up_in_flight(ctx, tokens, rank):
+    test_gives_up_in_flight(ctx, tokens, rank)
+
+
+@pytest.mark.gpu
+def test_starts_of_long_requests_out_of_order(ctx):
+    import torch
+    M, R, N = 3000, 200, 72
+    d = capi.make_lora_desc(M, R, 2, 16, 128, N, capi.F16, capi.F16)
+    x = torch.ones((M, 128), dtype=torch.float16, device="cuda")
+    a, b = torch.ones((2, 16, 128), dtype=torch.float16, device="cuda"), torch.ones((2, N, 16), dtype=torch.float16, device="cuda")
+    base = torch.zeros((M, N), dtype=torch.float16, device="cuda")
+    out = torch.full((M + 4, N), 7.0, dtype=torch.float16, device="cuda")
+    ws = torch.full((capi.lora_workspace_bytes(d) + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(0)
+    for starts in (rng.integers(-2 ** 31, 2 ** 31 - 1, R + 1), np.where(np.arange(R + 1) % 2, 10 ** 9, -5), np.arange(R, -1, -1)):
+        ctx.lora(d, x, torch.tensor(starts, dtype=torch.int32, device="cuda"), torch.tensor(rng.integers(-3, 5, R), dtype=torch.int32, device="cuda"), None,
+                 torch.ones(2, device="cuda"), a, b, base, out, ws[:capi.lora_workspace_bytes(d)])
+        ctx.sync()
+        assert (out[M:] == 7).all() and (ws[-64:] == 0xFF).all()
+        assert np.isin(out[:M].double().cpu().numpy(), [7.0, 0.0, 2048.0]).all()
+
+
+@pytest.mark.gpu
+def test_captured_short_requests(ctx):
+    """A captured call, replayed with other requests in the same buffers, gives what the call gives."""
+    import torch
+    out, args = check(ctx, [1] * 24, [i % 3 for i in range(24)], 16, 256, 1288, capi.BF16, capi.BF16)
+    stream = torch.cuda.Stream()
+    own = capi.Context(0, stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            own.lora(*args)
+        for turn in range(3):
+            args[3].copy_(torch.tensor([(i + turn) % 4 - 1 for i in range(24)], dtype=torch.int32))
+            torch.cuda.synchronize()
+            ctx.lora(*args)
+            ctx.sync()
+            want = out.clone()
+            out.fill_(7)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[:24], want[:24])
+        del graph
+    finally:
+        own.close()
