@@ -2,10 +2,11 @@
 //   dst[t] = base[t] + scale_a * (x[t] . A_a^T) . B_a^T          a: the adapter of the request that token t belongs to
 //
 // Long requests take two launches, short ones have one that does the same for tiles of 16 tokens (lora_few_kernel: 24 requests of a token,
-// 4096 -> 14336, rank 16, BF16 9.3 us, in two launches 13.3).  The first makes v = x . A^T: a tile of up to 64 tokens of one request per cluster, whose CTAs share K; their sums are added
-// up in a fixed order through distributed shared memory.  The second adds scale * v . B^T to base, 256 channels x a tile of tokens per
-// CTA.  Which tiles there are is known on the device only (the requests' lengths): every CTA counts them (a scan over the requests)
-// and takes the one with its number; the grid is the most that there can be.
+// 4096 -> 14336, rank 16, BF16 9.3 us, in two launches 13.3).  The first makes v = x . A^T: a tile of up to 64 tokens of one request per
+// cluster, whose CTAs share K; their sums are added up in a fixed order through distributed shared memory.  The second adds
+// scale * v . B^T to base, 256 channels x a tile of tokens per item.  Which tiles there are is known on the device only (the requests'
+// lengths): every CTA counts them (a scan over the requests) and takes the one with its number, or every gridDim.x-th item; the grid is the
+// most that there can be.
 //
 // What bounds it: bytes.  x, base and dst pass once, the adapters once per tile of tokens.  The first product is one for tcgen05.mma (K is
 // long, its sums few); the second has K of at most 128 ranks, and all the rest of its time goes to base and dst, hence mma.sync, whose

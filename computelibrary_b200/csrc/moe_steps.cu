@@ -348,8 +348,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
 
 // ---- combination ---------------------------------------------------------------------------------------------
 // dst[t] = sum_j weights[t][j] * src[slots[t][j]], in the order of j, in float, rounded once.  Eight columns of a token per thread: all
-// its slots and weights are asked for together, then all its rows, before the first is used (slot by slot 29.6 us, this 27.7: 4096 x
-// 2048 BF16, eight choices, 85 % of the copy rate).  The bytes bound it.
+// its slots and weights are asked for together, then all its rows, before the first is used (slot by slot 29.6 us, this 27.8: 4096 x
+// 2048 BF16, eight choices, 84 % of the copy rate).  The bytes bound it.
 struct CombineParams
 {
     const uint8_t *src;
