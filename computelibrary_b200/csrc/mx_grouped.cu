@@ -161,7 +161,8 @@ __device__ __forceinline__ Item get_item(const GroupedParams &p, const int *befo
 
 // ---- what happens to sums ------------------------------------------------------------------------------------
 // silu(g) * u.  16-bit results take 2^x of the rounded product -g log2(e): off by 2^-20 + |g| 2^-23 of the result, where half a step of
-// theirs is 2^-11 or 2^-8; eight instructions instead of seventeen (768 channels, K = 2048, 512 rows a group: 67 -> 64 us).
+// theirs is 2^-11 or 2^-8; eight instructions instead of seventeen (768 channels, K = 2048, 512 rows a group: 67 -> 64 us).  For gates
+// from kSiluTail up.
 template <bool kShort>
 __device__ __forceinline__ float swiglu(float g, float u)
 {
@@ -189,11 +190,36 @@ __device__ __forceinline__ float group_bias(const GroupedParams &p, int g, int n
 {
     return p.bias != nullptr && n < p.channels ? __ldg(p.bias + static_cast<int64_t>(g) * p.channels + n) : 0.f;
 }
-template <bool kSwiglu, bool kShort = false>
-__device__ __forceinline__ float finish(uint32_t a, uint32_t u, const Factors &f, float bias)
+// Sixteen sums (of both products) to results; bias(i): of the i-th.  Gates in silu's tail are rare: one test for all of them, and the
+// whole sixteen once more where there is one.
+template <bool kSwiglu, bool kShort, typename Bias>
+__device__ __forceinline__ void finish(const uint32_t (&a)[16], const uint32_t (&u)[16], const Factors &f, Bias bias, float (&x)[16])
 {
-    if constexpr (kSwiglu) return swiglu<kShort>(__uint_as_float(a) * f.alpha, __uint_as_float(u) * f.up);
-    return __fmaf_rn(__uint_as_float(a), f.alpha, bias);
+    if constexpr (kSwiglu)
+    {
+        float least = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) least = fminf(least, __uint_as_float(a[i]) * f.alpha);
+        if (least >= kSiluTail)
+        {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = swiglu<kShort>(__uint_as_float(a[i]) * f.alpha, __uint_as_float(u[i]) * f.up);
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                const float g = __uint_as_float(a[i]) * f.alpha, v = __uint_as_float(u[i]) * f.up;
+                x[i]          = g < kSiluTail ? swiglu_tail(g, v) : swiglu<kShort>(g, v);
+            }
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __fmaf_rn(__uint_as_float(a[i]), f.alpha, bias(i));
+    }
 }
 
 // Sixteen tokens (rows m and up, `cols` of them valid) of a lane's channel n to dst.  Two-byte results of neighbouring channels leave
@@ -472,8 +498,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 if constexpr (kSwiglu) tmem_ld_x16(up + j, u);
                 tmem_ld_wait();
                 float x[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = finish<kSwiglu>(r[i], kSwiglu ? u[i] : 0u, f, b);
+                finish<kSwiglu, false>(r, u, f, [&](int) { return b; }, x);
                 store_tokens(p, it.row + j, n, x, it.count - j);
             }
             tc_fence_before();
@@ -821,12 +846,8 @@ __global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                     {
-                        float x[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) // elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
-                        {
-                            x[k] = finish<kSwiglu, true>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[2 * h + ((k >> 1) & 1)]);
-                        }
+                        float x[16]; // elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
+                        finish<kSwiglu, true>(r[h], u[h], f, [&](int k) { return bias[2 * h + ((k >> 1) & 1)]; }, x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                         {
@@ -856,8 +877,7 @@ __global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
                     for (int h = 0; h < 2; ++h) // sixteen tokens
                     {
                         float x[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) x[k] = finish<kSwiglu>(r[h][k], kSwiglu ? u[h][k] : 0u, f, bias[0]);
+                        finish<kSwiglu, false>(r[h], u[h], f, [&](int) { return bias[0]; }, x);
                         const int left = cols - 16 * h;
                         store_tokens(p, m + 16 * h, n0 + lane, x, left);
                     }

@@ -344,6 +344,16 @@ __device__ __forceinline__ float4 sum_partial(const float *part, int at, int shi
     return sum;
 }
 
+// silu(g) * u of gates far below zero, where 1 / (1 + exp(-g)) is exp(g) to 32 bits.  From -87 down that reciprocal is subnormal, and the
+// fast divisions make it 0, while the result is a normal number for as long as u is large enough: hence exp(g) as the square of
+// h = exp(g / 2), half of it on either factor.  h is normal down to g = -174, where the result is below 2^-115 whatever u is.
+constexpr float kSiluTail = -80.f;
+__device__ __forceinline__ float swiglu_tail(float g, float u)
+{
+    const float h = expf(0.5f * g);
+    return (g * h) * (h * u);
+}
+
 // scale tiles as rows of 512 bytes; box = box_rows tiles
 inline bool encode_scale_map(CUtensorMap *map, const void *base, int64_t tiles, int box_rows)
 {
