@@ -296,9 +296,12 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, const in
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        const float x = g[i] * p.gate_alpha;
-        const float v = weight[t[i]] * __fdividef(x, 1.f + expf(-x)) * (u[i] * p.up_alpha); // SwiGLU, the gate's weight folded in
-        h[i]          = f < p.inner ? v : 0.f;
+        const float x = g[i] * p.gate_alpha, v = u[i] * p.up_alpha;
+        h[i]          = weight[t[i]] * __fdividef(x, 1.f + expf(-x)) * v; // SwiGLU, the gate's weight folded in
+        // (a branch each: 48 tokens, top 4 of 64, MXFP4, 40.65 us, without the tail 40.4; one for all four 40.8, none 41.1, and these two lengthen
+        // the call of a single token by 0.3)
+        if (x < kSiluTail) h[i] = weight[t[i]] * swiglu_tail(x, v);
+        h[i]          = f < p.inner ? h[i] : 0.f;
         amax[i]       = __float_as_uint(h[i]) & 0x7fffffffu;
     }
     if (kFormat == CUGL_MXFP4)
