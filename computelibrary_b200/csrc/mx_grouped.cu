@@ -193,7 +193,7 @@ __device__ __forceinline__ float group_bias(const GroupedParams &p, int g, int n
 // Sixteen sums (of both products) to results; bias(i): of the i-th.  Gates in silu's tail are rare: one test for all of them, and the
 // whole sixteen once more where there is one.
 template <bool kSwiglu, bool kShort, typename Bias>
-__device__ __forceinline__ void finish(const uint32_t (&a)[16], const uint32_t (&u)[16], const Factors &f, Bias bias, float (&x)[16])
+__device__ __forceinline__ void finish_as(const uint32_t (&a)[16], const uint32_t (&u)[16], const Factors &f, Bias bias, float (&x)[16])
 {
     if constexpr (kSwiglu)
     {
@@ -220,6 +220,14 @@ __device__ __forceinline__ void finish(const uint32_t (&a)[16], const uint32_t (
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = __fmaf_rn(__uint_as_float(a[i]), f.alpha, bias(i));
     }
+}
+
+// The same function for a type in every kernel: a result does not depend on which one a rule chose.
+template <bool kSwiglu, typename Bias>
+__device__ __forceinline__ void finish(const GroupedParams &p, const uint32_t (&a)[16], const uint32_t (&u)[16], const Factors &f, Bias bias, float (&x)[16])
+{
+    if (kSwiglu && p.dtype != CUGL_F32) finish_as<kSwiglu, true>(a, u, f, bias, x);
+    else finish_as<kSwiglu, false>(a, u, f, bias, x);
 }
 
 // Sixteen tokens (rows m and up, `cols` of them valid) of a lane's channel n to dst.  Two-byte results of neighbouring channels leave
@@ -498,7 +506,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 if constexpr (kSwiglu) tmem_ld_x16(up + j, u);
                 tmem_ld_wait();
                 float x[16];
-                finish<kSwiglu, false>(r, u, f, [&](int) { return b; }, x);
+                finish<kSwiglu>(p, r, u, f, [&](int) { return b; }, x);
                 store_tokens(p, it.row + j, n, x, it.count - j);
             }
             tc_fence_before();
@@ -847,7 +855,7 @@ __global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
                     for (int h = 0; h < 2; ++h)
                     {
                         float x[16]; // elements 4 i + 0, 1 belong to row lane / 4, 4 i + 2, 3 to row lane / 4 + 8
-                        finish<kSwiglu, true>(r[h], u[h], f, [&](int k) { return bias[2 * h + ((k >> 1) & 1)]; }, x);
+                        finish_as<kSwiglu, true>(r[h], u[h], f, [&](int k) { return bias[2 * h + ((k >> 1) & 1)]; }, x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                         {
@@ -877,7 +885,7 @@ __global__ void __launch_bounds__((PairPlan<kFormat, kSwiglu>::THREADS), 1)
                     for (int h = 0; h < 2; ++h) // sixteen tokens
                     {
                         float x[16];
-                        finish<kSwiglu, false>(r[h], u[h], f, [&](int) { return bias[0]; }, x);
+                        finish<kSwiglu>(p, r[h], u[h], f, [&](int) { return bias[0]; }, x);
                         const int left = cols - 16 * h;
                         store_tokens(p, m + 16 * h, n0 + lane, x, left);
                     }

@@ -74,3 +74,20 @@ def test_gates_far_below_zero(ctx, fmt, dtype, expected, pad):
             got, want, tol = (np.where(beyond, 0, v) for v in (got, want, tol))
         bad = ~(np.abs(got - want) <= tol)
         assert not bad.any(), f"{bad.sum()} of {bad.size} off at gates {np.unique(g[bad])[:8]}: {got[bad][:3]} for {want[bad][:3]}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_bits_depend_on_the_values_alone(ctx, fmt, swiglu, dtype):
+    """expected_rows and the alignment of dst choose kernels and stores, never a result."""
+    import torch
+    from test_mx_grouped import check
+    counts = [300, 64, 5, 900, 0, 128]
+    want, args, _ = check(ctx, counts, 640, 768, fmt, dtype, swiglu, factors=True, expected=FEW)
+    for expected in (FEW, 500, MANY):
+        for pad in (0, 1, 2):
+            out, _, _ = check(ctx, counts, 640, 768, fmt, dtype, swiglu, factors=True, expected=expected, pad=pad)
+            for start, count in args[3].tolist():
+                assert torch.equal(out[start:start + count, :640], want[start:start + count])
