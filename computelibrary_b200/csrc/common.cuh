@@ -16,7 +16,7 @@ struct cugl_context
     int          sm_count    = 0;
     cudaStream_t stream      = nullptr;
     bool         owns_stream = false;
-    int32_t     *d_status    = nullptr; // device word written by kernels whose bounded waits ran out
+    int32_t     *d_status    = nullptr; // device words, see DeviceStatus
     int32_t     *h_status    = nullptr; // pinned mirror read in cugl_sync
     long long   *d_trace     = nullptr; // optional event-timestamp buffer for the tensor-core GEMM kernels
     long long    spin_limit  = 4000000000ll; // clock64 ticks a device-side wait may last (about two seconds)
@@ -51,7 +51,13 @@ cugl_status check_cuda(cugl_context *ctx, cudaError_t e, const char *what);
         }                                \
     } while (0)
 
-// Device status codes (written to cugl_context::d_status)
+// Words of cugl_context::d_status, one for each kind of report: neither hides the other.
+enum DeviceStatus : int32_t
+{
+    STATUS_WAIT  = 0, // the first bounded wait that ran out (DEV_TIMEOUT_*): results are invalid
+    STATUS_GROUP = 1, // DEV_BAD_GROUP: a group was left out
+    STATUS_WORDS = 2
+};
 enum : int32_t
 {
     DEV_OK               = 0,
@@ -59,7 +65,7 @@ enum : int32_t
     DEV_TIMEOUT_MMA      = 2,
     DEV_TIMEOUT_EPILOGUE = 3,
     DEV_TIMEOUT_DRAIN    = 4,
-    DEV_BAD_GROUP        = 5 // cugl_mx_grouped_gemm: a group that does not lie within the rows
+    DEV_BAD_GROUP        = 1 // cugl_mx_grouped_gemm: a group that does not lie within the rows
 };
 
 // Everything an epilogue needs to turn a raw sum_k A*B accumulator into the function's output.

@@ -90,22 +90,22 @@ extern "C"
             }
             ctx->owns_stream = true;
         }
-        cudaError_t e = cudaMalloc(&ctx->d_status, sizeof(int32_t));
+        cudaError_t e = cudaMalloc(&ctx->d_status, cugl::STATUS_WORDS * sizeof(int32_t));
         if (e == cudaSuccess)
         {
-            e = cudaMemset(ctx->d_status, 0, sizeof(int32_t));
+            e = cudaMemset(ctx->d_status, 0, cugl::STATUS_WORDS * sizeof(int32_t));
         }
         if (e == cudaSuccess)
         {
-            e = cudaMallocHost(&ctx->h_status, sizeof(int32_t));
+            e = cudaMallocHost(&ctx->h_status, cugl::STATUS_WORDS * sizeof(int32_t));
         }
         if (e != cudaSuccess)
         {
             cugl_context_destroy(ctx);
-            return check_cuda(nullptr, e, "context status word");
+            return check_cuda(nullptr, e, "context status words");
         }
-        *ctx->h_status = 0;
-        *out           = ctx;
+        for (int i = 0; i < cugl::STATUS_WORDS; ++i) ctx->h_status[i] = 0;
+        *out = ctx;
         return CUGL_SUCCESS;
     }
 
@@ -370,22 +370,27 @@ extern "C"
     cugl_status cugl_sync(cugl_context *ctx)
     {
         CUGL_NEED_CTX(ctx);
-        CUGL_CUDA_TRY(ctx, cudaMemcpyAsync(ctx->h_status, ctx->d_status, sizeof(int32_t), cudaMemcpyDeviceToHost,
+        CUGL_CUDA_TRY(ctx, cudaMemcpyAsync(ctx->h_status, ctx->d_status, cugl::STATUS_WORDS * sizeof(int32_t), cudaMemcpyDeviceToHost,
                                            ctx->stream));
         CUGL_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
-        if (*ctx->h_status != 0)
+        const int32_t wait = ctx->h_status[cugl::STATUS_WAIT], group = ctx->h_status[cugl::STATUS_GROUP];
+        if (wait != 0 || group != 0)
         {
-            const int32_t code = *ctx->h_status;
-            *ctx->h_status     = 0;
-            cudaMemsetAsync(ctx->d_status, 0, sizeof(int32_t), ctx->stream);
+            for (int i = 0; i < cugl::STATUS_WORDS; ++i) ctx->h_status[i] = 0;
+            cudaMemsetAsync(ctx->d_status, 0, cugl::STATUS_WORDS * sizeof(int32_t), ctx->stream);
             cudaStreamSynchronize(ctx->stream);
-            if (code == cugl::DEV_BAD_GROUP)
+            std::string what;
+            if (wait != 0)
             {
-                return fail(ctx, CUGL_RUNTIME_ERROR, "cugl_mx_grouped_gemm: a group did not start at a multiple of 128 or did not lie within the rows, or groups overlapped; it was left out");
+                what = "device-side bounded wait ran out (code " + std::to_string(wait) +
+                       ": 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 4 = drain); results are invalid";
             }
-            return fail(ctx, CUGL_RUNTIME_ERROR,
-                        "device-side bounded wait ran out (code " + std::to_string(code) +
-                            ": 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 4 = drain); results are invalid");
+            if (group != 0)
+            {
+                what += std::string(wait != 0 ? "; besides, " : "") +
+                        "cugl_mx_grouped_gemm: a group did not start at a multiple of 128 or did not lie within the rows, or groups overlapped; it was left out";
+            }
+            return fail(ctx, CUGL_RUNTIME_ERROR, what);
         }
         return CUGL_SUCCESS;
     }

@@ -67,7 +67,7 @@ __device__ __forceinline__ int scan_groups(const GroupedParams &p, int *before)
         bool       bad;
         const int2 v  = load_group(p, g, bad);
         before[g + 1] = (v.y + kTile - 1) / kTile;
-        if (bad && blockIdx.x == 0) atomicCAS(p.status, 0, DEV_BAD_GROUP);
+        if (bad && blockIdx.x == 0) atomicExch(p.status + STATUS_GROUP, DEV_BAD_GROUP);
     }
     if (threadIdx.x == 0) before[0] = 0;
     __syncthreads();
@@ -94,7 +94,7 @@ __device__ __forceinline__ int scan_groups(const GroupedParams &p, int *before)
     const int tiles = before[p.n_groups];
     if (tiles > (p.rows + kSlab - 1) / kSlab)
     {
-        if (threadIdx.x == 0 && blockIdx.x == 0) atomicCAS(p.status, 0, DEV_BAD_GROUP);
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(p.status + STATUS_GROUP, DEV_BAD_GROUP);
         return 0;
     }
     return tiles;

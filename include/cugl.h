@@ -733,7 +733,7 @@ CUGL_API cugl_status cugl_mx_grouped_gemm_validate(const cugl_mx_grouped_gemm_de
 /* One launch, no workspace, nothing kept between calls.  d_b_alpha, d_up_alpha: float [groups] or NULL (1).  Operands and scale tiles
  * are 16-byte aligned, dst overlaps none of them.  Equal calls give equal bits.  A group that does not start at a multiple of 128 or does not
  * lie within the rows is left out; groups that overlap so much that they have more tiles than the rows are all left out.  The next cugl_sync()
- * reports either as CUGL_RUNTIME_ERROR.  rows == 0: nothing to do. */
+ * reports either as CUGL_RUNTIME_ERROR, beside a wait that ran out if there was one.  rows == 0: nothing to do. */
 CUGL_API cugl_status cugl_mx_grouped_gemm(cugl_context *ctx, const cugl_mx_grouped_gemm_desc *desc, const void *d_a,
                                           const void *d_a_scales, const int32_t *d_groups, const void *d_b,
                                           const void *d_b_scales, const float *d_b_alpha, const void *d_up,

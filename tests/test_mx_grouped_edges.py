@@ -91,3 +91,56 @@ def test_bits_depend_on_the_values_alone(ctx, fmt, swiglu, dtype):
             out, _, _ = check(ctx, counts, 640, 768, fmt, dtype, swiglu, factors=True, expected=expected, pad=pad)
             for start, count in args[3].tolist():
                 assert torch.equal(out[start:start + count, :640], want[start:start + count])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("expected", [FEW, MANY])
+def test_a_bad_group_does_not_hide_a_wait_that_ran_out(ctx, expected):
+    """Both in one launch: the sync says that results are invalid, and names the group too; the next call is as always."""
+    import torch
+    from test_mx_grouped import check
+    out, args, kw = check(ctx, [300, 0, 5, 900], 640, 2048, capi.NVFP4, capi.F32, expected=expected)
+    want, groups = out.clone(), args[3]
+    groups[1] = torch.tensor([64, 10], dtype=torch.int32, device="cuda")
+    ctx.set_wait_limit_us(20000)
+    try:
+        ctx.withhold_copy_once(1)
+        ctx.mx_grouped_gemm(*args, **kw)
+        with pytest.raises(capi.CuglError) as e:
+            ctx.sync()
+    finally:
+        ctx.set_wait_limit_us(0)
+    assert e.value.status == capi.RUNTIME_ERROR
+    assert "wait ran out" in e.value.message and "invalid" in e.value.message and "group" in e.value.message
+    ctx.mx_grouped_gemm(*args, **kw)  # each is forgotten by itself
+    with pytest.raises(capi.CuglError) as e:
+        ctx.sync()
+    assert "group" in e.value.message and "wait ran out" not in e.value.message
+    groups[1] = 0
+    out.fill_(7)
+    ctx.mx_grouped_gemm(*args, **kw)
+    ctx.sync()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("expected", [FEW, MANY])
+def test_a_bad_group_does_not_hide_an_earlier_or_later_wait(ctx, expected):
+    import torch
+    from test_mx_grouped import check
+    _, args, kw = check(ctx, [300, 0, 5, 900], 640, 2048, capi.NVFP4, capi.F32, expected=expected)
+    bad = (*args[:3], args[3].clone(), *args[4:])
+    bad[3][1] = torch.tensor([64, 10], dtype=torch.int32, device="cuda")
+    for order in ((args, bad), (bad, args)):
+        ctx.set_wait_limit_us(20000)
+        try:
+            for a in order:
+                if a is args:
+                    ctx.withhold_copy_once(1)
+                ctx.mx_grouped_gemm(*a, **kw)
+            with pytest.raises(capi.CuglError) as e:
+                ctx.sync()
+        finally:
+            ctx.set_wait_limit_us(0)
+        assert "wait ran out" in e.value.message and "group" in e.value.message
+        ctx.sync()
