@@ -255,7 +255,7 @@ __device__ __forceinline__ float token_v(const LoraParams &p, const Tile &t, con
         for (int q = 1; q < kMaxSplit; ++q) v[i] += parts[i][q];
         if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
     }
-    float factor = __ldg(p.scales + t.adapter);
+    float factor = p.scales[t.adapter];
     float mul    = 1.f;
     if constexpr (std::is_same<T, __half>::value)
     {

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
             const int   wb = tile % w_blocks, tb = tile / w_blocks;
             const int   as = it % P::ACC;
             const int   n  = wb * kMxRows + q * 32 + lane;
-            const float b  = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
+            const float b  = p.bias != nullptr && n < p.channels ? p.bias[n] : 0.f;
             if (!warp_wait(tfull_bar(as), static_cast<uint32_t>(it / P::ACC) & 1u, s_abort, DEV_TIMEOUT_EPILOGUE, p.spin_limit))
             {
                 break;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__((MxPlan<kFormat, NT, STAGES, kSplit>::THREADS)
         {
             const int    own = kMxRows >> shift, et = threadIdx.x - 32 * kFirstEpi;
             const int    n = wb * kMxRows + rank * own + (et & (own - 1));
-            const float  b = p.bias != nullptr && n < p.channels ? __ldg(p.bias + n) : 0.f;
+            const float  b = p.bias != nullptr && n < p.channels ? p.bias[n] : 0.f;
             const float *part = reinterpret_cast<const float *>(smem + P::OFF_PART);
             if (n < p.channels)
             {
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int i = 0; i < (kBulk == 2 ? 4 : 1); ++i)
                 {
                     const int n = n0 + (kBulk == 2 ? lane / 4 + 8 * i : lane);
-                    bias[i]     = n < p.channels ? __ldg(p.bias + n) : 0.f;
+                    bias[i]     = n < p.channels ? p.bias[n] : 0.f;
                 }
             }
 #pragma unroll 1

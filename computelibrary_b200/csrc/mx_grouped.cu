@@ -175,6 +175,8 @@ __device__ __forceinline__ float swiglu(float g, float u)
     }
     return __fdividef(g, 1.f + expf(-g)) * u;
 }
+// (Plain loads, here and wherever a kernel reads what a launch ahead may have written: read-only ones assume that nothing writes while the
+// kernel runs, and it has run since before griddepcontrol.wait.)
 struct Factors
 {
     float alpha, up;
@@ -182,13 +184,13 @@ struct Factors
 __device__ __forceinline__ Factors group_factors(const GroupedParams &p, int g)
 {
     Factors f{p.alpha, p.up_scale};
-    if (p.b_alpha != nullptr) f.alpha *= __ldg(p.b_alpha + g);
-    if (p.up_alpha != nullptr) f.up *= __ldg(p.up_alpha + g);
+    if (p.b_alpha != nullptr) f.alpha *= p.b_alpha[g];
+    if (p.up_alpha != nullptr) f.up *= p.up_alpha[g];
     return f;
 }
 __device__ __forceinline__ float group_bias(const GroupedParams &p, int g, int n)
 {
-    return p.bias != nullptr && n < p.channels ? __ldg(p.bias + static_cast<int64_t>(g) * p.channels + n) : 0.f;
+    return p.bias != nullptr && n < p.channels ? p.bias[static_cast<int64_t>(g) * p.channels + n] : 0.f;
 }
 // Sixteen sums (of both products) to results; bias(i): of the i-th.  Gates in silu's tail are rare: one test for all of them, and the
 // whole sixteen once more where there is one.

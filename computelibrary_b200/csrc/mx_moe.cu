@@ -69,7 +69,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
     for (int i = 0; i < kPer; ++i)
     {
         const int   e = i * 32 + lane;
-        const float v = e < p.experts ? __ldg(row + e) : -INFINITY;
+        const float v = e < p.experts ? row[e] : -INFINITY;
         const uint32_t b = __float_as_uint(v + 0.f); // -0 and 0 are equal logits
         key[i] = v > -INFINITY ? ((b >> 31) != 0 ? ~b : b | 0x80000000u) : 0u;
         if (v > top) top = v;
@@ -83,7 +83,7 @@ __device__ __forceinline__ void route_token(const MoeParams &p, int t, int lane)
         for (int i = 0; i < kPer; ++i)
         {
             const int e = i * 32 + lane;
-            if (e < p.experts && key[i] != 0) all += expf(__ldg(row + e) - top);
+            if (e < p.experts && key[i] != 0) all += expf(row[e] - top);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
@@ -143,7 +143,7 @@ __device__ __forceinline__ void quantize_tokens(const MoeParams &p, int block, i
     {
         if (p.vec_x != 0)
         {
-            uint4 q[2] = {__ldg(reinterpret_cast<const uint4 *>(src)), __ldg(reinterpret_cast<const uint4 *>(src) + 1)};
+            uint4 q[2] = {reinterpret_cast<const uint4 *>(src)[0], reinterpret_cast<const uint4 *>(src)[1]};
             const T *e = reinterpret_cast<const T *>(q);
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
@@ -298,8 +298,8 @@ __device__ __forceinline__ void store_hidden(const MoeParams &p, int a, const in
     {
         const float x = g[i] * p.gate_alpha, v = u[i] * p.up_alpha;
         h[i]          = weight[t[i]] * __fdividef(x, 1.f + expf(-x)) * v; // SwiGLU, the gate's weight folded in
-        // (a branch each: 48 tokens, top 4 of 64, MXFP4, 40.65 us, without the tail 40.4; one for all four 40.8, none 41.1, and these two lengthen
-        // the call of a single token by 0.3)
+        // (a branch each: 48 tokens, top 4 of 64, MXFP4, 40.65 us, without the tail 40.45; one for all four 40.8, none 41.1.  A single token: 14.85
+        // without, 15.0, 15.1 and 15.2)
         if (x < kSiluTail) h[i] = weight[t[i]] * swiglu_tail(x, v);
         h[i]          = f < p.inner ? h[i] : 0.f;
         amax[i]       = __float_as_uint(h[i]) & 0x7fffffffu;

@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint8_t *src, in
 #pragma unroll
         for (int j = 0; j < 4; ++j)
         {
-            if (b0 + j < blocks) w |= static_cast<uint32_t>(__ldg(src + row * ld + b0 + j)) << (8 * j);
+            if (b0 + j < blocks) w |= static_cast<uint32_t>(src[row * ld + b0 + j]) << (8 * j);
         }
         *reinterpret_cast<uint32_t *>(dst + mx_scale_offset(row, b0, tiles)) = w;
     }
