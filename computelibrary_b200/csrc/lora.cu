@@ -45,6 +45,7 @@ struct LoraParams
     int64_t        ld_x, ld_a, ld_b, ld_base, ld_dst; // bytes
     int            tokens, requests, n_adapters, max_rank, K, N, parts, tile;
     int            tiles; // at most
+    int            chains; // accumulators of a sum on tcgen05.mma: 1 or kChains
     uint32_t       idesc; // of no columns
     int32_t       *status;
     long long      spin_limit;
@@ -314,6 +315,28 @@ __device__ __forceinline__ void finish_v(const LoraParams &p, const Tile &t, con
 // instructions took twice as long (prompts of 4096 tokens, K = 4096, ranks up to 64: 20.6 -> 14.2 us under ncu).  Of the 128 rows of an MMA only
 // the adapter's count; the others are whatever shared memory holds behind them.  Rows of x behind the tile belong to other requests:
 // columns that nobody reads.
+//
+// An accumulator in tensor memory is cut to 24 bits at every step, not rounded, and v's error grows with their number.  Where results have 32
+// bits, four of them take the blocks of K in turn and are added up as floats (prompts of 4096 tokens, K = 4096, ranks up to 64, F16 to
+// F32, relative error against 64 bits: one 4.9e-7, four 1.6e-7, the plain 32-bit form 2.1e-7; 42.8 -> 43.1 us, 24 requests of a token at rank 16 6.9 -> 7.1); 16-bit results
+// have one.
+constexpr int kChains = 4;
+// The sums of sixteen columns of `chains` accumulators, `gap` columns apart.  (One at a time: registers that the first launch needs more than
+// 64 of keep the second from starting beside it, 11.2 -> 12.7 us for 8 requests of 32 tokens at rank 128.)
+__device__ __forceinline__ void add_chains(uint32_t tmem, int gap, int chains, float (&sum)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+#pragma unroll 1
+    for (int q = 0; q < chains; ++q)
+    {
+        uint32_t v[16];
+        tmem_ld_x16(tmem + q * gap, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i] += __uint_as_float(v[i]);
+    }
+}
 template <int kRank>
 struct ShrinkMma
 {
@@ -323,8 +346,8 @@ struct ShrinkMma
     static constexpr int kPitch  = kRank + 1;                                       // floats of a token's sums
     static constexpr int kOffBar = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384); // an MMA reads 16 KB from a stage's start on
     static constexpr int kSmem   = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
-    static constexpr int kColumns = 64;
-    static_assert(kTile * kPitch * 4 <= kOffBar && kTile <= kColumns, "sums fit where the stages were, and in tensor memory");
+    static constexpr int kColumns = kChains * kTile; // two CTAs to an SM
+    static_assert(kTile * kPitch * 4 <= kOffBar && 2 * kColumns <= 512, "sums fit where the stages were, and in tensor memory");
 };
 inline uint32_t f16_idesc(bool bf16) // float sums, 128 rows; add columns / 8 << 17
 {
@@ -427,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (el)
             {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16(tmem, a_desc + 2u * k, b_desc + 2u * k, idesc, (g | k) != 0 ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) umma_f16(tmem + (g & (p.chains - 1)) * S::kTile, a_desc + 2u * k, b_desc + 2u * k, idesc, g >= p.chains || k != 0 ? 1u : 0u);
                 umma_commit(empty_bar(s));
             }
             __syncwarp();
@@ -443,16 +466,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (ok && *s_abort == 0 && (warp & 3) * 32 < kRank && c0 < t.count)
     {
         tc_fence_after();
-        uint32_t v[32];
-        tmem_ld_x32(tmem + c0 + (static_cast<uint32_t>((warp & 3) * 32) << 16), v);
-        tmem_ld_wait();
-        if (r < kRank)
+#pragma unroll 1
+        for (int c = c0; c < min(c0 + 32, t.count); c += 16)
         {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
+            float v[16];
+            add_chains(tmem + c + (static_cast<uint32_t>((warp & 3) * 32) << 16), S::kTile, min(n_blocks, p.chains), v);
+            if (r < kRank)
             {
-                if (c0 + i < t.count) share[(c0 + i) * S::kPitch + r] = n_blocks > 0 && r < t.rank ? __uint_as_float(v[i]) : 0.f; // behind the adapter's ranks: zeros
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    if (c + i < t.count) share[(c + i) * S::kPitch + r] = r < t.rank ? v[i] : 0.f; // behind the adapter's ranks: zeros
+                }
             }
+            __syncwarp(); // aligned loads are next
         }
     }
     tc_fence_before();
@@ -966,13 +993,14 @@ struct Few
     static constexpr bool kKept   = kRank == 16;                           // v in registers
     static constexpr int kStages  = kRank == 64 ? 6 : 8;
     static constexpr int kA       = kRank * 128, kX = kTile * 128, kStage = kA + kX;
-    static constexpr int kSums    = kRank + 1;                                                   // floats of a token's sums
+    static constexpr int kShare   = kRank + 1;                                                   // floats of a token's sums
     static constexpr int kOffV    = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384);  // an MMA reads 16 KB from a stage's start on
     static constexpr int kPitch   = kRank * 2 + 16;                                              // bytes of a row of v, its factor included
     static constexpr int kOffBar  = kOffV + kParts * kTile * kPitch;
     static constexpr int kSmem    = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
-    static constexpr int kColumns = 32;
-    static_assert(kTile * kSums * 4 <= kOffV && kStage % 1024 == 0, "sums fit where the stages were");
+    static constexpr int kChained = sizeof(TD) == 4 ? kChains : 1;                               // see add_chains
+    static constexpr int kColumns = kChained == 1 ? 32 : kChained * kTile;
+    static_assert(kTile * kShare * 4 <= kOffV && kStage % 1024 == 0, "sums fit where the stages were");
 };
 template <typename T, typename TD, int kRank, bool kVec>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -1132,7 +1160,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (el)
             {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) umma_f16(tmem, a_desc + 2u * k, b_desc + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) umma_f16(tmem + i % S::kChained * S::kTile, a_desc + 2u * k, b_desc + 2u * k, idesc, i >= S::kChained || k != 0 ? 1u : 0u);
                 umma_commit(empty_bar(s));
             }
             __syncwarp();
@@ -1150,15 +1178,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (ok && *s_abort == 0 && warp * 32 < kRank) // sums to shared memory, [token][rank]: a lane has a rank
         {
             tc_fence_after();
-            uint32_t v[16];
-            tmem_ld_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16), v);
-            tmem_ld_wait();
+            float v[16];
+            add_chains(tmem + (static_cast<uint32_t>(warp * 32) << 16), S::kTile, min(n_blocks, S::kChained), v);
             if (r < kRank)
             {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                 {
-                    if (i < t.count) share[i * S::kSums + r] = n_blocks > 0 && r < t.rank ? __uint_as_float(v[i]) : 0.f; // behind the adapter's ranks: zeros
+                    if (i < t.count) share[i * S::kShare + r] = r < t.rank ? v[i] : 0.f; // behind the adapter's ranks: zeros
                 }
             }
         }
@@ -1183,7 +1210,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int tok = warp; tok < t.count; tok += kWarps) // (of a CTA that has given up: nothing of use)
         {
             uint8_t *const row    = area + tok * S::kPitch;
-            const float    factor = token_v<T, kRank>(p, t, share, S::kSums, ranks, tok, [&](int part, int place, uint16_t bits) {
+            const float    factor = token_v<T, kRank>(p, t, share, S::kShare, ranks, tok, [&](int part, int place, uint16_t bits) {
                 *reinterpret_cast<uint16_t *>(row + part * S::kTile * S::kPitch + place * 2) = bits;
             });
             if (lane == 0) *reinterpret_cast<float *>(row + kRank * 2) = factor;
@@ -1539,6 +1566,7 @@ extern "C"
         const bool vec_out = even(d_base, desc->ld_base) && even(d_dst, desc->ld_dst) && desc->N % 8 == 0;
         const int64_t tiles = most_tiles(*desc, p.tile), few_tiles = most_tiles(*desc, 16);
         p.tiles             = static_cast<int>(tiles);
+        p.chains            = desc->dst_dtype == CUGL_F32 ? kChains : 1;
         p.idesc             = f16_idesc(desc->dtype == CUGL_BF16);
         p.status            = ctx->d_status;
         p.spin_limit        = ctx->spin_limit;
