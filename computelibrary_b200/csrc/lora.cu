@@ -346,8 +346,12 @@ struct ShrinkMma
     static constexpr int kPitch  = kRank + 1;                                       // floats of a token's sums
     static constexpr int kOffBar = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384); // an MMA reads 16 KB from a stage's start on
     static constexpr int kSmem   = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
-    static constexpr int kColumns = kChains * kTile; // two CTAs to an SM
-    static_assert(kTile * kPitch * 4 <= kOffBar && 2 * kColumns <= 512, "sums fit where the stages were, and in tensor memory");
+    // Tensor-memory columns, and shared memory, of which a CTA takes at least as large a part of the SM's (512 columns, 228 KB).  Allocating
+    // columns waits until there are enough of them, and a CTA of a cluster that waits keeps the others of its cluster, and theirs, where they
+    // are: were there more CTAs on an SM than its tensor memory holds, of calls on two streams for instance, they could wait for each other.
+    __host__ __device__ static constexpr int columns(int chains) { return chains * kTile; }
+    static constexpr int smem(int chains) { return columns(chains) <= 128 ? kSmem : kSmem > 115200 ? kSmem : 115200; }
+    static_assert(kTile * kPitch * 4 <= kOffBar && columns(kChains) <= 256 && 128 * 456 <= kSmem, "sums fit where the stages were, and in tensor memory");
 };
 inline uint32_t f16_idesc(bool bf16) // float sums, 128 rows; add columns / 8 << 17
 {
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     if (warp == 1)
     {
-        tmem_alloc(smem_u32(s_tmem), S::kColumns);
+        tmem_alloc(smem_u32(s_tmem), static_cast<uint32_t>(S::columns(p.chains)));
     }
     tc_fence_before();
     __syncthreads();
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const Tile t     = find_tile(p, static_cast<int>(cluster_id_x()));
     if (t.count == 0 || t.adapter < 0) // the same for the cluster
     {
-        if (warp == 1) tmem_dealloc(tmem, S::kColumns);
+        if (warp == 1) tmem_dealloc(tmem, static_cast<uint32_t>(S::columns(p.chains)));
         return;
     }
     const int blocks = (p.K + 63) / 64; // of 64 columns, shared by the CTAs of the cluster
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     {
         if (gone) drain_mmas<false>(gone_bar, p.spin_limit);
         tc_fence_after();
-        tmem_dealloc(tmem, S::kColumns);
+        tmem_dealloc(tmem, static_cast<uint32_t>(S::columns(p.chains)));
     }
     if (threadIdx.x == 0 && gone)
     {
@@ -1000,6 +1004,7 @@ struct Few
     static constexpr int kSmem    = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
     static constexpr int kChained = sizeof(TD) == 4 ? kChains : 1;                               // see add_chains
     static constexpr int kColumns = kChained == 1 ? 32 : kChained * kTile;
+    static_assert(kColumns * 456 <= kSmem, "see ShrinkMma::columns");
     static_assert(kTile * kShare * 4 <= kOffV && kStage % 1024 == 0, "sums fit where the stages were");
 };
 template <typename T, typename TD, int kRank, bool kVec>
@@ -1376,9 +1381,9 @@ cugl_status launch_shrink_mma(cugl_context *ctx, const LoraParams &p, int64_t ti
     }
     auto                     kernel  = lora_shrink_mma_kernel<T, kRank>;
     static std::atomic<bool> set[64] = {};
-    CUGL_TRY(allow_smem(ctx, kernel, S::kSmem, set));
+    CUGL_TRY(allow_smem(ctx, kernel, S::smem(kChains), set));
     const int split = shrink_split(ctx, p, tiles);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, map_a, map_x, map_few, p));
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::smem(p.chains), split, tiles * split, map_a, map_x, map_few, p));
     return CUGL_SUCCESS;
 }
 template <typename T, int kRank, int kIn>

@@ -45,3 +45,41 @@ def test_long_sums_are_four_shorter_ones(ctx, requests, each, rank, dtype):
     tol = 2 * 2.0 ** -21 * want + 5 * 2.0 ** -24 * want.amax(1, keepdim=True) + 4 * 2.0 ** -24 * want  # (the quarters add up to one value)
     off = (got - want).abs()
     assert (off <= tol).all(), f"off by {(off / want).max().item():.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [capi.F16, capi.BF16])
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+def test_calls_on_three_streams(ctx, rank, dtype):
+    """Short requests, long ones and products at once, again and again: every call gives what it gives alone.  (Their clusters share SMs and
+    their tensor memory.)"""
+    import torch
+    from test_mx_inputs_ahead import stored
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    own = [capi.Context(0, s.cuda_stream) for s in streams]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a, b = stored(g, 48, 4096, capi.NVFP4), stored(g, 2048, 4096, capi.NVFP4)
+    product = torch.zeros((48, 2048), device="cuda")
+    d = capi.make_mx_gemm_desc(48, 2048, 4096, capi.NVFP4, capi.F32)
+    try:
+        short, short_args = check(ctx, [1] * 28, [i % 3 for i in range(28)], min(rank, 64), 4096, 1032, dtype, capi.F32)
+        long, long_args = check(ctx, [200, 1, 77, 300], [0, 1, 2, 0], rank, 4096, 1032, dtype, capi.F32)
+        ctx.mx_gemm(d, *a, *b, None, product)
+        ctx.sync()
+        outs = (short, long, product)
+        want = [o.clone() for o in outs]
+        for o in outs:
+            o.fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(200):
+            own[0].lora(*short_args)
+            own[1].lora(*long_args)
+            own[2].mx_gemm(d, *a, *b, None, product)
+        for c in own:
+            c.sync()
+        for o, w in zip(outs, want):
+            rows = w != 7
+            assert torch.equal(o[rows], w[rows])
+    finally:
+        for c in own:
+            c.close()
