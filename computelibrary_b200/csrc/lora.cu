@@ -318,7 +318,7 @@ __device__ __forceinline__ void finish_v(const LoraParams &p, const Tile &t, con
 //
 // An accumulator in tensor memory is cut to 24 bits at every step, not rounded, and v's error grows with their number.  Where results have 32
 // bits, four of them take the blocks of K in turn and are added up as floats (prompts of 4096 tokens, K = 4096, ranks up to 64, F16 to
-// F32, relative error against 64 bits: one 4.9e-7, four 1.6e-7, the plain 32-bit form 2.1e-7; 42.8 -> 43.1 us, 24 requests of a token at rank 16 6.9 -> 7.1); 16-bit results
+// F32, relative error against 64 bits: one 4.9e-7, four 1.6e-7, the plain 32-bit form 2.1e-7; 42.8 -> 43.1 us, 24 requests of a token at rank 16 6.9 -> 7.2); 16-bit results
 // have one.
 constexpr int kChains = 4;
 // The sums of sixteen columns of `chains` accumulators, `gap` columns apart.  (One at a time: registers that the first launch needs more than
@@ -346,12 +346,8 @@ struct ShrinkMma
     static constexpr int kPitch  = kRank + 1;                                       // floats of a token's sums
     static constexpr int kOffBar = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384); // an MMA reads 16 KB from a stage's start on
     static constexpr int kSmem   = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
-    // Tensor-memory columns, and shared memory, of which a CTA takes at least as large a part of the SM's (512 columns, 228 KB).  Allocating
-    // columns waits until there are enough of them, and a CTA of a cluster that waits keeps the others of its cluster, and theirs, where they
-    // are: were there more CTAs on an SM than its tensor memory holds, of calls on two streams for instance, they could wait for each other.
-    __host__ __device__ static constexpr int columns(int chains) { return chains * kTile; }
-    static constexpr int smem(int chains) { return columns(chains) <= 128 ? kSmem : kSmem > 115200 ? kSmem : 115200; }
-    static_assert(kTile * kPitch * 4 <= kOffBar && columns(kChains) <= 256 && 128 * 456 <= kSmem, "sums fit where the stages were, and in tensor memory");
+    __host__ __device__ static constexpr int columns(int chains) { return chains * kTile; } // of tensor memory; see Few::kSmem
+    static_assert(kTile * kPitch * 4 <= kOffBar && columns(kChains) <= 256, "sums fit where the stages were, and in tensor memory");
 };
 inline uint32_t f16_idesc(bool bf16) // float sums, 128 rows; add columns / 8 << 17
 {
@@ -1001,10 +997,15 @@ struct Few
     static constexpr int kOffV    = (kStages - 1) * kStage + (kStage > 16384 ? kStage : 16384);  // an MMA reads 16 KB from a stage's start on
     static constexpr int kPitch   = kRank * 2 + 16;                                              // bytes of a row of v, its factor included
     static constexpr int kOffBar  = kOffV + kParts * kTile * kPitch;
-    static constexpr int kSmem    = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
-    static constexpr int kChained = sizeof(TD) == 4 ? kChains : 1;                               // see add_chains
+    // Allocating columns of tensor memory waits until there are enough of them, and a CTA of a cluster that waits keeps the others of its
+    // cluster where they are: were there more CTAs on an SM than its tensor memory holds, of calls on two streams for instance, they could wait
+    // for each other.  So this CTA takes shared memory enough not to fit beside two that have half of tensor memory each (ShrinkMma's with four
+    // chains, 90 KB, and the products' and the expert layer's, 88 KB or more).
+    static constexpr int kNeeded  = kOffBar + (2 * kStages + 2) * 8 + 16 + 1024;
+    static constexpr int kSmem    = kNeeded > 57344 ? kNeeded : 57344;
+    static constexpr int kChained = sizeof(TD) == 4 ? kChains : 1; // see add_chains
     static constexpr int kColumns = kChained == 1 ? 32 : kChained * kTile;
-    static_assert(kColumns * 456 <= kSmem, "see ShrinkMma::columns");
+    static_assert(kSmem + 2 * 88176 > 228 * 1024 - 1024 && kSmem + 2 * (ShrinkMma<16>::kSmem + 1024) > 228 * 1024 - 1024, "no room beside two halves of tensor memory");
     static_assert(kTile * kShare * 4 <= kOffV && kStage % 1024 == 0, "sums fit where the stages were");
 };
 template <typename T, typename TD, int kRank, bool kVec>
@@ -1381,9 +1382,9 @@ cugl_status launch_shrink_mma(cugl_context *ctx, const LoraParams &p, int64_t ti
     }
     auto                     kernel  = lora_shrink_mma_kernel<T, kRank>;
     static std::atomic<bool> set[64] = {};
-    CUGL_TRY(allow_smem(ctx, kernel, S::smem(kChains), set));
+    CUGL_TRY(allow_smem(ctx, kernel, S::kSmem, set));
     const int split = shrink_split(ctx, p, tiles);
-    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::smem(p.chains), split, tiles * split, map_a, map_x, map_few, p));
+    CUGL_CUDA_TRY(ctx, launch_dependent_cluster(ctx, kernel, dim3(static_cast<unsigned>(tiles * split)), kThreads, S::kSmem, split, tiles * split, map_a, map_x, map_few, p));
     return CUGL_SUCCESS;
 }
 template <typename T, int kRank, int kIn>
