@@ -655,7 +655,6 @@ template <typename T, typename TD, int kRank>
 struct Expand
 {
     static constexpr int kSteps   = kRank / 16;
-    static constexpr int kCtas    = kRank == 128 ? 1 : 2; // per SM
     static constexpr bool kAhead  = kRank <= 32;          // the next item's B in registers
     static constexpr int kParts   = std::is_same<T, __nv_bfloat16>::value && sizeof(TD) == 4 ? 3 : 2;
     static constexpr int kTile    = Shrink<kRank>::kTile;
@@ -665,6 +664,11 @@ struct Expand
     static constexpr int kSlots   = 4;
     static constexpr int kOffBase = 2 * kV;
     static constexpr int kSmem    = kOffBase + kWarps * kSlots * 16 * kRow;
+    // CTAs per SM: as many as shared memory holds with the list, the scan and the 1 KB that goes with a CTA.  Rank 64 in three parts is one (a
+    // grid and registers for two of them, which ran one after the other: 4096 tokens of 7 requests, 4096 -> 4096, bf16 to F32 57 us, this 53).
+    static constexpr int kWhole   = kSmem + kListed * static_cast<int>(sizeof(Item)) + static_cast<int>(sizeof(ScanShared)) + 1024;
+    static constexpr int kCtas    = kRank == 128 || 2 * kWhole > 228 * 1024 ? 1 : 2;
+    static_assert(kWhole <= 228 * 1024 && kListed * sizeof(Item) <= 8192, "shared memory of an SM");
 };
 // the first channel of a lane's piece of 16 bytes
 template <typename TD>

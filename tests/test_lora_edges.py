@@ -83,3 +83,10 @@ def test_calls_on_three_streams(ctx, rank, dtype):
     finally:
         for c in own:
             c.close()
+
+
+@pytest.mark.gpu
+def test_wide_results_of_high_ranks_fill_the_gpu_once(ctx):
+    """Rank 64 in three parts leaves room for one CTA of the second launch to an SM: more items than CTAs, whole and ragged rows."""
+    check(ctx, [700, 3, 1000, 64], [0, 1, 2, 0], 64, 512, 4096, capi.BF16, capi.F32)
+    check(ctx, [700, 3, 1000, 64], [0, 1, -1, 0], 50, 512, 2051, capi.BF16, capi.F32, ranks=[50, 7, 33], adapters=3)
