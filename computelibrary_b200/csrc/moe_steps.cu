@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
 {
     __shared__ RouteShared s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
-    const int t0 = static_cast<int>(blockIdx.x) * p.chunk, end = min(t0 + p.chunk, p.tokens);
+    const int t0 = static_cast<int>(blockIdx.x) * p.chunk, end = t0 + min(p.chunk, p.tokens - t0); // (t0 + chunk may pass 32 bits)
     clear_mask(p, s);
     for (int e = threadIdx.x; e < p.experts; e += static_cast<int>(blockDim.x)) s.scan[e] = s.before[e] = 0;
     dependent_prologue();
@@ -506,7 +506,7 @@ int route_chunk(int tokens) // tokens of a block
 int route_chunks(int tokens)
 {
     const int chunk = route_chunk(tokens);
-    return tokens <= chunk ? 1 : (tokens + chunk - 1) / chunk;
+    return tokens <= chunk ? 1 : tokens / chunk + (tokens % chunk != 0 ? 1 : 0); // (tokens + chunk may pass 32 bits)
 }
 
 const char *validate_combine(const cugl_moe_combine_desc *d)
