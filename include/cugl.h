@@ -650,9 +650,9 @@ CUGL_API cugl_status cugl_mx_moe(cugl_context *ctx, const cugl_mx_moe_desc *desc
 CUGL_API int64_t     cugl_mx_group_rows(int32_t groups, int64_t rows);
 
 /* The gate: the top_k largest logits of every token, equal ones by index (NaN and -infinity are never chosen), and a row for every
- * choice.
+ * choice.  (+infinity is the largest logit; infinity over infinity is NaN, and so are all weights of its token.)
  *   ids      [tokens][top_k]  chosen experts, the largest logit first; -1: fewer than top_k could be chosen
- *   weights  [tokens][top_k]  exp(logit) over its sum, over the chosen ones (renormalize) or over all; 0 where there is no choice
+ *   weights  [tokens][top_k]  exp(logit) over its sum, over the chosen ones (renormalize) or over all but NaN; 0 where there is no choice
  *   slots    [tokens][top_k]  the choice's row: the rows of an expert follow each other in the order of the tokens; -1: no choice
  *   groups   [experts][2]     (start, count) of every expert's rows: whole multiples of 128 rows each, one behind the other, within the
  *                             first cugl_mx_group_rows(experts, tokens * top_k) */
