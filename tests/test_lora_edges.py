@@ -90,3 +90,29 @@ def test_wide_results_of_high_ranks_fill_the_gpu_once(ctx):
     """Rank 64 in three parts leaves room for one CTA of the second launch to an SM: more items than CTAs, whole and ragged rows."""
     check(ctx, [700, 3, 1000, 64], [0, 1, 2, 0], 64, 512, 4096, capi.BF16, capi.F32)
     check(ctx, [700, 3, 1000, 64], [0, 1, -1, 0], 50, 512, 2051, capi.BF16, capi.F32, ranks=[50, 7, 33], adapters=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dst", [capi.BF16, capi.F32])
+def test_two_calls_of_short_requests_at_once(ctx, dst):
+    """Each on its stream with its own workspace, again and again."""
+    import torch
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    own = [capi.Context(0, s.cuda_stream) for s in streams]
+    try:
+        calls = [check(ctx, [1] * 24, [(i + turn) % 4 - 1 for i in range(24)], rank, 1024, 2056, capi.BF16, dst, adapters=3, seed=turn)
+                 for turn, rank in enumerate((16, 64))]
+        want = [out.clone() for out, _ in calls]
+        for out, _ in calls:
+            out[:24] = 7
+        torch.cuda.synchronize()
+        for _ in range(100):
+            for c, (_, args) in zip(own, calls):
+                c.lora(*args)
+        for c in own:
+            c.sync()
+        for (out, _), w in zip(calls, want):
+            assert torch.equal(out, w)
+    finally:
+        for c in own:
+            c.close()
