@@ -1416,17 +1416,17 @@ cugl_status launch_expand(cugl_context *ctx, LoraParams p, int64_t tiles)
     return CUGL_SUCCESS;
 }
 // CTAs of a cluster that works on both products in one launch; 0: two launches.  One launch where requests are short, and are eight at least or
-// have little to add (few channels, low ranks).  us in two / in one, K = 4096, requests x tokens.  Rank 16, N = 14336, BF16: 1 x 1 6.8 / 7.9,
-// 8 x 1 8.5 / 8.4, 24 x 1 13.3 / 9.3, 148 x 1 47 / 26, 24 x 8 14.4 / 10.8, 24 x 16 15.7 / 19.2, 256 x 4 78 / 49.  Rank 64, N = 4096, BF16: 1 x 1
-// 7.4 / 7.8, 8 x 1 8.9 / 8.4, 24 x 8 14.0 / 12.2, 8 x 16 9.3 / 11.8.  Rank 16, N = 4096, F16 to F32: 1 x 1 6.7 / 6.1, 24 x 8 9.2 / 7.5.  Rank 128,
+// have little to add (few channels, low ranks).  us in two / in one, K = 4096, requests x tokens.  Rank 16, N = 14336, BF16: 1 x 1 6.7 / 7.9,
+// 8 x 1 8.5 / 8.4, 24 x 1 13.3 / 9.4, 148 x 1 47 / 26, 24 x 8 13.8 / 10.5, 24 x 16 15.7 / 14.2, 256 x 4 78 / 50.  Rank 64, N = 4096, BF16: 1 x 1
+// 7.2 / 7.8, 8 x 1 8.6 / 8.5, 24 x 8 13.8 / 12.1, 8 x 16 9.1 / 12.0.  Rank 16, N = 4096, F16 to F32: 1 x 1 6.6 / 6.3, 24 x 8 9.3 / 7.7.  Rank 128,
 // N = 4096, BF16: 1 x 1 8.7 / 11.6, 24 x 1 20.4 / 20.3.
-int few_split(const cugl_context *ctx, const LoraParams &p, int padded)
+int few_split(const LoraParams &p, int padded)
 {
     const int64_t some = std::min(p.requests, p.tokens), wide = (static_cast<int64_t>(p.N) + 32 * kWarps - 1) / (32 * kWarps);
     if (padded > kFewRank || p.tokens > 8 * some || (some < 8 && wide * padded > 256)) return 0;
-    int split = kMaxSplit; // clusters that run at once: 28 of eight CTAs 9.2 us, of four 13.7; 37 16.9 and 14.1
-    while (split > 1 && some * split * 5 > 8ll * ctx->sm_count) split /= 2;
-    return split;
+    // as many as run at once (see mx_split).  us with eight / four / two / one CTA, rank 16, N = 14336, requests of a token: 30 9.5 / 13.9 / 22 / 40,
+    // 40 17.1 / 14.7 / 24 / 41, 60 19 / 15.0 / 25 / 42, 74 27 / 26 / 23 / 41, 148 47 / 41 / 26 / 42, 160 48 / 43 / 48 / 46
+    return some <= 33 ? 8 : some <= 71 ? 4 : some <= 148 ? 2 : 1;
 }
 template <typename T, typename TD, int kRank>
 cugl_status launch_few(cugl_context *ctx, LoraParams p, int64_t tiles, int split, bool vec_out)
@@ -1450,7 +1450,7 @@ cugl_status launch_lora(cugl_context *ctx, const LoraParams &p, int64_t tiles, i
 {
     if constexpr (kRank <= kFewRank)
     {
-        const int split = rows_in == kUnits16 ? few_split(ctx, p, kRank) : 0;
+        const int split = rows_in == kUnits16 ? few_split(p, kRank) : 0;
         if (split > 0) return launch_few<T, TD, kRank>(ctx, p, few_tiles, split, vec_out);
     }
     CUGL_TRY((rows_in == kUnits16 ? launch_shrink_mma<T, kRank>(ctx, p, tiles)

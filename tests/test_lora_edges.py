@@ -116,3 +116,11 @@ def test_two_calls_of_short_requests_at_once(ctx, dst):
     finally:
         for c in own:
             c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [7, 8, 33, 34, 71, 72, 119, 148, 149])
+def test_numbers_of_short_requests_where_clusters_change(ctx, R):
+    rng = np.random.default_rng(R)
+    check(ctx, [1] * R, rng.integers(-1, 3, R).tolist(), 16, 1024, 2312, capi.BF16, capi.BF16, adapters=3)
+    check(ctx, rng.integers(1, 4, R).tolist(), rng.integers(-1, 3, R).tolist(), 40, 1000, 521, capi.F16, capi.F32, adapters=3, ranks=[40, 3, 17])
