@@ -17,7 +17,8 @@
 // of a warp's 32 channels are dealt out so that a lane's results are whole 16-byte pieces of a row.
 //
 // v is kept as two 16-bit parts, v = high + low (three where bf16 adapters add to 32-bit results): 16 (bf16) or 22 (f16) bits of it
-// count, 24 with three parts, so rounding v costs less than rounding the result.  f16 parts would leave that type's range: a token's
+// count, 24 with three parts, so rounding v costs less than rounding the result (prompts, K = 4096, ranks up to 64, F16 to F32: 1.7e-8 of it
+// beside 2.5e-8).  f16 parts would leave that type's range: a token's
 // v is first divided by a power of two that brings its largest rank into [1, 2).
 #include "mx_mma.cuh"
 
@@ -505,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 // ---- first launch, other rows ----------------------------------------------------------------------------------
 // Rows that are not 16-byte aligned: a warp takes a row, a lane two of its columns.  A block passes through registers, asked for before
 // the one ahead of it is multiplied by the warps' own matrix instructions: a warp takes 16 columns of a block and 32 (16) tokens; tiles of
-// few tokens leave every other block to the other half of the warps.
+// few tokens leave every other block to the other half of the warps.  What bounds it: one block of K in flight per CTA (404 tokens, K = 6319,
+// 25 us); and at ranks 64 and 128 rows that start anywhere take two registers a pair of columns and spill 192 and 372 bytes.
 template <typename T, int kRank, int kIn>
 __global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(const __grid_constant__ LoraParams p)
 {
@@ -986,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, (Expand<T, TD, kRank>::kCtas)) lora_
 // ranks-th block of 256 channels.  What bounds it is the chain requests -> tile (2 us) -> x and A -> sums (4 us) -> results (3 us, 24 requests
 // of a token, 14336 channels), and in the last part its instructions: addresses that are kept, v in registers at 16 ranks and no work for
 // rows that are not there took 10.8 to 9.3 us.  B and base of a warp's first blocks are on their way before the sums are there, those of the
-// blocks to come while others are multiplied.
+// blocks to come while others are multiplied (at rank 16 and 32-bit results 128 registers are 40 bytes too few).
 template <typename T, typename TD, int kRank>
 struct Few
 {
@@ -1356,7 +1358,7 @@ int64_t most_tiles(const cugl_lora_desc &d, int64_t tile) // of a request, all b
     return (d.tokens - some) / tile + some;
 }
 
-// CTAs that share a tile's K: as many as run at once, two to an SM, with four blocks of 64 columns each at least
+// CTAs that share a tile's K: as many as run at once, two to an SM, with two blocks of 64 columns each at least
 int shrink_split(const cugl_context *ctx, const LoraParams &p, int64_t tiles)
 {
     int split = 1;

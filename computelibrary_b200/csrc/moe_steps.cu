@@ -496,7 +496,7 @@ const char *validate_route(const cugl_moe_route_desc *d)
     if (static_cast<int64_t>(d->tokens) * d->top_k + static_cast<int64_t>(kSlab) * d->experts > INT32_MAX - 1024) return "more rows than 32 bits count";
     return nullptr;
 }
-int route_chunk(int tokens) // tokens of a block
+int route_chunk(int tokens) // tokens of a block; 148, the SMs of a B200: the workspace's size follows from it, and asking for that names no device
 {
     // one token a warp while there is an SM for every block: 8192 tokens, 128 experts, 256 blocks of 32 17.2 us, 128 of 64 13.3
     if (tokens <= 148 * kRouteSingle) return kRouteSingle;

@@ -90,7 +90,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // Programmatic dependent launch.  launch_dependents: the next kernel of the stream may be scheduled (it starts on SMs
 // this grid has left, or never used) and run its prologue; wait: returns once the preceding kernel has completed and
 // its memory operations are visible -- every access to global memory of a kernel launched that way comes after it, but for
-// prefetches into L2 and the expert layer's third launch, which reads what was complete before its predecessor let it start.
+// prefetches into L2 and two kernels that read what was complete before their predecessor let them start: the expert layer's third launch,
+// and lora_expand_kernel (starts, adapters, ranks, B, base).  Both rest on that predecessor's passing its own wait before it triggers.
 // Without the launch attribute both are no-ops.
 __device__ __forceinline__ void griddep_launch_dependents()
 {

@@ -746,7 +746,7 @@ CUGL_API cugl_status cugl_mx_grouped_gemm(cugl_context *ctx, const cugl_mx_group
  * The tokens of request i are [starts[i], starts[i + 1]); its adapter is request_adapters[i], any index outside 0 .. adapters - 1 for
  * none (dst[t] = base[t]).  Adapter a has ranks[a] ranks, at most max_rank; what lies behind them in A and B counts nothing.  Float sums;
  * x . A^T is kept to 16 bits or more (22 for CUGL_F16, 24 where bf16 adapters add to 32-bit results), the sum is rounded once.  Tokens of
- * no request are left as they were.  No counterpart in the reference.
+ * no request are left as they were.  An infinity in A or B gives infinities or NaN.  No counterpart in the reference.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct cugl_lora_desc
 {
@@ -767,8 +767,10 @@ CUGL_API cugl_status cugl_lora_validate(const cugl_lora_desc *desc, const char *
 CUGL_API size_t      cugl_lora_workspace_bytes(const cugl_lora_desc *desc);
 /* starts: int32 [requests + 1], in order; request_adapters: int32 [requests]; ranks: int32 [adapters] or NULL (max_rank); scales: float
  * [adapters].  B and the workspace are 16-byte aligned, B's rows are read in whole units of 8 bytes.  dst may be base (then ld_dst ==
- * ld_base), else it overlaps nothing.  One launch where requests are short (eight tokens or fewer on average), rows of x and A are 16-byte
- * aligned and ranks at most 64, two otherwise; equal calls give equal bits.  tokens == 0 or requests == 0: nothing to do. */
+ * ld_base), else it overlaps nothing.  Requests make at most 65535 tiles of 64 tokens (32 above 64 ranks).  One launch where max_rank is at
+ * most 64, rows of x and A are 16-byte aligned, requests are short (eight tokens or fewer on average) and are eight or more, or fewer with
+ * little to add (N / 256 and max_rank, each rounded up, the latter to 16, 32 or 64, multiply to at most 256); two otherwise.  Equal calls
+ * give equal bits.  tokens == 0 or requests == 0: nothing to do. */
 CUGL_API cugl_status cugl_lora(cugl_context *ctx, const cugl_lora_desc *desc, const void *d_x, const int32_t *d_starts,
                                const int32_t *d_request_adapters, const int32_t *d_ranks, const float *d_scales,
                                const void *d_a, const void *d_b, const void *d_base, void *d_dst, void *d_workspace,
