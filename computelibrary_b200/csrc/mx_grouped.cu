@@ -199,10 +199,10 @@ __device__ __forceinline__ void finish_as(const uint32_t (&a)[16], const uint32_
 {
     if constexpr (kSwiglu)
     {
-        float least = 0.f;
+        float top = 0.f; // of the gates' magnitudes: one instruction for two
 #pragma unroll
-        for (int i = 0; i < 16; ++i) least = fminf(least, __uint_as_float(a[i]) * f.alpha);
-        if (least >= kSiluTail)
+        for (int i = 0; i < 16; i += 2) asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(__uint_as_float(a[i])), "f"(__uint_as_float(a[i + 1])));
+        if (top * fabsf(f.alpha) <= -kSiluTail)
         {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = swiglu<kShort>(__uint_as_float(a[i]) * f.alpha, __uint_as_float(u[i]) * f.up);
