@@ -70,7 +70,7 @@ __device__ __forceinline__ int route_token(const RouteParams &p, int t, int lane
     constexpr int kBytes = kPer * static_cast<int>(sizeof(T)), kUnit = kBytes >= 16 ? 16 : kBytes;
     if (p.vec != 0 && (lane + 1) * kPer <= p.experts)
     {
-        T e[kPer];
+        alignas(16) T e[kPer];
 #pragma unroll
         for (int i = 0; i < kBytes / kUnit; ++i)
         {
